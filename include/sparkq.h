@@ -551,6 +551,118 @@ int sparkq_attention_gate(const void* x, const void* attn, const void* gate_w,
                           int64_t H, int64_t D, int64_t hidden, int dtype,
                           void* stream);
 
+/* ------------------------------------------------------------------------
+ * Many sequences over one paged INT8 KV cache (no counterpart in the
+ * reference, which serves one request at a time over contiguous caches).
+ *
+ * Cache: two code tensors int8 [pages,Hkv,page_size,D] of symmetric s8 codes,
+ *   each with fp16 scales [pages,Hkv,page_size] (the SPARKQ_KV_S8_F16SCALE
+ *   values: code * scale). page_size is a power of two from 16 to 1024; D is
+ *   64, 128 or 256.
+ * Batch: B sequences. Token t of sequence b lies in page page_table[b *
+ *   table_stride + t / page_size], slot t % page_size; an entry outside
+ *   [0, pages) is no page. lengths[b] counts b's tokens, the new ones
+ *   included. The new tokens' rows are packed: those of sequence b are rows
+ *   starts[b] .. starts[b+1] - 1 of T, the last of them its token lengths[b] - 1.
+ *   page_table int32 [B,max_pages], starts int32 [B+1], lengths int32 [B], all
+ *   on the device and read by the kernels only: nothing synchronises, and
+ *   nothing out of range in them is followed (starts are clamped to [0,T] and
+ *   to ascend, lengths to [0, max_pages * page_size]).
+ * strides[0..2] key codes (page, head, token) in bytes, multiples of 16;
+ *   strides[3..5] key scales (page, head, token) in elements; [6..11] values.
+ * ---------------------------------------------------------------------- */
+
+/* RMS norm of every query and key head with the rotary position embedding in
+ * the same pass: y = x * rsqrt(mean(x^2) + eps) * w over one head's D values,
+ * then pairs (i, i + dims/2) of y (or (2i, 2i+1) when traditional), i <
+ * dims/2, rotated by theta = scale * position * base^(-2i/dims); dims past
+ * `dims` are normed only. fp32 (the angle in fp64), one rounding.
+ *   q [T,Hq,D], k [T,Hkv,D] with strides[0..3] = q token, q head, k token,
+ *   k head in elements (views of a packed projection); weights [D] in dtype
+ *   (BF16 or F16); positions [T], int32 (position_bits 32) or int64 (64);
+ *   q_out [T,Hq,D] and k_out [T,Hkv,D] contiguous, apart from the inputs. */
+int sparkq_qk_norm_rope(const void* q, const void* k, const void* q_weight,
+                        const void* k_weight, const void* positions, int position_bits,
+                        void* q_out, void* k_out, int64_t T, int64_t Hq, int64_t Hkv,
+                        int64_t D, int dims, int traditional, float eps, double base,
+                        double scale, int dtype, const int64_t* strides, void* stream);
+
+/* Quantize-on-append of a batch's new tokens into their pages: k and v
+ * [T,Hkv,D] with x_strides[0..3] = k token, k head, v token, v head in
+ * elements, quantized by the sparkq_kv_quantize_s8 formula. Rows that fall to
+ * no sequence, tokens before position 0 and tokens without a page are
+ * skipped; the rest of the pool is untouched. Sequences that append must not
+ * share the page that they append to (sparkq_kv_pages_fork sees to that). */
+int sparkq_paged_kv_append(const void* k, const void* v, void* k_codes, void* k_scales,
+                           void* v_codes, void* v_scales, const int32_t* page_table,
+                           const int32_t* starts, const int32_t* lengths, int64_t T,
+                           int64_t B, int64_t Hkv, int64_t D, int64_t pages,
+                           int64_t max_pages, int64_t table_stride, int page_size,
+                           int x_dtype, const int64_t* x_strides, const int64_t* strides,
+                           void* stream);
+
+/* Attention of a batch's new tokens over their pages: q [T,Hq,D] (BF16 or
+ * F16) with q_strides[0..1] = token, head in elements (16-byte aligned rows),
+ * out [T,Hq,D] contiguous in out_dtype (q_dtype or F32). causal = 1: row i of
+ * a sequence's n sees its tokens 0 .. length - n + i; 0: all of them. Tokens
+ * without a page are hidden; a row that sees nothing is zero; rows of out
+ * that fall to no sequence are left as they were. max_new bounds the new
+ * tokens of one sequence: of longer ones the rows past it are left as they
+ * were too. A chunk of one token per sequence is the decode step. Workspace:
+ * sparkq_paged_sdpa_workspace_bytes (max_tokens = max_pages * page_size), any
+ * initial value. */
+size_t sparkq_paged_sdpa_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv,
+                                         int64_t D, int64_t max_new, int64_t max_tokens);
+int sparkq_paged_sdpa(const void* q, const void* k_codes, const void* k_scales,
+                      const void* v_codes, const void* v_scales, const int32_t* page_table,
+                      const int32_t* starts, const int32_t* lengths, void* out, int64_t T,
+                      int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages,
+                      int64_t max_pages, int64_t table_stride, int page_size,
+                      int64_t max_new, int causal, int q_dtype, int out_dtype, float scale,
+                      const int64_t* q_strides, const int64_t* strides, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* Pages of a batch, for one step of its sequences, in every layer of a pool.
+ * The four tensors (key codes, value codes, key scales, value scales: the
+ * order of bufs[0..3]) are [layers,pages,...] with buf_strides[2i],
+ * buf_strides[2i+1] = layer, page in bytes; one page of one layer is
+ * code_bytes (scale_bytes) in one piece. All of these are multiples of 16.
+ * A sequence holds the first ceil(length / page_size) entries of its row.
+ *
+ * fork: row i continues sequence parents[i] (itself where parents is NULL;
+ * outside [0,B): an empty row) and gets pages for new_tokens[i] more tokens
+ * (NULL: none; no more than its row of max_pages holds): out_table
+ * [rows,max_pages], out_lengths [rows] with the new tokens. Pages that no new
+ * row holds are free, and are dealt in ascending order to the rows in order.
+ * The partly filled last page of a row that gets tokens is its own to write:
+ * where another row holds it too the row gets a copy, except the first of its
+ * writers where all its holders are writers. out_missing[0] = pages short;
+ * when it is not 0 the entries that got none are -1 and no page is copied, so
+ * the batch before the call still stands. Dropping a sequence frees its pages.
+ *
+ * compact: with U pages in use (out_used[0]), the pages numbered U or higher
+ * move, in order, to the free numbers below U. out_table [B,max_pages].
+ *
+ * Entries past a row's pages are -1. out_table must not overlap page_table.
+ * Workspace: sparkq_kv_pages_workspace_bytes(rows (compact: B), pages), any
+ * initial value. */
+size_t sparkq_kv_pages_workspace_bytes(int64_t rows, int64_t pages);
+int sparkq_kv_pages_fork(void* k_codes, void* v_codes, void* k_scales, void* v_scales,
+                         const int32_t* page_table, const int32_t* lengths,
+                         const int32_t* parents, const int32_t* new_tokens,
+                         int64_t table_stride, int32_t* out_table, int32_t* out_lengths,
+                         int32_t* out_missing, const int64_t* buf_strides, int64_t B,
+                         int64_t rows, int64_t max_pages, int64_t pages, int64_t layers,
+                         int page_size, int64_t code_bytes, int64_t scale_bytes,
+                         void* workspace, size_t workspace_bytes, void* stream);
+int sparkq_kv_pages_compact(void* k_codes, void* v_codes, void* k_scales, void* v_scales,
+                            const int32_t* page_table, const int32_t* lengths,
+                            int64_t table_stride, int32_t* out_table, int32_t* out_used,
+                            const int64_t* buf_strides, int64_t B, int64_t max_pages,
+                            int64_t pages, int64_t layers, int page_size, int64_t code_bytes,
+                            int64_t scale_bytes, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

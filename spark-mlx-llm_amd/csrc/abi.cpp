@@ -12,6 +12,7 @@
 #include <mutex>
 
 #include "common.h"
+#include "paged.h"
 #include "sparkq.h"
 
 namespace sparkq {
@@ -50,6 +51,30 @@ int int8kv_sdpa_decode_noalloc(const void* q, const void* kc, const void* ks, co
                                int fmt, int qdt, int odt, float scale, const int64_t* strides,
                                hipStream_t st);
 size_t decode_scratch_bytes();
+// launchers (qknorm.hip, paged.hip, paged_sdpa.hip)
+int qk_norm_rope(const void* q, const void* k, const void* wq, const void* wk, const void* pos,
+                 int pos64, void* qo, void* ko, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                 int dims, int traditional, float eps, double base, double scale, int dt,
+                 const int64_t* st, hipStream_t stream);
+int paged_kv_append(const PagedBatch& p, const void* k, const void* v, const int64_t* xst,
+                    const PagedSide& ks, const PagedSide& vs, int64_t H, int64_t D, int xdt,
+                    hipStream_t st);
+size_t paged_sdpa_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                            int64_t max_new, int64_t max_tokens);
+int paged_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, const PagedSide& ks,
+               const PagedSide& vs, void* out, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
+               int causal, int qdt, int odt, float scale, void* ws, size_t wsb, hipStream_t st);
+size_t kv_pages_workspace(int64_t rows, int64_t pages);
+int kv_pages_fork(const int32_t* table, int64_t table_stride, const int32_t* lengths,
+                  const int32_t* parents, const int32_t* fresh, int32_t* out_table,
+                  int32_t* out_lengths, int32_t* missing, int64_t B, int64_t rows, int64_t width,
+                  int64_t pages, int page_size, int64_t layers, void* const* bufs,
+                  const int64_t* strides, int64_t code_bytes, int64_t scale_bytes, void* ws,
+                  hipStream_t st);
+int kv_pages_compact(const int32_t* table, int64_t table_stride, const int32_t* lengths,
+                     int32_t* out_table, int32_t* used, int64_t B, int64_t width, int64_t pages,
+                     int page_size, int64_t layers, void* const* bufs, const int64_t* strides,
+                     int64_t code_bytes, int64_t scale_bytes, void* ws, hipStream_t st);
 int kv_quantize_s8(const void* x, int8_t* codes, void* scales, int64_t R, int64_t D, int xdt,
                    hipStream_t st);
 int kv_append(const void* x, void* codes, void* scales, void* biases, int64_t B, int64_t H,
@@ -853,6 +878,196 @@ int sparkq_quantized_sdpa(const void* q, const void* k_packed, const void* k_sca
                       mask_kind, mask_dtype, mask_strides, out, B, Hq, Hkv, L, N, D, Dv,
                       group_size, bits, q_dtype, out_dtype, scale, strides, workspace,
                       workspace_bytes, (hipStream_t)stream);
+}
+
+int sparkq_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight,
+                        const void* positions, int position_bits, void* q_out, void* k_out,
+                        int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int dims, int traditional,
+                        float eps, double base, double scale, int dtype, const int64_t* strides,
+                        void* stream) {
+  REQUIRE(T >= 0 && Hq > 0 && Hkv > 0 && D > 0, "qk_norm_rope: bad shape");
+  REQUIRE(T <= kI32Max && Hq <= kI32Max && Hkv <= kI32Max && D <= kI32Max &&
+              T <= 4LL * kI32Max / (Hq + Hkv),
+          "qk_norm_rope: shape too large");
+  REQUIRE((T == 0 || (q && k && positions && q_out && k_out)) && q_weight && k_weight && strides,
+          "qk_norm_rope: null tensor pointer");
+  REQUIRE(position_bits == 32 || position_bits == 64, "qk_norm_rope: positions must be int32 or int64");
+  REQUIRE(is_half_dtype(dtype), "qk_norm_rope requires BF16 or F16 queries and keys");
+  REQUIRE(dims > 0 && dims % 2 == 0 && dims <= D,
+          "qk_norm_rope: dims must be positive, even and no larger than the head dim");
+  REQUIRE(std::isfinite(base) && base > 0 && std::isfinite(scale) && std::isfinite(eps) && eps >= 0,
+          "qk_norm_rope: base must be positive and finite, scale finite, eps nonnegative");
+  DEVICE_OK();
+  return qk_norm_rope(q, k, q_weight, k_weight, positions, position_bits == 64, q_out, k_out, T, Hq,
+                      Hkv, D, dims, traditional != 0, eps, base, scale, dtype, strides,
+                      (hipStream_t)stream);
+}
+
+// The checks that every entry point over a paged cache shares.
+static int paged_check(const char* op, int64_t T, int64_t B, int64_t Hkv, int64_t D, int64_t pages,
+                       int64_t max_pages, int64_t table_stride, int page_size, const void* kc,
+                       const void* ks, const void* vc, const void* vs, const int64_t* st) {
+  REQUIRE(T >= 0 && B >= 0 && Hkv > 0 && D > 0 && pages > 0 && max_pages > 0, "%s: bad shape", op);
+  REQUIRE(T <= kI32Max && B < kI32Max && Hkv <= 65535 && pages <= kI32Max && max_pages <= kI32Max,
+          "%s: shape too large", op);
+  REQUIRE_SUPPORTED(D == 64 || D == 128 || D == 256, "%s: head dim must be 64, 128 or 256 (got %lld)",
+                    op, (long long)D);
+  REQUIRE(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
+          "%s: page_size must be a power of two from 16 to 1024 (got %d)", op, page_size);
+  REQUIRE(max_pages <= kI32Max / page_size, "%s: more than 2^31 tokens in a row of pages", op);
+  REQUIRE(table_stride >= max_pages || B <= 1, "%s: table rows overlap", op);
+  REQUIRE(kc && ks && vc && vs && st, "%s: null tensor pointer", op);
+  for (int i = 0; i < 12; ++i) REQUIRE(st[i] >= 0, "%s: negative stride", op);
+  for (int i = 0; i < 12; i += 6)
+    REQUIRE(st[i] % 16 == 0 && st[i + 1] % 16 == 0 && st[i + 2] % 16 == 0,
+            "%s: code strides must be multiples of 16 bytes", op);
+  REQUIRE(aligned(kc, 16) && aligned(vc, 16) && aligned(ks, 2) && aligned(vs, 2),
+          "%s: codes must be 16-byte aligned", op);
+  return SPARKQ_OK;
+}
+
+static PagedSide paged_side(const void* codes, const void* scales, const int64_t* st) {
+  return PagedSide{(uint8_t*)const_cast<void*>(codes), (uint16_t*)const_cast<void*>(scales),
+                   st[0], st[1], st[2], st[3], st[4], st[5]};
+}
+
+static PagedBatch paged_batch(const int32_t* table, const int32_t* starts, const int32_t* lengths,
+                              int64_t T, int64_t B, int64_t pages, int64_t max_pages,
+                              int64_t table_stride, int page_size) {
+  return PagedBatch{table, starts, lengths, table_stride, (int)B, (int)T, (int)max_pages, (int)pages,
+                    __builtin_ctz((unsigned)page_size)};
+}
+
+int sparkq_paged_kv_append(const void* k, const void* v, void* k_codes, void* k_scales,
+                           void* v_codes, void* v_scales, const int32_t* page_table,
+                           const int32_t* starts, const int32_t* lengths, int64_t T, int64_t B,
+                           int64_t Hkv, int64_t D, int64_t pages, int64_t max_pages,
+                           int64_t table_stride, int page_size, int x_dtype,
+                           const int64_t* x_strides, const int64_t* strides, void* stream) {
+  if (int rc = paged_check("paged_kv_append", T, B, Hkv, D, pages, max_pages, table_stride, page_size,
+                           k_codes, k_scales, v_codes, v_scales, strides))
+    return rc;
+  REQUIRE((T == 0 || (k && v)) && x_strides && starts && (B == 0 || (page_table && lengths)),
+          "paged_kv_append: null tensor pointer");
+  REQUIRE(is_float_dtype(x_dtype), "paged_kv_append: keys and values must be float16, bfloat16 or float32");
+  REQUIRE(T <= 2 * kI32Max / Hkv, "paged_kv_append: shape too large");
+  DEVICE_OK();
+  return paged_kv_append(paged_batch(page_table, starts, lengths, T, B, pages, max_pages, table_stride,
+                                     page_size),
+                         k, v, x_strides, paged_side(k_codes, k_scales, strides),
+                         paged_side(v_codes, v_scales, strides + 6), Hkv, D, x_dtype,
+                         (hipStream_t)stream);
+}
+
+size_t sparkq_paged_sdpa_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                         int64_t max_new, int64_t max_tokens) {
+  if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || max_new <= 0 || max_tokens <= 0)
+    return 0;
+  return paged_sdpa_workspace(T, B, Hq, Hkv, D, max_new, max_tokens);
+}
+
+int sparkq_paged_sdpa(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                      const void* v_scales, const int32_t* page_table, const int32_t* starts,
+                      const int32_t* lengths, void* out, int64_t T, int64_t B, int64_t Hq,
+                      int64_t Hkv, int64_t D, int64_t pages, int64_t max_pages,
+                      int64_t table_stride, int page_size, int64_t max_new, int causal, int q_dtype,
+                      int out_dtype, float scale, const int64_t* q_strides, const int64_t* strides,
+                      void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = paged_check("paged_sdpa", T, B, Hkv, D, pages, max_pages, table_stride, page_size,
+                           k_codes, k_scales, v_codes, v_scales, strides))
+    return rc;
+  REQUIRE(Hq > 0 && Hq % Hkv == 0, "paged_sdpa: query heads must be divisible by KV heads");
+  REQUIRE(max_new > 0 && max_new <= kI32Max, "paged_sdpa: max_new must be positive");
+  REQUIRE(Hq <= 65535 && T <= kI32Max / Hq, "paged_sdpa: shape too large");
+  REQUIRE((T == 0 || (q && out)) && q_strides && starts && (B == 0 || (page_table && lengths)),
+          "paged_sdpa: null tensor pointer");
+  REQUIRE(is_half_dtype(q_dtype), "paged_sdpa requires float16 or bfloat16 queries");
+  REQUIRE(out_dtype == q_dtype || out_dtype == SPARKQ_F32,
+          "paged_sdpa: out dtype must be the query dtype or float32");
+  REQUIRE(std::isfinite(scale), "paged_sdpa: scale must be finite");
+  REQUIRE(q_strides[0] >= 0 && q_strides[1] >= 0 && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0 &&
+              aligned(q, 16) && aligned(out, 16),
+          "paged_sdpa: query rows must be 16-byte aligned");
+  DEVICE_OK();
+  return paged_sdpa(paged_batch(page_table, starts, lengths, T, B, pages, max_pages, table_stride,
+                                page_size),
+                    q, q_strides, paged_side(k_codes, k_scales, strides),
+                    paged_side(v_codes, v_scales, strides + 6), out, Hq, Hkv, D, max_new, causal != 0,
+                    q_dtype, out_dtype, scale, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+size_t sparkq_kv_pages_workspace_bytes(int64_t rows, int64_t pages) {
+  return rows < 0 || pages <= 0 ? 0 : kv_pages_workspace(rows, pages);
+}
+
+static int kv_pages_check(const char* op, void* const* bufs, const int64_t* st, int64_t B,
+                          int64_t rows, int64_t max_pages, int64_t pages, int64_t layers,
+                          int64_t table_stride, int page_size, int64_t code_bytes,
+                          int64_t scale_bytes, const void* ws, size_t wsb) {
+  REQUIRE(B >= 0 && rows >= 0 && max_pages > 0 && pages > 0 && layers > 0 && code_bytes > 0 &&
+              scale_bytes > 0,
+          "%s: bad shape", op);
+  REQUIRE(B < kI32Max && rows < kI32Max && layers <= kI32Max && pages <= kI32Max &&
+              code_bytes <= kI32Max && scale_bytes <= kI32Max && (rows == 0 || max_pages <= kI32Max / rows),
+          "%s: shape too large", op);
+  REQUIRE(page_size >= 16 && page_size <= 1024 && (page_size & (page_size - 1)) == 0,
+          "%s: page_size must be a power of two from 16 to 1024 (got %d)", op, page_size);
+  REQUIRE(max_pages <= kI32Max / page_size, "%s: more than 2^31 tokens in a row of pages", op);
+  REQUIRE(table_stride >= max_pages || B <= 1, "%s: table rows overlap", op);
+  REQUIRE(st, "%s: null strides", op);
+  REQUIRE(code_bytes % 16 == 0 && scale_bytes % 16 == 0, "%s: pages must be multiples of 16 bytes", op);
+  for (int i = 0; i < 4; ++i) {
+    REQUIRE(bufs[i], "%s: null tensor pointer", op);
+    const int64_t one = i < 2 ? code_bytes : scale_bytes;
+    REQUIRE(st[2 * i] >= 0 && st[2 * i + 1] >= one && st[2 * i] % 16 == 0 && st[2 * i + 1] % 16 == 0 &&
+                aligned(bufs[i], 16),
+            "%s: pages must be 16-byte aligned and apart", op);
+  }
+  if (!ws || wsb < kv_pages_workspace(rows, pages))
+    return set_error(SPARKQ_ERR_WORKSPACE, "%s needs a workspace of %zu bytes (got %zu)", op,
+                     kv_pages_workspace(rows, pages), ws ? wsb : (size_t)0);
+  REQUIRE(aligned(ws, 16), "%s: workspace must be 16-byte aligned", op);
+  return SPARKQ_OK;
+}
+
+int sparkq_kv_pages_fork(void* k_codes, void* v_codes, void* k_scales, void* v_scales,
+                         const int32_t* page_table, const int32_t* lengths, const int32_t* parents,
+                         const int32_t* new_tokens, int64_t table_stride, int32_t* out_table,
+                         int32_t* out_lengths, int32_t* out_missing, const int64_t* buf_strides,
+                         int64_t B, int64_t rows, int64_t max_pages, int64_t pages, int64_t layers,
+                         int page_size, int64_t code_bytes, int64_t scale_bytes, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  void* const bufs[4] = {k_codes, v_codes, k_scales, v_scales};
+  REQUIRE((B == 0 || (page_table && lengths)) && (rows == 0 || (out_table && out_lengths)) && out_missing,
+          "kv_pages_fork: null tensor pointer");
+  REQUIRE(parents || rows == B, "kv_pages_fork: without parents there is a row for each sequence");
+  if (int rc = kv_pages_check("kv_pages_fork", bufs, buf_strides, B, rows, max_pages, pages, layers,
+                              table_stride, page_size, code_bytes, scale_bytes, workspace,
+                              workspace_bytes))
+    return rc;
+  DEVICE_OK();
+  return kv_pages_fork(page_table, table_stride, lengths, parents, new_tokens, out_table, out_lengths,
+                       out_missing, B, rows, max_pages, pages, page_size, layers, bufs, buf_strides,
+                       code_bytes, scale_bytes, workspace, (hipStream_t)stream);
+}
+
+int sparkq_kv_pages_compact(void* k_codes, void* v_codes, void* k_scales, void* v_scales,
+                            const int32_t* page_table, const int32_t* lengths, int64_t table_stride,
+                            int32_t* out_table, int32_t* out_used, const int64_t* buf_strides,
+                            int64_t B, int64_t max_pages, int64_t pages, int64_t layers,
+                            int page_size, int64_t code_bytes, int64_t scale_bytes, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  void* const bufs[4] = {k_codes, v_codes, k_scales, v_scales};
+  REQUIRE((B == 0 || (page_table && lengths && out_table)) && out_used,
+          "kv_pages_compact: null tensor pointer");
+  if (int rc = kv_pages_check("kv_pages_compact", bufs, buf_strides, B, B, max_pages, pages, layers,
+                              table_stride, page_size, code_bytes, scale_bytes, workspace,
+                              workspace_bytes))
+    return rc;
+  DEVICE_OK();
+  return kv_pages_compact(page_table, table_stride, lengths, out_table, out_used, B, max_pages, pages,
+                          page_size, layers, bufs, buf_strides, code_bytes, scale_bytes, workspace,
+                          (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -1,0 +1,433 @@
+// paged.hip -- what keeps a paged INT8 KV cache: the quantized append of new
+// tokens, and forking and compacting of its pages (gfx950).
+//
+// A cache is two code tensors [P, Hkv, page, D] (symmetric s8) with one fp16
+// scale per (page, KV head, token). Sequence b's token t lies in page
+// table[b, t / page], slot t % page.
+#include <algorithm>
+
+#include "paged.h"
+
+namespace sparkq {
+namespace {
+
+// ---------------------------------------------------------------------------
+// quantize-on-append
+// ---------------------------------------------------------------------------
+// Row t of the packed new tokens is token length - count + (t - first) of the
+// sequence that it falls to. The formula is kv_append's: scale = fp16(amax /
+// 127), 1 where that is zero, code = clamp(rint(x / scale), -127, 127).
+struct PagedAppendArgs {
+  PagedBatch p;
+  const void *k, *v;
+  int64_t k_tok, k_head, v_tok, v_head;  // input strides (elements)
+  PagedSide ks, vs;
+  int H, D, x_dtype;
+};
+
+// the sequence whose rows hold packed row t, or -1
+__device__ __forceinline__ int seq_of_row(const PagedBatch& p, int t) {
+  int lo = 0, hi = p.B;  // the first b with starts[b + 1] > t
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (p.starts[mid + 1] > t)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo < p.B ? lo : -1;
+}
+
+__global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (int64_t)a.p.T * a.H * 2) return;
+  const bool isv = row & 1;
+  const int t = (int)((row >> 1) / a.H), h = (int)((row >> 1) - (int64_t)t * a.H);
+  const int b = seq_of_row(a.p, t);
+  if (b < 0) return;
+  const SeqRows s = seq_rows(a.p, b);
+  const int pos = s.length - s.count + (t - s.first);
+  if (t < s.first || t >= s.first + s.count || pos < 0) return;
+  const int id = page_of(a.p, b, pos);
+  if (id < 0) return;
+  const PagedSide& side = isv ? a.vs : a.ks;
+  const int64_t x0 = isv ? t * a.v_tok + h * a.v_head : t * a.k_tok + h * a.k_head;
+  const void* x = isv ? a.v : a.k;
+  float amax = 0.0f;
+  for (int d = lane; d < a.D; d += 64) amax = fmaxf(amax, fabsf(load_in(x, x0 + d, a.x_dtype)));
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+  uint16_t s16 = f32_to_f16(amax / 127.0f);
+  if (f16_to_f32(s16) == 0.0f) s16 = 0x3C00u;
+  const float sc = f16_to_f32(s16);
+  const int slot = pos & ((1 << a.p.page_log2) - 1);
+  if (lane == 0) side.scales[id * side.s_page + h * side.s_head + slot * side.s_tok] = s16;
+  int8_t* dst = reinterpret_cast<int8_t*>(side.codes) + id * side.c_page + h * side.c_head + slot * side.c_tok;
+  for (int d = lane; d < a.D; d += 64) {
+    const float v = __builtin_rintf(load_in(x, x0 + d, a.x_dtype) / sc);
+    dst[d] = (int8_t)fminf(fmaxf(v, -127.0f), 127.0f);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// pages: who holds them, which are free, and moving them
+// ---------------------------------------------------------------------------
+// Everything that decides (who holds a page, who gets which free one) is done
+// by one workgroup, so that free pages are dealt in order with no host and no
+// second pass; the tables and the pages themselves are written by a second
+// launch over the whole chip. Counts are integer atomics, so their order does
+// not matter.
+constexpr int kPlanThreads = 1024;
+
+// Workspace, in ints: head, then arrays of P (held, first, list) and of rows
+// (base, src, dst).
+enum { kPairs = 0, kShort = 1, kFree = 2, kUsed = 3, kHead = 16 };
+struct PageScratch {
+  int* head;
+  int *held, *first, *list;
+  int *base, *src, *dst;
+};
+
+__host__ __device__ inline PageScratch page_scratch(int* ws, int64_t pages, int64_t rows) {
+  PageScratch s;
+  s.head = ws;
+  s.held = ws + kHead;
+  s.first = s.held + pages;
+  s.list = s.first + pages;
+  s.base = s.list + pages;
+  s.src = s.base + rows;
+  s.dst = s.src + rows;
+  return s;
+}
+
+// One of the cache's four tensors, by its bytes: layers and pages of it.
+struct PageBuf {
+  uint8_t* p;
+  int64_t layer, page;  // strides (bytes)
+};
+
+struct PageArgs {
+  const int32_t* table;    // [B, width] before
+  const int32_t* lengths;  // [B]
+  const int32_t* parents;  // [rows] or null: row i continues sequence i
+  const int32_t* fresh;    // [rows] new tokens, or null: none
+  int32_t* out_table;      // [rows, width]
+  int32_t* out_lengths;    // [rows] (fork)
+  int32_t* out_count;      // [1] pages short (fork), pages in use (compact)
+  int64_t table_stride;
+  int B, rows, width, pages, page_log2;
+  PageScratch s;
+  PageBuf buf[4];       // codes, codes, scales, scales
+  int vec_codes, vec_scales;  // 16-byte pieces of a page in one layer
+  int layers, table_blocks;
+};
+
+struct RowPlan {
+  int src;            // sequence that the row continues, or -1
+  int before, after;  // tokens before and after the step
+  int held, need;     // pages before and after
+};
+
+__device__ __forceinline__ RowPlan row_plan(const PageArgs& a, int i) {
+  RowPlan r;
+  r.src = a.parents ? a.parents[i] : i;
+  if ((unsigned)r.src >= (unsigned)a.B) r.src = -1;
+  const int64_t room = (int64_t)a.width << a.page_log2;
+  const int64_t n = r.src < 0 ? 0 : min((int64_t)max(a.lengths[r.src], 0), room);
+  const int64_t m = min(n + (a.fresh ? max(a.fresh[i], 0) : 0), room);
+  r.before = (int)n;
+  r.after = (int)m;
+  const int64_t up = (1 << a.page_log2) - 1;
+  r.held = (int)((n + up) >> a.page_log2);
+  r.need = (int)((m + up) >> a.page_log2);
+  return r;
+}
+
+// entry j < held of row r, or -1
+__device__ __forceinline__ int held_page(const PageArgs& a, const RowPlan& r, int j) {
+  const int id = a.table[r.src * a.table_stride + j];
+  return (unsigned)id < (unsigned)a.pages ? id : -1;
+}
+
+// the partly filled last page that the row's new tokens go to, or -1
+__device__ __forceinline__ int write_page(const PageArgs& a, const RowPlan& r) {
+  if (r.after <= r.before || (r.before & ((1 << a.page_log2) - 1)) == 0) return -1;
+  return held_page(a, r, r.held - 1);
+}
+
+// The plan's counters are read and written by one workgroup through atomics
+// of device scope: they are coherent whatever its vector cache holds.
+__device__ __forceinline__ void put(int* p, int v) { splitk_store(p, v); }
+__device__ __forceinline__ int get(const int* p) { return splitk_load(p); }
+
+// exclusive prefix of v over the workgroup's threads; total in every thread
+__device__ __forceinline__ int block_prefix(int v, int* s_wave, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // the last call's readers are done with s_wave
+  if (lane == 63) s_wave[wave] = x;
+  __syncthreads();
+  int below = 0;
+  total = 0;
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    if (w < wave) below += s_wave[w];
+    total += s_wave[w];
+  }
+  return below + x - v;
+}
+
+// held[p] = rows' entries that name page p
+__device__ void count_held(const PageArgs& a) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int p = tid; p < a.pages; p += kPlanThreads) {
+    put(a.s.held + p, 0);
+    put(a.s.first + p, 0x7FFFFFFF);
+  }
+  __threadfence();
+  __syncthreads();
+  for (int i = wave; i < a.rows; i += kPlanThreads / 64) {
+    const RowPlan r = row_plan(a, i);
+    for (int j = lane; j < r.held; j += 64) {
+      const int id = held_page(a, r, j);
+      if (id >= 0) atomicAdd(a.s.held + id, 1);
+    }
+  }
+  __threadfence();
+  __syncthreads();
+}
+
+__global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PageArgs a) {
+  __shared__ int s_wave[kPlanThreads / 64];
+  const int tid = threadIdx.x;
+  count_held(a);
+  // free pages in order: each thread takes a run of pages
+  const int per = (a.pages + kPlanThreads - 1) / kPlanThreads;
+  const int p0 = min(tid * per, a.pages), p1 = min(p0 + per, a.pages);
+  int n = 0, nfree;
+  for (int p = p0; p < p1; ++p) n += get(a.s.held + p) == 0;
+  int at = block_prefix(n, s_wave, nfree);
+  for (int p = p0; p < p1; ++p)
+    if (get(a.s.held + p) == 0) put(a.s.list + at++, p);
+  __threadfence();
+  __syncthreads();
+  // holders that do not write: what is left of held without the writers
+  for (int i = tid; i < a.rows; i += kPlanThreads) {
+    const int w = write_page(a, row_plan(a, i));
+    if (w >= 0) {
+      atomicSub(a.s.held + w, 1);
+      atomicMin(a.s.first + w, i);
+    }
+  }
+  __threadfence();
+  __syncthreads();
+  int wanted = 0, pairs = 0;
+  for (int i0 = 0; i0 < a.rows; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    int copy = 0, w = -1, want = 0;
+    if (i < a.rows) {
+      const RowPlan r = row_plan(a, i);
+      w = write_page(a, r);
+      copy = w >= 0 && (get(a.s.held + w) > 0 || get(a.s.first + w) != i);
+      want = copy + (r.need - r.held);
+    }
+    int t_want, t_copy;
+    const int base = wanted + block_prefix(want, s_wave, t_want);
+    const int pair = pairs + block_prefix(copy, s_wave, t_copy);
+    if (i < a.rows) a.s.base[i] = copy ? ~base : base;  // negative: its first page is a copy
+    if (copy) {
+      a.s.src[pair] = w;
+      a.s.dst[pair] = base < nfree ? get(a.s.list + base) : -1;
+    }
+    wanted += t_want;
+    pairs += t_copy;
+  }
+  if (tid == 0) {
+    const int missing = max(wanted - nfree, 0);
+    a.s.head[kPairs] = missing ? 0 : pairs;
+    a.s.head[kFree] = nfree;
+    *a.out_count = missing;
+  }
+}
+
+__global__ __launch_bounds__(kPlanThreads) void pages_compact_plan_kernel(PageArgs a) {
+  __shared__ int s_wave[kPlanThreads / 64];
+  const int tid = threadIdx.x;
+  count_held(a);
+  const int per = (a.pages + kPlanThreads - 1) / kPlanThreads;
+  const int p0 = min(tid * per, a.pages), p1 = min(p0 + per, a.pages);
+  int n = 0, used, movers;
+  for (int p = p0; p < p1; ++p) n += get(a.s.held + p) != 0;
+  const int below = block_prefix(n, s_wave, used);
+  int m = 0;  // pages in use at or past `used`
+  for (int p = max(p0, used); p < p1; ++p) m += get(a.s.held + p) != 0;
+  int mover = block_prefix(m, s_wave, movers);
+  int hole = p0 - below;  // free pages before p0
+  for (int p = p0; p < p1; ++p) {
+    const bool live = get(a.s.held + p) != 0;
+    if (p < used && !live) a.s.list[hole] = p;
+    if (p >= used && live) {
+      a.s.first[mover] = p;
+      a.s.held[p] = ~mover;  // its new number is list[mover]
+      ++mover;
+    }
+    hole += !live;
+  }
+  if (tid == 0) {
+    a.s.head[kPairs] = movers;
+    *a.out_count = used;
+  }
+}
+
+// Copies page src[i] to dst[i] in every layer of the four tensors, in pieces
+// of 16 KB dealt over the workgroups. No page is both a source and a
+// destination.
+__device__ void copy_pages(const PageArgs& a, const int* src, const int* dst, int pairs, int block,
+                           int blocks) {
+  const int vecs = 2 * (a.vec_codes + a.vec_scales), units = (vecs + 1023) / 1024;
+  const int64_t total = (int64_t)pairs * a.layers * units;
+  for (int64_t u = block; u < total; u += blocks) {
+    const int piece = (int)(u % units);
+    const int64_t pl = u / units;
+    const int layer = (int)(pl % a.layers), pair = (int)(pl / a.layers);
+    const int64_t from = src[pair], to = dst[pair];
+    u32x4_t v[4];
+    uint8_t* out[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      int e = piece * 1024 + k * 256 + threadIdx.x;
+      out[k] = nullptr;
+      if (e < vecs) {
+        const bool sc = e >= 2 * a.vec_codes;
+        if (sc) e -= 2 * a.vec_codes;
+        const int n = sc ? a.vec_scales : a.vec_codes, second = e >= n;
+        const PageBuf& b = a.buf[2 * sc + second];
+        uint8_t* at = b.p + layer * b.layer + 16 * (int64_t)(e - second * n);
+        v[k] = *reinterpret_cast<const u32x4_t*>(at + from * b.page);
+        out[k] = at + to * b.page;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (out[k]) *reinterpret_cast<u32x4_t*>(out[k]) = v[k];
+  }
+}
+
+__global__ __launch_bounds__(256) void pages_fork_kernel(PageArgs a) {
+  if ((int)blockIdx.x >= a.table_blocks) {
+    copy_pages(a, a.s.src, a.s.dst, a.s.head[kPairs], blockIdx.x - a.table_blocks,
+               gridDim.x - a.table_blocks);
+    return;
+  }
+  const int nfree = a.s.head[kFree];
+  for (int i = blockIdx.x; i < a.rows; i += a.table_blocks) {
+    const RowPlan r = row_plan(a, i);
+    const int b = a.s.base[i], copy = b < 0, base = copy ? ~b : b;
+    if (threadIdx.x == 0) a.out_lengths[i] = r.after;
+    for (int j = threadIdx.x; j < a.width; j += 256) {
+      int id = -1, k = -1;
+      if (j < r.held - copy)
+        id = held_page(a, r, j);
+      else if (j < r.need)
+        k = base + (j - (r.held - copy));
+      if (k >= 0 && k < nfree) id = a.s.list[k];
+      a.out_table[(int64_t)i * a.width + j] = id;
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void pages_compact_kernel(PageArgs a) {
+  if ((int)blockIdx.x >= a.table_blocks) {
+    copy_pages(a, a.s.first, a.s.list, a.s.head[kPairs], blockIdx.x - a.table_blocks,
+               gridDim.x - a.table_blocks);
+    return;
+  }
+  for (int i = blockIdx.x; i < a.rows; i += a.table_blocks) {
+    const RowPlan r = row_plan(a, i);
+    for (int j = threadIdx.x; j < a.width; j += 256) {
+      int id = j < r.held ? held_page(a, r, j) : -1;
+      if (id >= 0 && a.s.held[id] < 0) id = a.s.list[~a.s.held[id]];
+      a.out_table[(int64_t)i * a.width + j] = id;
+    }
+  }
+}
+
+}  // namespace
+
+int paged_kv_append(const PagedBatch& p, const void* k, const void* v, const int64_t* xst,
+                    const PagedSide& ks, const PagedSide& vs, int64_t H, int64_t D, int xdt,
+                    hipStream_t st) {
+  if (p.T == 0 || p.B == 0) return SPARKQ_OK;
+  const PagedAppendArgs a{p, k, v, xst[0], xst[1], xst[2], xst[3], ks, vs, (int)H, (int)D, xdt};
+  hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)cdiv((int64_t)p.T * H * 2, 4)), dim3(256),
+                     0, st, a);
+  return check_launch("paged_append_kernel");
+}
+
+size_t kv_pages_workspace(int64_t rows, int64_t pages) {
+  return (size_t)(kHead + 3 * pages + 3 * rows) * sizeof(int);
+}
+
+// what fork and compact have in common; the output pointers are theirs
+static PageArgs page_args(const int32_t* table, int64_t table_stride, const int32_t* lengths,
+                          int64_t B, int64_t rows, int64_t width, int64_t pages, int page_size,
+                          int64_t layers, void* const* bufs, const int64_t* strides,
+                          int64_t code_bytes, int64_t scale_bytes, void* ws) {
+  PageArgs a{};
+  a.table = table;
+  a.lengths = lengths;
+  a.table_stride = table_stride;
+  a.B = (int)B;
+  a.rows = (int)rows;
+  a.width = (int)width;
+  a.pages = (int)pages;
+  a.page_log2 = __builtin_ctz((unsigned)page_size);
+  a.s = page_scratch((int*)ws, pages, rows);
+  for (int i = 0; i < 4; ++i)
+    a.buf[i] = PageBuf{(uint8_t*)bufs[i], strides[2 * i], strides[2 * i + 1]};
+  a.vec_codes = (int)(code_bytes / 16);
+  a.vec_scales = (int)(scale_bytes / 16);
+  a.layers = (int)layers;
+  a.table_blocks = (int)std::min<int64_t>(std::max<int64_t>(rows, 1), 512);
+  return a;
+}
+
+static dim3 page_grid(const PageArgs& a) { return dim3((unsigned)(a.table_blocks + 4 * device_cus())); }
+
+int kv_pages_fork(const int32_t* table, int64_t table_stride, const int32_t* lengths,
+                  const int32_t* parents, const int32_t* fresh, int32_t* out_table,
+                  int32_t* out_lengths, int32_t* missing, int64_t B, int64_t rows, int64_t width,
+                  int64_t pages, int page_size, int64_t layers, void* const* bufs,
+                  const int64_t* strides, int64_t code_bytes, int64_t scale_bytes, void* ws,
+                  hipStream_t st) {
+  PageArgs a = page_args(table, table_stride, lengths, B, rows, width, pages, page_size, layers, bufs,
+                         strides, code_bytes, scale_bytes, ws);
+  a.parents = parents;
+  a.fresh = fresh;
+  a.out_table = out_table;
+  a.out_lengths = out_lengths;
+  a.out_count = missing;
+  hipLaunchKernelGGL(pages_fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+  hipLaunchKernelGGL(pages_fork_kernel, page_grid(a), dim3(256), 0, st, a);
+  return check_launch("pages_fork_kernel");
+}
+
+int kv_pages_compact(const int32_t* table, int64_t table_stride, const int32_t* lengths,
+                     int32_t* out_table, int32_t* used, int64_t B, int64_t width, int64_t pages,
+                     int page_size, int64_t layers, void* const* bufs, const int64_t* strides,
+                     int64_t code_bytes, int64_t scale_bytes, void* ws, hipStream_t st) {
+  PageArgs a = page_args(table, table_stride, lengths, B, B, width, pages, page_size, layers, bufs,
+                         strides, code_bytes, scale_bytes, ws);
+  a.out_table = out_table;
+  a.out_count = used;
+  hipLaunchKernelGGL(pages_compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+  hipLaunchKernelGGL(pages_compact_kernel, page_grid(a), dim3(256), 0, st, a);
+  return check_launch("pages_compact_kernel");
+}
+
+}  // namespace sparkq

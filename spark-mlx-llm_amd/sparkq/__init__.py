@@ -20,6 +20,7 @@ from .ext import (
     kv_quantize_s8,
     prepare_w4a16,
     prepare_w4a16_nax4,
+    qk_norm_rope,
     quantize_per_token,
     rms_norm,
     rope,
@@ -28,6 +29,13 @@ from .ext import (
     w4a16_qmv,
     w8a16_per_channel,
     w8a8_linear,
+)
+from .paged import (
+    PagedKVCache,
+    kv_pages_compact,
+    kv_pages_fork,
+    paged_kv_append,
+    paged_quantized_sdpa,
 )
 from . import torch_ops  # registers torch.ops.sparkq.* (custom ops with fake kernels)
 
@@ -42,10 +50,16 @@ __all__ = [
     "int8_matmul_int32",
     "int8_quantized_sdpa",
     "is_w8a8_available",
+    "PagedKVCache",
     "kv_append",
+    "kv_pages_compact",
+    "kv_pages_fork",
     "kv_quantize_s8",
+    "paged_kv_append",
+    "paged_quantized_sdpa",
     "prepare_w4a16",
     "prepare_w4a16_nax4",
+    "qk_norm_rope",
     "quantize_per_token",
     "rms_norm",
     "rope",

@@ -28,8 +28,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _LIB = None
 _LOCK = threading.Lock()
 
-P, I64, I, F, SZ = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float,
-                    ctypes.c_size_t)
+P, I64, I, F, DB, SZ = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float,
+                        ctypes.c_double, ctypes.c_size_t)
 
 # name -> (restype, argtypes); mirrors include/sparkq.h
 SIGNATURES = {
@@ -72,6 +72,18 @@ SIGNATURES = {
                             P]),
     "sparkq_rope": (I, [P, P, I64, I64, I64, I, I, F, F, I64, I, P]),
     "sparkq_rms_norm": (I, [P, P, P, F, P, P, I64, I64, I, P]),
+    "sparkq_qk_norm_rope": (I, [P, P, P, P, P, I, P, P, I64, I64, I64, I64, I, I, F, DB, DB, I, P,
+                                P]),
+    "sparkq_paged_kv_append": (I, [P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I,
+                                   I, P, P, P]),
+    "sparkq_paged_sdpa_workspace_bytes": (SZ, [I64, I64, I64, I64, I64, I64, I64]),
+    "sparkq_paged_sdpa": (I, [P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I,
+                              I64, I, I, I, F, P, P, P, SZ, P]),
+    "sparkq_kv_pages_workspace_bytes": (SZ, [I64, I64]),
+    "sparkq_kv_pages_fork": (I, [P, P, P, P, P, P, P, P, I64, P, P, P, P, I64, I64, I64, I64, I64,
+                                 I, I64, I64, P, SZ, P]),
+    "sparkq_kv_pages_compact": (I, [P, P, P, P, P, P, I64, P, P, P, I64, I64, I64, I64, I, I64,
+                                    I64, P, SZ, P]),
     "sparkq_attention_gate": (I, [P, P, P, P, P, I64, I64, I64, I64, I64, I, P]),
     "sparkq_quantized_sdpa_workspace_bytes": (SZ, [I64, I64, I64, I64, I64, I64]),
     "sparkq_quantized_sdpa_call_workspace_bytes": (SZ, [I64, I64, I64, I64, I64, I64, I64, I]),

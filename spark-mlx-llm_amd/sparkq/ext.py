@@ -36,6 +36,7 @@ __all__ = [
     "kv_append",
     "prepare_w4a16",
     "prepare_w4a16_nax4",
+    "qk_norm_rope",
     "quantize_per_token",
     "rms_norm",
     "rope",
@@ -963,6 +964,51 @@ def rope(x, dims: int, *, traditional: bool = False, base: float = 10000.0,
               float(base), float(scale), int(offset), _lib.dtype_code(x.dtype),
               _lib.stream_handle(x.device), device=x.device)
     return out
+
+
+def qk_norm_rope(queries, keys, q_weight, k_weight, positions, *, dims: int, eps: float,
+                 base: float = 10000.0, scale: float = 1.0, traditional: bool = False):
+    """RMS norm of every query and key head and the rotary position embedding
+    in one pass (no counterpart in the reference, whose models rotate without
+    it): queries [T,Hq,D] and keys [T,Hkv,D] (bfloat16 or float16; views of a
+    packed projection are read in place), weights [D], a position for each row
+    (int32 or int64 [T]) -> new [T,Hq,D] and [T,Hkv,D]. Each head is normed
+    over its D values and multiplied by its weight, then the first `dims` of
+    them rotate as in rope: pairs (i, i + dims/2), or (2i, 2i+1) when
+    traditional, by (scale * position) * base^(-2i/dims). All of it is fp32
+    (the angle fp64) with one rounding at the end, where rms_norm and rope in
+    turn round three times."""
+    tensors = (queries, keys, q_weight, k_weight, positions)
+    if any(not isinstance(v, torch.Tensor) for v in tensors):
+        raise TypeError("queries, keys, weights and positions must be tensors")
+    if queries.ndim != 3 or keys.ndim != 3 or keys.shape[0] != queries.shape[0] \
+            or keys.shape[2] != queries.shape[2] or 0 in queries.shape[1:] or not keys.shape[1]:
+        raise ValueError("qk_norm_rope requires queries [T,Hq,D] and keys [T,Hkv,D]")
+    t, hq, d = queries.shape
+    hkv = keys.shape[1]
+    dtype, dev = queries.dtype, queries.device
+    if dtype not in _HALF or any(v.dtype != dtype for v in (keys, q_weight, k_weight)):
+        raise ValueError("qk_norm_rope requires BF16 or F16 queries, keys and weights of one dtype")
+    if q_weight.shape != (d,) or k_weight.shape != (d,):
+        raise ValueError(f"qk_norm_rope weights must have shape [{d}]")
+    if positions.shape != (t,) or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"qk_norm_rope positions must be int32 or int64 of shape [{t}]")
+    if type(dims) is not int:
+        raise ValueError("qk_norm_rope dims must be an int")
+    _require_device("qk_norm_rope", *tensors)
+    if any(v.device != dev for v in tensors):
+        raise ValueError("qk_norm_rope tensors must live on one device")
+    q = queries if queries.stride(2) == 1 or d == 1 else queries.contiguous()
+    k = keys if keys.stride(2) == 1 or d == 1 else keys.contiguous()
+    q_out = torch.empty((t, hq, d), dtype=dtype, device=dev)
+    k_out = torch.empty((t, hkv, d), dtype=dtype, device=dev)
+    st = (ctypes.c_int64 * 4)(*q.stride()[:2], *k.stride()[:2])
+    _lib.call("sparkq_qk_norm_rope", _ptr(q), _ptr(k), _ptr(q_weight.contiguous()),
+              _ptr(k_weight.contiguous()), _ptr(positions.contiguous()),
+              32 if positions.dtype == torch.int32 else 64, _ptr(q_out), _ptr(k_out), t, hq, hkv,
+              d, dims, int(bool(traditional)), float(eps), float(base), float(scale),
+              _lib.dtype_code(dtype), st, _lib.stream_handle(dev), device=dev)
+    return q_out, k_out
 
 
 def spark_qkv_rope(x, weight, scales, biases, q_size: int, kv_size: int, num_heads: int,
