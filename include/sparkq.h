@@ -603,12 +603,15 @@ int sparkq_paged_kv_append(const void* k, const void* v, void* k_codes, void* k_
 
 /* Attention of a batch's new tokens over their pages: q [T,Hq,D] (BF16 or
  * F16) with q_strides[0..1] = token, head in elements (16-byte aligned rows),
- * out [T,Hq,D] contiguous in out_dtype (q_dtype or F32). causal = 1: row i of
- * a sequence's n sees its tokens 0 .. length - n + i; 0: all of them. Tokens
- * without a page are hidden; a row that sees nothing is zero; rows of out
- * that fall to no sequence are left as they were. max_new bounds the new
- * tokens of one sequence: of longer ones the rows past it are left as they
- * were too. A chunk of one token per sequence is the decode step. Workspace:
+ * out [T,Hq,D] contiguous in out_dtype (q_dtype or F32). The scales of a page
+ * and head are contiguous (token stride 1), page and head strides multiples of
+ * 8, both scale tensors 16-byte aligned. causal = 1: row i of a sequence's n
+ * sees its tokens 0 .. length - n + i; 0: all of them. Tokens without a page are
+ * hidden; a row that sees nothing is zero; rows of out that fall to no sequence
+ * are left as they were. max_new bounds the new tokens of one sequence: of
+ * longer ones the rows past it are left as they were too. A chunk of one token
+ * per sequence is the decode step. Scores, normalizer and sums are fp32; a
+ * weight times its value's scale is rounded to fp16 once. Workspace:
  * sparkq_paged_sdpa_workspace_bytes (max_tokens = max_pages * page_size), any
  * initial value. */
 size_t sparkq_paged_sdpa_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv,

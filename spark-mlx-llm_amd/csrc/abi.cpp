@@ -978,7 +978,13 @@ int sparkq_paged_sdpa(const void* q, const void* k_codes, const void* k_scales, 
     return rc;
   REQUIRE(Hq > 0 && Hq % Hkv == 0, "paged_sdpa: query heads must be divisible by KV heads");
   REQUIRE(max_new > 0 && max_new <= kI32Max, "paged_sdpa: max_new must be positive");
-  REQUIRE(Hq <= 65535 && T <= kI32Max / Hq, "paged_sdpa: shape too large");
+  REQUIRE(Hq <= 65535 && T <= kI32Max / Hq && B <= kI32Max / (4 * Hkv), "paged_sdpa: shape too large");
+  for (int i = 3; i < 12; i += 6)
+    REQUIRE_SUPPORTED(strides[i] % 8 == 0 && strides[i + 1] % 8 == 0 && strides[i + 2] == 1,
+                      "paged_sdpa: scales must be contiguous over a page's tokens, pages and heads "
+                      "multiples of 8 scales apart");
+  REQUIRE_SUPPORTED(aligned(k_scales, 16) && aligned(v_scales, 16),
+                    "paged_sdpa: scales must be 16-byte aligned");
   REQUIRE((T == 0 || (q && out)) && q_strides && starts && (B == 0 || (page_table && lengths)),
           "paged_sdpa: null tensor pointer");
   REQUIRE(is_half_dtype(q_dtype), "paged_sdpa requires float16 or bfloat16 queries");

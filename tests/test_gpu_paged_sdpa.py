@@ -1,10 +1,13 @@
 """paged_quantized_sdpa against the float64 form.
 
 Tolerance of an output o = sum p v / sum p, with mass = sum p|v| / sum p:
- - its rounding: eps/2 of it, none in fp32;
- - the weights' one rounding to fp16, half a step 2^-12 of each, both in the
-   numerator alone: 2^-12 mass (weights are scaled so that only those under
-   2^-28 of the largest fall below fp16's normal range);
+ - its rounding: eps/2 of the value that is rounded (the errors below included),
+   none in fp32;
+ - the weights' one rounding to fp16, in the numerator alone: fp16 has 11 bits,
+   so half a step of a weight is at most 2^-11 of it (1 + 2^-11 lies halfway
+   between 1 and the next fp16, 1 + 2^-10), in all 2^-11 mass (weights are
+   scaled so that only those under 2^-19 of the largest fall below fp16's
+   normal range);
  - the scores: fp32 products of exact operands, summed D at a time, times three
    factors: (D + 8) 2^-24 of scale * sum|q||k| (`size`), twice (numerator and
    normalizer), and exp2's 2^-22;
@@ -29,10 +32,11 @@ def check(got, q, cache, table, starts, lengths, scale, causal=True, max_new=1 <
     want, mass, size, done = ref.attention(q, cache, table, starts, lengths, scale, causal, max_new)
     d = q.shape[-1]
     n = max([0, *lengths])
-    part = 2.0 ** -12 + 2 * (d + 8) * 2.0 ** -24 * size[..., None] + 2.0 ** -20 + n * 2.0 ** -23
+    part = 2.0 ** -11 + 2 * (d + 8) * 2.0 ** -24 * size[..., None] + 2.0 ** -20 + n * 2.0 ** -23
     half = 0 if got.dtype == torch.float32 else torch.finfo(got.dtype).eps / 2
     tiny = 2.0 ** -25 if got.dtype == torch.float16 else 2.0 ** -60
-    tol = (half * want.abs()).clamp(min=tiny) + 1.01 * part * mass
+    part = 1.01 * part * mass
+    tol = (half * (want.abs() + part)).clamp(min=tiny) + part
     off = ((got.cpu().double() - want).abs() / tol)[done]
     worst = off.max().item() if off.numel() else 0.0
     print(f"[paged sdpa] {tuple(got.shape)} n={n} largest error {worst:.3f} of its bound", flush=True)
