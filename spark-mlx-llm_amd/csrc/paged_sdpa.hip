@@ -48,11 +48,11 @@ struct PagedSdpaArgs {
   float *pm, *pz, *pacc;  // [Hkv][slots][rows], [...], [...][D]: parts of split contexts
   int Hq, Hkv, max_new, causal, q_dtype, out_dtype;
   int slots;       // parts of split contexts, at most, per KV head
-  int min_blocks;  // blocks of a part, at least
+  int min_part;    // tokens of a part, at least
   float scale_log2;
 };
 
-constexpr int kBlock = 32;  // tokens of a block
+constexpr int kFewBlock = 32, kTileBlock = 64;  // tokens of a block
 
 // ---------------------------------------------------------------------------
 // which work is whose
@@ -66,12 +66,12 @@ struct Item {
 };
 
 struct SeqWork {
-  int first, count, length, rows, tiles, blocks;
+  int first, count, length, rows, tiles;
 };
 
-template <int R>
+template <int R>  // rows of a tile: 16 or 128
 __device__ __forceinline__ SeqWork seq_work(const PagedSdpaArgs& a, int b) {
-  SeqWork w{0, 0, 0, 0, 0, 0};
+  SeqWork w{0, 0, 0, 0, 0};
   if (b < a.p.B) {
     const SeqRows s = seq_rows(a.p, b);
     w.first = s.first;
@@ -79,7 +79,6 @@ __device__ __forceinline__ SeqWork seq_work(const PagedSdpaArgs& a, int b) {
     w.length = s.length;
     w.rows = min(s.count, a.max_new) * (a.Hq / a.Hkv);
     w.tiles = (w.rows + R - 1) / R;
-    w.blocks = (s.length + kBlock - 1) / kBlock;
   }
   return w;
 }
@@ -94,8 +93,8 @@ __device__ __forceinline__ int wave_prefix(int v, int lane) {  // inclusive
 }
 
 // Item x of the batch's items in order (SPLIT false: every tile and part), or
-// tile x of those whose context is split. A context of n blocks is split into
-// floor(n / C) parts, C = max(min_blocks, ceil(all tiles' blocks / slots)), so
+// tile x of those whose context is split. A context of n tokens is split into
+// floor(n / C) parts, C = max(min_part, ceil(all tiles' tokens / slots)), so
 // split contexts have no more than `slots` parts together. All lanes of a wave
 // take part and get the same answer.
 template <int R, bool SPLIT>
@@ -104,16 +103,16 @@ __device__ Item find_item(const PagedSdpaArgs& a, int x) {
   long long all = 0;
   for (int b0 = 0; b0 < a.p.B; b0 += 64) {
     const SeqWork w = seq_work<R>(a, b0 + lane);
-    all += (long long)w.tiles * w.blocks;
+    all += (long long)w.tiles * w.length;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
-  const long long C = max((all + a.slots - 1) / a.slots, (long long)a.min_blocks);
+  const long long C = max((all + a.slots - 1) / a.slots, (long long)a.min_part);
   Item it{-1, 0, 0, 1, 0, 0, 0, 0, 0};
   int items = 0, slots = 0;
   for (int b0 = 0; b0 < a.p.B; b0 += 64) {
     const SeqWork w = seq_work<R>(a, b0 + lane);
-    const int parts = max(1, (int)(w.blocks / C));
+    const int parts = max(1, (int)(w.length / C));
     const int own = SPLIT ? (parts > 1 ? w.tiles : 0) : w.tiles * parts;
     const int used = parts > 1 ? w.tiles * parts : 0;
     const int end = items + wave_prefix(own, lane), slot_end = slots + wave_prefix(used, lane);
@@ -132,11 +131,14 @@ __device__ Item find_item(const PagedSdpaArgs& a, int x) {
       it.part = SPLIT ? 0 : i - k * it.parts;
       it.tile = tiles - 1 - k;  // the last tiles see the most: they start first
       it.slot = of(slot_end - used) + k * it.parts;
-      return it;
+      break;
     }
     items = __builtin_amdgcn_readlane(end, 63);
     slots = __builtin_amdgcn_readlane(slot_end, 63);
   }
+  // (the compiler does not see that a loop left on a ballot leaves scalars)
+  for (int* f : {&it.b, &it.tile, &it.part, &it.parts, &it.slot, &it.first, &it.count, &it.length, &it.rows})
+    *f = __builtin_amdgcn_readfirstlane(*f);
   return it;
 }
 
@@ -188,6 +190,19 @@ __device__ __forceinline__ float load_query(const PagedSdpaArgs& a, const uint16
   return ldexpf(1.0f, e);
 }
 
+// v, in a way that what depends on it stays in its branch: the compiler would
+// otherwise rescale the sums of every block and select, at twice the registers
+__device__ __forceinline__ float pinned(float v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// two values rounded (to nearest even) into packed fp16: one instruction
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){a, b}, f16x2_t));
+}
+
 // max / sum over the four 16-lane rows of a wave, the same value in all of them
 __device__ __forceinline__ float max_groups(float v) {
   auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -229,24 +244,18 @@ __device__ __forceinline__ float part_max(const RowState& st, float z) {
   return st.m != kNegInf ? unit(st) : (z != 0.0f ? 0.0f : kNegInf);
 }
 
-// The block's 8 scores of this lane's row (raw sums times the key scales times
-// the softmax scale: s * mul is in log2 units), `ok` where visible; `size` is
-// the block's largest finite value scale, used where all of it is visible.
-// Writes the packed fp16 weights of its 8 values; returns the factor for what
-// is summed so far (up: it is not 1).
-template <bool MASK>
-__device__ __forceinline__ float row_block(RowState& st, const float s[8], const bool ok[8], float mul,
-                                           const float vsc[8], float size, u32x4_t& w, bool& up) {
-  float top = kNegInf;
+// A block's N scores of this lane's row (raw sums times the key scales times
+// the softmax scale: s * mul is in log2 units), of which those in `ok` are
+// visible where MASK; `size` is the block's largest finite value scale, used
+// where all of it is visible. Writes the packed fp16 weights of the lane's N
+// values; returns the factor for what is summed so far (up: it is not 1).
+template <int N>
+__device__ __forceinline__ float row_block(RowState& st, const float s[N], float mul, const float vsc[N],
+                                           float size, u32x4_t w[N / 8], bool& up) {
+  float top = s[0];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, MASK ? (ok[i] ? s[i] : kNegInf) : s[i]);
+  for (int i = 1; i < N; ++i) top = fmaxf(top, s[i]);
   top = max_groups(top) * mul;
-  if (MASK) {
-    size = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) size = fmaxf(size, scale_size(vsc[i], ok[i]));
-    size = max_groups(size);
-  }
   const float e = fmaxf(st.e, (float)((int)(__float_as_uint(size) >> 23) - 127));
   const bool raise = top > st.m + kRoom;
   up = raise || e != st.e;
@@ -255,19 +264,37 @@ __device__ __forceinline__ float row_block(RowState& st, const float s[8], const
   st.e = e;
   const float M = st.m == kNegInf ? 0.0f : unit(st);
   const float alpha = old == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(old - M);
-  float p[8], sum = 0.0f;
+  float p[N], sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < N; ++i) {
     p[i] = __builtin_amdgcn_exp2f(fmaf(s[i], mul, -M));
-    if (MASK) p[i] = ok[i] ? p[i] : 0.0f;
     sum += p[i];
     p[i] *= vsc[i];
-    if (MASK) p[i] = ok[i] ? p[i] : 0.0f;
   }
   st.z = fmaf(st.z, up ? alpha : 1.0f, sum);
-  w = u32x4_t{pack_round<F16>(p[0], p[1]), pack_round<F16>(p[2], p[3]), pack_round<F16>(p[4], p[5]),
-              pack_round<F16>(p[6], p[7])};
+#pragma unroll
+  for (int i = 0; i < N; i += 2) w[i / 8][i / 2 % 4] = pack_f16(p[i], p[i + 1]);
   return alpha;
+}
+
+// A value scale as the tile kernel keeps it: what is not finite is -0, so that a
+// hidden token's weight of 0 times its scale is 0, and a visible one is found.
+__device__ __forceinline__ float kept_scale(float v) {
+  return fabsf(v) <= 65504.0f ? v + 0.0f : -0.0f;
+}
+
+// Hides the scores that are not in `ok` and turns those of values that are not
+// finite to NaN; returns the largest value scale of the others.
+template <int N>
+__device__ __forceinline__ float hide(uint32_t ok, float s[N], const float vsc[N]) {
+  float size = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const bool live = (ok >> i) & 1u;
+    s[i] = live ? (__float_as_uint(vsc[i]) == 0x80000000u ? __builtin_nanf("") : s[i]) : kNegInf;
+    size = fmaxf(size, live ? fabsf(vsc[i]) : 0.0f);
+  }
+  return max_groups(size);
 }
 
 // Four outputs (dims d .. d + 3) of a row.
@@ -287,20 +314,32 @@ __device__ __forceinline__ int64_t out_row(const PagedSdpaArgs& a, const Item& i
   return ((int64_t)(it.first + rr / gqa) * a.Hq + kh * gqa + rr % gqa);
 }
 
-// Pages of a block's two 16-token halves; a half without one reads page 0 and
-// is hidden. Past the table's row the last entry stands in (those tokens lie
+// Pages of a block's Q runs of 16 tokens; a run without one reads page 0 and is
+// hidden (ok). Past the table's row the last entry stands in (those tokens lie
 // past every length).
+template <int Q>
 struct BlockPages {
-  int id[2];
-  bool ok[2];
+  int id[Q];
+  uint32_t ok;
 };
-__device__ __forceinline__ BlockPages block_pages(const PagedSdpaArgs& a, const int32_t* row, int t0) {
-  BlockPages r;
+//
+// The table is read by scalar loads (its constant address space says that no
+// store of this kernel changes it): a vector load among those of the codes
+// would be waited for in their order.
+typedef const __attribute__((address_space(4))) int32_t* TableRow;
+__device__ __forceinline__ TableRow table_row(const PagedSdpaArgs& a, int b) {
+  return (TableRow)(uintptr_t)(a.p.table + b * a.p.table_stride);
+}
+template <int Q>
+__device__ __forceinline__ BlockPages<Q> block_pages(const PagedSdpaArgs& a, TableRow row, int t0) {
+  BlockPages<Q> r;
+  r.ok = 0;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < Q; ++h) {
     const int id = row[min((t0 + 16 * h) >> a.p.page_log2, a.p.width - 1)];
-    r.ok[h] = (unsigned)id < (unsigned)a.p.pages;
-    r.id[h] = r.ok[h] ? id : 0;
+    const bool in = (unsigned)id < (unsigned)a.p.pages;
+    r.ok |= (uint32_t)in << h;
+    r.id[h] = in ? id : 0;
   }
   return r;
 }
@@ -316,7 +355,7 @@ __device__ __forceinline__ BlockPages block_pages(const PagedSdpaArgs& a, const 
 template <int D>
 struct FewLds {
   static constexpr int VROW = D + 16;
-  static constexpr int VT = kBlock * VROW;          // one wave's V block
+  static constexpr int VT = kFewBlock * VROW;          // one wave's V block
   static constexpr int LOOP = 4 * VT;
   static constexpr int JOIN = 4 * 16 * (2 + D) * 4;  // the waves' maxima, sums and outputs
   static constexpr int BYTES = LOOP > JOIN ? LOOP : JOIN;
@@ -329,6 +368,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedS
   __shared__ __attribute__((aligned(16))) unsigned char smem[L::BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int kBlock = kFewBlock;
   const int n16 = lane & 15, grp = lane >> 4;
   const int kh = blockIdx.x % a.Hkv, gqa = a.Hq / a.Hkv;
   const Item it = find_item<16, false>(a, blockIdx.x / a.Hkv);
@@ -337,11 +377,10 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedS
   const int rr = 16 * it.tile + min(n16, rows - 1);
   const int lim = last_seen(a, it, rr, gqa);
   const int seen = last_seen(a, it, 16 * it.tile + rows - 1, gqa) + 1;  // by the last row: the most
-  const int all = last_seen(a, it, 16 * it.tile, gqa) + 1;              // by every row
   const int nblocks = (seen + kBlock - 1) / kBlock;
   const int ib0 = (int)((int64_t)it.part * nblocks / it.parts);
   const int ib1 = (int)((int64_t)(it.part + 1) * nblocks / it.parts);
-  const int32_t* trow = a.p.table + it.b * a.p.table_stride;
+  const TableRow trow = table_row(a, it.b);
   unsigned char* vtile = smem + wave * L::VT;
 
   u32x4_t qb[NK];
@@ -350,12 +389,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedS
   const float mul = load_query<NK>(a, qrow, true, [&](int c) { return 16 * (grp + 4 * (c >> 1)) + 8 * (c & 1); }, qb);
 
   u32x4_t kr[2][2][PL], vr[2][VL], skr[2], svr[2];
-  BlockPages pg[2], next;
+  BlockPages<2> pg[2], next;
   const int ktok = 8 * (n16 >> 2) + (n16 & 3);
   const int slot_mask = (1 << a.p.page_log2) - 1;
   const int last = ib1 - 1;
   // block ib (no further than the last) through the pages found for it
-  auto load = [&](int set, int ib, const BlockPages& bp) {
+  auto load = [&](int set, int ib, const BlockPages<2>& bp) {
     const int t0 = kBlock * min(ib, last);
     const int s0 = t0 & slot_mask, s1 = (t0 + 16) & slot_mask;
     auto base = [&](const PagedSide& s, int h) {
@@ -407,29 +446,32 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedS
       }
     }
     float s[8], vsc[8];
-    bool ok[8];
-    float big = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t kw = skr[set][i >> 1], vw = svr[set][i >> 1];
       s[i] = sc[i >> 2][i & 3] * (((i & 1) ? hi16<F16>(kw) : lo16<F16>(kw)) * a.scale_log2);
       vsc[i] = (i & 1) ? hi16<F16>(vw) : lo16<F16>(vw);
     }
-    const bool half_ok[2] = {pg[set].ok[0], pg[set].ok[1]};
-    const bool whole = t0 + kBlock <= all && half_ok[0] && half_ok[1];
+    uint32_t ok = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      ok[i] = whole || (t0 + 8 * grp + i <= lim && (grp < 2 ? half_ok[0] : half_ok[1]));
-      big = fmaxf(big, scale_size(vsc[i], true));
-    }
+    for (int i = 0; i < 8; ++i) ok |= (uint32_t)(t0 + 8 * grp + i <= lim) << i;
+    if (!((pg[set].ok >> (grp >> 1)) & 1u)) ok = 0;
     load(set, ib + 8, next);
-    next = block_pages(a, trow, kBlock * min(ib + 12, last));
+    next = block_pages<2>(a, trow, kBlock * min(ib + 12, last));
     u32x4_t w;
     bool up;
-    const float alpha = whole ? row_block<false>(st, s, ok, mul, vsc, max_groups(big), w, up)
-                              : row_block<true>(st, s, ok, mul, vsc, 0.0f, w, up);
+    float size = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const bool live = (ok >> i) & 1u;
+      s[i] = live ? s[i] : kNegInf;
+      vsc[i] = live ? vsc[i] : 0.0f;
+      size = fmaxf(size, scale_size(vsc[i], true));
+    }
+    size = max_groups(size);
+    const float alpha = row_block<8>(st, s, mul, vsc, size, &w, up);
     if (__ballot(up)) {
-      const float f = up ? alpha : 1.0f;
+      const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[j] *= f;
     }
@@ -445,9 +487,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedS
 
   int ib = ib0 + wave;
   if (ib < ib1) {
-    load(0, ib, block_pages(a, trow, kBlock * ib));
-    load(1, ib + 4, block_pages(a, trow, kBlock * min(ib + 4, last)));
-    next = block_pages(a, trow, kBlock * min(ib + 8, last));
+    load(0, ib, block_pages<2>(a, trow, kBlock * ib));
+    load(1, ib + 4, block_pages<2>(a, trow, kBlock * min(ib + 4, last)));
+    next = block_pages<2>(a, trow, kBlock * min(ib + 8, last));
     for (; ib + 4 < ib1; ib += 8) {
       block(ib, std::integral_constant<int, 0>{});
       block(ib + 4, std::integral_constant<int, 1>{});
@@ -508,25 +550,27 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedS
 // 16-byte chunks XOR-swizzled by the token, V token-major with its 32-byte runs
 // swizzled (read transposed), two buffers deep: the next block's codes are
 // converted while this one is computed, and the one after is in flight.
+//
+// A wave takes 32 rows up to D = 128, where the products' operands and sums fit
+// 256 registers and two workgroups a CU; at 256 eight waves take 16 each, or
+// there would be one wave a SIMD with nothing to hide its waits.
+constexpr int tile_waves(int D) { return D <= 128 ? 4 : 8; }
 template <int D>
 struct TileLds {
-  static constexpr int ROW = 2 * D;
-  static constexpr int TILE = kBlock * ROW;
-  static constexpr int BUF = 2 * TILE + 2 * kBlock * 4 + 16;  // K, V, key and value scales, the largest of these
+  static constexpr int KROW = 2 * D + 16, VROW = 2 * D + 32;  // padded: no two lanes of a read share banks
+  static constexpr int V = kTileBlock * KROW;
+  static constexpr int SCALES = V + kTileBlock * VROW;        // of keys, of values, the largest of each 16 of these
+  static constexpr int BUF = SCALES + 2 * kTileBlock * 4 + 16;
   static constexpr int BYTES = 2 * BUF;
 };
-template <int D>
-__device__ __forceinline__ int kswz(int t) { return D >= 128 ? (t & 15) : ((t >> 1) & 7); }
-template <int D>
-__device__ __forceinline__ int vswz(int t) { return D >= 128 ? (t & 7) : ((t >> 1) & 3); }
 
 template <int D>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_tile_kernel(PagedSdpaArgs a) {
+__global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_tile_kernel(PagedSdpaArgs a) {
   using L = TileLds<D>;
+  constexpr int kBlock = kTileBlock, Q = kBlock / 16;
+  constexpr int NW = tile_waves(D), RT = 8 / NW;  // waves, 16-row tiles of each
   constexpr int NK = D / 32, NJ = D / 16;
-  constexpr int PIECES = 2 * D;  // 16-code pieces of a K (or V) block
-  constexpr int PPT = PIECES >= 256 ? PIECES / 256 : 1;
-  constexpr int NVB = NJ < 8 ? NJ : 8;
+  constexpr int PPT = kBlock * D / 16 / (64 * NW);  // 16-code pieces of a K (or V) block per thread
   __shared__ __attribute__((aligned(16))) unsigned char smem[L::BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -540,133 +584,136 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_tile_kernel(Paged
   const int nblocks = (seen + kBlock - 1) / kBlock;
   const int ib0 = (int)((int64_t)it.part * nblocks / it.parts);
   const int ib1 = (int)((int64_t)(it.part + 1) * nblocks / it.parts);
-  const int32_t* trow = a.p.table + it.b * a.p.table_stride;
+  const TableRow trow = table_row(a, it.b);
 
-  u32x4_t qb[2][NK];
-  int lim[2];
-  float mul[2];
+  u32x4_t qb[RT][NK];
+  int lim[RT];
+  float mul[RT];
 #pragma unroll
-  for (int rt = 0; rt < 2; ++rt) {
-    const int rr = rw0 + 32 * wave + 16 * rt + n16, rq = min(rr, it.rows - 1);
+  for (int rt = 0; rt < RT; ++rt) {
+    const int rr = rw0 + 16 * (RT * wave + rt) + n16, rq = min(rr, it.rows - 1);
     lim[rt] = last_seen(a, it, rr, gqa);
     const uint16_t* qrow = a.q + (it.first + rq / gqa) * a.q_tok + (kh * gqa + rq % gqa) * a.q_head;
     mul[rt] = load_query<NK>(a, qrow, rr < it.rows, [&](int c) { return 32 * c + 8 * grp; }, qb[rt]);
   }
-  // what every row of the wave sees, and what its last one does
-  const int wr0 = rw0 + 32 * wave;
-  const int all = last_seen(a, it, wr0, gqa) + 1 > 0 && wr0 + 31 < it.rows ? last_seen(a, it, wr0, gqa) + 1 : 0;
-  const int most = wr0 < it.rows ? last_seen(a, it, min(wr0 + 31, it.rows - 1), gqa) + 1 : 0;
+  // what every row of the tile sees
+  const int all = __builtin_amdgcn_readfirstlane(last_seen(a, it, rw0, gqa) + 1);
 
   const int slot_mask = (1 << a.p.page_log2) - 1;
-  const bool stager = PIECES >= 256 || tid < PIECES;  // wave-uniform
   u32x4_t kcr[PPT], vcr[PPT];
   uint16_t sr;
   const int last = ib1 - 1;
-  // piece p = tid + 256 i: token p / (D / 16), codes 16 (p % (D / 16)); thread
-  // t < 64 also takes a scale: key t, or value t - 32
-  auto load = [&](int ib, const BlockPages& bp) {
+  // Piece p = tid + 64 NW i of a block: token p / (D / 16), codes 16 (p % (D /
+  // 16)). All tokens of a wave's i-th piece lie in one run of 16, and so in one
+  // page: its address is a scalar plus the lane's offset. Wave w < Q also takes
+  // the scales of run w: keys in its first 16 lanes, values in the next.
+  const uint32_t koff = (uint32_t)((tid / (D / 16)) & 15) * (uint32_t)a.ks.c_tok + 16 * (tid % (D / 16));
+  const uint32_t voff = (uint32_t)((tid / (D / 16)) & 15) * (uint32_t)a.vs.c_tok + 16 * (tid % (D / 16));
+  auto page_id = [&](const BlockPages<Q>& bp, int run) {
+    return (int64_t)(run == 0 ? bp.id[0] : Q == 2 || run == 1 ? bp.id[1] : run == 2 ? bp.id[Q - 2] : bp.id[Q - 1]);
+  };
+  auto load = [&](int ib, const BlockPages<Q>& bp) {
     const int t0 = kBlock * min(ib, last);
-    const int s0 = t0 & slot_mask, s1 = (t0 + 16) & slot_mask;
-    if (stager) {
 #pragma unroll
-      for (int i = 0; i < PPT; ++i) {
-        const int p = tid + 256 * i, tk = p / (D / 16), jb = p % (D / 16), h = tk >> 4;
-        const int64_t id = h ? bp.id[1] : bp.id[0];
-        const int64_t slot = (h ? s1 : s0) + (tk & 15);
-        kcr[i] = *reinterpret_cast<const u32x4_t*>(a.ks.codes + id * a.ks.c_page + kh * a.ks.c_head + slot * a.ks.c_tok + 16 * jb);
-        vcr[i] = *reinterpret_cast<const u32x4_t*>(a.vs.codes + id * a.vs.c_page + kh * a.vs.c_head + slot * a.vs.c_tok + 16 * jb);
-      }
+    for (int i = 0; i < PPT; ++i) {
+      const int run = wave * 64 / D + i * (64 * NW / D);
+      const int64_t id = page_id(bp, run), slot = (t0 + 16 * run) & slot_mask;
+      const uint8_t* kp = a.ks.codes + (id * a.ks.c_page + kh * a.ks.c_head + slot * a.ks.c_tok);
+      const uint8_t* vp = a.vs.codes + (id * a.vs.c_page + kh * a.vs.c_head + slot * a.vs.c_tok);
+      kcr[i] = *reinterpret_cast<const u32x4_t*>(kp + koff);
+      vcr[i] = *reinterpret_cast<const u32x4_t*>(vp + voff);
     }
-    if (wave == 0) {
-      const PagedSide& s = lane < 32 ? a.ks : a.vs;
-      const int h = (lane >> 4) & 1;
-      sr = s.scales[(h ? bp.id[1] : bp.id[0]) * s.s_page + kh * s.s_head + (h ? s1 : s0) + (lane & 15)];
+    if (wave < Q) {
+      const int64_t id = page_id(bp, wave), slot = (t0 + 16 * wave) & slot_mask;
+      const uint16_t* kp = a.ks.scales + (id * a.ks.s_page + kh * a.ks.s_head + slot);
+      const uint16_t* vp = a.vs.scales + (id * a.vs.s_page + kh * a.vs.s_head + slot);
+      sr = (lane < 16 ? kp : vp)[n16];
     }
   };
-  auto stage = [&](unsigned char* buf) {
-    if (stager) {
+  const int tk0 = tid / (D / 16), jb = tid % (D / 16);
+  unsigned char* const kput = smem + tk0 * L::KROW + 32 * jb;
+  unsigned char* const vput = smem + L::V + tk0 * L::VROW + 32 * jb;
+  auto stage = [&](auto bufc) {
+    constexpr int at = decltype(bufc)::value * L::BUF, TPP = 64 * NW / (D / 16);  // tokens of a round of pieces
 #pragma unroll
-      for (int i = 0; i < PPT; ++i) {
-        const int p = tid + 256 * i, tk = p / (D / 16), jb = p % (D / 16), ks = kswz<D>(tk);
-        unsigned char* kt = buf + tk * L::ROW;
-        *reinterpret_cast<u32x4_t*>(kt + ((2 * jb) ^ ks) * 16) = s8x8_exact(kcr[i].x, kcr[i].y);
-        *reinterpret_cast<u32x4_t*>(kt + ((2 * jb + 1) ^ ks) * 16) = s8x8_exact(kcr[i].z, kcr[i].w);
-        unsigned char* vt = buf + L::TILE + tk * L::ROW + (jb ^ vswz<D>(tk)) * 32;
-        *reinterpret_cast<u32x4_t*>(vt) = s8x8_exact(vcr[i].x, vcr[i].y);
-        *reinterpret_cast<u32x4_t*>(vt + 16) = s8x8_exact(vcr[i].z, vcr[i].w);
-      }
+    for (int i = 0; i < PPT; ++i) {
+      unsigned char* kt = kput + at + i * TPP * L::KROW;
+      *reinterpret_cast<u32x4_t*>(kt) = s8x8_exact(kcr[i].x, kcr[i].y);
+      *reinterpret_cast<u32x4_t*>(kt + 16) = s8x8_exact(kcr[i].z, kcr[i].w);
+      unsigned char* vt = vput + at + i * TPP * L::VROW;
+      *reinterpret_cast<u32x4_t*>(vt) = s8x8_exact(vcr[i].x, vcr[i].y);
+      *reinterpret_cast<u32x4_t*>(vt + 16) = s8x8_exact(vcr[i].z, vcr[i].w);
     }
-    if (wave == 0) {
-      float* sc = reinterpret_cast<float*>(buf + 2 * L::TILE);
+    if (wave < Q) {
+      float* sc = reinterpret_cast<float*>(smem + at + L::SCALES);
       const float v = f16_to_f32(sr);
-      sc[lane] = lane < 32 ? v * a.scale_log2 : v;
-      const float big = max_groups(max_row16(scale_size(v, lane >= 32)));
-      if (lane == 0) sc[64] = big;
+      const float big = max_row16(fabsf(v) <= 65504.0f ? fabsf(v) : __builtin_huge_valf());
+      if (lane < 32) sc[(lane < 16 ? 0 : kBlock) + 16 * wave + n16] = lane < 16 ? v * a.scale_log2 : kept_scale(v);
+      if (lane == 16) sc[2 * kBlock + wave] = big;
     }
   };
 
-  int ka[NK], va[NVB];
+  const unsigned char* const kget = smem + n16 * L::KROW + 16 * grp;
+  const unsigned char* const vget = smem + L::V + (4 * grp + (n16 >> 2)) * L::VROW + 8 * (n16 & 3);
+  const float* const sget = reinterpret_cast<const float*>(smem + L::SCALES) + 4 * grp;
+  RowState st[RT];
+  f32x4_t acc[RT][NJ];
 #pragma unroll
-  for (int kk = 0; kk < NK; ++kk) ka[kk] = n16 * L::ROW + ((4 * kk + grp) ^ kswz<D>(n16)) * 16;
-  {
-    const int tv = 4 * grp + (n16 >> 2), sw = vswz<D>(tv);
-#pragma unroll
-    for (int v = 0; v < NVB; ++v) va[v] = L::TILE + tv * L::ROW + ((v ^ sw) * 32) + 8 * (n16 & 3);
-  }
-  RowState st[2];
-  f32x4_t acc[2][NJ];
-#pragma unroll
-  for (int rt = 0; rt < 2; ++rt)
+  for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-  auto compute = [&](const unsigned char* buf, int t0, bool ok0, bool ok1) {
-    f32x4_t sc[2][2];
+  // One block; MASK where some row of the tile does not see all of it.
+  auto compute = [&](auto bufc, int t0, uint32_t pages_ok) {
+    constexpr int at = decltype(bufc)::value * L::BUF;
+    f32x4_t sc[Q][RT];
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt)
+    for (int tt = 0; tt < Q; ++tt)
 #pragma unroll
-      for (int rt = 0; rt < 2; ++rt) sc[tt][rt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int rt = 0; rt < RT; ++rt) sc[tt][rt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk)
+    for (int tt = 0; tt < Q; ++tt)
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt) {
-        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(buf + ka[kk] + tt * 16 * L::ROW);
-        sc[tt][0] = mfma16x16x32_f16(kf, qb[0][kk], sc[tt][0]);
-        sc[tt][1] = mfma16x16x32_f16(kf, qb[1][kk], sc[tt][1]);
+      for (int kk = 0; kk < NK; ++kk) {
+        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kget + at + tt * 16 * L::KROW + 64 * kk);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sc[tt][rt] = mfma16x16x32_f16(kf, qb[rt][kk], sc[tt][rt]);
       }
-    const float* scl = reinterpret_cast<const float*>(buf + 2 * L::TILE);
-    float ksc[8], vsc[8];
+    const float* scl = sget + at / 4;
+    float vsc[4 * Q], s[RT][4 * Q];
 #pragma unroll
-    for (int tt = 0; tt < 2; ++tt) {
-      const f32x4_t k4 = *reinterpret_cast<const f32x4_t*>(scl + 16 * tt + 4 * grp);
-      const f32x4_t v4 = *reinterpret_cast<const f32x4_t*>(scl + 32 + 16 * tt + 4 * grp);
+    for (int tt = 0; tt < Q; ++tt) {
+      const f32x4_t k4 = *reinterpret_cast<const f32x4_t*>(scl + 16 * tt);
+      const f32x4_t v4 = *reinterpret_cast<const f32x4_t*>(scl + kBlock + 16 * tt);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        ksc[4 * tt + r] = k4[r];
         vsc[4 * tt + r] = v4[r];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s[rt][4 * tt + r] = sc[tt][rt][r] * k4[r];
       }
     }
-    const float size = scl[64];
-    const bool whole = t0 + kBlock <= all && ok0 && ok1;
-    u32x4_t pb[2];
-    float alpha[2];
-    bool up[2];
+    u32x4_t pb[RT][Q / 2];
+    float alpha[RT];
+    bool up[RT];
+    float size[RT];
+    const f32x4_t big = *reinterpret_cast<const f32x4_t*>(smem + at + L::SCALES + 8 * kBlock);
+    size[0] = size[RT - 1] = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+    if (__builtin_expect(t0 + kBlock > all || pages_ok != (1u << Q) - 1 || size[0] > 65504.0f, 0)) {
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-      float s[8];
-      bool ok[8];
+      for (int rt = 0; rt < RT; ++rt) {
+        uint32_t ok = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        s[i] = sc[i >> 2][rt][i & 3] * ksc[i];
-        ok[i] = t0 + 16 * (i >> 2) + 4 * grp + (i & 3) <= lim[rt] && (i < 4 ? ok0 : ok1);
+        for (int i = 0; i < 4 * Q; ++i)
+          ok |= (uint32_t)(t0 + 16 * (i >> 2) + 4 * grp + (i & 3) <= lim[rt] && ((pages_ok >> (i >> 2)) & 1u)) << i;
+        size[rt] = hide<4 * Q>(__float_as_uint(pinned(__uint_as_float(ok))), s[rt], vsc);
       }
-      alpha[rt] = whole ? row_block<false>(st[rt], s, ok, mul[rt], vsc, size, pb[rt], up[rt])
-                        : row_block<true>(st[rt], s, ok, mul[rt], vsc, 0.0f, pb[rt], up[rt]);
     }
-    if (__ballot(up[0] || up[1])) {
 #pragma unroll
-      for (int rt = 0; rt < 2; ++rt) {
-        const float f = up[rt] ? alpha[rt] : 1.0f;
+    for (int rt = 0; rt < RT; ++rt) alpha[rt] = row_block<4 * Q>(st[rt], s[rt], mul[rt], vsc, size[rt], pb[rt], up[rt]);
+    if (__builtin_expect(__ballot(up[0] || up[RT - 1]) != 0, 0)) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float f = pinned(up[rt] ? alpha[rt] : 1.0f);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[rt][j] *= f;
       }
@@ -674,42 +721,50 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_tile_kernel(Paged
     typedef short s16x4_t __attribute__((ext_vector_type(4)));
     typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const unsigned char* vp = buf + va[j % NVB] + 256 * (j / NVB);
-      const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4_t*)(vp)));
-      const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4_t*)(vp + 16 * L::ROW)));
-      const u32x4_t vf = u32x4_t{lo.x, lo.y, hi.x, hi.y};
-      acc[0][j] = mfma16x16x32_f16(vf, pb[0], acc[0][j]);
-      acc[1][j] = mfma16x16x32_f16(vf, pb[1], acc[1][j]);
-    }
+    for (int k = 0; k < Q / 2; ++k)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const unsigned char* vp = vget + at + 32 * k * L::VROW + 32 * j;
+        const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4_t*)(vp)));
+        const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4_t*)(vp + 16 * L::VROW)));
+        const u32x4_t vf = u32x4_t{lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt][j] = mfma16x16x32_f16(vf, pb[rt][k], acc[rt][j]);
+      }
   };
 
   if (ib0 < ib1) {
-    BlockPages now = block_pages(a, trow, kBlock * ib0);
-    BlockPages next = block_pages(a, trow, kBlock * min(ib0 + 1, last));
-    load(ib0, now);
-    stage(smem);
-    load(ib0 + 1, next);
-    BlockPages after = block_pages(a, trow, kBlock * min(ib0 + 2, last));
+    BlockPages<Q> bp = block_pages<Q>(a, trow, kBlock * ib0);
+    uint32_t ok_now = bp.ok, ok_next;
+    load(ib0, bp);
+    bp = block_pages<Q>(a, trow, kBlock * min(ib0 + 1, last));
+    stage(std::integral_constant<int, 0>{});
+    load(ib0 + 1, bp);
+    ok_next = bp.ok;
     __syncthreads();
-    for (int ib = ib0; ib < ib1; ++ib) {
-      const int cur = (ib - ib0) & 1;
-      if (kBlock * ib < most) compute(smem + cur * L::BUF, kBlock * ib, now.ok[0], now.ok[1]);
-      stage(smem + (cur ^ 1) * L::BUF);
+    auto step = [&](int ib, auto cur) {
+      const BlockPages<Q> after = block_pages<Q>(a, trow, kBlock * min(ib + 2, last));
+      compute(cur, kBlock * ib, ok_now);
+      stage(std::integral_constant<int, 1 - decltype(cur)::value>{});
       load(ib + 2, after);
-      now = next;
-      next = after;
-      after = block_pages(a, trow, kBlock * min(ib + 3, last));
+      ok_now = ok_next;
+      ok_next = after.ok;
       __syncthreads();
+    };
+    int ib = ib0;
+    for (; ib + 2 <= ib1; ib += 2) {
+      step(ib, std::integral_constant<int, 0>{});
+      step(ib + 1, std::integral_constant<int, 1>{});
     }
+    if (ib < ib1) compute(std::integral_constant<int, 0>{}, kBlock * ib, ok_now);
   }
 
 #pragma unroll
-  for (int rt = 0; rt < 2; ++rt) {
+  for (int rt = 0; rt < RT; ++rt) {
     const float z = sum_groups(st[rt].z);
-    const int r = 32 * wave + 16 * rt + n16;
+    const int r = 16 * (RT * wave + rt) + n16;
     if (r >= rows) continue;
     if (it.parts == 1) {
       const int64_t at = out_row(a, it, kh, rw0 + r, gqa) * D;
@@ -774,7 +829,7 @@ struct PagedPlan {
   int rows;           // of a tile
   int64_t max_tiles;  // of the whole batch, at most
   int64_t slots;
-  int min_blocks;
+  int min_part;
 };
 
 PagedPlan paged_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t max_tokens) {
@@ -783,10 +838,10 @@ PagedPlan paged_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_
   max_new = std::min(max_new, T);
   p.few = max_new * gqa <= 16;
   p.rows = p.few ? 16 : 128;
-  p.min_blocks = 4;
+  p.min_part = 128;
   p.max_tiles = std::min(T * gqa / p.rows + B, B * cdiv(max_new * gqa, p.rows));
-  const int64_t blocks = p.max_tiles * cdiv(max_tokens, kBlock);
-  p.slots = std::max<int64_t>(1, std::min<int64_t>(cdiv(env_int("SPARKQ_PAGED_WGS", 4) * device_cus(), Hkv), cdiv(blocks, p.min_blocks)));
+  p.slots = std::max<int64_t>(1, std::min<int64_t>(cdiv((p.few ? 4 : 2) * device_cus(), Hkv),
+                                                   p.max_tiles * cdiv(max_tokens, p.min_part)));
   return p;
 }
 
@@ -797,7 +852,7 @@ void launch_paged(const PagedSdpaArgs& a, const PagedPlan& p, hipStream_t st) {
   if (p.few)
     hipLaunchKernelGGL(paged_few_kernel<D>, grid, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL(paged_tile_kernel<D>, grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL(paged_tile_kernel<D>, grid, dim3(64 * tile_waves(D)), 0, st, a);
   if (merge.x == 0) return;
   if (p.few)
     hipLaunchKernelGGL((paged_merge_kernel<D, 16>), merge, dim3(256), 0, st, a);
@@ -829,7 +884,7 @@ int paged_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, const Pag
   float* acc = (float*)ws;
   const PagedSdpaArgs a{p, (const uint16_t*)q, qst[0], qst[1], ks, vs, out, acc + n * D, acc + n * (D + 1), acc,
                         (int)Hq, (int)Hkv, (int)std::min<int64_t>(max_new, p.T), causal, qdt, odt,
-                        (int)plan.slots, plan.min_blocks, scale * 1.44269504088896340736f};
+                        (int)plan.slots, plan.min_part, scale * 1.44269504088896340736f};
   if (D == 64)
     launch_paged<64>(a, plan, st);
   else if (D == 128)
