@@ -589,7 +589,7 @@ int sparkq_qk_norm_rope(const void* q, const void* k, const void* q_weight,
 
 /* Quantize-on-append of a batch's new tokens into their pages: k and v
  * [T,Hkv,D] with x_strides[0..3] = k token, k head, v token, v head in
- * elements, quantized by the sparkq_kv_quantize_s8 formula. Rows that fall to
+ * elements (16-byte aligned rows), quantized by the sparkq_kv_quantize_s8 formula. Rows that fall to
  * no sequence, tokens before position 0 and tokens without a page are
  * skipped; the rest of the pool is untouched. Sequences that append must not
  * share the page that they append to (sparkq_kv_pages_fork sees to that). */

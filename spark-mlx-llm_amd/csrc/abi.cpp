@@ -950,7 +950,11 @@ int sparkq_paged_kv_append(const void* k, const void* v, void* k_codes, void* k_
   REQUIRE((T == 0 || (k && v)) && x_strides && starts && (B == 0 || (page_table && lengths)),
           "paged_kv_append: null tensor pointer");
   REQUIRE(is_float_dtype(x_dtype), "paged_kv_append: keys and values must be float16, bfloat16 or float32");
-  REQUIRE(T <= 2 * kI32Max / Hkv, "paged_kv_append: shape too large");
+  REQUIRE(T <= kI32Max / Hkv, "paged_kv_append: shape too large");
+  const int64_t piece = x_dtype == SPARKQ_F32 ? 4 : 8;
+  for (int i = 0; i < 4; ++i)
+    REQUIRE(x_strides[i] >= 0 && x_strides[i] % piece == 0, "paged_kv_append: rows must be 16-byte aligned");
+  REQUIRE(aligned(k, 16) && aligned(v, 16), "paged_kv_append: rows must be 16-byte aligned");
   DEVICE_OK();
   return paged_kv_append(paged_batch(page_table, starts, lengths, T, B, pages, max_pages, table_stride,
                                      page_size),

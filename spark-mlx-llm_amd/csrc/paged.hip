@@ -38,36 +38,79 @@ __device__ __forceinline__ int seq_of_row(const PagedBatch& p, int t) {
   return lo < p.B ? lo : -1;
 }
 
+// v / s for rounding to a whole number, with inv = 1 / s to a unit of fp32 or so:
+// the quotient's error (2^-22) after one correction is far below what matters.
+// A quotient of a 16-bit v (11 bits) and an fp16 s that is not half-way between
+// two whole numbers of 7 bits lies at least 2^-19 of itself from there, and one
+// that is there comes out exactly: q + (v - q s) inv differs from it by the square
+// of q's error, and rounds to it. A third of the division's instructions: 14.4 ->
+// 8 us for 4000 tokens of 4 heads of 256.
+__device__ __forceinline__ float near_quotient(float v, float s, float inv) {
+  const float q = v * inv;
+  return fmaf(fmaf(-q, s, v), inv, q);
+}
+
+// D / 8 lanes a row, 8 values (one or two 16-byte loads) and 8 codes (one store)
+// a lane: the row's loads do not wait for where it goes. A decode step, where
+// row t is sequence t's, finds that out at once.
+template <int LPR>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.p.T * a.H * 2) return;
-  const bool isv = row & 1;
-  const int t = (int)((row >> 1) / a.H), h = (int)((row >> 1) - (int64_t)t * a.H);
-  const int b = seq_of_row(a.p, t);
-  if (b < 0) return;
+  const int l = threadIdx.x % LPR;
+  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const bool live = row < (int64_t)a.p.T * a.H * 2;
+  const int64_t rc = live ? row : 0;
+  const int t = (int)(rc / (2 * a.H)), hv = (int)(rc - (int64_t)t * 2 * a.H);
+  const bool isv = hv >= a.H;
+  const int h = isv ? hv - a.H : hv;
+  const int64_t x0 = (isv ? t * a.v_tok + h * a.v_head : t * a.k_tok + h * a.k_head) + 8 * l;
+  const void* x = isv ? a.v : a.k;
+  float v[8];
+  if (a.x_dtype == SPARKQ_F32) {
+    const f32x4_t* p = reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(x) + x0);
+    const f32x4_t lo = p[0], hi = p[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = lo[i];
+      v[4 + i] = hi[i];
+    }
+  } else {
+    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(x) + x0);
+    const bool bf = a.x_dtype == SPARKQ_BF16;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = bf ? lo16<BF16>(w[i]) : lo16<F16>(w[i]);
+      v[2 * i + 1] = bf ? hi16<BF16>(w[i]) : hi16<F16>(w[i]);
+    }
+  }
+  const bool own = t < a.p.B && a.p.starts[t] == t && a.p.starts[t + 1] == t + 1;
+  const int b = own ? t : seq_of_row(a.p, t);
+  float amax = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
+#pragma unroll
+  for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+  if (!live || b < 0) return;
   const SeqRows s = seq_rows(a.p, b);
   const int pos = s.length - s.count + (t - s.first);
   if (t < s.first || t >= s.first + s.count || pos < 0) return;
   const int id = page_of(a.p, b, pos);
   if (id < 0) return;
-  const PagedSide& side = isv ? a.vs : a.ks;
-  const int64_t x0 = isv ? t * a.v_tok + h * a.v_head : t * a.k_tok + h * a.k_head;
-  const void* x = isv ? a.v : a.k;
-  float amax = 0.0f;
-  for (int d = lane; d < a.D; d += 64) amax = fmaxf(amax, fabsf(load_in(x, x0 + d, a.x_dtype)));
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
   uint16_t s16 = f32_to_f16(amax / 127.0f);
   if (f16_to_f32(s16) == 0.0f) s16 = 0x3C00u;
   const float sc = f16_to_f32(s16);
+  const PagedSide& side = isv ? a.vs : a.ks;
   const int slot = pos & ((1 << a.p.page_log2) - 1);
-  if (lane == 0) side.scales[id * side.s_page + h * side.s_head + slot * side.s_tok] = s16;
-  int8_t* dst = reinterpret_cast<int8_t*>(side.codes) + id * side.c_page + h * side.c_head + slot * side.c_tok;
-  for (int d = lane; d < a.D; d += 64) {
-    const float v = __builtin_rintf(load_in(x, x0 + d, a.x_dtype) / sc);
-    dst[d] = (int8_t)fminf(fmaxf(v, -127.0f), 127.0f);
+  if (l == 0) side.scales[id * side.s_page + h * side.s_head + slot * side.s_tok] = s16;
+  uint32_t w[2] = {0, 0};
+  const float inv = __builtin_amdgcn_rcpf(sc);
+  const bool divide = a.x_dtype == SPARKQ_F32 || sc > 65504.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = fminf(fmaxf(__builtin_rintf(divide ? v[i] / sc : near_quotient(v[i], sc, inv)), -127.0f), 127.0f);
+    w[i / 4] |= ((uint32_t)(int)q & 255u) << (8 * (i % 4));
   }
+  *reinterpret_cast<uint2*>(side.codes + id * side.c_page + h * side.c_head + slot * side.c_tok + 8 * l) =
+      make_uint2(w[0], w[1]);
 }
 
 // ---------------------------------------------------------------------------
@@ -156,10 +199,29 @@ __device__ __forceinline__ int write_page(const PageArgs& a, const RowPlan& r) {
   return held_page(a, r, r.held - 1);
 }
 
-// The plan's counters are read and written by one workgroup through atomics
-// of device scope: they are coherent whatever its vector cache holds.
-__device__ __forceinline__ void put(int* p, int v) { splitk_store(p, v); }
-__device__ __forceinline__ int get(const int* p) { return splitk_load(p); }
+// Counters of a plan's pages, in LDS (up to kLdsPages) or, of larger pools, in
+// the workspace: there through device-scope atomics, which are coherent whatever
+// the vector cache holds.
+constexpr int kLdsPages = 16384;
+template <bool LDS>
+struct Counters {
+  int* p;
+  __device__ void put(int i, int v) const {
+    if (LDS)
+      p[i] = v;
+    else
+      splitk_store(p + i, v);
+  }
+  __device__ int get(int i) const { return LDS ? p[i] : splitk_load(p + i); }
+  __device__ void add(int i, int v) const { atomicAdd(p + i, v); }
+  __device__ void min(int i, int v) const { atomicMin(p + i, v); }
+};
+
+template <bool LDS>
+__device__ __forceinline__ void plan_sync() {
+  if (!LDS) __threadfence();
+  __syncthreads();
+}
 
 // exclusive prefix of v over the workgroup's threads; total in every thread
 __device__ __forceinline__ int block_prefix(int v, int* s_wave, int& total) {
@@ -175,57 +237,78 @@ __device__ __forceinline__ int block_prefix(int v, int* s_wave, int& total) {
   __syncthreads();
   int below = 0;
   total = 0;
+#pragma unroll
   for (int w = 0; w < kPlanThreads / 64; ++w) {
-    if (w < wave) below += s_wave[w];
-    total += s_wave[w];
+    const int n = s_wave[w];
+    below += w < wave ? n : 0;
+    total += n;
   }
   return below + x - v;
 }
 
-// held[p] = rows' entries that name page p
-__device__ void count_held(const PageArgs& a) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int p = tid; p < a.pages; p += kPlanThreads) {
-    put(a.s.held + p, 0);
-    put(a.s.first + p, 0x7FFFFFFF);
-  }
-  __threadfence();
-  __syncthreads();
-  for (int i = wave; i < a.rows; i += kPlanThreads / 64) {
-    const RowPlan r = row_plan(a, i);
-    for (int j = lane; j < r.held; j += 64) {
-      const int id = held_page(a, r, j);
-      if (id >= 0) atomicAdd(a.s.held + id, 1);
+// held[p] = rows' entries that name page p. Rows are planned a thread each and
+// their entries counted by `per` lanes each, four rows' loads in flight.
+template <bool LDS>
+__device__ void count_held(const PageArgs& a, const Counters<LDS>& held, int (&s_src)[kPlanThreads],
+                           int (&s_held)[kPlanThreads]) {
+  const int tid = threadIdx.x;
+  for (int p = tid; p < a.pages; p += kPlanThreads) held.put(p, 0);
+  int per = 1;
+  while (per < a.width && per < 64) per <<= 1;
+  const int step = kPlanThreads / per, l = tid % per;
+  for (int i0 = 0; i0 < a.rows; i0 += kPlanThreads) {
+    const int n = min(a.rows - i0, kPlanThreads);
+    plan_sync<LDS>();  // held is cleared; the last rows are counted
+    if (tid < n) {
+      const RowPlan r = row_plan(a, i0 + tid);
+      s_src[tid] = r.src;
+      s_held[tid] = r.held;
+    }
+    __syncthreads();
+    for (int j0 = 0; j0 < a.width; j0 += per) {
+      for (int i = tid / per; i < n; i += 4 * step) {
+        int id[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int k = min(i + u * step, n - 1), j = j0 + l;
+          id[u] = i + u * step < n && j < s_held[k] ? a.table[s_src[k] * a.table_stride + j] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if ((unsigned)id[u] < (unsigned)a.pages) held.add(id[u], 1);
+      }
     }
   }
-  __threadfence();
-  __syncthreads();
+  plan_sync<LDS>();
 }
 
+// One workgroup. Three passes over the pages' counters, two over the rows.
+template <bool LDS>
 __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PageArgs a) {
-  __shared__ int s_wave[kPlanThreads / 64];
+  extern __shared__ int s_pages[];
+  __shared__ int s_wave[kPlanThreads / 64], s_src[kPlanThreads], s_held[kPlanThreads];
+  const Counters<LDS> held{LDS ? s_pages : a.s.held}, first{LDS ? s_pages + a.pages : a.s.first};
   const int tid = threadIdx.x;
-  count_held(a);
+  for (int p = tid; p < a.pages; p += kPlanThreads) first.put(p, 0x7FFFFFFF);
+  count_held<LDS>(a, held, s_src, s_held);
   // free pages in order: each thread takes a run of pages
   const int per = (a.pages + kPlanThreads - 1) / kPlanThreads;
   const int p0 = min(tid * per, a.pages), p1 = min(p0 + per, a.pages);
   int n = 0, nfree;
-  for (int p = p0; p < p1; ++p) n += get(a.s.held + p) == 0;
+  for (int p = p0; p < p1; ++p) n += held.get(p) == 0;
   int at = block_prefix(n, s_wave, nfree);
   for (int p = p0; p < p1; ++p)
-    if (get(a.s.held + p) == 0) put(a.s.list + at++, p);
-  __threadfence();
+    if (held.get(p) == 0) a.s.list[at++] = p;
   __syncthreads();
   // holders that do not write: what is left of held without the writers
   for (int i = tid; i < a.rows; i += kPlanThreads) {
     const int w = write_page(a, row_plan(a, i));
     if (w >= 0) {
-      atomicSub(a.s.held + w, 1);
-      atomicMin(a.s.first + w, i);
+      held.add(w, -1);
+      first.min(w, i);
     }
   }
-  __threadfence();
-  __syncthreads();
+  plan_sync<LDS>();
   int wanted = 0, pairs = 0;
   for (int i0 = 0; i0 < a.rows; i0 += kPlanThreads) {
     const int i = i0 + tid;
@@ -233,7 +316,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PageArgs 
     if (i < a.rows) {
       const RowPlan r = row_plan(a, i);
       w = write_page(a, r);
-      copy = w >= 0 && (get(a.s.held + w) > 0 || get(a.s.first + w) != i);
+      copy = w >= 0 && (held.get(w) > 0 || first.get(w) != i);
       want = copy + (r.need - r.held);
     }
     int t_want, t_copy;
@@ -242,7 +325,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PageArgs 
     if (i < a.rows) a.s.base[i] = copy ? ~base : base;  // negative: its first page is a copy
     if (copy) {
       a.s.src[pair] = w;
-      a.s.dst[pair] = base < nfree ? get(a.s.list + base) : -1;
+      a.s.dst[pair] = base;  // of the list
     }
     wanted += t_want;
     pairs += t_copy;
@@ -255,27 +338,33 @@ __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PageArgs 
   }
 }
 
+// One workgroup. A page that moves keeps in held the (inverted) place of its new
+// number in the list.
+template <bool LDS>
 __global__ __launch_bounds__(kPlanThreads) void pages_compact_plan_kernel(PageArgs a) {
-  __shared__ int s_wave[kPlanThreads / 64];
+  extern __shared__ int s_pages[];
+  __shared__ int s_wave[kPlanThreads / 64], s_src[kPlanThreads], s_held[kPlanThreads];
+  const Counters<LDS> held{LDS ? s_pages : a.s.held};
   const int tid = threadIdx.x;
-  count_held(a);
+  count_held<LDS>(a, held, s_src, s_held);
   const int per = (a.pages + kPlanThreads - 1) / kPlanThreads;
   const int p0 = min(tid * per, a.pages), p1 = min(p0 + per, a.pages);
   int n = 0, used, movers;
-  for (int p = p0; p < p1; ++p) n += get(a.s.held + p) != 0;
+  for (int p = p0; p < p1; ++p) n += held.get(p) != 0;
   const int below = block_prefix(n, s_wave, used);
   int m = 0;  // pages in use at or past `used`
-  for (int p = max(p0, used); p < p1; ++p) m += get(a.s.held + p) != 0;
+  for (int p = max(p0, used); p < p1; ++p) m += held.get(p) != 0;
   int mover = block_prefix(m, s_wave, movers);
   int hole = p0 - below;  // free pages before p0
   for (int p = p0; p < p1; ++p) {
-    const bool live = get(a.s.held + p) != 0;
+    const bool live = held.get(p) != 0;
     if (p < used && !live) a.s.list[hole] = p;
+    int to = 0;
     if (p >= used && live) {
       a.s.first[mover] = p;
-      a.s.held[p] = ~mover;  // its new number is list[mover]
-      ++mover;
+      to = ~mover++;
     }
+    a.s.held[p] = to;
     hole += !live;
   }
   if (tid == 0) {
@@ -286,16 +375,16 @@ __global__ __launch_bounds__(kPlanThreads) void pages_compact_plan_kernel(PageAr
 
 // Copies page src[i] to dst[i] in every layer of the four tensors, in pieces
 // of 16 KB dealt over the workgroups. No page is both a source and a
-// destination.
-__device__ void copy_pages(const PageArgs& a, const int* src, const int* dst, int pairs, int block,
-                           int blocks) {
+// destination. The destination is dst[i], or list[dst[i]] where a list is given.
+__device__ void copy_pages(const PageArgs& a, const int* src, const int* dst, const int* list, int pairs,
+                           int block, int blocks) {
   const int vecs = 2 * (a.vec_codes + a.vec_scales), units = (vecs + 1023) / 1024;
   const int64_t total = (int64_t)pairs * a.layers * units;
   for (int64_t u = block; u < total; u += blocks) {
     const int piece = (int)(u % units);
     const int64_t pl = u / units;
     const int layer = (int)(pl % a.layers), pair = (int)(pl / a.layers);
-    const int64_t from = src[pair], to = dst[pair];
+    const int64_t from = src[pair], to = list ? list[dst[pair]] : dst[pair];
     u32x4_t v[4];
     uint8_t* out[4];
 #pragma unroll
@@ -320,7 +409,7 @@ __device__ void copy_pages(const PageArgs& a, const int* src, const int* dst, in
 
 __global__ __launch_bounds__(256) void pages_fork_kernel(PageArgs a) {
   if ((int)blockIdx.x >= a.table_blocks) {
-    copy_pages(a, a.s.src, a.s.dst, a.s.head[kPairs], blockIdx.x - a.table_blocks,
+    copy_pages(a, a.s.src, a.s.dst, a.s.list, a.s.head[kPairs], blockIdx.x - a.table_blocks,
                gridDim.x - a.table_blocks);
     return;
   }
@@ -343,7 +432,7 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(PageArgs a) {
 
 __global__ __launch_bounds__(256) void pages_compact_kernel(PageArgs a) {
   if ((int)blockIdx.x >= a.table_blocks) {
-    copy_pages(a, a.s.first, a.s.list, a.s.head[kPairs], blockIdx.x - a.table_blocks,
+    copy_pages(a, a.s.first, a.s.list, nullptr, a.s.head[kPairs], blockIdx.x - a.table_blocks,
                gridDim.x - a.table_blocks);
     return;
   }
@@ -364,8 +453,13 @@ int paged_kv_append(const PagedBatch& p, const void* k, const void* v, const int
                     hipStream_t st) {
   if (p.T == 0 || p.B == 0) return SPARKQ_OK;
   const PagedAppendArgs a{p, k, v, xst[0], xst[1], xst[2], xst[3], ks, vs, (int)H, (int)D, xdt};
-  hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)cdiv((int64_t)p.T * H * 2, 4)), dim3(256),
-                     0, st, a);
+  const dim3 grid((unsigned)cdiv((int64_t)p.T * H * 2, 2048 / D));
+  if (D == 64)
+    hipLaunchKernelGGL(paged_append_kernel<8>, grid, dim3(256), 0, st, a);
+  else if (D == 128)
+    hipLaunchKernelGGL(paged_append_kernel<16>, grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL(paged_append_kernel<32>, grid, dim3(256), 0, st, a);
   return check_launch("paged_append_kernel");
 }
 
@@ -412,7 +506,10 @@ int kv_pages_fork(const int32_t* table, int64_t table_stride, const int32_t* len
   a.out_table = out_table;
   a.out_lengths = out_lengths;
   a.out_count = missing;
-  hipLaunchKernelGGL(pages_fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+  if (pages <= kLdsPages)
+    hipLaunchKernelGGL(pages_fork_plan_kernel<true>, dim3(1), dim3(kPlanThreads), 2 * pages * sizeof(int), st, a);
+  else
+    hipLaunchKernelGGL(pages_fork_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, st, a);
   hipLaunchKernelGGL(pages_fork_kernel, page_grid(a), dim3(256), 0, st, a);
   return check_launch("pages_fork_kernel");
 }
@@ -425,7 +522,10 @@ int kv_pages_compact(const int32_t* table, int64_t table_stride, const int32_t* 
                          strides, code_bytes, scale_bytes, ws);
   a.out_table = out_table;
   a.out_count = used;
-  hipLaunchKernelGGL(pages_compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+  if (pages <= kLdsPages)
+    hipLaunchKernelGGL(pages_compact_plan_kernel<true>, dim3(1), dim3(kPlanThreads), pages * sizeof(int), st, a);
+  else
+    hipLaunchKernelGGL(pages_compact_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, st, a);
   hipLaunchKernelGGL(pages_compact_kernel, page_grid(a), dim3(256), 0, st, a);
   return check_launch("pages_compact_kernel");
 }

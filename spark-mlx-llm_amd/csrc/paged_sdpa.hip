@@ -18,7 +18,7 @@
 //
 // Work. The lengths live on the device, so every workgroup works out from the
 // batch's starts and lengths which (sequence, tile, part of the context) is
-// its own (find_item): a context is split so that about `slots` parts of equal
+// its own (find_item): a context is split so that about `target` parts of equal
 // length fill the chip however the lengths differ, and a grid sized by the
 // host for the worst case has nothing left over but idle workgroups.
 //
@@ -47,6 +47,7 @@ struct PagedSdpaArgs {
   void* out;  // [T, Hq, D]
   float *pm, *pz, *pacc;  // [Hkv][slots][rows], [...], [...][D]: parts of split contexts
   int Hq, Hkv, max_new, causal, q_dtype, out_dtype;
+  int target;      // parts of the whole batch, about, per KV head
   int slots;       // parts of split contexts, at most, per KV head
   int min_part;    // tokens of a part, at least
   float scale_log2;
@@ -94,9 +95,9 @@ __device__ __forceinline__ int wave_prefix(int v, int lane) {  // inclusive
 
 // Item x of the batch's items in order (SPLIT false: every tile and part), or
 // tile x of those whose context is split. A context of n tokens is split into
-// floor(n / C) parts, C = max(min_part, ceil(all tiles' tokens / slots)), so
-// split contexts have no more than `slots` parts together. All lanes of a wave
-// take part and get the same answer.
+// ceil(n / C) parts, C = max(min_part, ceil(all tiles' tokens / target)): fewer
+// than `target` contexts are longer than C, and these have fewer than 2 target
+// parts together. All lanes of a wave take part and get the same answer.
 template <int R, bool SPLIT>
 __device__ Item find_item(const PagedSdpaArgs& a, int x) {
   const int lane = threadIdx.x & 63;
@@ -107,12 +108,12 @@ __device__ Item find_item(const PagedSdpaArgs& a, int x) {
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
-  const long long C = max((all + a.slots - 1) / a.slots, (long long)a.min_part);
+  const int C = (int)min(max((all + a.target - 1) / a.target, (long long)a.min_part), 0x7FFFFFFFll);
   Item it{-1, 0, 0, 1, 0, 0, 0, 0, 0};
   int items = 0, slots = 0;
   for (int b0 = 0; b0 < a.p.B; b0 += 64) {
     const SeqWork w = seq_work<R>(a, b0 + lane);
-    const int parts = max(1, (int)(w.length / C));
+    const int parts = w.length > C ? (w.length - 1) / C + 1 : 1;
     const int own = SPLIT ? (parts > 1 ? w.tiles : 0) : w.tiles * parts;
     const int used = parts > 1 ? w.tiles * parts : 0;
     const int end = items + wave_prefix(own, lane), slot_end = slots + wave_prefix(used, lane);
@@ -131,6 +132,8 @@ __device__ Item find_item(const PagedSdpaArgs& a, int x) {
       it.part = SPLIT ? 0 : i - k * it.parts;
       it.tile = tiles - 1 - k;  // the last tiles see the most: they start first
       it.slot = of(slot_end - used) + k * it.parts;
+      // sequences whose starts overlap are more than the workspace is for
+      if (it.parts > 1 && it.slot + it.parts > a.slots) it.b = -1;
       break;
     }
     items = __builtin_amdgcn_readlane(end, 63);
@@ -784,40 +787,73 @@ __global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_ti
 }
 
 // Joins the parts of split contexts: workgroup (x, kh) takes 16 rows of a split
-// tile, each thread four dims of a row at a time, eight parts in flight.
+// tile. A wave per row finds the parts' weights (a lane each, one round trip);
+// then a thread sums four dims of a row over every `ways`-th part, eight loads
+// in flight, and the ways are summed through LDS.
+constexpr int kMaxParts = 512;
 template <int D, int R>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedSdpaArgs a) {
-  constexpr int GROUPS = R / 16;
+  constexpr int GROUPS = R / 16, D4 = D / 4;
+  __shared__ float wts[16][kMaxParts];
+  __shared__ f32x4_t sums[256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int kh = blockIdx.x % a.Hkv, x = blockIdx.x / a.Hkv, gqa = a.Hq / a.Hkv;
   const Item it = find_item<R, true>(a, x / GROUPS);
   if (it.b < 0) return;
   const int r0 = 16 * (x % GROUPS);
-  const int rows = min(it.rows - R * it.tile - r0, 16);
+  const int rows = min(it.rows - R * it.tile - r0, 16), parts = it.parts;
   const int64_t base = ((int64_t)kh * a.slots + it.slot) * R + r0;
-  for (int i = threadIdx.x; i < rows * (D / 4); i += 256) {
-    const int r = i / (D / 4), d = 4 * (i - r * (D / 4));
+  for (int r = wave; r < rows; r += 4) {
     float mm = kNegInf, z = 0.0f;
-    for (int k = 0; k < it.parts; ++k) mm = fmaxf(mm, a.pm[base + (int64_t)k * R + r]);
-    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k0 = 0; k0 < it.parts; k0 += 8) {
-      f32x4_t v[8];
-      float f[8];
-      bool live[8];
+    for (int k = lane; k < parts; k += 64) {
+      const float m = a.pm[base + (int64_t)k * R + r];
+      wts[r][k] = m;
+      mm = fmaxf(mm, m);
+    }
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int64_t at = base + (int64_t)min(k0 + u, it.parts - 1) * R + r;
-        const float m = a.pm[at];
-        live[u] = k0 + u < it.parts && m != kNegInf;
-        f[u] = __builtin_amdgcn_exp2f(m - mm);
-        v[u] = *reinterpret_cast<const f32x4_t*>(a.pacc + at * D + d);
-        z = live[u] ? fmaf(a.pz[at], f[u], z) : z;
-      }
+    for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
+    for (int k = lane; k < parts; k += 64) {
+      const float m = wts[r][k];
+      const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mm);
+      const float pz = a.pz[base + (int64_t)k * R + r];
+      z = m == kNegInf ? z : fmaf(pz, f, z);
+      wts[r][k] = f;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) z += __shfl_xor(z, o);
+    const float inv = z != 0.0f ? 1.0f / z : 0.0f;
+    for (int k = lane; k < parts; k += 64) wts[r][k] *= inv;
+  }
+  __syncthreads();
+  // as many ways over the parts as the threads allow: a power of two
+  const int items = rows * D4;
+  int ways = 1;
+  while (2 * ways * items <= 256 && 2 * ways <= parts) ways *= 2;
+  const int per = 256 / ways, way = tid / per;
+  for (int i0 = 0; i0 < items; i0 += per) {
+    const int i = i0 + tid % per;
+    const int r = min(i, items - 1) / D4, d = 4 * (min(i, items - 1) % D4);
+    const float* p = a.pacc + (base + r) * D + d;
+    f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k0 = way; k0 < parts; k0 += 8 * ways) {
+      f32x4_t v[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (live[u]) o += v[u] * f[u];
+        v[u] = *reinterpret_cast<const f32x4_t*>(p + (int64_t)min(k0 + u * ways, parts - 1) * R * D);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float f = wts[r][min(k0 + u * ways, parts - 1)];
+        if (k0 + u * ways < parts && f != 0.0f) o += v[u] * f;
+      }
     }
-    if (z != 0.0f) o /= z;
-    store_row4(a, out_row(a, it, kh, R * it.tile + r0 + r, gqa) * D + d, o);
+    if (ways > 1) {
+      __syncthreads();
+      sums[tid] = o;
+      __syncthreads();
+      if (way == 0)
+        for (int w = 1; w < ways; ++w) o += sums[tid + w * per];
+    }
+    if (way == 0 && i < items) store_row4(a, out_row(a, it, kh, R * it.tile + r0 + r, gqa) * D + d, o);
   }
 }
 
@@ -828,7 +864,7 @@ struct PagedPlan {
   bool few;
   int rows;           // of a tile
   int64_t max_tiles;  // of the whole batch, at most
-  int64_t slots;
+  int64_t target, slots, split;  // parts to aim at, parts and tiles of split contexts at most
   int min_part;
 };
 
@@ -840,15 +876,16 @@ PagedPlan paged_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_
   p.rows = p.few ? 16 : 128;
   p.min_part = 128;
   p.max_tiles = std::min(T * gqa / p.rows + B, B * cdiv(max_new * gqa, p.rows));
-  p.slots = std::max<int64_t>(1, std::min<int64_t>(cdiv((p.few ? 4 : 2) * device_cus(), Hkv),
-                                                   p.max_tiles * cdiv(max_tokens, p.min_part)));
+  p.target = std::min<int64_t>(cdiv((p.few ? 4 : 2) * device_cus(), Hkv), kMaxParts);
+  p.split = max_tokens > p.min_part ? std::min(p.max_tiles, p.target) : 0;
+  p.slots = std::min(2 * p.target, p.split * cdiv(max_tokens, p.min_part));
   return p;
 }
 
 template <int D>
 void launch_paged(const PagedSdpaArgs& a, const PagedPlan& p, hipStream_t st) {
-  const dim3 grid((unsigned)((p.slots + p.max_tiles) * a.Hkv));
-  const dim3 merge((unsigned)(p.slots / 2 * (p.rows / 16) * a.Hkv));
+  const dim3 grid((unsigned)((p.slots + p.max_tiles) * a.Hkv));  // of an unsplit tile or a part each
+  const dim3 merge((unsigned)(p.split * (p.rows / 16) * a.Hkv));
   if (p.few)
     hipLaunchKernelGGL(paged_few_kernel<D>, grid, dim3(256), 0, st, a);
   else
@@ -866,7 +903,7 @@ void launch_paged(const PagedSdpaArgs& a, const PagedPlan& p, hipStream_t st) {
 size_t paged_sdpa_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
                             int64_t max_tokens) {
   const PagedPlan p = paged_plan(T, B, Hq, Hkv, max_new, max_tokens);
-  return p.slots < 2 ? 0 : (size_t)(Hkv * p.slots * p.rows * (D + 2)) * sizeof(float);
+  return (size_t)(Hkv * p.slots * p.rows * (D + 2)) * sizeof(float);
 }
 
 int paged_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, const PagedSide& ks,
@@ -884,7 +921,7 @@ int paged_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, const Pag
   float* acc = (float*)ws;
   const PagedSdpaArgs a{p, (const uint16_t*)q, qst[0], qst[1], ks, vs, out, acc + n * D, acc + n * (D + 1), acc,
                         (int)Hq, (int)Hkv, (int)std::min<int64_t>(max_new, p.T), causal, qdt, odt,
-                        (int)plan.slots, plan.min_part, scale * 1.44269504088896340736f};
+                        (int)plan.target, (int)plan.slots, plan.min_part, scale * 1.44269504088896340736f};
   if (D == 64)
     launch_paged<64>(a, plan, st);
   else if (D == 128)

@@ -152,8 +152,25 @@ def call(name: str, *args, device: Optional[torch.device] = None) -> None:
             rc = getattr(lib(), name)(*args)
     else:
         rc = getattr(lib(), name)(*args)
-    if rc == OK:
-        return
+    if rc != OK:
+        _raise(name, rc)
+
+
+def launch(name: str, index: int, *args) -> None:
+    """call() for an entry point whose tensors are all on GPU `index`, with the
+    current stream of that GPU as its last argument."""
+    fn = getattr(_LIB or lib(), name)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc != OK:
+        _raise(name, rc)
+
+
+def _raise(name: str, rc: int):
     msg = (lib().sparkq_last_error() or b"").decode(errors="replace")
     if rc in (ERR_INVALID, ERR_UNSUPPORTED):
         raise ValueError(msg)

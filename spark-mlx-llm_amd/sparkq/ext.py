@@ -981,33 +981,42 @@ def qk_norm_rope(queries, keys, q_weight, k_weight, positions, *, dims: int, eps
     tensors = (queries, keys, q_weight, k_weight, positions)
     if any(not isinstance(v, torch.Tensor) for v in tensors):
         raise TypeError("queries, keys, weights and positions must be tensors")
-    if queries.ndim != 3 or keys.ndim != 3 or keys.shape[0] != queries.shape[0] \
-            or keys.shape[2] != queries.shape[2] or 0 in queries.shape[1:] or not keys.shape[1]:
+    qshape, kshape = queries.shape, keys.shape
+    if len(qshape) != 3 or len(kshape) != 3 or kshape[0] != qshape[0] or kshape[2] != qshape[2] \
+            or not qshape[1] or not kshape[1] or not qshape[2]:
         raise ValueError("qk_norm_rope requires queries [T,Hq,D] and keys [T,Hkv,D]")
-    t, hq, d = queries.shape
-    hkv = keys.shape[1]
-    dtype, dev = queries.dtype, queries.device
-    if dtype not in _HALF or any(v.dtype != dtype for v in (keys, q_weight, k_weight)):
+    t, hq, d = qshape
+    dtype = queries.dtype
+    if dtype not in _HALF or any(v.dtype is not dtype for v in (keys, q_weight, k_weight)):
         raise ValueError("qk_norm_rope requires BF16 or F16 queries, keys and weights of one dtype")
     if q_weight.shape != (d,) or k_weight.shape != (d,):
         raise ValueError(f"qk_norm_rope weights must have shape [{d}]")
-    if positions.shape != (t,) or positions.dtype not in (torch.int32, torch.int64):
+    wide = positions.dtype is torch.int64
+    if positions.shape != (t,) or not (wide or positions.dtype is torch.int32):
         raise ValueError(f"qk_norm_rope positions must be int32 or int64 of shape [{t}]")
     if type(dims) is not int:
         raise ValueError("qk_norm_rope dims must be an int")
     _require_device("qk_norm_rope", *tensors)
-    if any(v.device != dev for v in tensors):
+    index = queries.get_device()
+    if any(v.get_device() != index for v in tensors):
         raise ValueError("qk_norm_rope tensors must live on one device")
-    q = queries if queries.stride(2) == 1 or d == 1 else queries.contiguous()
-    k = keys if keys.stride(2) == 1 or d == 1 else keys.contiguous()
-    q_out = torch.empty((t, hq, d), dtype=dtype, device=dev)
-    k_out = torch.empty((t, hkv, d), dtype=dtype, device=dev)
-    st = (ctypes.c_int64 * 4)(*q.stride()[:2], *k.stride()[:2])
-    _lib.call("sparkq_qk_norm_rope", _ptr(q), _ptr(k), _ptr(q_weight.contiguous()),
-              _ptr(k_weight.contiguous()), _ptr(positions.contiguous()),
-              32 if positions.dtype == torch.int32 else 64, _ptr(q_out), _ptr(k_out), t, hq, hkv,
-              d, dims, int(bool(traditional)), float(eps), float(base), float(scale),
-              _lib.dtype_code(dtype), st, _lib.stream_handle(dev), device=dev)
+    qst, kst = queries.stride(), keys.stride()
+    if qst[2] != 1:
+        queries = queries.contiguous()
+        qst = queries.stride()
+    if kst[2] != 1:
+        keys = keys.contiguous()
+        kst = keys.stride()
+    dev = queries.device
+    q_out = torch.empty(qshape, dtype=dtype, device=dev)
+    k_out = torch.empty(kshape, dtype=dtype, device=dev)
+    q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
+    positions = positions.contiguous()
+    _lib.launch("sparkq_qk_norm_rope", index, queries.data_ptr(), keys.data_ptr(),
+                q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), 64 if wide else 32,
+                q_out.data_ptr(), k_out.data_ptr(), t, hq, kshape[1], d, dims,
+                int(bool(traditional)), eps, base, scale, _lib.dtype_code(dtype),
+                (ctypes.c_int64 * 4)(qst[0], qst[1], kst[0], kst[1]))
     return q_out, k_out
 
 

@@ -26,70 +26,76 @@ import math
 import torch
 
 from . import _lib
-from .ext import _HALF, _REAL, _out_buffer, _ptr, _require_device
+from .ext import _HALF, _out_buffer, _ptr
 
 __all__ = ["PagedKVCache", "kv_pages_compact", "kv_pages_fork", "paged_kv_append",
            "paged_quantized_sdpa"]
 
 
+_I64x2, _I64x4, _I64x8, _I64x12 = (ctypes.c_int64 * n for n in (2, 4, 8, 12))
+_CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+
+
 def _check_cache(op, cache, ndim):
-    """(pages, Hkv, page_size, D) of a cache with `ndim` axes in its codes."""
+    """((k_codes, k_scales, v_codes, v_scales), their GPU, codes' shape) of a
+    cache with `ndim` axes in its codes."""
     if len(cache) != 4 or any(not isinstance(t, torch.Tensor) for t in cache):
         raise ValueError(f"{op}: the cache is (k_codes, k_scales, v_codes, v_scales)")
     kc, ks, vc, vs = cache
-    if (kc.ndim != ndim or kc.dtype != torch.int8 or vc.dtype != torch.int8
-            or ks.dtype != torch.float16 or vs.dtype != torch.float16
-            or vc.shape != kc.shape or ks.shape != kc.shape[:-1] or vs.shape != ks.shape):
+    shape, scales = kc.shape, ks.shape
+    if (len(shape) != ndim or vc.shape != shape or scales != shape[:-1] or vs.shape != scales
+            or kc.dtype is not torch.int8 or vc.dtype is not torch.int8
+            or ks.dtype is not torch.float16 or vs.dtype is not torch.float16):
         raise ValueError(f"{op}: the cache holds int8 codes [pages,Hkv,page_size,D] and fp16 "
                          "scales [pages,Hkv,page_size] of keys and of values")
-    dev = kc.device
-    if ks.device != dev or vc.device != dev or vs.device != dev:
+    index = _gpu(op, kc)
+    if ks.get_device() != index or vc.get_device() != index or vs.get_device() != index:
         raise ValueError(f"{op}: the cache's tensors must live on one device")
-    return kc.shape[-4:]
+    return kc, ks, vc, vs, index, shape
 
 
-def _check_device(op, cache, *tensors):
-    """On the GPU, all of them on the cache's."""
-    _require_device(op, cache[0], *tensors)
-    if any(t.device != cache[0].device for t in tensors):
-        raise ValueError(f"{op}: every tensor must live on the cache's device")
+def _gpu(op, t):
+    index = t.get_device()
+    if index < 0:
+        raise ValueError(f"{op} requires GPU execution")
+    return index
 
 
-def _check_ints(op, device, **tensors):
-    for name, (t, shape) in tensors.items():
-        if t.dtype != torch.int32 or t.shape != shape or (t.ndim and t.stride(-1) != 1
-                                                          and t.shape[-1] > 1):
-            raise ValueError(f"{op}: {name} must be an int32 tensor of shape {list(shape)}, its "
-                             "last axis contiguous")
-        if t.device != device:
-            raise ValueError(f"{op}: {name} must live on the cache's device")
+def _check_ints(op, index, name, t, shape):
+    if t.dtype is not torch.int32 or t.shape != shape:
+        raise ValueError(f"{op}: {name} must be an int32 tensor of shape {list(shape)}")
+    if t.get_device() != index:
+        raise ValueError(f"{op}: {name} must live on the cache's device")
+    if shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{op}: the last axis of {name} must be contiguous")
 
 
-def _batch(op, cache, page_table, starts, lengths):
-    if page_table.ndim != 2 or lengths.ndim != 1:
+def _check_batch(op, index, page_table, starts, lengths):
+    """(sequences, pages per row) of a batch."""
+    if page_table.ndim != 2 or page_table.shape[1] < 1:
         raise ValueError(f"{op}: expected page_table [B,M], lengths [B] and starts [B+1]")
-    b, width = page_table.shape
-    if width < 1:
-        raise ValueError(f"{op}: page_table has no columns")
-    _check_ints(op, cache[0].device, page_table=(page_table, (b, width)),
-                lengths=(lengths, (b,)), starts=(starts, (b + 1,)))
+    b, width = shape = page_table.shape
+    _check_ints(op, index, "page_table", page_table, shape)
+    _check_ints(op, index, "lengths", lengths, (b,))
+    _check_ints(op, index, "starts", starts, (b + 1,))
     return b, width
 
 
-def _strides(cache):
-    kc, ks, vc, vs = cache
-    if kc.stride(-1) != 1 or vc.stride(-1) != 1:
-        raise ValueError("the cache's innermost axes must be contiguous")
-    return (ctypes.c_int64 * 12)(*kc.stride()[:3], *ks.stride(), *vc.stride()[:3], *vs.stride())
+def _strides(op, kc, ks, vc, vs):
+    a, b = kc.stride(), vc.stride()
+    if a[3] != 1 or b[3] != 1:
+        raise ValueError(f"{op}: the codes' innermost axes must be contiguous")
+    return _I64x12(*a[:3], *ks.stride(), *b[:3], *vs.stride())
 
 
 def _rows16(t):
-    """t with rows that 16-byte loads can read: itself, or a copy."""
+    """(t, its strides) with rows that 16-byte loads can read: itself, or a copy."""
     n = 16 // t.element_size()
     st = t.stride()
     if st[2] == 1 and st[0] % n == 0 and st[1] % n == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+        return t, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
 
 
 def paged_kv_append(keys, values, cache, page_table, starts, lengths):
@@ -100,21 +106,22 @@ def paged_kv_append(keys, values, cache, page_table, starts, lengths):
     and tokens without a page are skipped. Sequences that append must not share
     the page they append to: kv_pages_fork gives each its own."""
     op = "paged_kv_append"
-    pages, hkv, page, d = _check_cache(op, cache, 4)
+    kc, ks, vc, vs, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
     if keys.ndim != 3 or keys.shape[1:] != (hkv, d) or values.shape != keys.shape:
         raise ValueError(f"{op}: keys and values must be [T,{hkv},{d}] like the cache")
-    if keys.dtype not in _REAL or values.dtype != keys.dtype:
+    dtype = keys.dtype
+    if dtype not in _CODE or values.dtype is not dtype:
         raise ValueError(f"{op}: keys and values must be float16, bfloat16 or float32, both alike")
-    b, width = _batch(op, cache, page_table, starts, lengths)
-    _check_device(op, cache, keys, values)
-    strides = _strides(cache)
-    keys, values = _rows16(keys), _rows16(values)
-    xst = (ctypes.c_int64 * 4)(*keys.stride()[:2], *values.stride()[:2])
-    kc, ks, vc, vs = cache
-    _lib.call("sparkq_paged_kv_append", _ptr(keys), _ptr(values), _ptr(kc), _ptr(ks), _ptr(vc),
-              _ptr(vs), _ptr(page_table), _ptr(starts), _ptr(lengths), keys.shape[0], b, hkv, d,
-              pages, width, page_table.stride(0), page, _lib.dtype_code(keys.dtype), xst, strides,
-              _lib.stream_handle(kc.device), device=kc.device)
+    if keys.get_device() != index or values.get_device() != index:
+        raise ValueError(f"{op}: keys and values must live on the cache's device")
+    b, width = _check_batch(op, index, page_table, starts, lengths)
+    strides = _strides(op, kc, ks, vc, vs)
+    (keys, kst), (values, vst) = _rows16(keys), _rows16(values)
+    _lib.launch("sparkq_paged_kv_append", index, keys.data_ptr(), values.data_ptr(), kc.data_ptr(),
+                ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), page_table.data_ptr(),
+                starts.data_ptr(), lengths.data_ptr(), keys.shape[0], b, hkv, d, pages, width,
+                page_table.stride(0), page, _CODE[dtype], _I64x4(kst[0], kst[1], vst[0], vst[1]),
+                strides)
 
 
 def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, max_new: int,
@@ -127,59 +134,67 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
     step). Rows that fall to no sequence, or to more than max_new of one, are
     left as they are in `out`, and hold anything in a new tensor."""
     op = "paged_quantized_sdpa"
-    pages, hkv, page, d = _check_cache(op, cache, 4)
-    if queries.ndim != 3 or queries.shape[2] != d or queries.shape[1] < 1 \
+    kc, ks, vc, vs, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
+    if queries.ndim != 3 or queries.shape[2] != d or not queries.shape[1] \
             or queries.shape[1] % hkv:
         raise ValueError(f"{op}: queries must be [T,Hq,{d}] with Hq divisible by {hkv}")
-    if queries.dtype not in _HALF:
+    t, heads, _ = shape = queries.shape
+    dtype = queries.dtype
+    if dtype not in _HALF:
         raise ValueError(f"{op} requires float16 or bfloat16 queries")
-    if mask not in (None, "causal"):
+    if queries.get_device() != index:
+        raise ValueError(f"{op}: queries must live on the cache's device")
+    if mask is not None and mask != "causal":
         raise ValueError(f"{op} takes mask=None or mask='causal'")
     if not isinstance(scale, (float, int)) or not math.isfinite(scale):
         raise ValueError("scale must be a finite Python number")
     if type(max_new) is not int or max_new < 1:
         raise ValueError(f"{op}: max_new must be a positive Python int")
-    out_dtype = queries.dtype if out_dtype is None else out_dtype
-    if out_dtype not in (queries.dtype, torch.float32):
+    out_dtype = dtype if out_dtype is None else out_dtype
+    if out_dtype is not dtype and out_dtype is not torch.float32:
         raise ValueError("out_dtype must be the query dtype or torch.float32")
-    b, width = _batch(op, cache, page_table, starts, lengths)
-    _check_device(op, cache, queries)
-    strides = _strides(cache)
-    t, heads = queries.shape[:2]
-    q = _rows16(queries)
-    y = _out_buffer(out, (t, heads, d), out_dtype, queries.device)
-    lib = _lib.lib()
-    need = lib.sparkq_paged_sdpa_workspace_bytes(t, b, heads, hkv, d, max_new, width * page)
-    ws = _lib.scratch(q.device, need)
-    qst = (ctypes.c_int64 * 2)(*q.stride()[:2])
-    kc, ks, vc, vs = cache
-    code = _lib.dtype_code
-    _lib.call("sparkq_paged_sdpa", _ptr(q), _ptr(kc), _ptr(ks), _ptr(vc), _ptr(vs),
-              _ptr(page_table), _ptr(starts), _ptr(lengths), _ptr(y), t, b, heads, hkv, d, pages,
-              width, page_table.stride(0), page, max_new, 1 if mask is not None else 0,
-              code(q.dtype), code(out_dtype), float(scale), qst, strides, _ptr(ws), need,
-              _lib.stream_handle(q.device), device=q.device)
-    return y
+    b, width = _check_batch(op, index, page_table, starts, lengths)
+    strides = _strides(op, kc, ks, vc, vs)
+    queries, qst = _rows16(queries)
+    dev = kc.device
+    out = torch.empty(shape, dtype=out_dtype, device=dev) if out is None \
+        else _out_buffer(out, shape, out_dtype, dev)
+    need = _lib.lib().sparkq_paged_sdpa_workspace_bytes(t, b, heads, hkv, d, max_new, width * page)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _lib.launch("sparkq_paged_sdpa", index, queries.data_ptr(), kc.data_ptr(), ks.data_ptr(),
+                vc.data_ptr(), vs.data_ptr(), page_table.data_ptr(), starts.data_ptr(),
+                lengths.data_ptr(), out.data_ptr(), t, b, heads, hkv, d, pages, width,
+                page_table.stride(0), page, max_new, 1 if mask is not None else 0, _CODE[dtype],
+                _CODE[out_dtype], scale, _I64x2(qst[0], qst[1]), strides, _ptr(ws), need)
+    return out
 
 
 def _pool(op, cache):
-    """(layers, pages, page_size, code and scale bytes of a page, strides) of a
-    pool [layers,pages,...] or of one layer [pages,...]."""
-    ndim = cache[0].ndim if len(cache) == 4 and isinstance(cache[0], torch.Tensor) else 0
-    pages, hkv, page, d = _check_cache(op, cache, 5 if ndim == 5 else 4)
-    kc, ks, vc, vs = cache
+    """(tensors in the C order, their GPU, layers, pages, page_size, bytes of a
+    page's codes and scales, strides) of a pool [layers,pages,...] or of one
+    layer [pages,...]."""
+    layered = len(cache) == 4 and getattr(cache[0], "ndim", 0) == 5
+    kc, ks, vc, vs, index, shape = _check_cache(op, cache, 5 if layered else 4)
+    pages, hkv, page, d = shape[-4:]
     st = []
-    for t in (kc, vc, ks, vs):
-        e, s = t.element_size(), t.stride()
-        inner = (page * d, d, 1) if t.dtype == torch.int8 else (page, 1)
-        if s[-len(inner):] != inner:
+    for t, inner, size in ((kc, (page * d, d, 1), 1), (vc, (page * d, d, 1), 1),
+                           (ks, (page, 1), 2), (vs, (page, 1), 2)):
+        s = t.stride()
+        k = len(inner)
+        if s[-k:] != inner:
             raise ValueError(f"{op}: a page must be contiguous in every tensor of the cache")
-        lead = s[:-len(inner)]
-        st += [lead[0] * e if ndim == 5 else 0, lead[-1] * e]
-    layers = kc.shape[0] if ndim == 5 else 1
-    if layers < 1:
-        raise ValueError(f"{op}: the pool has no layers")
-    return layers, pages, page, hkv * page * d, hkv * page * 2, (ctypes.c_int64 * 8)(*st)
+        st += (s[0] * size if layered else 0, s[-k - 1] * size)
+    return (kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr()), index, \
+        shape[0] if layered else 1, pages, page, hkv * page * d, hkv * page * 2, _I64x8(*st)
+
+
+def _check_rows(op, index, page_table, lengths):
+    if page_table.ndim != 2 or page_table.shape[1] < 1:
+        raise ValueError(f"{op}: expected page_table [B,M] and lengths [B]")
+    b, width = shape = page_table.shape
+    _check_ints(op, index, "page_table", page_table, shape)
+    _check_ints(op, index, "lengths", lengths, (b,))
+    return b, width
 
 
 def kv_pages_fork(cache, page_table, lengths, parents=None, new_tokens=None):
@@ -197,29 +212,24 @@ def kv_pages_fork(cache, page_table, lengths, parents=None, new_tokens=None):
     their entries are -1 and nothing was copied, so the old table and lengths
     still stand."""
     op = "kv_pages_fork"
-    layers, pages, page, cb, sb, st = _pool(op, cache)
-    if page_table.ndim != 2 or page_table.shape[1] < 1 or lengths.ndim != 1:
-        raise ValueError(f"{op}: expected page_table [B,M] and lengths [B]")
-    b, width = page_table.shape
-    rows = b if parents is None else parents.shape[0] if parents.ndim == 1 else -1
-    checks = {"page_table": (page_table, (b, width)), "lengths": (lengths, (b,))}
+    bufs, index, layers, pages, page, cb, sb, st = _pool(op, cache)
+    b, width = _check_rows(op, index, page_table, lengths)
+    rows = b
     if parents is not None:
-        checks["parents"] = (parents, (rows,))
+        rows = parents.shape[0] if parents.ndim == 1 else -1
+        _check_ints(op, index, "parents", parents, (rows,))
     if new_tokens is not None:
-        checks["new_tokens"] = (new_tokens, (rows,))
-    kc, ks, vc, vs = cache
-    dev = kc.device
-    _check_ints(op, dev, **checks)
-    _check_device(op, cache)
+        _check_ints(op, index, "new_tokens", new_tokens, (rows,))
+    dev = page_table.device
     table = torch.empty((rows, width), dtype=torch.int32, device=dev)
-    after = torch.empty((rows,), dtype=torch.int32, device=dev)
-    missing = torch.empty((1,), dtype=torch.int32, device=dev)
+    after = torch.empty(rows, dtype=torch.int32, device=dev)
+    missing = torch.empty(1, dtype=torch.int32, device=dev)
     need = _lib.lib().sparkq_kv_pages_workspace_bytes(rows, pages)
-    ws = _lib.scratch(dev, need)
-    _lib.call("sparkq_kv_pages_fork", _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), _ptr(page_table),
-              _ptr(lengths), _ptr(parents), _ptr(new_tokens), page_table.stride(0), _ptr(table),
-              _ptr(after), _ptr(missing), st, b, rows, width, pages, layers, page, cb, sb,
-              _ptr(ws), need, _lib.stream_handle(dev), device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.launch("sparkq_kv_pages_fork", index, *bufs, page_table.data_ptr(), lengths.data_ptr(),
+                _ptr(parents), _ptr(new_tokens), page_table.stride(0), table.data_ptr(),
+                after.data_ptr(), missing.data_ptr(), st, b, rows, width, pages, layers, page, cb,
+                sb, ws.data_ptr(), need)
     return table, after, missing
 
 
@@ -228,21 +238,16 @@ def kv_pages_compact(cache, page_table, lengths):
     of them, those numbered U or higher go, in order, to the free numbers below
     U. Returns (page_table [B,M], used [1] = U)."""
     op = "kv_pages_compact"
-    layers, pages, page, cb, sb, st = _pool(op, cache)
-    if page_table.ndim != 2 or page_table.shape[1] < 1 or lengths.ndim != 1:
-        raise ValueError(f"{op}: expected page_table [B,M] and lengths [B]")
-    b, width = page_table.shape
-    kc, ks, vc, vs = cache
-    dev = kc.device
-    _check_ints(op, dev, page_table=(page_table, (b, width)), lengths=(lengths, (b,)))
-    _check_device(op, cache)
+    bufs, index, layers, pages, page, cb, sb, st = _pool(op, cache)
+    b, width = _check_rows(op, index, page_table, lengths)
+    dev = page_table.device
     table = torch.empty((b, width), dtype=torch.int32, device=dev)
-    used = torch.empty((1,), dtype=torch.int32, device=dev)
+    used = torch.empty(1, dtype=torch.int32, device=dev)
     need = _lib.lib().sparkq_kv_pages_workspace_bytes(b, pages)
-    ws = _lib.scratch(dev, need)
-    _lib.call("sparkq_kv_pages_compact", _ptr(kc), _ptr(vc), _ptr(ks), _ptr(vs), _ptr(page_table),
-              _ptr(lengths), page_table.stride(0), _ptr(table), _ptr(used), st, b, width, pages,
-              layers, page, cb, sb, _ptr(ws), need, _lib.stream_handle(dev), device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _lib.launch("sparkq_kv_pages_compact", index, *bufs, page_table.data_ptr(), lengths.data_ptr(),
+                page_table.stride(0), table.data_ptr(), used.data_ptr(), st, b, width, pages,
+                layers, page, cb, sb, ws.data_ptr(), need)
     return table, used
 
 

@@ -132,7 +132,8 @@ def _moved(cpu, pairs):
 @pytest.mark.parametrize("seed,b,page,width,pages,most", [
     (0, 1, 16, 1, 2, 16), (1, 8, 32, 6, 60, 100), (2, 50, 16, 12, 300, 150),
     (3, 7, 64, 3, 20, 192), (4, 300, 16, 4, 700, 60), (5, 1300, 16, 2, 1500, 30),
-    (6, 20, 128, 4, 2500, 500)])
+    (6, 20, 128, 4, 2500, 500),
+    (7, 40, 16, 3, 16384, 40), (8, 40, 16, 90, 17000, 1400)])
 @pytest.mark.parametrize("reorder", [False, True])
 def test_fork(gpu, seed, b, page, width, pages, most, reorder):
     import sparkq
@@ -173,7 +174,8 @@ def test_fork_short_of_pages_changes_nothing(gpu):
 
 @pytest.mark.parametrize("seed,b,page,width,pages,most", [
     (0, 1, 16, 1, 2, 16), (1, 8, 32, 6, 60, 100), (2, 50, 16, 12, 500, 150),
-    (3, 0, 16, 2, 5, 0), (4, 300, 16, 4, 3000, 60), (5, 5, 1024, 2, 30, 2000)])
+    (3, 0, 16, 2, 5, 0), (4, 300, 16, 4, 3000, 60), (5, 5, 1024, 2, 30, 2000),
+    (6, 1100, 16, 3, 16384, 40), (7, 40, 16, 90, 17000, 1400)])
 def test_compact(gpu, seed, b, page, width, pages, most):
     import sparkq
 
