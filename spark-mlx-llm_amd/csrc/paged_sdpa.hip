@@ -84,39 +84,42 @@ __device__ __forceinline__ SeqWork seq_work(const PagedSdpaArgs& a, int b) {
   return w;
 }
 
-__device__ __forceinline__ int wave_prefix(int v, int lane) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(v, o);
-    if (lane >= o) v += y;
-  }
+// inclusive prefix over the wave's lanes: row shifts, then the rows' totals
+__device__ __forceinline__ int wave_prefix(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
   return v;
 }
 
 // Item x of the batch's items in order (SPLIT false: every tile and part), or
 // tile x of those whose context is split. A context of n tokens is split into
-// ceil(n / C) parts, C = max(min_part, ceil(all tiles' tokens / target)): fewer
+// ceil(n / C) parts, C = max(min_part, W / target + 1), W all tiles' tokens: fewer
 // than `target` contexts are longer than C, and these have fewer than 2 target
-// parts together. All lanes of a wave take part and get the same answer.
+// parts together. (W is summed in fp32, to 2^-17 of itself, which C is enlarged
+// by.) All lanes of a wave take part, and every wave gets the same answers.
 template <int R, bool SPLIT>
 __device__ Item find_item(const PagedSdpaArgs& a, int x) {
   const int lane = threadIdx.x & 63;
-  long long all = 0;
-  for (int b0 = 0; b0 < a.p.B; b0 += 64) {
+  const SeqWork w0 = seq_work<R>(a, lane);
+  float all = (float)w0.tiles * (float)w0.length;
+  for (int b0 = 64; b0 < a.p.B; b0 += 64) {
     const SeqWork w = seq_work<R>(a, b0 + lane);
-    all += (long long)w.tiles * w.length;
+    all = fmaf((float)w.tiles, (float)w.length, all);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o);
-  const int C = (int)min(max((all + a.target - 1) / a.target, (long long)a.min_part), 0x7FFFFFFFll);
+  const float share = wave_sum(all) / (float)a.target;
+  const int C = (int)fminf(fmaxf(share + share * 0x1p-16f + 1.0f, (float)a.min_part), 0x1p30f);
   Item it{-1, 0, 0, 1, 0, 0, 0, 0, 0};
   int items = 0, slots = 0;
   for (int b0 = 0; b0 < a.p.B; b0 += 64) {
-    const SeqWork w = seq_work<R>(a, b0 + lane);
+    const SeqWork w = b0 == 0 ? w0 : seq_work<R>(a, b0 + lane);
     const int parts = w.length > C ? (w.length - 1) / C + 1 : 1;
     const int own = SPLIT ? (parts > 1 ? w.tiles : 0) : w.tiles * parts;
     const int used = parts > 1 ? w.tiles * parts : 0;
-    const int end = items + wave_prefix(own, lane), slot_end = slots + wave_prefix(used, lane);
+    const int end = items + wave_prefix(own), slot_end = slots + wave_prefix(used);
     const unsigned long long hit = __ballot(x < end);
     if (hit) {
       const int l = __builtin_ctzll(hit);
@@ -365,7 +368,7 @@ struct FewLds {
 };
 
 template <int D>
-__global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedSdpaArgs a) {
+__global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedSdpaArgs a) {
   constexpr int NK = D / 32, PL = D / 64, NJ = D / 16, VL = D / 32;
   using L = FewLds<D>;
   __shared__ __attribute__((aligned(16))) unsigned char smem[L::BYTES];
@@ -391,13 +394,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedS
   // chunk c: dims 16 (g + 4 (c / 2)) + 8 (c % 2), as the 16-byte pieces of K lie
   const float mul = load_query<NK>(a, qrow, true, [&](int c) { return 16 * (grp + 4 * (c >> 1)) + 8 * (c & 1); }, qb);
 
-  u32x4_t kr[2][2][PL], vr[2][VL], skr[2], svr[2];
-  BlockPages<2> pg[2], next;
+  u32x4_t kr[2][PL], vr[VL], skr, svr;
+  BlockPages<2> next;
+  uint32_t pages_ok;
   const int ktok = 8 * (n16 >> 2) + (n16 & 3);
   const int slot_mask = (1 << a.p.page_log2) - 1;
   const int last = ib1 - 1;
   // block ib (no further than the last) through the pages found for it
-  auto load = [&](int set, int ib, const BlockPages<2>& bp) {
+  auto load = [&](int ib, const BlockPages<2>& bp) {
     const int t0 = kBlock * min(ib, last);
     const int s0 = t0 & slot_mask, s1 = (t0 + 16) & slot_mask;
     auto base = [&](const PagedSide& s, int h) {
@@ -409,20 +413,20 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedS
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < PL; ++i)
-        kr[set][t][i] = *reinterpret_cast<const u32x4_t*>(kp + 4 * t * a.ks.c_tok + 16 * (grp + 4 * i));
+        kr[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kp + 4 * t * a.ks.c_tok + 16 * (grp + 4 * i)));
 #pragma unroll
     for (int v = 0; v < VL; ++v) {
       const int f = lane + 64 * v, tok = f / (D / 16), pc = f % (D / 16);
-      vr[set][v] = *reinterpret_cast<const u32x4_t*>((2 * v >= VL ? v1 : v0) + (tok & 15) * a.vs.c_tok + 16 * pc);
+      vr[v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>((2 * v >= VL ? v1 : v0) + (tok & 15) * a.vs.c_tok + 16 * pc));
     }
     auto scales = [&](const PagedSide& s) {
       const int h = grp >> 1;
       const uint16_t* p = s.scales + (h ? bp.id[1] : bp.id[0]) * s.s_page + kh * s.s_head + (h ? s1 : s0) + 8 * (grp & 1);
       return *reinterpret_cast<const u32x4_t*>(p);
     };
-    skr[set] = scales(a.ks);
-    svr[set] = scales(a.vs);
-    pg[set] = bp;
+    skr = scales(a.ks);
+    svr = scales(a.vs);
+    pages_ok = bp.ok;
   };
 
   RowState st;
@@ -430,13 +434,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedS
 #pragma unroll
   for (int j = 0; j < NJ; ++j) acc[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-  auto block = [&](int ib, auto setc) {
-    constexpr int set = decltype(setc)::value;
+  auto block = [&](int ib) {
     const int t0 = kBlock * ib;
 #pragma unroll
     for (int v = 0; v < VL; ++v) {
       const int f = lane + 64 * v, tok = f / (D / 16), pc = f % (D / 16);
-      *reinterpret_cast<u32x4_t*>(vtile + tok * L::VROW + 16 * pc) = vr[set][v];
+      *reinterpret_cast<u32x4_t*>(vtile + tok * L::VROW + 16 * pc) = vr[v];
     }
     f32x4_t sc[2];
 #pragma unroll
@@ -444,23 +447,23 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedS
       sc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int c = 0; c < NK; ++c) {
-        const u32x4_t kp = kr[set][t][c >> 1];
+        const u32x4_t kp = kr[t][c >> 1];
         sc[t] = mfma16x16x32_f16((c & 1) ? s8x8_exact(kp.z, kp.w) : s8x8_exact(kp.x, kp.y), qb[c], sc[t]);
       }
     }
     float s[8], vsc[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t kw = skr[set][i >> 1], vw = svr[set][i >> 1];
+      const uint32_t kw = skr[i >> 1], vw = svr[i >> 1];
       s[i] = sc[i >> 2][i & 3] * (((i & 1) ? hi16<F16>(kw) : lo16<F16>(kw)) * a.scale_log2);
       vsc[i] = (i & 1) ? hi16<F16>(vw) : lo16<F16>(vw);
     }
     uint32_t ok = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ok |= (uint32_t)(t0 + 8 * grp + i <= lim) << i;
-    if (!((pg[set].ok >> (grp >> 1)) & 1u)) ok = 0;
-    load(set, ib + 8, next);
-    next = block_pages<2>(a, trow, kBlock * min(ib + 12, last));
+    if (!((pages_ok >> (grp >> 1)) & 1u)) ok = 0;
+    load(ib + 4, next);
+    next = block_pages<2>(a, trow, kBlock * min(ib + 8, last));
     u32x4_t w;
     bool up;
     float size = 0.0f;
@@ -490,14 +493,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 2 : 1) void paged_few_kernel(PagedS
 
   int ib = ib0 + wave;
   if (ib < ib1) {
-    load(0, ib, block_pages<2>(a, trow, kBlock * ib));
-    load(1, ib + 4, block_pages<2>(a, trow, kBlock * min(ib + 4, last)));
-    next = block_pages<2>(a, trow, kBlock * min(ib + 8, last));
-    for (; ib + 4 < ib1; ib += 8) {
-      block(ib, std::integral_constant<int, 0>{});
-      block(ib + 4, std::integral_constant<int, 1>{});
-    }
-    if (ib < ib1) block(ib, std::integral_constant<int, 0>{});
+    load(ib, block_pages<2>(a, trow, kBlock * ib));
+    next = block_pages<2>(a, trow, kBlock * min(ib + 4, last));
+    for (; ib < ib1; ib += 4) block(ib);
   }
 
   // combine the waves
