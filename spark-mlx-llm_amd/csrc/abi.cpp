@@ -989,6 +989,11 @@ int sparkq_paged_sdpa(const void* q, const void* k_codes, const void* k_scales, 
                       "multiples of 8 scales apart");
   REQUIRE_SUPPORTED(aligned(k_scales, 16) && aligned(v_scales, 16),
                     "paged_sdpa: scales must be 16-byte aligned");
+  for (int i = 0; i < 12; i += 6)
+    REQUIRE_SUPPORTED(strides[i] / 16 <= kI32Max && strides[i + 3] / 8 <= kI32Max &&
+                          strides[i + 2] <= kI32Max / page_size,
+                      "paged_sdpa: pages must be less than 32 GiB apart and a head's tokens span less "
+                      "than 2 GiB");
   REQUIRE((T == 0 || (q && out)) && q_strides && starts && (B == 0 || (page_table && lengths)),
           "paged_sdpa: null tensor pointer");
   REQUIRE(is_half_dtype(q_dtype), "paged_sdpa requires float16 or bfloat16 queries");

@@ -39,11 +39,21 @@
 namespace sparkq {
 namespace {
 
+// One side of the cache as the attention addresses it: the page stride in units
+// of 16 bytes (codes) and 8 scales, so that a page's address is one 32-bit
+// product, and a page's own extent in 32 bits.
+struct CodeSide {
+  const uint8_t* codes;
+  const uint16_t* scales;
+  int64_t c_head, s_head;
+  uint32_t c_page, s_page, c_tok;
+};
+
 struct PagedSdpaArgs {
   PagedBatch p;
   const uint16_t* q;
   int64_t q_tok, q_head;  // elements
-  PagedSide ks, vs;
+  CodeSide ks, vs;
   void* out;  // [T, Hq, D]
   float *pm, *pz, *pacc;  // [Hkv][slots][rows], [...], [...][D]: parts of split contexts
   int Hq, Hkv, max_new, causal, q_dtype, out_dtype;
@@ -95,6 +105,19 @@ __device__ __forceinline__ int wave_prefix(int v) {
   return v;
 }
 
+// Reorders the sequences of up to 64 lanes, the longest first: a batch's short
+// tiles come last and fill the gaps that the long ones leave.
+__device__ __forceinline__ void longest_first(SeqWork& w, int& b, int n) {
+  const int lane = threadIdx.x & 63, key = w.tiles ? w.length : -1;
+  int rank = 0;
+  for (int j = 0; j < n; ++j) {
+    const int k = __builtin_amdgcn_readlane(key, j);
+    rank += k > key || (k == key && j < lane);
+  }
+  const int to = 4 * (lane < n ? rank : lane);
+  for (int* f : {&w.first, &w.count, &w.length, &w.rows, &w.tiles, &b}) *f = __builtin_amdgcn_ds_permute(to, *f);
+}
+
 // Item x of the batch's items in order (SPLIT false: every tile and part), or
 // tile x of those whose context is split. A context of n tokens is split into
 // ceil(n / C) parts, C = max(min_part, W / target + 1), W all tiles' tokens: fewer
@@ -104,7 +127,9 @@ __device__ __forceinline__ int wave_prefix(int v) {
 template <int R, bool SPLIT>
 __device__ Item find_item(const PagedSdpaArgs& a, int x) {
   const int lane = threadIdx.x & 63;
-  const SeqWork w0 = seq_work<R>(a, lane);
+  int b_of = lane;
+  SeqWork w0 = seq_work<R>(a, lane);
+  if (R == 128 && a.p.B > 1 && a.p.B <= 64) longest_first(w0, b_of, a.p.B);
   float all = (float)w0.tiles * (float)w0.length;
   for (int b0 = 64; b0 < a.p.B; b0 += 64) {
     const SeqWork w = seq_work<R>(a, b0 + lane);
@@ -124,7 +149,7 @@ __device__ Item find_item(const PagedSdpaArgs& a, int x) {
     if (hit) {
       const int l = __builtin_ctzll(hit);
       auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-      it.b = b0 + l;
+      it.b = b0 + of(b_of);
       it.first = of(w.first);
       it.count = of(w.count);
       it.length = of(w.length);
@@ -320,6 +345,14 @@ __device__ __forceinline__ int64_t out_row(const PagedSdpaArgs& a, const Item& i
   return ((int64_t)(it.first + rr / gqa) * a.Hq + kh * gqa + rr % gqa);
 }
 
+// This KV head's codes and scales of a page: run `slot` / 16 of it
+__device__ __forceinline__ const uint8_t* code_run(const uint8_t* head, const CodeSide& s, int id, int slot) {
+  return head + (((uint64_t)(uint32_t)id * s.c_page << 4) + (uint32_t)slot * s.c_tok);
+}
+__device__ __forceinline__ const uint16_t* scale_run(const uint16_t* head, const CodeSide& s, int id, int slot) {
+  return head + (((uint64_t)(uint32_t)id * s.s_page << 3) + (uint32_t)slot);
+}
+
 // Pages of a block's Q runs of 16 tokens; a run without one reads page 0 and is
 // hidden (ok). Past the table's row the last entry stands in (those tokens lie
 // past every length).
@@ -339,13 +372,24 @@ __device__ __forceinline__ TableRow table_row(const PagedSdpaArgs& a, int b) {
 template <int Q>
 __device__ __forceinline__ BlockPages<Q> block_pages(const PagedSdpaArgs& a, TableRow row, int t0) {
   BlockPages<Q> r;
-  r.ok = 0;
-#pragma unroll
-  for (int h = 0; h < Q; ++h) {
+  auto look = [&](int h) {
     const int id = row[min((t0 + 16 * h) >> a.p.page_log2, a.p.width - 1)];
+    return id;
+  };
+  auto keep = [&](int h, int id) {
     const bool in = (unsigned)id < (unsigned)a.p.pages;
     r.ok |= (uint32_t)in << h;
     r.id[h] = in ? id : 0;
+  };
+  r.ok = 0;
+  if ((1 << a.p.page_log2) >= 16 * Q) {  // blocks do not straddle pages
+    keep(0, look(0));
+#pragma unroll
+    for (int h = 1; h < Q; ++h) r.id[h] = r.id[0];
+    r.ok = r.ok ? (1u << Q) - 1 : 0;
+  } else {
+#pragma unroll
+    for (int h = 0; h < Q; ++h) keep(h, look(h));
   }
   return r;
 }
@@ -398,34 +442,31 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
   BlockPages<2> next;
   uint32_t pages_ok;
   const int ktok = 8 * (n16 >> 2) + (n16 & 3);
+  const uint32_t koff = (ktok & 15) * a.ks.c_tok + 16 * grp;
+  const uint8_t *const khead = a.ks.codes + kh * a.ks.c_head, *const vhead = a.vs.codes + kh * a.vs.c_head;
+  const uint16_t *const kshead = a.ks.scales + kh * a.ks.s_head, *const vshead = a.vs.scales + kh * a.vs.s_head;
   const int slot_mask = (1 << a.p.page_log2) - 1;
   const int last = ib1 - 1;
   // block ib (no further than the last) through the pages found for it
   auto load = [&](int ib, const BlockPages<2>& bp) {
     const int t0 = kBlock * min(ib, last);
     const int s0 = t0 & slot_mask, s1 = (t0 + 16) & slot_mask;
-    auto base = [&](const PagedSide& s, int h) {
-      return s.codes + bp.id[h] * s.c_page + kh * s.c_head + (h ? s1 : s0) * s.c_tok;
-    };
-    const uint8_t *k0 = base(a.ks, 0), *k1 = base(a.ks, 1), *v0 = base(a.vs, 0), *v1 = base(a.vs, 1);
-    const uint8_t* kp = (n16 < 8 ? k0 : k1) + (ktok & 15) * a.ks.c_tok;
+    const uint8_t* kp = (n16 < 8 ? code_run(khead, a.ks, bp.id[0], s0) : code_run(khead, a.ks, bp.id[1], s1)) + koff;
+    const uint8_t *v0 = code_run(vhead, a.vs, bp.id[0], s0), *v1 = code_run(vhead, a.vs, bp.id[1], s1);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < PL; ++i)
-        kr[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kp + 4 * t * a.ks.c_tok + 16 * (grp + 4 * i)));
+        kr[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kp + (4 * t * a.ks.c_tok + 64 * i)));
 #pragma unroll
     for (int v = 0; v < VL; ++v) {
       const int f = lane + 64 * v, tok = f / (D / 16), pc = f % (D / 16);
-      vr[v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>((2 * v >= VL ? v1 : v0) + (tok & 15) * a.vs.c_tok + 16 * pc));
+      vr[v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>((2 * v >= VL ? v1 : v0) + ((tok & 15) * a.vs.c_tok + 16 * pc)));
     }
-    auto scales = [&](const PagedSide& s) {
-      const int h = grp >> 1;
-      const uint16_t* p = s.scales + (h ? bp.id[1] : bp.id[0]) * s.s_page + kh * s.s_head + (h ? s1 : s0) + 8 * (grp & 1);
-      return *reinterpret_cast<const u32x4_t*>(p);
-    };
-    skr = scales(a.ks);
-    svr = scales(a.vs);
+    const bool h = grp >= 2;
+    const int id = h ? bp.id[1] : bp.id[0], run = (h ? s1 : s0) + 8 * (grp & 1);
+    skr = *reinterpret_cast<const u32x4_t*>(scale_run(kshead, a.ks, id, run));
+    svr = *reinterpret_cast<const u32x4_t*>(scale_run(vshead, a.vs, id, run));
     pages_ok = bp.ok;
   };
 
@@ -547,18 +588,24 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
 // ---------------------------------------------------------------------------
 // The products run as above with 2 x 16 rows a wave; the lane with a row's
 // scores of tokens 16 t + 4 g + r holds those k-slots. A block of codes is read
-// once by the workgroup and written to LDS as fp16, K token-major with its
-// 16-byte chunks XOR-swizzled by the token, V token-major with its 32-byte runs
-// swizzled (read transposed), two buffers deep: the next block's codes are
-// converted while this one is computed, and the one after is in flight.
+// once by the workgroup and written to LDS as fp16, token-major, two buffers deep:
+// the next block's codes are converted while this one is computed, and the one
+// after is in flight. V is read transposed.
 //
 // A wave takes 32 rows up to D = 128, where the products' operands and sums fit
 // 256 registers and two workgroups a CU; at 256 eight waves take 16 each, or
 // there would be one wave a SIMD with nothing to hide its waits.
 constexpr int tile_waves(int D) { return D <= 128 ? 4 : 8; }
+//
+// K rows are as long as all banks: the 16-byte chunks of token t are XOR-swizzled
+// by t, so that any 16 lanes of a read that the LDS takes together (16 tokens, or
+// 4 tokens of each lane group) hit different banks. V rows are padded by 32 bytes,
+// which does the same for the transposed reads.
+template <int D>
+__device__ __forceinline__ int kswz(int t) { return D >= 128 ? (t & 15) : ((t >> 1) & 7); }
 template <int D>
 struct TileLds {
-  static constexpr int KROW = 2 * D + 16, VROW = 2 * D + 32;  // padded: no two lanes of a read share banks
+  static constexpr int KROW = 2 * D, VROW = 2 * D + 32;
   static constexpr int V = kTileBlock * KROW;
   static constexpr int SCALES = V + kTileBlock * VROW;        // of keys, of values, the largest of each 16 of these
   static constexpr int BUF = SCALES + 2 * kTileBlock * 4 + 16;
@@ -597,6 +644,7 @@ __global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_ti
     const uint16_t* qrow = a.q + (it.first + rq / gqa) * a.q_tok + (kh * gqa + rq % gqa) * a.q_head;
     mul[rt] = load_query<NK>(a, qrow, rr < it.rows, [&](int c) { return 32 * c + 8 * grp; }, qb[rt]);
   }
+  const int wr0 = rw0 + 16 * RT * wave;  // the wave's first row
   // what every row of the tile sees
   const int all = __builtin_amdgcn_readfirstlane(last_seen(a, it, rw0, gqa) + 1);
 
@@ -608,39 +656,39 @@ __global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_ti
   // 16)). All tokens of a wave's i-th piece lie in one run of 16, and so in one
   // page: its address is a scalar plus the lane's offset. Wave w < Q also takes
   // the scales of run w: keys in its first 16 lanes, values in the next.
-  const uint32_t koff = (uint32_t)((tid / (D / 16)) & 15) * (uint32_t)a.ks.c_tok + 16 * (tid % (D / 16));
-  const uint32_t voff = (uint32_t)((tid / (D / 16)) & 15) * (uint32_t)a.vs.c_tok + 16 * (tid % (D / 16));
+  const uint8_t *const khead = a.ks.codes + kh * a.ks.c_head, *const vhead = a.vs.codes + kh * a.vs.c_head;
+  const uint16_t *const kshead = a.ks.scales + kh * a.ks.s_head, *const vshead = a.vs.scales + kh * a.vs.s_head;
+  const uint32_t koff = ((tid / (D / 16)) & 15) * a.ks.c_tok + 16 * (tid % (D / 16));
+  const uint32_t voff = ((tid / (D / 16)) & 15) * a.vs.c_tok + 16 * (tid % (D / 16));
   auto page_id = [&](const BlockPages<Q>& bp, int run) {
-    return (int64_t)(run == 0 ? bp.id[0] : Q == 2 || run == 1 ? bp.id[1] : run == 2 ? bp.id[Q - 2] : bp.id[Q - 1]);
+    return (run == 0 ? bp.id[0] : Q == 2 || run == 1 ? bp.id[1] : run == 2 ? bp.id[Q - 2] : bp.id[Q - 1]);
   };
   auto load = [&](int ib, const BlockPages<Q>& bp) {
     const int t0 = kBlock * min(ib, last);
 #pragma unroll
     for (int i = 0; i < PPT; ++i) {
       const int run = wave * 64 / D + i * (64 * NW / D);
-      const int64_t id = page_id(bp, run), slot = (t0 + 16 * run) & slot_mask;
-      const uint8_t* kp = a.ks.codes + (id * a.ks.c_page + kh * a.ks.c_head + slot * a.ks.c_tok);
-      const uint8_t* vp = a.vs.codes + (id * a.vs.c_page + kh * a.vs.c_head + slot * a.vs.c_tok);
-      kcr[i] = *reinterpret_cast<const u32x4_t*>(kp + koff);
-      vcr[i] = *reinterpret_cast<const u32x4_t*>(vp + voff);
+      const int id = page_id(bp, run), slot = (t0 + 16 * run) & slot_mask;
+      kcr[i] = *reinterpret_cast<const u32x4_t*>(code_run(khead, a.ks, id, slot) + koff);
+      vcr[i] = *reinterpret_cast<const u32x4_t*>(code_run(vhead, a.vs, id, slot) + voff);
     }
     if (wave < Q) {
-      const int64_t id = page_id(bp, wave), slot = (t0 + 16 * wave) & slot_mask;
-      const uint16_t* kp = a.ks.scales + (id * a.ks.s_page + kh * a.ks.s_head + slot);
-      const uint16_t* vp = a.vs.scales + (id * a.vs.s_page + kh * a.vs.s_head + slot);
+      const int id = page_id(bp, wave), slot = (t0 + 16 * wave) & slot_mask;
+      const uint16_t *kp = scale_run(kshead, a.ks, id, slot), *vp = scale_run(vshead, a.vs, id, slot);
       sr = (lane < 16 ? kp : vp)[n16];
     }
   };
   const int tk0 = tid / (D / 16), jb = tid % (D / 16);
-  unsigned char* const kput = smem + tk0 * L::KROW + 32 * jb;
+  constexpr int TPP = 64 * NW / (D / 16);  // tokens of a round of pieces: whole swizzle periods
+  unsigned char* const kput0 = smem + tk0 * L::KROW + 16 * ((2 * jb) ^ kswz<D>(tk0));
+  unsigned char* const kput1 = smem + tk0 * L::KROW + 16 * ((2 * jb + 1) ^ kswz<D>(tk0));
   unsigned char* const vput = smem + L::V + tk0 * L::VROW + 32 * jb;
   auto stage = [&](auto bufc) {
-    constexpr int at = decltype(bufc)::value * L::BUF, TPP = 64 * NW / (D / 16);  // tokens of a round of pieces
+    constexpr int at = decltype(bufc)::value * L::BUF;
 #pragma unroll
     for (int i = 0; i < PPT; ++i) {
-      unsigned char* kt = kput + at + i * TPP * L::KROW;
-      *reinterpret_cast<u32x4_t*>(kt) = s8x8_exact(kcr[i].x, kcr[i].y);
-      *reinterpret_cast<u32x4_t*>(kt + 16) = s8x8_exact(kcr[i].z, kcr[i].w);
+      *reinterpret_cast<u32x4_t*>(kput0 + at + i * TPP * L::KROW) = s8x8_exact(kcr[i].x, kcr[i].y);
+      *reinterpret_cast<u32x4_t*>(kput1 + at + i * TPP * L::KROW) = s8x8_exact(kcr[i].z, kcr[i].w);
       unsigned char* vt = vput + at + i * TPP * L::VROW;
       *reinterpret_cast<u32x4_t*>(vt) = s8x8_exact(vcr[i].x, vcr[i].y);
       *reinterpret_cast<u32x4_t*>(vt + 16) = s8x8_exact(vcr[i].z, vcr[i].w);
@@ -654,7 +702,9 @@ __global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_ti
     }
   };
 
-  const unsigned char* const kget = smem + n16 * L::KROW + 16 * grp;
+  const unsigned char* kget[4];  // chunk 4 kk + g of token n16: kk and kk + 4 are 256 bytes apart
+#pragma unroll
+  for (int kk = 0; kk < 4 && kk < NK; ++kk) kget[kk] = smem + n16 * L::KROW + 16 * ((4 * kk + grp) ^ kswz<D>(n16));
   const unsigned char* const vget = smem + L::V + (4 * grp + (n16 >> 2)) * L::VROW + 8 * (n16 & 3);
   const float* const sget = reinterpret_cast<const float*>(smem + L::SCALES) + 4 * grp;
   RowState st[RT];
@@ -676,7 +726,7 @@ __global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_ti
     for (int tt = 0; tt < Q; ++tt)
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) {
-        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kget + at + tt * 16 * L::KROW + 64 * kk);
+        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kget[kk % 4] + at + tt * 16 * L::KROW + 256 * (kk / 4));
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) sc[tt][rt] = mfma16x16x32_f16(kf, qb[rt][kk], sc[tt][rt]);
       }
@@ -747,7 +797,7 @@ __global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_ti
     __syncthreads();
     auto step = [&](int ib, auto cur) {
       const BlockPages<Q> after = block_pages<Q>(a, trow, kBlock * min(ib + 2, last));
-      compute(cur, kBlock * ib, ok_now);
+      if (wr0 < it.rows) compute(cur, kBlock * ib, ok_now);
       stage(std::integral_constant<int, 1 - decltype(cur)::value>{});
       load(ib + 2, after);
       ok_now = ok_next;
@@ -759,7 +809,7 @@ __global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_ti
       step(ib, std::integral_constant<int, 0>{});
       step(ib + 1, std::integral_constant<int, 1>{});
     }
-    if (ib < ib1) compute(std::integral_constant<int, 0>{}, kBlock * ib, ok_now);
+    if (ib < ib1 && wr0 < it.rows) compute(std::integral_constant<int, 0>{}, kBlock * ib, ok_now);
   }
 
 #pragma unroll
@@ -917,7 +967,10 @@ int paged_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, const Pag
   if (!aligned(ws, 16)) return set_error(SPARKQ_ERR_INVALID, "paged_sdpa: workspace must be 16-byte aligned");
   const int64_t n = Hkv * plan.slots * plan.rows;
   float* acc = (float*)ws;
-  const PagedSdpaArgs a{p, (const uint16_t*)q, qst[0], qst[1], ks, vs, out, acc + n * D, acc + n * (D + 1), acc,
+  const auto side = [](const PagedSide& s) {
+    return CodeSide{s.codes, s.scales, s.c_head, s.s_head, (uint32_t)(s.c_page / 16), (uint32_t)(s.s_page / 8), (uint32_t)s.c_tok};
+  };
+  const PagedSdpaArgs a{p, (const uint16_t*)q, qst[0], qst[1], side(ks), side(vs), out, acc + n * D, acc + n * (D + 1), acc,
                         (int)Hq, (int)Hkv, (int)std::min<int64_t>(max_new, p.T), causal, qdt, odt,
                         (int)plan.target, (int)plan.slots, plan.min_part, scale * 1.44269504088896340736f};
   if (D == 64)
