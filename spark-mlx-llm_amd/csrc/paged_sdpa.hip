@@ -12,8 +12,8 @@
 //   paged_few_kernel   at most 16 of them (decode, a few drafted tokens): the
 //                      waves of a workgroup take turns at 32-token blocks and
 //                      combine at the end.
-//   paged_tile_kernel  tiles of 128 rows, 32 a wave: a block is turned to fp16
-//                      in LDS once for all of them.
+//   paged_tile_kernel  tiles of 128 rows (64 at D = 256): a block is turned to
+//                      fp16 in LDS once for all of them.
 //   paged_merge_kernel joins the parts of a context that was split.
 //
 // Work. The lengths live on the device, so every workgroup works out from the
@@ -63,7 +63,9 @@ struct PagedSdpaArgs {
   float scale_log2;
 };
 
-constexpr int kFewBlock = 32, kTileBlock = 64;  // tokens of a block
+constexpr int kFewBlock = 32;  // tokens of a block
+constexpr int tile_block(int D) { return D <= 128 ? 64 : 32; }
+constexpr int tile_rows(int D) { return D <= 128 ? 128 : 64; }
 
 // ---------------------------------------------------------------------------
 // which work is whose
@@ -80,7 +82,7 @@ struct SeqWork {
   int first, count, length, rows, tiles;
 };
 
-template <int R>  // rows of a tile: 16 or 128
+template <int R>  // rows of a tile: 16, 64 or 128
 __device__ __forceinline__ SeqWork seq_work(const PagedSdpaArgs& a, int b) {
   SeqWork w{0, 0, 0, 0, 0};
   if (b < a.p.B) {
@@ -129,7 +131,7 @@ __device__ Item find_item(const PagedSdpaArgs& a, int x) {
   const int lane = threadIdx.x & 63;
   int b_of = lane;
   SeqWork w0 = seq_work<R>(a, lane);
-  if (R == 128 && a.p.B > 1 && a.p.B <= 64) longest_first(w0, b_of, a.p.B);
+  if (R > 16 && a.p.B > 1 && a.p.B <= 64) longest_first(w0, b_of, a.p.B);
   float all = (float)w0.tiles * (float)w0.length;
   for (int b0 = 64; b0 < a.p.B; b0 += 64) {
     const SeqWork w = seq_work<R>(a, b0 + lane);
@@ -584,7 +586,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
 }
 
 // ---------------------------------------------------------------------------
-// tiles of 128 rows
+// tiles of 128 or 64 rows
 // ---------------------------------------------------------------------------
 // The products run as above with 2 x 16 rows a wave; the lane with a row's
 // scores of tokens 16 t + 4 g + r holds those k-slots. A block of codes is read
@@ -592,10 +594,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
 // the next block's codes are converted while this one is computed, and the one
 // after is in flight. V is read transposed.
 //
-// A wave takes 32 rows up to D = 128, where the products' operands and sums fit
-// 256 registers and two workgroups a CU; at 256 eight waves take 16 each, or
-// there would be one wave a SIMD with nothing to hide its waits.
-constexpr int tile_waves(int D) { return D <= 128 ? 4 : 8; }
+// A workgroup is four waves of 32 rows up to D = 128 and of 16 at 256, with blocks
+// of 64 and 32 tokens: what fits two workgroups a CU in registers and LDS. They
+// are at different places of their blocks, so that one's products and LDS reads
+// run beside the other's softmax; eight waves of 16 rows in one workgroup a CU,
+// all in step, took 368 us for 24 sequences of up to 1000 new tokens at D = 256,
+// two of four waves 356.
 //
 // K rows are as long as all banks: the 16-byte chunks of token t are XOR-swizzled
 // by t, so that any 16 lanes of a read that the LDS takes together (16 tokens, or
@@ -606,28 +610,28 @@ __device__ __forceinline__ int kswz(int t) { return D >= 128 ? (t & 15) : ((t >>
 template <int D>
 struct TileLds {
   static constexpr int KROW = 2 * D, VROW = 2 * D + 32;
-  static constexpr int V = kTileBlock * KROW;
-  static constexpr int SCALES = V + kTileBlock * VROW;        // of keys, of values, the largest of each 16 of these
-  static constexpr int BUF = SCALES + 2 * kTileBlock * 4 + 16;
+  static constexpr int V = tile_block(D) * KROW;
+  static constexpr int SCALES = V + tile_block(D) * VROW;        // of keys, of values, the largest of each 16 of these
+  static constexpr int BUF = SCALES + 2 * tile_block(D) * 4 + 16;
   static constexpr int BYTES = 2 * BUF;
 };
 
 template <int D>
-__global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_tile_kernel(PagedSdpaArgs a) {
+__global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
   using L = TileLds<D>;
-  constexpr int kBlock = kTileBlock, Q = kBlock / 16;
-  constexpr int NW = tile_waves(D), RT = 8 / NW;  // waves, 16-row tiles of each
-  constexpr int NK = D / 32, NJ = D / 16;
+  constexpr int kBlock = tile_block(D), Q = kBlock / 16;
+  constexpr int NW = 4, RT = tile_rows(D) / 64;  // waves, 16-row tiles of each
+  constexpr int R = tile_rows(D), NK = D / 32, NJ = D / 16;
   constexpr int PPT = kBlock * D / 16 / (64 * NW);  // 16-code pieces of a K (or V) block per thread
   __shared__ __attribute__((aligned(16))) unsigned char smem[L::BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n16 = lane & 15, grp = lane >> 4;
   const int kh = blockIdx.x % a.Hkv, gqa = a.Hq / a.Hkv;
-  const Item it = find_item<128, false>(a, blockIdx.x / a.Hkv);
+  const Item it = find_item<R, false>(a, blockIdx.x / a.Hkv);
   if (it.b < 0) return;
-  const int rw0 = 128 * it.tile;
-  const int rows = min(it.rows - rw0, 128);
+  const int rw0 = R * it.tile;
+  const int rows = min(it.rows - rw0, R);
   const int seen = last_seen(a, it, rw0 + rows - 1, gqa) + 1;
   const int nblocks = (seen + kBlock - 1) / kBlock;
   const int ib0 = (int)((int64_t)it.part * nblocks / it.parts);
@@ -661,7 +665,7 @@ __global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_ti
   const uint32_t koff = ((tid / (D / 16)) & 15) * a.ks.c_tok + 16 * (tid % (D / 16));
   const uint32_t voff = ((tid / (D / 16)) & 15) * a.vs.c_tok + 16 * (tid % (D / 16));
   auto page_id = [&](const BlockPages<Q>& bp, int run) {
-    return (run == 0 ? bp.id[0] : Q == 2 || run == 1 ? bp.id[1] : run == 2 ? bp.id[Q - 2] : bp.id[Q - 1]);
+    return run == 0 ? bp.id[0] : Q == 2 || run == 1 ? bp.id[1] : run == 2 ? bp.id[Q - 2] : bp.id[Q - 1];
   };
   auto load = [&](int ib, const BlockPages<Q>& bp) {
     const int t0 = kBlock * min(ib, last);
@@ -747,8 +751,11 @@ __global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_ti
     float alpha[RT];
     bool up[RT];
     float size[RT];
-    const f32x4_t big = *reinterpret_cast<const f32x4_t*>(smem + at + L::SCALES + 8 * kBlock);
-    size[0] = size[RT - 1] = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+    const float* big = reinterpret_cast<const float*>(smem + at + L::SCALES) + 2 * kBlock;
+    size[0] = big[0];
+#pragma unroll
+    for (int i = 1; i < Q; ++i) size[0] = fmaxf(size[0], big[i]);
+    size[RT - 1] = size[0];
     if (__builtin_expect(t0 + kBlock > all || pages_ok != (1u << Q) - 1 || size[0] > 65504.0f, 0)) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
@@ -823,7 +830,7 @@ __global__ __launch_bounds__(64 * tile_waves(D), D <= 128 ? 2 : 1) void paged_ti
 #pragma unroll
       for (int j = 0; j < NJ; ++j) store_row4(a, at + 16 * j + 4 * grp, z != 0.0f ? acc[rt][j] * inv : acc[rt][j]);
     } else {
-      const int64_t at = ((int64_t)kh * a.slots + it.slot + it.part) * 128 + r;
+      const int64_t at = ((int64_t)kh * a.slots + it.slot + it.part) * R + r;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) *reinterpret_cast<f32x4_t*>(a.pacc + at * D + 16 * j + 4 * grp) = acc[rt][j];
       if (grp == 0) {
@@ -916,12 +923,13 @@ struct PagedPlan {
   int min_part;
 };
 
-PagedPlan paged_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t max_new, int64_t max_tokens) {
+PagedPlan paged_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
+                     int64_t max_tokens) {
   PagedPlan p;
   const int64_t gqa = Hq / Hkv;
   max_new = std::min(max_new, T);
   p.few = max_new * gqa <= 16;
-  p.rows = p.few ? 16 : 128;
+  p.rows = p.few ? 16 : tile_rows((int)D);
   p.min_part = 128;
   p.max_tiles = std::min(T * gqa / p.rows + B, B * cdiv(max_new * gqa, p.rows));
   p.target = std::min<int64_t>(cdiv((p.few ? 4 : 2) * device_cus(), Hkv), kMaxParts);
@@ -937,12 +945,12 @@ void launch_paged(const PagedSdpaArgs& a, const PagedPlan& p, hipStream_t st) {
   if (p.few)
     hipLaunchKernelGGL(paged_few_kernel<D>, grid, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL(paged_tile_kernel<D>, grid, dim3(64 * tile_waves(D)), 0, st, a);
+    hipLaunchKernelGGL(paged_tile_kernel<D>, grid, dim3(256), 0, st, a);
   if (merge.x == 0) return;
   if (p.few)
     hipLaunchKernelGGL((paged_merge_kernel<D, 16>), merge, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((paged_merge_kernel<D, 128>), merge, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_merge_kernel<D, tile_rows(D)>), merge, dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -950,7 +958,7 @@ void launch_paged(const PagedSdpaArgs& a, const PagedPlan& p, hipStream_t st) {
 // Parts of split contexts: their outputs, then maxima and sums.
 size_t paged_sdpa_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
                             int64_t max_tokens) {
-  const PagedPlan p = paged_plan(T, B, Hq, Hkv, max_new, max_tokens);
+  const PagedPlan p = paged_plan(T, B, Hq, Hkv, D, max_new, max_tokens);
   return (size_t)(Hkv * p.slots * p.rows * (D + 2)) * sizeof(float);
 }
 
@@ -959,7 +967,7 @@ int paged_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, const Pag
                int causal, int qdt, int odt, float scale, void* ws, size_t wsb, hipStream_t st) {
   if (p.T == 0 || p.B == 0) return SPARKQ_OK;
   const int64_t max_tokens = (int64_t)p.width << p.page_log2;
-  const PagedPlan plan = paged_plan(p.T, p.B, Hq, Hkv, max_new, max_tokens);
+  const PagedPlan plan = paged_plan(p.T, p.B, Hq, Hkv, D, max_new, max_tokens);
   const size_t need = paged_sdpa_workspace(p.T, p.B, Hq, Hkv, D, max_new, max_tokens);
   if (need > 0 && (!ws || wsb < need))
     return set_error(SPARKQ_ERR_WORKSPACE, "paged_sdpa needs a workspace of %zu bytes (got %zu)", need,
