@@ -983,17 +983,17 @@ int sparkq_paged_sdpa(const void* q, const void* k_codes, const void* k_scales, 
   REQUIRE(Hq > 0 && Hq % Hkv == 0, "paged_sdpa: query heads must be divisible by KV heads");
   REQUIRE(max_new > 0 && max_new <= kI32Max, "paged_sdpa: max_new must be positive");
   REQUIRE(Hq <= 65535 && T <= kI32Max / Hq && B <= kI32Max / (4 * Hkv), "paged_sdpa: shape too large");
-  for (int i = 3; i < 12; i += 6)
-    REQUIRE_SUPPORTED(strides[i] % 8 == 0 && strides[i + 1] % 8 == 0 && strides[i + 2] == 1,
-                      "paged_sdpa: scales must be contiguous over a page's tokens, pages and heads "
-                      "multiples of 8 scales apart");
+  REQUIRE_SUPPORTED(strides[3] % 8 == 0 && strides[4] % 8 == 0 && strides[5] == 1,
+                    "paged_sdpa: scales must be contiguous over a page's tokens, pages and heads "
+                    "multiples of 8 scales apart");
   REQUIRE_SUPPORTED(aligned(k_scales, 16) && aligned(v_scales, 16),
                     "paged_sdpa: scales must be 16-byte aligned");
-  for (int i = 0; i < 12; i += 6)
-    REQUIRE_SUPPORTED(strides[i] / 16 <= kI32Max && strides[i + 3] / 8 <= kI32Max &&
-                          strides[i + 2] <= kI32Max / page_size,
-                      "paged_sdpa: pages must be less than 32 GiB apart and a head's tokens span less "
-                      "than 2 GiB");
+  for (int i = 0; i < 6; ++i)
+    REQUIRE_SUPPORTED(strides[i] == strides[6 + i], "paged_sdpa: keys and values must have the same strides");
+  REQUIRE_SUPPORTED(strides[0] / 16 <= kI32Max && strides[3] / 8 <= kI32Max &&
+                        strides[2] <= kI32Max / page_size,
+                    "paged_sdpa: pages must be less than 32 GiB apart and a head's tokens span less "
+                    "than 2 GiB");
   REQUIRE((T == 0 || (q && out)) && q_strides && starts && (B == 0 || (page_table && lengths)),
           "paged_sdpa: null tensor pointer");
   REQUIRE(is_half_dtype(q_dtype), "paged_sdpa requires float16 or bfloat16 queries");

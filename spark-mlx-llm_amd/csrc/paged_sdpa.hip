@@ -39,12 +39,13 @@
 namespace sparkq {
 namespace {
 
-// One side of the cache as the attention addresses it: the page stride in units
-// of 16 bytes (codes) and 8 scales, so that a page's address is one 32-bit
-// product, and a page's own extent in 32 bits.
-struct CodeSide {
-  const uint8_t* codes;
-  const uint16_t* scales;
+// The cache as the attention addresses it. Keys and values lie alike, so that one
+// offset serves both; the page strides are in units of 16 bytes (codes) and 8
+// scales, so that a page's offset is one 32-bit product, and a head's tokens
+// within a page span less than 32 bits.
+struct CodeLayout {
+  const uint8_t *k, *v;
+  const uint16_t *ks, *vs;
   int64_t c_head, s_head;
   uint32_t c_page, s_page, c_tok;
 };
@@ -53,7 +54,7 @@ struct PagedSdpaArgs {
   PagedBatch p;
   const uint16_t* q;
   int64_t q_tok, q_head;  // elements
-  CodeSide ks, vs;
+  CodeLayout c;
   void* out;  // [T, Hq, D]
   float *pm, *pz, *pacc;  // [Hkv][slots][rows], [...], [...][D]: parts of split contexts
   int Hq, Hkv, max_new, causal, q_dtype, out_dtype;
@@ -64,8 +65,6 @@ struct PagedSdpaArgs {
 };
 
 constexpr int kFewBlock = 32;  // tokens of a block
-constexpr int tile_block(int D) { return D <= 128 ? 64 : 32; }
-constexpr int tile_rows(int D) { return D <= 128 ? 128 : 64; }
 
 // ---------------------------------------------------------------------------
 // which work is whose
@@ -195,31 +194,50 @@ __device__ __forceinline__ u32x4_t s8x8_exact(uint32_t lo, uint32_t hi) {
   return u32x4_t{pair(x, 0x04010400u), pair(x, 0x04030402u), pair(y, 0x04010400u), pair(y, 0x04030402u)};
 }
 
-// A row's query values as exact fp16 under a power of two: chunk c of lane
-// group g holds dims dim0(c) .. +8. The row's lanes are l, l^16, l^32, l^48.
-// Returns the factor that undoes the shift.
-template <int NK, typename F>
+// max / sum over a row's lanes (l, l ^ 32 and, in four groups of 16, l ^ 16 and
+// l ^ 48), the same value in all of them
+template <int G>
+__device__ __forceinline__ float max_groups(float v) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  if (G == 2) return v;
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <int G>
+__device__ __forceinline__ float sum_groups(float v) {
+  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  if (G == 2) return v;
+  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// A row's query values as exact fp16 under a power of two: chunk c of this lane
+// holds dims dim0(c) .. +8. Returns the factor that undoes the shift.
+template <int NK, int G, typename F>
 __device__ __forceinline__ float load_query(const PagedSdpaArgs& a, const uint16_t* row, bool live, F dim0,
                                             u32x4_t qb[NK]) {
-  float qv[NK][8], top = 0.0f;
+  float top = 0.0f;
+  auto value = [&](u32x4_t w, int i) {
+    const uint16_t bits = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+    return live ? (a.q_dtype == SPARKQ_BF16 ? bf16_to_f32(bits) : f16_to_f32(bits)) : 0.0f;
+  };
 #pragma unroll
   for (int c = 0; c < NK; ++c) {
-    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(row + dim0(c));
+    qb[c] = *reinterpret_cast<const u32x4_t*>(row + dim0(c));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint16_t bits = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-      qv[c][i] = live ? (a.q_dtype == SPARKQ_BF16 ? bf16_to_f32(bits) : f16_to_f32(bits)) : 0.0f;
-      top = fmaxf(top, fabsf(qv[c][i]));
-    }
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(value(qb[c], i)));
   }
-  top = fmaxf(top, __shfl_xor(top, 16));
-  top = fmaxf(top, __shfl_xor(top, 32));
+  top = max_groups<G>(top);
   const int e = top > 0.0f && top <= 3.4028235e38f ? ilogbf(top) - 14 : 0;
 #pragma unroll
-  for (int c = 0; c < NK; ++c)
+  for (int c = 0; c < NK; ++c) {
+    const u32x4_t w = qb[c];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      qb[c][i] = pack_round<F16>(ldexpf(qv[c][2 * i], -e), ldexpf(qv[c][2 * i + 1], -e));
+      qb[c][i] = pack_round<F16>(ldexpf(value(w, 2 * i), -e), ldexpf(value(w, 2 * i + 1), -e));
+  }
   return ldexpf(1.0f, e);
 }
 
@@ -234,20 +252,6 @@ __device__ __forceinline__ float pinned(float v) {
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
   typedef float f32x2_t __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){a, b}, f16x2_t));
-}
-
-// max / sum over the four 16-lane rows of a wave, the same value in all of them
-__device__ __forceinline__ float max_groups(float v) {
-  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sum_groups(float v) {
-  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // ---------------------------------------------------------------------------
@@ -282,13 +286,13 @@ __device__ __forceinline__ float part_max(const RowState& st, float z) {
 // visible where MASK; `size` is the block's largest finite value scale, used
 // where all of it is visible. Writes the packed fp16 weights of the lane's N
 // values; returns the factor for what is summed so far (up: it is not 1).
-template <int N>
+template <int N, int G>
 __device__ __forceinline__ float row_block(RowState& st, const float s[N], float mul, const float vsc[N],
                                            float size, u32x4_t w[N / 8], bool& up) {
   float top = s[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) top = fmaxf(top, s[i]);
-  top = max_groups(top) * mul;
+  top = max_groups<G>(top) * mul;
   const float e = fmaxf(st.e, (float)((int)(__float_as_uint(size) >> 23) - 127));
   const bool raise = top > st.m + kRoom;
   up = raise || e != st.e;
@@ -318,7 +322,7 @@ __device__ __forceinline__ float kept_scale(float v) {
 
 // Hides the scores that are not in `ok` and turns those of values that are not
 // finite to NaN; returns the largest value scale of the others.
-template <int N>
+template <int N, int G>
 __device__ __forceinline__ float hide(uint32_t ok, float s[N], const float vsc[N]) {
   float size = 0.0f;
 #pragma unroll
@@ -327,7 +331,7 @@ __device__ __forceinline__ float hide(uint32_t ok, float s[N], const float vsc[N
     s[i] = live ? (__float_as_uint(vsc[i]) == 0x80000000u ? __builtin_nanf("") : s[i]) : kNegInf;
     size = fmaxf(size, live ? fabsf(vsc[i]) : 0.0f);
   }
-  return max_groups(size);
+  return max_groups<G>(size);
 }
 
 // Four outputs (dims d .. d + 3) of a row.
@@ -347,12 +351,12 @@ __device__ __forceinline__ int64_t out_row(const PagedSdpaArgs& a, const Item& i
   return ((int64_t)(it.first + rr / gqa) * a.Hq + kh * gqa + rr % gqa);
 }
 
-// This KV head's codes and scales of a page: run `slot` / 16 of it
-__device__ __forceinline__ const uint8_t* code_run(const uint8_t* head, const CodeSide& s, int id, int slot) {
-  return head + (((uint64_t)(uint32_t)id * s.c_page << 4) + (uint32_t)slot * s.c_tok);
+// Offsets within a KV head's codes (bytes) and scales (elements) of a page's slot
+__device__ __forceinline__ uint64_t code_at(const CodeLayout& c, int id, int slot) {
+  return ((uint64_t)(uint32_t)id * c.c_page << 4) + (uint32_t)slot * c.c_tok;
 }
-__device__ __forceinline__ const uint16_t* scale_run(const uint16_t* head, const CodeSide& s, int id, int slot) {
-  return head + (((uint64_t)(uint32_t)id * s.s_page << 3) + (uint32_t)slot);
+__device__ __forceinline__ uint64_t scale_at(const CodeLayout& c, int id, int slot) {
+  return ((uint64_t)(uint32_t)id * c.s_page << 3) + (uint32_t)slot;
 }
 
 // Pages of a block's Q runs of 16 tokens; a run without one reads page 0 and is
@@ -438,37 +442,37 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
   u32x4_t qb[NK];
   const uint16_t* qrow = a.q + (it.first + rr / gqa) * a.q_tok + (kh * gqa + rr % gqa) * a.q_head;
   // chunk c: dims 16 (g + 4 (c / 2)) + 8 (c % 2), as the 16-byte pieces of K lie
-  const float mul = load_query<NK>(a, qrow, true, [&](int c) { return 16 * (grp + 4 * (c >> 1)) + 8 * (c & 1); }, qb);
+  const float mul = load_query<NK, 4>(a, qrow, true, [&](int c) { return 16 * (grp + 4 * (c >> 1)) + 8 * (c & 1); }, qb);
 
   u32x4_t kr[2][PL], vr[VL], skr, svr;
   BlockPages<2> next;
   uint32_t pages_ok;
   const int ktok = 8 * (n16 >> 2) + (n16 & 3);
-  const uint32_t koff = (ktok & 15) * a.ks.c_tok + 16 * grp;
-  const uint8_t *const khead = a.ks.codes + kh * a.ks.c_head, *const vhead = a.vs.codes + kh * a.vs.c_head;
-  const uint16_t *const kshead = a.ks.scales + kh * a.ks.s_head, *const vshead = a.vs.scales + kh * a.vs.s_head;
+  const uint32_t koff = (ktok & 15) * a.c.c_tok + 16 * grp;
+  const uint8_t *const khead = a.c.k + kh * a.c.c_head, *const vhead = a.c.v + kh * a.c.c_head;
+  const uint16_t *const kshead = a.c.ks + kh * a.c.s_head, *const vshead = a.c.vs + kh * a.c.s_head;
   const int slot_mask = (1 << a.p.page_log2) - 1;
   const int last = ib1 - 1;
   // block ib (no further than the last) through the pages found for it
   auto load = [&](int ib, const BlockPages<2>& bp) {
     const int t0 = kBlock * min(ib, last);
     const int s0 = t0 & slot_mask, s1 = (t0 + 16) & slot_mask;
-    const uint8_t* kp = (n16 < 8 ? code_run(khead, a.ks, bp.id[0], s0) : code_run(khead, a.ks, bp.id[1], s1)) + koff;
-    const uint8_t *v0 = code_run(vhead, a.vs, bp.id[0], s0), *v1 = code_run(vhead, a.vs, bp.id[1], s1);
+    const uint64_t o0 = code_at(a.c, bp.id[0], s0), o1 = code_at(a.c, bp.id[1], s1);
+    const uint8_t *kp = khead + (n16 < 8 ? o0 : o1) + koff, *v0 = vhead + o0, *v1 = vhead + o1;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < PL; ++i)
-        kr[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kp + (4 * t * a.ks.c_tok + 64 * i)));
+        kr[t][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kp + (4 * t * a.c.c_tok + 64 * i)));
 #pragma unroll
     for (int v = 0; v < VL; ++v) {
       const int f = lane + 64 * v, tok = f / (D / 16), pc = f % (D / 16);
-      vr[v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>((2 * v >= VL ? v1 : v0) + ((tok & 15) * a.vs.c_tok + 16 * pc)));
+      vr[v] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>((2 * v >= VL ? v1 : v0) + ((tok & 15) * a.c.c_tok + 16 * pc)));
     }
     const bool h = grp >= 2;
-    const int id = h ? bp.id[1] : bp.id[0], run = (h ? s1 : s0) + 8 * (grp & 1);
-    skr = *reinterpret_cast<const u32x4_t*>(scale_run(kshead, a.ks, id, run));
-    svr = *reinterpret_cast<const u32x4_t*>(scale_run(vshead, a.vs, id, run));
+    const uint64_t so = scale_at(a.c, h ? bp.id[1] : bp.id[0], (h ? s1 : s0) + 8 * (grp & 1));
+    skr = *reinterpret_cast<const u32x4_t*>(kshead + so);
+    svr = *reinterpret_cast<const u32x4_t*>(vshead + so);
     pages_ok = bp.ok;
   };
 
@@ -517,8 +521,8 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
       vsc[i] = live ? vsc[i] : 0.0f;
       size = fmaxf(size, scale_size(vsc[i], true));
     }
-    size = max_groups(size);
-    const float alpha = row_block<8>(st, s, mul, vsc, size, &w, up);
+    size = max_groups<4>(size);
+    const float alpha = row_block<8, 4>(st, s, mul, vsc, size, &w, up);
     if (__ballot(up)) {
       const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
@@ -542,7 +546,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
   }
 
   // combine the waves
-  const float z = sum_groups(st.z);
+  const float z = sum_groups<4>(st.z);
   __syncthreads();
   float* wm = reinterpret_cast<float*>(smem);  // [4][16]
   float* wz = wm + 64;                         // [4][16]
@@ -588,45 +592,57 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
 // ---------------------------------------------------------------------------
 // tiles of 128 or 64 rows
 // ---------------------------------------------------------------------------
-// The products run as above with 2 x 16 rows a wave; the lane with a row's
-// scores of tokens 16 t + 4 g + r holds those k-slots. A block of codes is read
-// once by the workgroup and written to LDS as fp16, token-major, two buffers deep:
-// the next block's codes are converted while this one is computed, and the one
-// after is in flight. V is read transposed.
+// Four waves of MT rows each. The products run as above on the MT x MT MFMA: 32
+// rows a wave up to D = 128, 16 at 256, with blocks of 64 and 32 tokens, which is
+// what fits two workgroups a CU in registers and LDS. These are at different
+// places of their blocks, so that one's products and LDS reads run beside the
+// other's softmax (at D = 256 eight waves of 16 rows in one workgroup a CU, all in
+// step, took 368 us for 24 sequences of up to 1000 new tokens, two of four 356).
+// A lane has one row, and of a block the scores i of tokens 4 G (i / 4) + 4 g + i %
+// 4, g its group of the G = 64 / MT: scores 8 s .. +8 are its k-slots of the second
+// product's step s.
 //
-// A workgroup is four waves of 32 rows up to D = 128 and of 16 at 256, with blocks
-// of 64 and 32 tokens: what fits two workgroups a CU in registers and LDS. They
-// are at different places of their blocks, so that one's products and LDS reads
-// run beside the other's softmax; eight waves of 16 rows in one workgroup a CU,
-// all in step, took 368 us for 24 sequences of up to 1000 new tokens at D = 256,
-// two of four waves 356.
-//
-// K rows are as long as all banks: the 16-byte chunks of token t are XOR-swizzled
-// by t, so that any 16 lanes of a read that the LDS takes together (16 tokens, or
-// 4 tokens of each lane group) hit different banks. V rows are padded by 32 bytes,
-// which does the same for the transposed reads.
+// A block of codes is read once by the workgroup and written to LDS as fp16,
+// token-major, two buffers deep: the next block's codes are converted while this
+// one is computed, and the one after is in flight. K rows are padded by 16 bytes,
+// or at D = 256 their 16-byte chunks XOR-swizzled by the token, so that any 16
+// lanes of a read that the LDS takes together hit different banks; V rows, read
+// transposed, are padded to the same end.
 template <int D>
-__device__ __forceinline__ int kswz(int t) { return D >= 128 ? (t & 15) : ((t >> 1) & 7); }
-template <int D>
-struct TileLds {
-  static constexpr int KROW = 2 * D, VROW = 2 * D + 32;
-  static constexpr int V = tile_block(D) * KROW;
-  static constexpr int SCALES = V + tile_block(D) * VROW;        // of keys, of values, the largest of each 16 of these
-  static constexpr int BUF = SCALES + 2 * tile_block(D) * 4 + 16;
+struct TileShape {
+  static constexpr int MT = D <= 128 ? 32 : 16, G = 64 / MT;
+  static constexpr int ROWS = 4 * MT;                 // of a workgroup
+  static constexpr int BLOCK = D <= 128 ? 64 : 32;    // tokens
+  static constexpr int N = BLOCK * MT / 64;           // scores a lane
+  static constexpr int KROW = 2 * D + (MT == 32 ? 16 : 0), VROW = 2 * D + (MT == 32 ? 64 : 32);
+  static constexpr int V = BLOCK * KROW;
+  static constexpr int SCALES = V + BLOCK * VROW;     // of keys, of values, the largest of each 16 of these
+  static constexpr int BUF = SCALES + 2 * BLOCK * 4 + 16;
   static constexpr int BYTES = 2 * BUF;
 };
 
+template <int MT>
+struct TileSum {
+  typedef f32x4_t type;
+};
+template <>
+struct TileSum<32> {
+  typedef f32x16_t type;
+};
+__device__ __forceinline__ f32x4_t tile_mfma(u32x4_t x, u32x4_t y, f32x4_t c) { return mfma16x16x32_f16(x, y, c); }
+__device__ __forceinline__ f32x16_t tile_mfma(u32x4_t x, u32x4_t y, f32x16_t c) { return mfma32x32x16<F16>(x, y, c); }
+
 template <int D>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
-  using L = TileLds<D>;
-  constexpr int kBlock = tile_block(D), Q = kBlock / 16;
-  constexpr int NW = 4, RT = tile_rows(D) / 64;  // waves, 16-row tiles of each
-  constexpr int R = tile_rows(D), NK = D / 32, NJ = D / 16;
-  constexpr int PPT = kBlock * D / 16 / (64 * NW);  // 16-code pieces of a K (or V) block per thread
-  __shared__ __attribute__((aligned(16))) unsigned char smem[L::BYTES];
+  using S = TileShape<D>;
+  constexpr int MT = S::MT, G = S::G, R = S::ROWS, kBlock = S::BLOCK, N = S::N, Q = kBlock / 16;
+  constexpr int NK = D / (8 * G), NJ = D / MT, NT = kBlock / MT, NV = MT * MT / 64;
+  constexpr int PPT = kBlock * D / 16 / 256;  // 16-code pieces of a K (or V) block per thread
+  using Sum = typename TileSum<MT>::type;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[S::BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n16 = lane & 15, grp = lane >> 4;
+  const int n16 = lane & 15, row = lane % MT, grp = lane / MT;
   const int kh = blockIdx.x % a.Hkv, gqa = a.Hq / a.Hkv;
   const Item it = find_item<R, false>(a, blockIdx.x / a.Hkv);
   if (it.b < 0) return;
@@ -638,67 +654,74 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
   const int ib1 = (int)((int64_t)(it.part + 1) * nblocks / it.parts);
   const TableRow trow = table_row(a, it.b);
 
-  u32x4_t qb[RT][NK];
-  int lim[RT];
-  float mul[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int rr = rw0 + 16 * (RT * wave + rt) + n16, rq = min(rr, it.rows - 1);
-    lim[rt] = last_seen(a, it, rr, gqa);
-    const uint16_t* qrow = a.q + (it.first + rq / gqa) * a.q_tok + (kh * gqa + rq % gqa) * a.q_head;
-    mul[rt] = load_query<NK>(a, qrow, rr < it.rows, [&](int c) { return 32 * c + 8 * grp; }, qb[rt]);
-  }
-  const int wr0 = rw0 + 16 * RT * wave;  // the wave's first row
+  const int wr0 = rw0 + MT * wave;  // the wave's first row
+  const int rr = wr0 + row, rq = min(rr, it.rows - 1);
+  const int lim = last_seen(a, it, rr, gqa);
+  u32x4_t qb[NK];
+  const uint16_t* qrow = a.q + (it.first + rq / gqa) * a.q_tok + (kh * gqa + rq % gqa) * a.q_head;
+  const float mul = load_query<NK, G>(a, qrow, rr < it.rows, [&](int c) { return 8 * G * c + 8 * grp; }, qb);
   // what every row of the tile sees
   const int all = __builtin_amdgcn_readfirstlane(last_seen(a, it, rw0, gqa) + 1);
 
+  // Piece p = tid + 256 i of a block: token p / (D / 16), codes 16 (p % (D / 16)).
+  // All tokens of a wave's i-th piece lie in one run of 16, and so in one page.
+  // Wave w < Q also takes the scales of run w: keys in its first 16 lanes, values
+  // in the next. Where blocks do not straddle pages all of a block's addresses are
+  // one offset and the lane's own.
   const int slot_mask = (1 << a.p.page_log2) - 1;
+  const bool one_page = slot_mask + 1 >= kBlock;
   u32x4_t kcr[PPT], vcr[PPT];
   uint16_t sr;
   const int last = ib1 - 1;
-  // Piece p = tid + 64 NW i of a block: token p / (D / 16), codes 16 (p % (D /
-  // 16)). All tokens of a wave's i-th piece lie in one run of 16, and so in one
-  // page: its address is a scalar plus the lane's offset. Wave w < Q also takes
-  // the scales of run w: keys in its first 16 lanes, values in the next.
-  const uint8_t *const khead = a.ks.codes + kh * a.ks.c_head, *const vhead = a.vs.codes + kh * a.vs.c_head;
-  const uint16_t *const kshead = a.ks.scales + kh * a.ks.s_head, *const vshead = a.vs.scales + kh * a.vs.s_head;
-  const uint32_t koff = ((tid / (D / 16)) & 15) * a.ks.c_tok + 16 * (tid % (D / 16));
-  const uint32_t voff = ((tid / (D / 16)) & 15) * a.vs.c_tok + 16 * (tid % (D / 16));
-  auto page_id = [&](const BlockPages<Q>& bp, int run) {
-    return run == 0 ? bp.id[0] : Q == 2 || run == 1 ? bp.id[1] : run == 2 ? bp.id[Q - 2] : bp.id[Q - 1];
-  };
+  const uint8_t *const khead = a.c.k + kh * a.c.c_head, *const vhead = a.c.v + kh * a.c.c_head;
+  const uint16_t* const shead = (lane < 16 ? a.c.ks : a.c.vs) + kh * a.c.s_head + n16;
+  const int tk0 = tid / (D / 16), jb = tid % (D / 16);
+  constexpr int TPP = 256 / (D / 16);  // tokens of a round of pieces
+  const uint32_t run_off = (tk0 & 15) * a.c.c_tok + 16 * jb;
+  uint32_t off[PPT];
+#pragma unroll
+  for (int i = 0; i < PPT; ++i) off[i] = (tk0 + i * TPP) * a.c.c_tok + 16 * jb;
   auto load = [&](int ib, const BlockPages<Q>& bp) {
     const int t0 = kBlock * min(ib, last);
+    if (one_page) {
+      const uint64_t at = code_at(a.c, bp.id[0], t0 & slot_mask);
+      const uint8_t *kp = khead + at, *vp = vhead + at;
 #pragma unroll
-    for (int i = 0; i < PPT; ++i) {
-      const int run = wave * 64 / D + i * (64 * NW / D);
-      const int id = page_id(bp, run), slot = (t0 + 16 * run) & slot_mask;
-      kcr[i] = *reinterpret_cast<const u32x4_t*>(code_run(khead, a.ks, id, slot) + koff);
-      vcr[i] = *reinterpret_cast<const u32x4_t*>(code_run(vhead, a.vs, id, slot) + voff);
-    }
-    if (wave < Q) {
-      const int id = page_id(bp, wave), slot = (t0 + 16 * wave) & slot_mask;
-      const uint16_t *kp = scale_run(kshead, a.ks, id, slot), *vp = scale_run(vshead, a.vs, id, slot);
-      sr = (lane < 16 ? kp : vp)[n16];
+      for (int i = 0; i < PPT; ++i) {
+        kcr[i] = *reinterpret_cast<const u32x4_t*>(kp + off[i]);
+        vcr[i] = *reinterpret_cast<const u32x4_t*>(vp + off[i]);
+      }
+      if (wave < Q) sr = shead[scale_at(a.c, bp.id[0], (t0 & slot_mask) + 16 * wave)];
+    } else {
+      auto page_id = [&](int run) {
+        return run == 0 ? bp.id[0] : Q == 2 || run == 1 ? bp.id[1] : run == 2 ? bp.id[Q - 2] : bp.id[Q - 1];
+      };
+#pragma unroll
+      for (int i = 0; i < PPT; ++i) {
+        const int run = wave * 64 / D + i * (TPP / 16);
+        const uint64_t at = code_at(a.c, page_id(run), (t0 + 16 * run) & slot_mask);
+        kcr[i] = *reinterpret_cast<const u32x4_t*>(khead + at + run_off);
+        vcr[i] = *reinterpret_cast<const u32x4_t*>(vhead + at + run_off);
+      }
+      if (wave < Q) sr = shead[scale_at(a.c, page_id(wave), (t0 + 16 * wave) & slot_mask)];
     }
   };
-  const int tk0 = tid / (D / 16), jb = tid % (D / 16);
-  constexpr int TPP = 64 * NW / (D / 16);  // tokens of a round of pieces: whole swizzle periods
-  unsigned char* const kput0 = smem + tk0 * L::KROW + 16 * ((2 * jb) ^ kswz<D>(tk0));
-  unsigned char* const kput1 = smem + tk0 * L::KROW + 16 * ((2 * jb + 1) ^ kswz<D>(tk0));
-  unsigned char* const vput = smem + L::V + tk0 * L::VROW + 32 * jb;
+  auto kswz = [](int t) { return MT == 32 ? 0 : t & 15; };
+  unsigned char* const kput0 = smem + tk0 * S::KROW + 16 * ((2 * jb) ^ kswz(tk0));
+  unsigned char* const kput1 = smem + tk0 * S::KROW + 16 * ((2 * jb + 1) ^ kswz(tk0));
+  unsigned char* const vput = smem + S::V + tk0 * S::VROW + 32 * jb;
   auto stage = [&](auto bufc) {
-    constexpr int at = decltype(bufc)::value * L::BUF;
+    constexpr int at = decltype(bufc)::value * S::BUF;
 #pragma unroll
     for (int i = 0; i < PPT; ++i) {
-      *reinterpret_cast<u32x4_t*>(kput0 + at + i * TPP * L::KROW) = s8x8_exact(kcr[i].x, kcr[i].y);
-      *reinterpret_cast<u32x4_t*>(kput1 + at + i * TPP * L::KROW) = s8x8_exact(kcr[i].z, kcr[i].w);
-      unsigned char* vt = vput + at + i * TPP * L::VROW;
+      *reinterpret_cast<u32x4_t*>(kput0 + at + i * TPP * S::KROW) = s8x8_exact(kcr[i].x, kcr[i].y);
+      *reinterpret_cast<u32x4_t*>(kput1 + at + i * TPP * S::KROW) = s8x8_exact(kcr[i].z, kcr[i].w);
+      unsigned char* vt = vput + at + i * TPP * S::VROW;
       *reinterpret_cast<u32x4_t*>(vt) = s8x8_exact(vcr[i].x, vcr[i].y);
       *reinterpret_cast<u32x4_t*>(vt + 16) = s8x8_exact(vcr[i].z, vcr[i].w);
     }
     if (wave < Q) {
-      float* sc = reinterpret_cast<float*>(smem + at + L::SCALES);
+      float* sc = reinterpret_cast<float*>(smem + at + S::SCALES);
       const float v = f16_to_f32(sr);
       const float big = max_row16(fabsf(v) <= 65504.0f ? fabsf(v) : __builtin_huge_valf());
       if (lane < 32) sc[(lane < 16 ? 0 : kBlock) + 16 * wave + n16] = lane < 16 ? v * a.scale_log2 : kept_scale(v);
@@ -706,90 +729,76 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
     }
   };
 
-  const unsigned char* kget[4];  // chunk 4 kk + g of token n16: kk and kk + 4 are 256 bytes apart
+  // chunk G kk + g of token `row`; swizzled chunks kk and kk + 4 are 256 bytes apart
+  constexpr int KP = MT == 32 ? 1 : 4;
+  const unsigned char* kget[KP];
 #pragma unroll
-  for (int kk = 0; kk < 4 && kk < NK; ++kk) kget[kk] = smem + n16 * L::KROW + 16 * ((4 * kk + grp) ^ kswz<D>(n16));
-  const unsigned char* const vget = smem + L::V + (4 * grp + (n16 >> 2)) * L::VROW + 8 * (n16 & 3);
-  const float* const sget = reinterpret_cast<const float*>(smem + L::SCALES) + 4 * grp;
-  RowState st[RT];
-  f32x4_t acc[RT][NJ];
+  for (int kk = 0; kk < KP; ++kk) kget[kk] = smem + row * S::KROW + 16 * ((G * kk + grp) ^ kswz(row));
+  const unsigned char* const vget = smem + S::V + (4 * grp + (n16 >> 2)) * S::VROW + 8 * (n16 & 3) +
+                                    (MT == 32 ? 32 * ((lane >> 4) & 1) : 0);
+  const float* const sget = reinterpret_cast<const float*>(smem + S::SCALES) + 4 * grp;
+  RowState st;
+  Sum acc[NJ];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[rt][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int j = 0; j < NJ; ++j) acc[j] = Sum{};
 
-  // One block; MASK where some row of the tile does not see all of it.
   auto compute = [&](auto bufc, int t0, uint32_t pages_ok) {
-    constexpr int at = decltype(bufc)::value * L::BUF;
-    f32x4_t sc[Q][RT];
+    constexpr int at = decltype(bufc)::value * S::BUF;
+    Sum sc[NT];
 #pragma unroll
-    for (int tt = 0; tt < Q; ++tt)
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) sc[tt][rt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int tt = 0; tt < Q; ++tt)
+    for (int tt = 0; tt < NT; ++tt) {
+      sc[tt] = Sum{};
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) {
-        const u32x4_t kf = *reinterpret_cast<const u32x4_t*>(kget[kk % 4] + at + tt * 16 * L::KROW + 256 * (kk / 4));
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) sc[tt][rt] = mfma16x16x32_f16(kf, qb[rt][kk], sc[tt][rt]);
+        const unsigned char* kp = kget[kk % KP] + at + tt * MT * S::KROW + 16 * G * KP * (kk / KP);
+        sc[tt] = tile_mfma(*reinterpret_cast<const u32x4_t*>(kp), qb[kk], sc[tt]);
       }
+    }
     const float* scl = sget + at / 4;
-    float vsc[4 * Q], s[RT][4 * Q];
+    float vsc[N], s[N];
 #pragma unroll
-    for (int tt = 0; tt < Q; ++tt) {
-      const f32x4_t k4 = *reinterpret_cast<const f32x4_t*>(scl + 16 * tt);
-      const f32x4_t v4 = *reinterpret_cast<const f32x4_t*>(scl + kBlock + 16 * tt);
+    for (int i = 0; i < N; i += 4) {
+      const f32x4_t k4 = *reinterpret_cast<const f32x4_t*>(scl + G * i);
+      const f32x4_t v4 = *reinterpret_cast<const f32x4_t*>(scl + kBlock + G * i);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        vsc[4 * tt + r] = v4[r];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][4 * tt + r] = sc[tt][rt][r] * k4[r];
+        vsc[i + r] = v4[r];
+        s[i + r] = sc[i / NV][i % NV + r] * k4[r];
       }
     }
-    u32x4_t pb[RT][Q / 2];
-    float alpha[RT];
-    bool up[RT];
-    float size[RT];
-    const float* big = reinterpret_cast<const float*>(smem + at + L::SCALES) + 2 * kBlock;
-    size[0] = big[0];
+    const float* big = reinterpret_cast<const float*>(smem + at + S::SCALES) + 2 * kBlock;
+    float size = big[0];
 #pragma unroll
-    for (int i = 1; i < Q; ++i) size[0] = fmaxf(size[0], big[i]);
-    size[RT - 1] = size[0];
-    if (__builtin_expect(t0 + kBlock > all || pages_ok != (1u << Q) - 1 || size[0] > 65504.0f, 0)) {
+    for (int i = 1; i < Q; ++i) size = fmaxf(size, big[i]);
+    if (__builtin_expect(t0 + kBlock > all || pages_ok != (1u << Q) - 1 || size > 65504.0f, 0)) {
+      uint32_t ok = 0;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        uint32_t ok = 0;
-#pragma unroll
-        for (int i = 0; i < 4 * Q; ++i)
-          ok |= (uint32_t)(t0 + 16 * (i >> 2) + 4 * grp + (i & 3) <= lim[rt] && ((pages_ok >> (i >> 2)) & 1u)) << i;
-        size[rt] = hide<4 * Q>(__float_as_uint(pinned(__uint_as_float(ok))), s[rt], vsc);
+      for (int i = 0; i < N; ++i) {
+        const int t = 4 * G * (i >> 2) + 4 * grp + (i & 3);
+        ok |= (uint32_t)(t0 + t <= lim && ((pages_ok >> (t / 16)) & 1u)) << i;
       }
+      size = hide<N, G>(__float_as_uint(pinned(__uint_as_float(ok))), s, vsc);
     }
+    u32x4_t w[N / 8];
+    bool up;
+    const float alpha = row_block<N, G>(st, s, mul, vsc, size, w, up);
+    if (__builtin_expect(__ballot(up) != 0, 0)) {
+      const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) alpha[rt] = row_block<4 * Q>(st[rt], s[rt], mul[rt], vsc, size[rt], pb[rt], up[rt]);
-    if (__builtin_expect(__ballot(up[0] || up[RT - 1]) != 0, 0)) {
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        const float f = pinned(up[rt] ? alpha[rt] : 1.0f);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[rt][j] *= f;
-      }
+      for (int j = 0; j < NJ; ++j) acc[j] *= f;
     }
     typedef short s16x4_t __attribute__((ext_vector_type(4)));
     typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
-    for (int k = 0; k < Q / 2; ++k)
+    for (int k = 0; k < N / 8; ++k)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const unsigned char* vp = vget + at + 32 * k * L::VROW + 32 * j;
+        const unsigned char* vp = vget + at + 8 * G * k * S::VROW + 2 * MT * j;
         const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (__attribute__((address_space(3))) s16x4_t*)(vp)));
         const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4_t*)(vp + 16 * L::VROW)));
-        const u32x4_t vf = u32x4_t{lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][j] = mfma16x16x32_f16(vf, pb[rt][k], acc[rt][j]);
+            (__attribute__((address_space(3))) s16x4_t*)(vp + 4 * G * S::VROW)));
+        acc[j] = tile_mfma(u32x4_t{lo.x, lo.y, hi.x, hi.y}, w[k], acc[j]);
       }
   };
 
@@ -819,24 +828,29 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
     if (ib < ib1 && wr0 < it.rows) compute(std::integral_constant<int, 0>{}, kBlock * ib, ok_now);
   }
 
+  const float z = sum_groups<G>(st.z);
+  const int r = MT * wave + row;
+  if (r >= rows) return;
+  if (it.parts == 1) {
+    const int64_t at = out_row(a, it, kh, rw0 + r, gqa) * D;
+    const float inv = z != 0.0f ? 1.0f / z : 1.0f;
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const float z = sum_groups(st[rt].z);
-    const int r = 16 * (RT * wave + rt) + n16;
-    if (r >= rows) continue;
-    if (it.parts == 1) {
-      const int64_t at = out_row(a, it, kh, rw0 + r, gqa) * D;
-      const float inv = z != 0.0f ? 1.0f / z : 0.0f;
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) store_row4(a, at + 16 * j + 4 * grp, z != 0.0f ? acc[rt][j] * inv : acc[rt][j]);
-    } else {
-      const int64_t at = ((int64_t)kh * a.slots + it.slot + it.part) * R + r;
+      for (int v = 0; v < NV; v += 4)
+        store_row4(a, at + MT * j + G * v + 4 * grp,
+                   f32x4_t{acc[j][v], acc[j][v + 1], acc[j][v + 2], acc[j][v + 3]} * inv);
+  } else {
+    const int64_t at = ((int64_t)kh * a.slots + it.slot + it.part) * R + r;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) *reinterpret_cast<f32x4_t*>(a.pacc + at * D + 16 * j + 4 * grp) = acc[rt][j];
-      if (grp == 0) {
-        a.pm[at] = part_max(st[rt], z);
-        a.pz[at] = z;
-      }
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int v = 0; v < NV; v += 4)
+        *reinterpret_cast<f32x4_t*>(a.pacc + at * D + MT * j + G * v + 4 * grp) =
+            f32x4_t{acc[j][v], acc[j][v + 1], acc[j][v + 2], acc[j][v + 3]};
+    if (grp == 0) {
+      a.pm[at] = part_max(st, z);
+      a.pz[at] = z;
     }
   }
 }
@@ -929,7 +943,7 @@ PagedPlan paged_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
   const int64_t gqa = Hq / Hkv;
   max_new = std::min(max_new, T);
   p.few = max_new * gqa <= 16;
-  p.rows = p.few ? 16 : tile_rows((int)D);
+  p.rows = p.few ? 16 : D <= 128 ? TileShape<128>::ROWS : TileShape<256>::ROWS;
   p.min_part = 128;
   p.max_tiles = std::min(T * gqa / p.rows + B, B * cdiv(max_new * gqa, p.rows));
   p.target = std::min<int64_t>(cdiv((p.few ? 4 : 2) * device_cus(), Hkv), kMaxParts);
@@ -950,7 +964,7 @@ void launch_paged(const PagedSdpaArgs& a, const PagedPlan& p, hipStream_t st) {
   if (p.few)
     hipLaunchKernelGGL((paged_merge_kernel<D, 16>), merge, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((paged_merge_kernel<D, tile_rows(D)>), merge, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_merge_kernel<D, TileShape<D>::ROWS>), merge, dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -975,10 +989,9 @@ int paged_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, const Pag
   if (!aligned(ws, 16)) return set_error(SPARKQ_ERR_INVALID, "paged_sdpa: workspace must be 16-byte aligned");
   const int64_t n = Hkv * plan.slots * plan.rows;
   float* acc = (float*)ws;
-  const auto side = [](const PagedSide& s) {
-    return CodeSide{s.codes, s.scales, s.c_head, s.s_head, (uint32_t)(s.c_page / 16), (uint32_t)(s.s_page / 8), (uint32_t)s.c_tok};
-  };
-  const PagedSdpaArgs a{p, (const uint16_t*)q, qst[0], qst[1], side(ks), side(vs), out, acc + n * D, acc + n * (D + 1), acc,
+  const CodeLayout c{ks.codes, vs.codes, ks.scales, vs.scales, ks.c_head, ks.s_head, (uint32_t)(ks.c_page / 16),
+                     (uint32_t)(ks.s_page / 8), (uint32_t)ks.c_tok};
+  const PagedSdpaArgs a{p, (const uint16_t*)q, qst[0], qst[1], c, out, acc + n * D, acc + n * (D + 1), acc,
                         (int)Hq, (int)Hkv, (int)std::min<int64_t>(max_new, p.T), causal, qdt, odt,
                         (int)plan.target, (int)plan.slots, plan.min_part, scale * 1.44269504088896340736f};
   if (D == 64)
