@@ -43,74 +43,108 @@ __device__ __forceinline__ int seq_of_row(const PagedBatch& p, int t) {
 // A quotient of a 16-bit v (11 bits) and an fp16 s that is not half-way between
 // two whole numbers of 7 bits lies at least 2^-19 of itself from there, and one
 // that is there comes out exactly: q + (v - q s) inv differs from it by the square
-// of q's error, and rounds to it. A third of the division's instructions: 14.4 ->
-// 8 us for 4000 tokens of 4 heads of 256.
+// of q's error, and rounds to it. A third of the division's instructions: 3501
+// tokens of 4 heads of 256 14.4 -> 12.8 us.
 __device__ __forceinline__ float near_quotient(float v, float s, float inv) {
   const float q = v * inv;
   return fmaf(fmaf(-q, s, v), inv, q);
 }
 
 // D / 8 lanes a row, 8 values (one or two 16-byte loads) and 8 codes (one store)
-// a lane: the row's loads do not wait for where it goes. A decode step, where
-// row t is sequence t's, finds that out at once.
-template <int LPR>
+// a lane, U rows in flight. A workgroup's tokens are placed by a thread each while
+// the rows' loads are under way; a decode step, where row t is sequence t's, finds
+// its place at once. A chain of five loads and a store, so bound by latency: one
+// row a lane where the rows fill the chip no more than once over, else two (3501
+// tokens of 4 heads of 256, 21 MB: 11.1 us, 1.9 TB/s; one row 11.9, four 12.0).
+template <int LPR, int U>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
+  constexpr int RPP = 256 / LPR;
+  __shared__ int s_page[RPP * U / 2 + 2], s_slot[RPP * U / 2 + 2];
   const int l = threadIdx.x % LPR;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const bool live = row < (int64_t)a.p.T * a.H * 2;
-  const int64_t rc = live ? row : 0;
-  const int t = (int)(rc / (2 * a.H)), hv = (int)(rc - (int64_t)t * 2 * a.H);
-  const bool isv = hv >= a.H;
-  const int h = isv ? hv - a.H : hv;
-  const int64_t x0 = (isv ? t * a.v_tok + h * a.v_head : t * a.k_tok + h * a.k_head) + 8 * l;
-  const void* x = isv ? a.v : a.k;
-  float v[8];
-  if (a.x_dtype == SPARKQ_F32) {
-    const f32x4_t* p = reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(x) + x0);
-    const f32x4_t lo = p[0], hi = p[1];
+  // rows are counted in 32 bits, unsigned: T * H is less than 2^31
+  const uint32_t heads = 2 * (uint32_t)a.H, total = (uint32_t)a.p.T * heads, row0 = blockIdx.x * (RPP * U);
+  const int t0 = (int)(row0 / heads);
+  const int t1 = (int)((min(total - row0, (uint32_t)(RPP * U)) - 1 + row0) / heads);  // the last token
+  float v[U][8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = lo[i];
-      v[4 + i] = hi[i];
-    }
-  } else {
-    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(x) + x0);
-    const bool bf = a.x_dtype == SPARKQ_BF16;
+  for (int u = 0; u < U; ++u) {
+    const uint32_t row = row0 + min(total - row0 - 1, u * RPP + threadIdx.x / LPR);
+    const int t = (int)(row / heads), hv = (int)(row - t * heads);
+    const bool isv = hv >= a.H;
+    const int h = isv ? hv - a.H : hv;
+    const int64_t x0 = (isv ? t * a.v_tok + h * a.v_head : t * a.k_tok + h * a.k_head) + 8 * l;
+    const void* x = isv ? a.v : a.k;
+    if (a.x_dtype == SPARKQ_F32) {
+      const f32x4_t* p = reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(x) + x0);
+      const f32x4_t lo = p[0], hi = p[1];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = bf ? lo16<BF16>(w[i]) : lo16<F16>(w[i]);
-      v[2 * i + 1] = bf ? hi16<BF16>(w[i]) : hi16<F16>(w[i]);
+      for (int i = 0; i < 4; ++i) {
+        v[u][i] = lo[i];
+        v[u][4 + i] = hi[i];
+      }
+    } else {
+      const u32x4_t w = *reinterpret_cast<const u32x4_t*>(reinterpret_cast<const uint16_t*>(x) + x0);
+      const bool bf = a.x_dtype == SPARKQ_BF16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[u][2 * i] = bf ? lo16<BF16>(w[i]) : lo16<F16>(w[i]);
+        v[u][2 * i + 1] = bf ? hi16<BF16>(w[i]) : hi16<F16>(w[i]);
+      }
     }
   }
-  const bool own = t < a.p.B && a.p.starts[t] == t && a.p.starts[t + 1] == t + 1;
-  const int b = own ? t : seq_of_row(a.p, t);
-  float amax = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[i]));
-#pragma unroll
-  for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
-  if (!live || b < 0) return;
-  const SeqRows s = seq_rows(a.p, b);
-  const int pos = s.length - s.count + (t - s.first);
-  if (t < s.first || t >= s.first + s.count || pos < 0) return;
-  const int id = page_of(a.p, b, pos);
-  if (id < 0) return;
-  uint16_t s16 = f32_to_f16(amax / 127.0f);
-  if (f16_to_f32(s16) == 0.0f) s16 = 0x3C00u;
-  const float sc = f16_to_f32(s16);
-  const PagedSide& side = isv ? a.vs : a.ks;
-  const int slot = pos & ((1 << a.p.page_log2) - 1);
-  if (l == 0) side.scales[id * side.s_page + h * side.s_head + slot * side.s_tok] = s16;
-  uint32_t w[2] = {0, 0};
-  const float inv = __builtin_amdgcn_rcpf(sc);
-  const bool divide = a.x_dtype == SPARKQ_F32 || sc > 65504.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = fminf(fmaxf(__builtin_rintf(divide ? v[i] / sc : near_quotient(v[i], sc, inv)), -127.0f), 127.0f);
-    w[i / 4] |= ((uint32_t)(int)q & 255u) << (8 * (i % 4));
+  if ((int)threadIdx.x <= t1 - t0) {
+    const int t = t0 + threadIdx.x;
+    const bool own = t < a.p.B && a.p.starts[t] == t && a.p.starts[t + 1] == t + 1;
+    const int b = own ? t : seq_of_row(a.p, t);
+    int id = -1, slot = 0;
+    if (b >= 0) {
+      const SeqRows s = seq_rows(a.p, b);
+      const int pos = s.length - s.count + (t - s.first);
+      if (t >= s.first && t < s.first + s.count && pos >= 0) id = page_of(a.p, b, pos);
+      slot = pos & ((1 << a.p.page_log2) - 1);
+    }
+    s_page[threadIdx.x] = id;
+    s_slot[threadIdx.x] = slot;
   }
-  *reinterpret_cast<uint2*>(side.codes + id * side.c_page + h * side.c_head + slot * side.c_tok + 8 * l) =
-      make_uint2(w[0], w[1]);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t rel = u * RPP + threadIdx.x / LPR, row = row0 + min(total - row0 - 1, rel);
+    const bool live = rel < total - row0;
+    const int t = (int)(row / heads), hv = (int)(row - t * heads);
+    const bool isv = hv >= a.H;
+    const int h = isv ? hv - a.H : hv;
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(v[u][i]));
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor(amax, o));
+    uint16_t s16 = f32_to_f16(amax / 127.0f);
+    if (f16_to_f32(s16) == 0.0f) s16 = 0x3C00u;
+    const float sc = f16_to_f32(s16), inv = __builtin_amdgcn_rcpf(sc);
+    const bool divide = a.x_dtype == SPARKQ_F32 || sc > 65504.0f;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float q = __builtin_rintf(divide ? v[u][i] / sc : near_quotient(v[u][i], sc, inv));
+      w[i / 4] |= ((uint32_t)(int)fminf(fmaxf(q, -127.0f), 127.0f) & 255u) << (8 * (i % 4));
+    }
+    const int64_t id = s_page[t - t0], slot = s_slot[t - t0];
+    if (!live || id < 0) continue;
+    const PagedSide& side = isv ? a.vs : a.ks;
+    if (l == 0) side.scales[id * side.s_page + h * side.s_head + slot * side.s_tok] = s16;
+    *reinterpret_cast<uint2*>(side.codes + id * side.c_page + h * side.c_head + slot * side.c_tok + 8 * l) =
+        make_uint2(w[0], w[1]);
+  }
+}
+
+template <int LPR>
+void launch_append(const PagedAppendArgs& a, hipStream_t st) {
+  const int64_t rows = (int64_t)a.p.T * a.H * 2, groups = cdiv(rows, 256 / LPR);
+  if (groups <= 8 * device_cus())
+    hipLaunchKernelGGL((paged_append_kernel<LPR, 1>), dim3((unsigned)groups), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((paged_append_kernel<LPR, 2>), dim3((unsigned)cdiv(groups, 2)), dim3(256), 0, st, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -374,7 +408,9 @@ __global__ __launch_bounds__(kPlanThreads) void pages_compact_plan_kernel(PageAr
 }
 
 // Copies page src[i] to dst[i] in every layer of the four tensors, in pieces
-// of 16 KB dealt over the workgroups. No page is both a source and a
+// of 16 KB dealt over the workgroups, past the caches (read and written once).
+// Bound by HBM: 0.9 GB moved and written in 163 us, 5.5 TB/s; half the workgroups
+// 205 us, cached accesses 171. No page is both a source and a
 // destination. The destination is dst[i], or list[dst[i]] where a list is given.
 __device__ void copy_pages(const PageArgs& a, const int* src, const int* dst, const int* list, int pairs,
                            int block, int blocks) {
@@ -397,13 +433,13 @@ __device__ void copy_pages(const PageArgs& a, const int* src, const int* dst, co
         const int n = sc ? a.vec_scales : a.vec_codes, second = e >= n;
         const PageBuf& b = a.buf[2 * sc + second];
         uint8_t* at = b.p + layer * b.layer + 16 * (int64_t)(e - second * n);
-        v[k] = *reinterpret_cast<const u32x4_t*>(at + from * b.page);
+        v[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(at + from * b.page));
         out[k] = at + to * b.page;
       }
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (out[k]) *reinterpret_cast<u32x4_t*>(out[k]) = v[k];
+      if (out[k]) __builtin_nontemporal_store(v[k], reinterpret_cast<u32x4_t*>(out[k]));
   }
 }
 
@@ -453,13 +489,12 @@ int paged_kv_append(const PagedBatch& p, const void* k, const void* v, const int
                     hipStream_t st) {
   if (p.T == 0 || p.B == 0) return SPARKQ_OK;
   const PagedAppendArgs a{p, k, v, xst[0], xst[1], xst[2], xst[3], ks, vs, (int)H, (int)D, xdt};
-  const dim3 grid((unsigned)cdiv((int64_t)p.T * H * 2, 2048 / D));
   if (D == 64)
-    hipLaunchKernelGGL(paged_append_kernel<8>, grid, dim3(256), 0, st, a);
+    launch_append<8>(a, st);
   else if (D == 128)
-    hipLaunchKernelGGL(paged_append_kernel<16>, grid, dim3(256), 0, st, a);
+    launch_append<16>(a, st);
   else
-    hipLaunchKernelGGL(paged_append_kernel<32>, grid, dim3(256), 0, st, a);
+    launch_append<32>(a, st);
   return check_launch("paged_append_kernel");
 }
 
@@ -491,7 +526,7 @@ static PageArgs page_args(const int32_t* table, int64_t table_stride, const int3
   return a;
 }
 
-static dim3 page_grid(const PageArgs& a) { return dim3((unsigned)(a.table_blocks + 4 * device_cus())); }
+static dim3 page_grid(const PageArgs& a) { return dim3((unsigned)(a.table_blocks + 8 * device_cus())); }
 
 int kv_pages_fork(const int32_t* table, int64_t table_stride, const int32_t* lengths,
                   const int32_t* parents, const int32_t* fresh, int32_t* out_table,
