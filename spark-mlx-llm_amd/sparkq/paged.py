@@ -48,17 +48,15 @@ def _check_cache(op, cache, ndim):
             or ks.dtype is not torch.float16 or vs.dtype is not torch.float16):
         raise ValueError(f"{op}: the cache holds int8 codes [pages,Hkv,page_size,D] and fp16 "
                          "scales [pages,Hkv,page_size] of keys and of values")
-    index = _gpu(op, kc)
+    index = kc.get_device()
     if ks.get_device() != index or vc.get_device() != index or vs.get_device() != index:
         raise ValueError(f"{op}: the cache's tensors must live on one device")
     return kc, ks, vc, vs, index, shape
 
 
-def _gpu(op, t):
-    index = t.get_device()
+def _need_gpu(op, index):
     if index < 0:
         raise ValueError(f"{op} requires GPU execution")
-    return index
 
 
 def _check_ints(op, index, name, t, shape):
@@ -104,7 +102,8 @@ def paged_kv_append(keys, values, cache, page_table, starts, lengths):
     projection are read in place), one layer's cache. The formula is
     kv_quantize_s8's. Rows that fall to no sequence, tokens before position 0
     and tokens without a page are skipped. Sequences that append must not share
-    the page they append to: kv_pages_fork gives each its own."""
+    the page they append to: kv_pages_fork gives each its own. Calls that write
+    one cache are ordered by their stream."""
     op = "paged_kv_append"
     kc, ks, vc, vs, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
     if keys.ndim != 3 or keys.shape[1:] != (hkv, d) or values.shape != keys.shape:
@@ -116,6 +115,7 @@ def paged_kv_append(keys, values, cache, page_table, starts, lengths):
         raise ValueError(f"{op}: keys and values must live on the cache's device")
     b, width = _check_batch(op, index, page_table, starts, lengths)
     strides = _strides(op, kc, ks, vc, vs)
+    _need_gpu(op, index)
     (keys, kst), (values, vst) = _rows16(keys), _rows16(values)
     _lib.launch("sparkq_paged_kv_append", index, keys.data_ptr(), values.data_ptr(), kc.data_ptr(),
                 ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), page_table.data_ptr(),
@@ -132,7 +132,10 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
     of them; tokens without a page are hidden, and a row that sees nothing is
     zero. max_new is the most new tokens that a sequence has (1: a decode
     step). Rows that fall to no sequence, or to more than max_new of one, are
-    left as they are in `out`, and hold anything in a new tensor."""
+    left as they are in `out`, and hold anything in a new tensor. Codes and
+    scales of keys lie as those of values do (the same strides), a page's scales
+    of a head together. A weight times its value's scale is rounded to float16
+    once; scores, normalizer and sums are fp32."""
     op = "paged_quantized_sdpa"
     kc, ks, vc, vs, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
     if queries.ndim != 3 or queries.shape[2] != d or not queries.shape[1] \
@@ -155,6 +158,7 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
         raise ValueError("out_dtype must be the query dtype or torch.float32")
     b, width = _check_batch(op, index, page_table, starts, lengths)
     strides = _strides(op, kc, ks, vc, vs)
+    _need_gpu(op, index)
     queries, qst = _rows16(queries)
     dev = kc.device
     out = torch.empty(shape, dtype=out_dtype, device=dev) if out is None \
@@ -220,6 +224,7 @@ def kv_pages_fork(cache, page_table, lengths, parents=None, new_tokens=None):
         _check_ints(op, index, "parents", parents, (rows,))
     if new_tokens is not None:
         _check_ints(op, index, "new_tokens", new_tokens, (rows,))
+    _need_gpu(op, index)
     dev = page_table.device
     table = torch.empty((rows, width), dtype=torch.int32, device=dev)
     after = torch.empty(rows, dtype=torch.int32, device=dev)
@@ -240,6 +245,7 @@ def kv_pages_compact(cache, page_table, lengths):
     op = "kv_pages_compact"
     bufs, index, layers, pages, page, cb, sb, st = _pool(op, cache)
     b, width = _check_rows(op, index, page_table, lengths)
+    _need_gpu(op, index)
     dev = page_table.device
     table = torch.empty((b, width), dtype=torch.int32, device=dev)
     used = torch.empty(1, dtype=torch.int32, device=dev)

@@ -26,6 +26,16 @@ Registered ops:
   fused_ffn(x, attention_output, norm_weight, eps, gate_w, gate_s, gate_b, up_w, up_s,
             up_b, down_w, down_s, down_b, group_size, bits)
   attention_gate(x, output, gate_weight)
+  qk_norm_rope(queries, keys, q_weight, k_weight, positions, dims, eps, base, scale,
+               traditional) -> (q, k)
+  paged_sdpa(queries, k_codes, k_scales, v_codes, v_scales, page_table, starts, lengths, scale,
+             max_new, causal, out_dtype)
+and, writing the cache's four tensors in place:
+  paged_kv_append(keys, values, k_codes, k_scales, v_codes, v_scales, page_table, starts, lengths)
+  kv_pages_fork(k_codes, k_scales, v_codes, v_scales, page_table, lengths, parents, new_tokens)
+      -> (page_table, lengths, missing)
+  kv_pages_compact(k_codes, k_scales, v_codes, v_scales, page_table, lengths)
+      -> (page_table, used)
 """
 
 from __future__ import annotations
@@ -36,7 +46,7 @@ import torch
 from torch import Tensor
 from torch.library import custom_op
 
-from . import ext
+from . import ext, paged
 
 _NS = "sparkq"
 
@@ -212,8 +222,82 @@ def _(x, output, gate_weight):
     return output.new_empty((b, length, h * d))
 
 
+# --- many sequences over one paged cache -----------------------------------------
+
+_CACHE = ("k_codes", "k_scales", "v_codes", "v_scales")
+
+
+@custom_op(f"{_NS}::qk_norm_rope", mutates_args=())
+def qk_norm_rope(queries: Tensor, keys: Tensor, q_weight: Tensor, k_weight: Tensor,
+                 positions: Tensor, dims: int, eps: float, base: float, scale: float,
+                 traditional: bool) -> Tuple[Tensor, Tensor]:
+    return ext.qk_norm_rope(queries, keys, q_weight, k_weight, positions, dims=dims, eps=eps,
+                            base=base, scale=scale, traditional=traditional)
+
+
+@qk_norm_rope.register_fake
+def _(queries, keys, q_weight, k_weight, positions, dims, eps, base, scale, traditional):
+    return queries.new_empty(queries.shape), keys.new_empty(keys.shape)
+
+
+@custom_op(f"{_NS}::paged_sdpa", mutates_args=())
+def paged_sdpa(queries: Tensor, k_codes: Tensor, k_scales: Tensor, v_codes: Tensor,
+               v_scales: Tensor, page_table: Tensor, starts: Tensor, lengths: Tensor,
+               scale: float, max_new: int, causal: bool,
+               out_dtype: Optional[torch.dtype]) -> Tensor:
+    return paged.paged_quantized_sdpa(queries, (k_codes, k_scales, v_codes, v_scales), page_table,
+                                      starts, lengths, scale=scale, max_new=max_new,
+                                      mask="causal" if causal else None, out_dtype=out_dtype)
+
+
+@paged_sdpa.register_fake
+def _(queries, k_codes, k_scales, v_codes, v_scales, page_table, starts, lengths, scale, max_new,
+      causal, out_dtype):
+    return queries.new_empty(queries.shape, dtype=out_dtype or queries.dtype)
+
+
+@custom_op(f"{_NS}::paged_kv_append", mutates_args=_CACHE)
+def paged_kv_append(keys: Tensor, values: Tensor, k_codes: Tensor, k_scales: Tensor,
+                    v_codes: Tensor, v_scales: Tensor, page_table: Tensor, starts: Tensor,
+                    lengths: Tensor) -> None:
+    paged.paged_kv_append(keys, values, (k_codes, k_scales, v_codes, v_scales), page_table, starts,
+                          lengths)
+
+
+@paged_kv_append.register_fake
+def _(keys, values, k_codes, k_scales, v_codes, v_scales, page_table, starts, lengths):
+    return None
+
+
+@custom_op(f"{_NS}::kv_pages_fork", mutates_args=_CACHE)
+def kv_pages_fork(k_codes: Tensor, k_scales: Tensor, v_codes: Tensor, v_scales: Tensor,
+                  page_table: Tensor, lengths: Tensor, parents: Optional[Tensor],
+                  new_tokens: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    return paged.kv_pages_fork((k_codes, k_scales, v_codes, v_scales), page_table, lengths,
+                               parents, new_tokens)
+
+
+@kv_pages_fork.register_fake
+def _(k_codes, k_scales, v_codes, v_scales, page_table, lengths, parents, new_tokens):
+    rows = page_table.shape[0] if parents is None else parents.shape[0]
+    return (page_table.new_empty((rows, page_table.shape[1])), lengths.new_empty((rows,)),
+            lengths.new_empty((1,)))
+
+
+@custom_op(f"{_NS}::kv_pages_compact", mutates_args=_CACHE)
+def kv_pages_compact(k_codes: Tensor, k_scales: Tensor, v_codes: Tensor, v_scales: Tensor,
+                     page_table: Tensor, lengths: Tensor) -> Tuple[Tensor, Tensor]:
+    return paged.kv_pages_compact((k_codes, k_scales, v_codes, v_scales), page_table, lengths)
+
+
+@kv_pages_compact.register_fake
+def _(k_codes, k_scales, v_codes, v_scales, page_table, lengths):
+    return page_table.new_empty(page_table.shape), lengths.new_empty((1,))
+
+
 __all__ = [
     "affine_quantized_matmul", "w8a8_linear", "w8a16_per_channel", "quantize_per_token",
     "int8_matmul_int32", "int8_sdpa_s8", "int8_sdpa_affine", "rms_norm", "rope", "qkv_rope",
-    "fused_ffn", "attention_gate",
+    "fused_ffn", "attention_gate", "qk_norm_rope", "paged_sdpa", "paged_kv_append",
+    "kv_pages_fork", "kv_pages_compact",
 ]
