@@ -566,8 +566,10 @@ int sparkq_attention_gate(const void* x, const void* attn, const void* gate_w,
  *   starts[b] .. starts[b+1] - 1 of T, the last of them its token lengths[b] - 1.
  *   page_table int32 [B,max_pages], starts int32 [B+1], lengths int32 [B], all
  *   on the device and read by the kernels only: nothing synchronises, and
- *   nothing out of range in them is followed (starts are clamped to [0,T] and
- *   to ascend, lengths to [0, max_pages * page_size]).
+ *   nothing out of range in them is followed (starts are clamped to [0,T], a
+ *   sequence that ends before it starts has no rows, lengths are clamped to [0,
+ *   max_pages * page_size]). Starts that descend make rows overlap: what these
+ *   hold afterwards is not said.
  * strides[0..2] key codes (page, head, token) in bytes, multiples of 16;
  *   strides[3..5] key scales (page, head, token) in elements; [6..11] values.
  * ---------------------------------------------------------------------- */
@@ -589,10 +591,11 @@ int sparkq_qk_norm_rope(const void* q, const void* k, const void* q_weight,
 
 /* Quantize-on-append of a batch's new tokens into their pages: k and v
  * [T,Hkv,D] with x_strides[0..3] = k token, k head, v token, v head in
- * elements (16-byte aligned rows), quantized by the sparkq_kv_quantize_s8 formula. Rows that fall to
- * no sequence, tokens before position 0 and tokens without a page are
- * skipped; the rest of the pool is untouched. Sequences that append must not
- * share the page that they append to (sparkq_kv_pages_fork sees to that). */
+ * elements (16-byte aligned rows), quantized by the sparkq_kv_quantize_s8
+ * formula. Rows that fall to no sequence, tokens before position 0 and tokens
+ * without a page are skipped; the rest of the pool is untouched. Sequences that
+ * append must not share the page that they append to (sparkq_kv_pages_fork sees
+ * to that). */
 int sparkq_paged_kv_append(const void* k, const void* v, void* k_codes, void* k_scales,
                            void* v_codes, void* v_scales, const int32_t* page_table,
                            const int32_t* starts, const int32_t* lengths, int64_t T,
@@ -603,17 +606,20 @@ int sparkq_paged_kv_append(const void* k, const void* v, void* k_codes, void* k_
 
 /* Attention of a batch's new tokens over their pages: q [T,Hq,D] (BF16 or
  * F16) with q_strides[0..1] = token, head in elements (16-byte aligned rows),
- * out [T,Hq,D] contiguous in out_dtype (q_dtype or F32). The scales of a page
- * and head are contiguous (token stride 1), page and head strides multiples of
- * 8, both scale tensors 16-byte aligned. causal = 1: row i of a sequence's n
- * sees its tokens 0 .. length - n + i; 0: all of them. Tokens without a page are
- * hidden; a row that sees nothing is zero; rows of out that fall to no sequence
- * are left as they were. max_new bounds the new tokens of one sequence: of
- * longer ones the rows past it are left as they were too. A chunk of one token
- * per sequence is the decode step. Scores, normalizer and sums are fp32; a
- * weight times its value's scale is rounded to fp16 once. Workspace:
- * sparkq_paged_sdpa_workspace_bytes (max_tokens = max_pages * page_size), any
- * initial value. */
+ * out [T,Hq,D] contiguous in out_dtype (q_dtype or F32), apart from the inputs.
+ * Keys and values have the same strides; the scales of a page and head are
+ * contiguous (token stride 1), page and head strides multiples of 8, both scale
+ * tensors 16-byte aligned; pages lie less than 32 GiB apart and a head's tokens
+ * within a page span less than 2 GiB (each SPARKQ_ERR_UNSUPPORTED). causal =
+ * 1: row i of a sequence's n sees its tokens 0 .. length - n + i; 0: all of
+ * them. Tokens without a page are hidden; a row that sees nothing is zero; rows
+ * of out that fall to no sequence are left as they were. max_new bounds the new
+ * tokens of one sequence: of longer ones the rows past it are left as they were
+ * too. A chunk of one token per sequence is the decode step. Scores, normalizer
+ * and sums are fp32; a weight times its value's scale is rounded to fp16 once
+ * (from 2^-19 of the row's largest down, to 2^-29 of that).
+ * Workspace: sparkq_paged_sdpa_workspace_bytes (max_tokens = max_pages *
+ * page_size), any initial value. */
 size_t sparkq_paged_sdpa_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv,
                                          int64_t D, int64_t max_new, int64_t max_tokens);
 int sparkq_paged_sdpa(const void* q, const void* k_codes, const void* k_scales,

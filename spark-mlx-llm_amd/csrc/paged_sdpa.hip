@@ -161,8 +161,9 @@ __device__ Item find_item(const PagedSdpaArgs& a, int x) {
       it.part = SPLIT ? 0 : i - k * it.parts;
       it.tile = tiles - 1 - k;  // the last tiles see the most: they start first
       it.slot = of(slot_end - used) + k * it.parts;
-      // sequences whose starts overlap are more than the workspace is for
-      if (it.parts > 1 && it.slot + it.parts > a.slots) it.b = -1;
+      // sequences whose starts overlap are more than the workspace is for, and may be
+      // more than 32 bits count
+      if ((it.parts > 1 && it.slot + it.parts > a.slots) || (unsigned)i >= (unsigned)of(own)) it.b = -1;
       break;
     }
     items = __builtin_amdgcn_readlane(end, 63);

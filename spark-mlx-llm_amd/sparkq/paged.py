@@ -135,7 +135,8 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
     left as they are in `out`, and hold anything in a new tensor. Codes and
     scales of keys lie as those of values do (the same strides), a page's scales
     of a head together. A weight times its value's scale is rounded to float16
-    once; scores, normalizer and sums are fp32."""
+    once (from 2^-19 of the row's largest down, to 2^-29 of that); scores,
+    normalizer and sums are fp32."""
     op = "paged_quantized_sdpa"
     kc, ks, vc, vs, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
     if queries.ndim != 3 or queries.shape[2] != d or not queries.shape[1] \
@@ -185,7 +186,7 @@ def _pool(op, cache):
                            (ks, (page, 1), 2), (vs, (page, 1), 2)):
         s = t.stride()
         k = len(inner)
-        if s[-k:] != inner:
+        if any(x != y and n > 1 for x, y, n in zip(s[-k:], inner, t.shape[-k:])):
             raise ValueError(f"{op}: a page must be contiguous in every tensor of the cache")
         st += (s[0] * size if layered else 0, s[-k - 1] * size)
     return (kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr()), index, \
@@ -263,7 +264,7 @@ class PagedKVCache:
     sequence. A step is
 
         starts = cache.step(new_tokens, parents)     # pages for the new tokens
-        for each layer l:
+        for each layer l:                            # positions: lengths - n .. lengths - 1
             cache.append(l, keys, values)            # packed rows [T,Hkv,D]
             out = cache.attend(l, queries, scale=...)
 
@@ -288,12 +289,14 @@ class PagedKVCache:
         self.starts = torch.zeros((batch + 1,), dtype=torch.int32, device=dev)
         self.missing = torch.zeros((1,), dtype=torch.int32, device=dev)
         self.max_new = 0
+        self._last = None
 
     def step(self, new_tokens, parents=None):
         """Start a step: the batch's rows continue `parents` (itself without)
         and get new_tokens[i] tokens each (a list of Python ints). Returns the
         packed rows' starts. `missing` then counts the pages that the pool was
-        short of (on the device)."""
+        short of (on the device): a caller that may run short reads it before
+        the step's first append, and takes the step back with undo()."""
         new_tokens = [int(n) for n in new_tokens]
         if any(n < 0 for n in new_tokens):
             raise ValueError("new_tokens must not be negative")
@@ -308,10 +311,19 @@ class PagedKVCache:
         ints = torch.tensor(host, dtype=torch.int32, device=dev)
         if parents is not None:
             parents = ints[2 * rows + 1:]
+        self._last = self.page_table, self.lengths, self.starts, self.max_new
         self.page_table, self.lengths, self.missing = kv_pages_fork(
             self.cache, self.page_table, self.lengths, parents, ints[:rows])
         self.starts, self.max_new = ints[rows:2 * rows + 1], max(new_tokens, default=0)
         return self.starts
+
+    def undo(self):
+        """Take back a step that was short of pages, before anything of it was
+        appended: the batch is what it was, and a smaller step can follow."""
+        if self._last is None:
+            raise ValueError("there is no step to take back")
+        self.page_table, self.lengths, self.starts, self.max_new = self._last
+        self._last = None
 
     def layer(self, index: int):
         return tuple(t[index] for t in self.cache)
@@ -328,5 +340,6 @@ class PagedKVCache:
     def compact(self):
         """Returns the number of pages in use (on the device): the pages from
         it on are free."""
+        self._last = None
         self.page_table, used = kv_pages_compact(self.cache, self.page_table, self.lengths)
         return used

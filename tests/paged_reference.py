@@ -61,7 +61,8 @@ def append(keys, values, cache, table, starts, lengths):
 
 
 def attention(q, cache, table, starts, lengths, scale, causal=True, max_new=1 << 30):
-    """(out, sum p|v| / sum p, largest scale * sum |q||k| of the row, written)."""
+    """(out, sum p|v| / sum p, largest scale * sum |q||k| of the row, written, the
+    largest p / sum p times the largest value scale times sum |code|)."""
     kc, ks, vc, vs = cache
     pages, hkv, page, d = kc.shape
     t, hq, _ = q.shape
@@ -69,6 +70,7 @@ def attention(q, cache, table, starts, lengths, scale, causal=True, max_new=1 <<
     mass = torch.zeros((t, hq, d), dtype=torch.float64)
     size = torch.zeros((t, hq), dtype=torch.float64)
     done = torch.zeros(t, dtype=torch.bool)
+    steps = torch.zeros((t, hq, d), dtype=torch.float64)
     g = hq // hkv
     qd = q.double()
     for b in range(len(lengths)):
@@ -85,13 +87,15 @@ def attention(q, cache, table, starts, lengths, scale, causal=True, max_new=1 <<
             p, s = ids[see], pos[see] % page
             k = kc[p, :, s].double() * ks[p, :, s].double()[..., None]  # [n, hkv, d]
             v = vc[p, :, s].double() * vs[p, :, s].double()[..., None]
+            codes, most = vc[p, :, s].double().abs().sum(0), vs[p, :, s].double().abs().amax(0)
             for h in range(hq):
                 sc = (k[:, h // g] @ qd[first + i, h]) * scale
                 w = torch.softmax(sc, 0)
                 out[first + i, h] = w @ v[:, h // g]
                 mass[first + i, h] = w @ v[:, h // g].abs()
+                steps[first + i, h] = w.max() * most[h // g] * codes[h // g]
                 size[first + i, h] = abs(scale) * (k[:, h // g].abs() @ qd[first + i, h].abs()).max()
-    return out, mass, size, done
+    return out, mass, size, done, steps
 
 
 def held(table, lengths, b, pages, page):

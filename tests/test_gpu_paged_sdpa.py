@@ -5,9 +5,14 @@ Tolerance of an output o = sum p v / sum p, with mass = sum p|v| / sum p:
    none in fp32;
  - the weights' one rounding to fp16, in the numerator alone: fp16 has 11 bits,
    so half a step of a weight is at most 2^-11 of it (1 + 2^-11 lies halfway
-   between 1 and the next fp16, 1 + 2^-10), in all 2^-11 mass (weights are
-   scaled so that only those under 2^-19 of the largest fall below fp16's
-   normal range);
+   between 1 and the next fp16, 1 + 2^-10), in all 2^-11 mass;
+ - weights under fp16's normal range, which are rounded to its step of 2^-24
+   instead, by 2^-25 of the unit at most. With s the largest score (log2) and V
+   the largest value scale a row has seen, the unit is 2^(m + e - 6) with m <=
+   ceil(s) < s + 1 and 2^e <= V, so under 2^-5 V 2^s, and all these roundings
+   together add up to less than 2^-30 V 2^s sum |code| / sum p, sum p in units of
+   1: 2^-30 of `steps`. (A sharp softmax needs it: where the code of the one
+   token that counts is 0, the rest is all there is of want and mass.)
  - the scores: fp32 products of exact operands, summed D at a time, times three
    factors: (D + 8) 2^-24 of scale * sum|q||k| (`size`), twice (numerator and
    normalizer), and exp2's 2^-22;
@@ -29,13 +34,14 @@ def _ints(v, gpu):
 
 
 def check(got, q, cache, table, starts, lengths, scale, causal=True, max_new=1 << 30):
-    want, mass, size, done = ref.attention(q, cache, table, starts, lengths, scale, causal, max_new)
+    want, mass, size, done, steps = ref.attention(q, cache, table, starts, lengths, scale, causal,
+                                                  max_new)
     d = q.shape[-1]
     n = max([0, *lengths])
     part = 2.0 ** -11 + 2 * (d + 8) * 2.0 ** -24 * size[..., None] + 2.0 ** -20 + n * 2.0 ** -23
     half = 0 if got.dtype == torch.float32 else torch.finfo(got.dtype).eps / 2
     tiny = 2.0 ** -25 if got.dtype == torch.float16 else 2.0 ** -60
-    part = 1.01 * part * mass
+    part = 1.01 * part * mass + 2.0 ** -30 * steps
     tol = (half * (want.abs() + part)).clamp(min=tiny) + part
     off = ((got.cpu().double() - want).abs() / tol)[done]
     worst = off.max().item() if off.numel() else 0.0
@@ -157,7 +163,7 @@ def test_values_that_no_row_may_see(gpu, new):
         out = run(gpu, q, cache, table, starts, lengths, new).cpu()
         assert out[starts[1] - 1].isnan().all()
         keep = [i for i in range(starts[2]) if i != starts[1] - 1]
-        want, mass, _, _ = ref.attention(q, cache, table, starts, lengths, 128 ** -0.5)
+        want, mass, *_ = ref.attention(q, cache, table, starts, lengths, 128 ** -0.5)
         assert ((out[keep].double() - want[keep]).abs() <= 2.0 ** -7 * mass[keep] + 1e-9).all()
 
 

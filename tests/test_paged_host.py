@@ -280,7 +280,7 @@ def test_fakes_and_a_traced_step():
 
 def test_reference_attention_is_softmax_attention():
     q, _, _, cache_, table, starts = ref.batch(1, [40, 9], [7, 9], 4, 2, 64, 16)
-    out, mass, _, done = ref.attention(q, cache_, table, starts, [40, 9], 0.125)
+    out, mass, _, done, _ = ref.attention(q, cache_, table, starts, [40, 9], 0.125)
     assert done.all() and (mass >= out.abs() - 1e-12).all()
     kc, ks, vc, vs = cache_
     for b, n in ((0, 40), (1, 9)):
