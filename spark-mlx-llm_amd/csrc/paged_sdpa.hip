@@ -12,8 +12,9 @@
 //   paged_few_kernel   at most 16 of them (decode, a few drafted tokens): the
 //                      waves of a workgroup take turns at 32-token blocks and
 //                      combine at the end.
-//   paged_tile_kernel  tiles of 128 rows (64 at D = 256): a block is turned to
-//                      fp16 in LDS once for all of them.
+//   paged_tile_kernel  tiles of 128 rows, D up to 128: a block of 64 tokens is
+//                      turned to fp16 in LDS once for all of them.
+//   paged_pair_kernel  the same at D = 256, where a pair of waves shares its rows.
 //   paged_merge_kernel joins the parts of a context that was split.
 //
 // Work. The lengths live on the device, so every workgroup works out from the
@@ -61,10 +62,12 @@ struct PagedSdpaArgs {
   int target;      // parts of the whole batch, about, per KV head
   int slots;       // parts of split contexts, at most, per KV head
   int min_part;    // tokens of a part, at least
+  int snake;       // items that the chip's CUs take a round of, per KV head (0: in order)
   float scale_log2;
 };
 
-constexpr int kFewBlock = 32;  // tokens of a block
+constexpr int kFewBlock = 32;    // tokens of a block
+constexpr int kTileRows = 128;  // rows of a tile
 
 // ---------------------------------------------------------------------------
 // which work is whose
@@ -81,7 +84,7 @@ struct SeqWork {
   int first, count, length, rows, tiles;
 };
 
-template <int R>  // rows of a tile: 16, 64 or 128
+template <int R>  // rows of a tile: 16 or 128
 __device__ __forceinline__ SeqWork seq_work(const PagedSdpaArgs& a, int b) {
   SeqWork w{0, 0, 0, 0, 0};
   if (b < a.p.B) {
@@ -126,7 +129,7 @@ __device__ __forceinline__ void longest_first(SeqWork& w, int& b, int n) {
 // parts together. (W is summed in fp32, to 2^-17 of itself, which C is enlarged
 // by.) All lanes of a wave take part, and every wave gets the same answers.
 template <int R, bool SPLIT>
-__device__ Item find_item(const PagedSdpaArgs& a, int x) {
+__device__ __forceinline__ Item find_item(const PagedSdpaArgs& a, int x) {
   const int lane = threadIdx.x & 63;
   int b_of = lane;
   SeqWork w0 = seq_work<R>(a, lane);
@@ -214,31 +217,38 @@ __device__ __forceinline__ float sum_groups(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// A row's query values as exact fp16 under a power of two: chunk c of this lane
-// holds dims dim0(c) .. +8. Returns the factor that undoes the shift.
+// two values rounded (to nearest even) into packed fp16: one instruction
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){a, b}, f16x2_t));
+}
+
+// A row's query values as exact fp16: chunk c of this lane holds dims dim0(c) ..
+// +8. bf16 rows are shifted by a power of two for that; returns the factor that
+// undoes it. (What bf16 can hold below 2^-28 of the row's largest is rounded.)
 template <int NK, int G, typename F>
 __device__ __forceinline__ float load_query(const PagedSdpaArgs& a, const uint16_t* row, bool live, F dim0,
                                             u32x4_t qb[NK]) {
-  float top = 0.0f;
-  auto value = [&](u32x4_t w, int i) {
-    const uint16_t bits = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
-    return live ? (a.q_dtype == SPARKQ_BF16 ? bf16_to_f32(bits) : f16_to_f32(bits)) : 0.0f;
-  };
 #pragma unroll
   for (int c = 0; c < NK; ++c) {
     qb[c] = *reinterpret_cast<const u32x4_t*>(row + dim0(c));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(value(qb[c], i)));
+    if (!live) qb[c] = u32x4_t{0, 0, 0, 0};
   }
-  top = max_groups<G>(top);
-  const int e = top > 0.0f && top <= 3.4028235e38f ? ilogbf(top) - 14 : 0;
+  if (a.q_dtype == SPARKQ_F16) return 1.0f;
+  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+  u16x2_t most = {0, 0};
 #pragma unroll
-  for (int c = 0; c < NK; ++c) {
-    const u32x4_t w = qb[c];
+  for (int c = 0; c < NK; ++c)
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      qb[c][i] = pack_round<F16>(ldexpf(value(w, 2 * i), -e), ldexpf(value(w, 2 * i + 1), -e));
-  }
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, qb[c][i] & 0x7FFF7FFFu));
+  const float top = max_groups<G>(bf16_to_f32(most[0] > most[1] ? most[0] : most[1]));
+  const int e = top > 0.0f && top <= 3.4028235e38f ? ilogbf(top) - 14 : 0;
+#pragma unroll
+  for (int c = 0; c < NK; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      qb[c][i] = pack_f16(ldexpf(lo16<BF16>(qb[c][i]), -e), ldexpf(hi16<BF16>(qb[c][i]), -e));
   return ldexpf(1.0f, e);
 }
 
@@ -247,12 +257,6 @@ __device__ __forceinline__ float load_query(const PagedSdpaArgs& a, const uint16
 __device__ __forceinline__ float pinned(float v) {
   asm volatile("" : "+v"(v));
   return v;
-}
-
-// two values rounded (to nearest even) into packed fp16: one instruction
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-  typedef float f32x2_t __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t){a, b}, f16x2_t));
 }
 
 // ---------------------------------------------------------------------------
@@ -593,59 +597,88 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
 // ---------------------------------------------------------------------------
 // tiles of 128 or 64 rows
 // ---------------------------------------------------------------------------
-// Four waves of MT rows each. The products run as above on the MT x MT MFMA: 32
-// rows a wave up to D = 128, 16 at 256, with blocks of 64 and 32 tokens, which is
-// what fits two workgroups a CU in registers and LDS. These are at different
-// places of their blocks, so that one's products and LDS reads run beside the
-// other's softmax (at D = 256 eight waves of 16 rows in one workgroup a CU, all in
-// step, took 368 us for 24 sequences of up to 1000 new tokens, two of four 356).
-// A lane has one row, and of a block the scores i of tokens 4 G (i / 4) + 4 g + i %
-// 4, g its group of the G = 64 / MT: scores 8 s .. +8 are its k-slots of the second
-// product's step s.
+// Four waves of 32 rows each. The products run as above on the 32 x 32 MFMA, a
+// lane has one row, and of a block the scores i of tokens 8 (i / 4) + 4 g + i % 4, g
+// its half of the wave: scores 8 s .. +8 are its k-slots of the second product's
+// step s. 16-row waves read every K and V operand from LDS for half the work: 334
+// us where these took 309 (2048 new tokens of 8192, 32 heads).
 //
 // A block of codes is read once by the workgroup and written to LDS as fp16,
 // token-major, two buffers deep: the next block's codes are converted while this
-// one is computed, and the one after is in flight. K rows are padded by 16 bytes,
-// or at D = 256 their 16-byte chunks XOR-swizzled by the token, so that any 16
-// lanes of a read that the LDS takes together hit different banks; V rows, read
-// transposed, are padded to the same end.
+// one is computed, and the one after is in flight. K rows are padded by 16 bytes, so
+// that any 16 lanes of a read that the LDS takes together hit different banks; V
+// rows, read transposed, are padded to the same end.
+//
+// Two workgroups a CU is what registers (240) and LDS (76 KB) allow; being at
+// different places of their blocks, one's products and LDS reads run beside the
+// other's softmax. 2048 new tokens of 8192, 32 heads of 128, 240 GFLOP: 304 us, 790
+// TFLOP/s. Bound by what a wave can issue: per block of 64 tokens 32 products (1024
+// cycles of the matrix cores), about 350 vector and 75 LDS instructions, 3200
+// cycles in all. Scores one block ahead, so that products and exponentials are
+// independent neighbours in one wave, saved 4% of the cycles and lost as much in
+// clock (2.34 -> 2.22 GHz).
 template <int D>
 struct TileShape {
-  static constexpr int MT = D <= 128 ? 32 : 16, G = 64 / MT;
-  static constexpr int ROWS = 4 * MT;                 // of a workgroup
-  static constexpr int BLOCK = D <= 128 ? 64 : 32;    // tokens
-  static constexpr int N = BLOCK * MT / 64;           // scores a lane
-  static constexpr int KROW = 2 * D + (MT == 32 ? 16 : 0), VROW = 2 * D + (MT == 32 ? 64 : 32);
+  static constexpr int BLOCK = 64;                    // tokens
+  static constexpr int KROW = 2 * D + 16, VROW = 2 * D + 64;
   static constexpr int V = BLOCK * KROW;
   static constexpr int SCALES = V + BLOCK * VROW;     // of keys, of values, the largest of each 16 of these
-  static constexpr int BUF = SCALES + 2 * BLOCK * 4 + 16;
+  static constexpr int BUF = SCALES + 2 * BLOCK * 4 + 32;  // (as many again that are not read)
   static constexpr int BYTES = 2 * BUF;
 };
 
-template <int MT>
-struct TileSum {
-  typedef f32x4_t type;
+// The pages of a block of 64 tokens, PG of them (1, 2 or 4), as offsets into a
+// head's codes and scales: of a wave's pieces i, which lie in runs run0 + i * step
+// of 16 tokens, and of the run srun whose scales it takes. A lane's own offset
+// counts from the block's first token where PG is 1, else from its page's.
+// `ok` says which runs have a page; page 0 stands in for the others, whose tokens
+// are hidden.
+template <int PG, int PPT>
+struct TilePages {
+  uint64_t at[PG == 1 ? 1 : PPT], sat;
+  uint32_t ok;
 };
-template <>
-struct TileSum<32> {
-  typedef f32x16_t type;
-};
-__device__ __forceinline__ f32x4_t tile_mfma(u32x4_t x, u32x4_t y, f32x4_t c) { return mfma16x16x32_f16(x, y, c); }
+template <int PG, int PPT>
+__device__ __forceinline__ TilePages<PG, PPT> tile_pages(const PagedSdpaArgs& a, TableRow row, int t0, int run0,
+                                                         int step, int srun) {
+  const int mask = (1 << a.p.page_log2) - 1;
+  auto look = [&](int run) { return row[min((t0 + 16 * run) >> a.p.page_log2, a.p.width - 1)]; };
+  auto valid = [&](int id) { return (unsigned)id < (unsigned)a.p.pages; };
+  auto keep = [&](int id) { return valid(id) ? id : 0; };
+  TilePages<PG, PPT> r;
+  if constexpr (PG == 1) {
+    const int id = look(0);
+    r.ok = valid(id) ? 15 : 0;
+    r.at[0] = code_at(a.c, keep(id), t0 & mask);
+    r.sat = scale_at(a.c, keep(id), (t0 & mask) + 16 * srun);
+  } else {
+    r.ok = 0;
+#pragma unroll
+    for (int h = 0; h < PG; ++h) r.ok |= (valid(look(4 / PG * h)) ? (1u << 4 / PG) - 1 : 0) << (4 / PG * h);
+#pragma unroll
+    for (int i = 0; i < PPT; ++i) r.at[i] = code_at(a.c, keep(look(run0 + i * step)), 0);
+    r.sat = scale_at(a.c, keep(look(srun)), 16 * srun & mask);
+  }
+  return r;
+}
+
 __device__ __forceinline__ f32x16_t tile_mfma(u32x4_t x, u32x4_t y, f32x16_t c) { return mfma32x32x16<F16>(x, y, c); }
 
-template <int D>
+template <int D, int PG>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
   using S = TileShape<D>;
-  constexpr int MT = S::MT, G = S::G, R = S::ROWS, kBlock = S::BLOCK, N = S::N, Q = kBlock / 16;
-  constexpr int NK = D / (8 * G), NJ = D / MT, NT = kBlock / MT, NV = MT * MT / 64;
+  constexpr int R = kTileRows, kBlock = S::BLOCK, G = 2, N = kBlock / G, Q = kBlock / 16;
+  constexpr int NK = D / 16, NJ = D / 32, NT = kBlock / 32;
   constexpr int PPT = kBlock * D / 16 / 256;  // 16-code pieces of a K (or V) block per thread
-  using Sum = typename TileSum<MT>::type;
+  using Sum = f32x16_t;
   __shared__ __attribute__((aligned(16))) unsigned char smem[S::BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n16 = lane & 15, row = lane % MT, grp = lane / MT;
+  const int n16 = lane & 15, row = lane & 31, grp = lane >> 5;
   const int kh = blockIdx.x % a.Hkv, gqa = a.Hq / a.Hkv;
-  const Item it = find_item<R, false>(a, blockIdx.x / a.Hkv);
+  // the CUs' second workgroups in reverse order: the longest with the shortest
+  const int x = blockIdx.x / a.Hkv;
+  const Item it = find_item<R, false>(a, x >= a.snake && x < 2 * a.snake ? 3 * a.snake - 1 - x : x);
   if (it.b < 0) return;
   const int rw0 = R * it.tile;
   const int rows = min(it.rows - rw0, R);
@@ -655,88 +688,64 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
   const int ib1 = (int)((int64_t)(it.part + 1) * nblocks / it.parts);
   const TableRow trow = table_row(a, it.b);
 
-  const int wr0 = rw0 + MT * wave;  // the wave's first row
+  const int wr0 = rw0 + 32 * wave;  // the wave's first row
   const int rr = wr0 + row, rq = min(rr, it.rows - 1);
   const int lim = last_seen(a, it, rr, gqa);
   u32x4_t qb[NK];
   const uint16_t* qrow = a.q + (it.first + rq / gqa) * a.q_tok + (kh * gqa + rq % gqa) * a.q_head;
-  const float mul = load_query<NK, G>(a, qrow, rr < it.rows, [&](int c) { return 8 * G * c + 8 * grp; }, qb);
+  const float mul = load_query<NK, G>(a, qrow, rr < it.rows, [&](int c) { return 16 * c + 8 * grp; }, qb);
   // what every row of the tile sees
   const int all = __builtin_amdgcn_readfirstlane(last_seen(a, it, rw0, gqa) + 1);
 
-  // Piece p = tid + 256 i of a block: token p / (D / 16), codes 16 (p % (D / 16)).
-  // All tokens of a wave's i-th piece lie in one run of 16, and so in one page.
-  // Wave w < Q also takes the scales of run w: keys in its first 16 lanes, values
-  // in the next. Where blocks do not straddle pages all of a block's addresses are
-  // one offset and the lane's own.
-  const int slot_mask = (1 << a.p.page_log2) - 1;
-  const bool one_page = slot_mask + 1 >= kBlock;
+  // Piece i of a block: token tk0 + i TPP, codes 16 jb .. +16. All tokens of a
+  // wave's piece lie in one run of 16, and so in one page. Wave w also takes the
+  // scales of run w: keys in its first 16 lanes, values in the next, and the same
+  // again in the upper half, which spares branches.
   u32x4_t kcr[PPT], vcr[PPT];
   uint16_t sr;
   const int last = ib1 - 1;
   const uint8_t *const khead = a.c.k + kh * a.c.c_head, *const vhead = a.c.v + kh * a.c.c_head;
-  const uint16_t* const shead = (lane < 16 ? a.c.ks : a.c.vs) + kh * a.c.s_head + n16;
+  const bool ks_lane = !(lane & 16);
+  const uint16_t* const shead = (ks_lane ? a.c.ks : a.c.vs) + kh * a.c.s_head + n16;
   const int tk0 = tid / (D / 16), jb = tid % (D / 16);
   constexpr int TPP = 256 / (D / 16);  // tokens of a round of pieces
-  const uint32_t run_off = (tk0 & 15) * a.c.c_tok + 16 * jb;
   uint32_t off[PPT];
 #pragma unroll
-  for (int i = 0; i < PPT; ++i) off[i] = (tk0 + i * TPP) * a.c.c_tok + 16 * jb;
-  auto load = [&](int ib, const BlockPages<Q>& bp) {
-    const int t0 = kBlock * min(ib, last);
-    if (one_page) {
-      const uint64_t at = code_at(a.c, bp.id[0], t0 & slot_mask);
-      const uint8_t *kp = khead + at, *vp = vhead + at;
-#pragma unroll
-      for (int i = 0; i < PPT; ++i) {
-        kcr[i] = *reinterpret_cast<const u32x4_t*>(kp + off[i]);
-        vcr[i] = *reinterpret_cast<const u32x4_t*>(vp + off[i]);
-      }
-      if (wave < Q) sr = shead[scale_at(a.c, bp.id[0], (t0 & slot_mask) + 16 * wave)];
-    } else {
-      auto page_id = [&](int run) {
-        return run == 0 ? bp.id[0] : Q == 2 || run == 1 ? bp.id[1] : run == 2 ? bp.id[Q - 2] : bp.id[Q - 1];
-      };
-#pragma unroll
-      for (int i = 0; i < PPT; ++i) {
-        const int run = wave * 64 / D + i * (TPP / 16);
-        const uint64_t at = code_at(a.c, page_id(run), (t0 + 16 * run) & slot_mask);
-        kcr[i] = *reinterpret_cast<const u32x4_t*>(khead + at + run_off);
-        vcr[i] = *reinterpret_cast<const u32x4_t*>(vhead + at + run_off);
-      }
-      if (wave < Q) sr = shead[scale_at(a.c, page_id(wave), (t0 + 16 * wave) & slot_mask)];
-    }
+  for (int i = 0; i < PPT; ++i) off[i] = ((tk0 + i * TPP) & (kBlock / PG - 1)) * a.c.c_tok + 16 * jb;
+  using Pages = TilePages<PG, PPT>;
+  auto pages = [&](int ib) {
+    return tile_pages<PG, PPT>(a, trow, kBlock * min(ib, last), wave * 64 / D, TPP / 16, wave);
   };
-  auto kswz = [](int t) { return MT == 32 ? 0 : t & 15; };
-  unsigned char* const kput0 = smem + tk0 * S::KROW + 16 * ((2 * jb) ^ kswz(tk0));
-  unsigned char* const kput1 = smem + tk0 * S::KROW + 16 * ((2 * jb + 1) ^ kswz(tk0));
+  auto load = [&](const Pages& bp) {
+#pragma unroll
+    for (int i = 0; i < PPT; ++i) {
+      kcr[i] = *reinterpret_cast<const u32x4_t*>(khead + bp.at[PG == 1 ? 0 : i] + off[i]);
+      vcr[i] = *reinterpret_cast<const u32x4_t*>(vhead + bp.at[PG == 1 ? 0 : i] + off[i]);
+    }
+    sr = shead[bp.sat];
+  };
+  unsigned char* const kput = smem + tk0 * S::KROW + 32 * jb;
   unsigned char* const vput = smem + S::V + tk0 * S::VROW + 32 * jb;
+  float* const sput = reinterpret_cast<float*>(smem + S::SCALES) + (ks_lane ? 0 : kBlock) + 16 * wave + n16;
+  float* const bput = reinterpret_cast<float*>(smem + S::SCALES) + 2 * kBlock + (ks_lane ? 4 : 0) + wave;
   auto stage = [&](auto bufc) {
     constexpr int at = decltype(bufc)::value * S::BUF;
 #pragma unroll
     for (int i = 0; i < PPT; ++i) {
-      *reinterpret_cast<u32x4_t*>(kput0 + at + i * TPP * S::KROW) = s8x8_exact(kcr[i].x, kcr[i].y);
-      *reinterpret_cast<u32x4_t*>(kput1 + at + i * TPP * S::KROW) = s8x8_exact(kcr[i].z, kcr[i].w);
-      unsigned char* vt = vput + at + i * TPP * S::VROW;
+      unsigned char *kt = kput + at + i * TPP * S::KROW, *vt = vput + at + i * TPP * S::VROW;
+      *reinterpret_cast<u32x4_t*>(kt) = s8x8_exact(kcr[i].x, kcr[i].y);
+      *reinterpret_cast<u32x4_t*>(kt + 16) = s8x8_exact(kcr[i].z, kcr[i].w);
       *reinterpret_cast<u32x4_t*>(vt) = s8x8_exact(vcr[i].x, vcr[i].y);
       *reinterpret_cast<u32x4_t*>(vt + 16) = s8x8_exact(vcr[i].z, vcr[i].w);
     }
-    if (wave < Q) {
-      float* sc = reinterpret_cast<float*>(smem + at + S::SCALES);
-      const float v = f16_to_f32(sr);
-      const float big = max_row16(fabsf(v) <= 65504.0f ? fabsf(v) : __builtin_huge_valf());
-      if (lane < 32) sc[(lane < 16 ? 0 : kBlock) + 16 * wave + n16] = lane < 16 ? v * a.scale_log2 : kept_scale(v);
-      if (lane == 16) sc[2 * kBlock + wave] = big;
-    }
+    const float v = f16_to_f32(sr);
+    sput[at / 4] = ks_lane ? v * a.scale_log2 : kept_scale(v);
+    bput[at / 4] = max_row16(fabsf(v) <= 65504.0f ? fabsf(v) : __builtin_huge_valf());
   };
 
-  // chunk G kk + g of token `row`; swizzled chunks kk and kk + 4 are 256 bytes apart
-  constexpr int KP = MT == 32 ? 1 : 4;
-  const unsigned char* kget[KP];
-#pragma unroll
-  for (int kk = 0; kk < KP; ++kk) kget[kk] = smem + row * S::KROW + 16 * ((G * kk + grp) ^ kswz(row));
+  const unsigned char* const kget = smem + row * S::KROW + 16 * grp;  // chunk 2 kk + g of token `row`
   const unsigned char* const vget = smem + S::V + (4 * grp + (n16 >> 2)) * S::VROW + 8 * (n16 & 3) +
-                                    (MT == 32 ? 32 * ((lane >> 4) & 1) : 0);
+                                    32 * ((lane >> 4) & 1);
   const float* const sget = reinterpret_cast<const float*>(smem + S::SCALES) + 4 * grp;
   RowState st;
   Sum acc[NJ];
@@ -750,10 +759,8 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
     for (int tt = 0; tt < NT; ++tt) {
       sc[tt] = Sum{};
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) {
-        const unsigned char* kp = kget[kk % KP] + at + tt * MT * S::KROW + 16 * G * KP * (kk / KP);
-        sc[tt] = tile_mfma(*reinterpret_cast<const u32x4_t*>(kp), qb[kk], sc[tt]);
-      }
+      for (int kk = 0; kk < NK; ++kk)
+        sc[tt] = tile_mfma(*reinterpret_cast<const u32x4_t*>(kget + at + tt * 32 * S::KROW + 32 * kk), qb[kk], sc[tt]);
     }
     const float* scl = sget + at / 4;
     float vsc[N], s[N];
@@ -764,7 +771,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         vsc[i + r] = v4[r];
-        s[i + r] = sc[i / NV][i % NV + r] * k4[r];
+        s[i + r] = sc[i / 16][i % 16 + r] * k4[r];
       }
     }
     const float* big = reinterpret_cast<const float*>(smem + at + S::SCALES) + 2 * kBlock;
@@ -794,29 +801,29 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
     for (int k = 0; k < N / 8; ++k)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const unsigned char* vp = vget + at + 8 * G * k * S::VROW + 2 * MT * j;
+        const unsigned char* vp = vget + at + 16 * k * S::VROW + 64 * j;
         const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (__attribute__((address_space(3))) s16x4_t*)(vp)));
         const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4_t*)(vp + 4 * G * S::VROW)));
+            (__attribute__((address_space(3))) s16x4_t*)(vp + 8 * S::VROW)));
         acc[j] = tile_mfma(u32x4_t{lo.x, lo.y, hi.x, hi.y}, w[k], acc[j]);
       }
   };
 
   if (ib0 < ib1) {
-    BlockPages<Q> bp = block_pages<Q>(a, trow, kBlock * ib0);
+    Pages bp = pages(ib0);
     uint32_t ok_now = bp.ok, ok_next;
-    load(ib0, bp);
-    bp = block_pages<Q>(a, trow, kBlock * min(ib0 + 1, last));
+    load(bp);
+    bp = pages(ib0 + 1);
     stage(std::integral_constant<int, 0>{});
-    load(ib0 + 1, bp);
+    load(bp);
     ok_next = bp.ok;
     __syncthreads();
     auto step = [&](int ib, auto cur) {
-      const BlockPages<Q> after = block_pages<Q>(a, trow, kBlock * min(ib + 2, last));
+      const Pages after = pages(ib + 2);
       if (wr0 < it.rows) compute(cur, kBlock * ib, ok_now);
       stage(std::integral_constant<int, 1 - decltype(cur)::value>{});
-      load(ib + 2, after);
+      load(after);
       ok_now = ok_next;
       ok_next = after.ok;
       __syncthreads();
@@ -830,7 +837,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
   }
 
   const float z = sum_groups<G>(st.z);
-  const int r = MT * wave + row;
+  const int r = 32 * wave + row;
   if (r >= rows) return;
   if (it.parts == 1) {
     const int64_t at = out_row(a, it, kh, rw0 + r, gqa) * D;
@@ -838,18 +845,286 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int v = 0; v < NV; v += 4)
-        store_row4(a, at + MT * j + G * v + 4 * grp,
+      for (int v = 0; v < 16; v += 4)
+        store_row4(a, at + 32 * j + 2 * v + 4 * grp,
                    f32x4_t{acc[j][v], acc[j][v + 1], acc[j][v + 2], acc[j][v + 3]} * inv);
   } else {
     const int64_t at = ((int64_t)kh * a.slots + it.slot + it.part) * R + r;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int v = 0; v < NV; v += 4)
-        *reinterpret_cast<f32x4_t*>(a.pacc + at * D + MT * j + G * v + 4 * grp) =
+      for (int v = 0; v < 16; v += 4)
+        *reinterpret_cast<f32x4_t*>(a.pacc + at * D + 32 * j + 2 * v + 4 * grp) =
             f32x4_t{acc[j][v], acc[j][v + 1], acc[j][v + 2], acc[j][v + 3]};
     if (grp == 0) {
+      a.pm[at] = part_max(st, z);
+      a.pz[at] = z;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// tiles of 128 rows, D = 256
+// ---------------------------------------------------------------------------
+// The outputs of 32 rows of 256 take 128 registers a lane and their queries 64: one
+// wave a SIMD. So a pair of waves shares 32 rows: each scores one half of a block's
+// 64 tokens over all dims, hands its weights to the other through LDS, and sums all
+// 64 tokens' values of its half of the dims. Eight waves a CU, every operand from
+// LDS is used for 32 rows, and a block's conversion is shared by 512 threads.
+// (24 sequences of up to 1000 new tokens, 166 GFLOP, 16 heads of 256: 296 us, 560
+// TFLOP/s; waves of 16 rows with all dims 346, waves of 32 rows alone on their SIMDs
+// 376.)
+//
+// Both waves weigh in the units of their own running maxima; where these differ
+// after a block (hardly ever: they move in steps of 2^8) both go on with the larger.
+//
+// A block has two phases. In the first its keys are read and its values are written
+// to LDS, in the second the values are read and the next keys are written: one buffer
+// of each and a barrier after each phase. (Half the waves a phase behind the others,
+// with two buffers, took 306 us.) Bound by the latency of a wave's own chain through
+// these phases.
+struct PairShape {
+  static constexpr int D = 256, BLOCK = 64;
+  static constexpr int KROW = 2 * D + 16, VROW = 2 * D + 64;
+  static constexpr int V = BLOCK * KROW, P = V + BLOCK * VROW;
+  static constexpr int STATE = P + 8 * 2 * 1024;      // of each wave's rows: maximum, scale exponent
+  static constexpr int SCALES = STATE + 8 * 32 * 8;   // of keys, of values, the largest of each 16 of these
+  static constexpr int BYTES = SCALES + 2 * BLOCK * 4 + 16;
+};
+
+template <int PG>  // pages that a block lies in: 1, 2 or 4
+__global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
+  using S = PairShape;
+  constexpr int D = S::D, R = kTileRows, kBlock = S::BLOCK, N = 16, Q = kBlock / 16, G = 2;
+  constexpr int NK = D / 16, NJ = 4, PPT = 2;
+  using Sum = f32x16_t;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[S::BYTES];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = wave & 1;
+  const int n16 = lane & 15, row = lane & 31, grp = lane >> 5;
+  const int kh = blockIdx.x % a.Hkv, gqa = a.Hq / a.Hkv;
+  const Item it = find_item<R, false>(a, blockIdx.x / a.Hkv);
+  if (it.b < 0) return;
+  const int rw0 = R * it.tile;
+  const int rows = min(it.rows - rw0, R);
+  const int seen = last_seen(a, it, rw0 + rows - 1, gqa) + 1;
+  const int nblocks = (seen + kBlock - 1) / kBlock;
+  const int ib0 = (int)((int64_t)it.part * nblocks / it.parts);
+  const int ib1 = (int)((int64_t)(it.part + 1) * nblocks / it.parts);
+  const TableRow trow = table_row(a, it.b);
+
+  const int wr0 = rw0 + 32 * (wave >> 1);  // the pair's first row
+  const int rr = wr0 + row, rq = min(rr, it.rows - 1);
+  const int lim = last_seen(a, it, rr, gqa);
+  const bool live = wr0 < it.rows;
+  u32x4_t qb[NK];
+  const uint16_t* qrow = a.q + (it.first + rq / gqa) * a.q_tok + (kh * gqa + rq % gqa) * a.q_head;
+  const float mul = load_query<NK, G>(a, qrow, rr < it.rows, [&](int c) { return 16 * c + 8 * grp; }, qb);
+  const int all = __builtin_amdgcn_readfirstlane(last_seen(a, it, rw0, gqa) + 1);
+
+  // Piece i of a block: token tk0 + 32 i, codes 16 jb .. +16. A wave's pieces lie in
+  // runs 2 i + wave / 4 of 16 tokens, and it takes the scales of run wave % 4.
+  u32x4_t kcr[PPT], vcr[PPT];
+  uint16_t skr, svr;
+  const int last = ib1 - 1, srun = wave & 3;
+  const uint8_t *const khead = a.c.k + kh * a.c.c_head, *const vhead = a.c.v + kh * a.c.c_head;
+  const uint16_t *const kshead = a.c.ks + kh * a.c.s_head + n16, *const vshead = a.c.vs + kh * a.c.s_head + n16;
+  const int tk0 = tid >> 4, jb = tid & 15;
+  uint32_t off[PPT];
+#pragma unroll
+  for (int i = 0; i < PPT; ++i) off[i] = ((tk0 + 32 * i) & (kBlock / PG - 1)) * a.c.c_tok + 16 * jb;
+  using Pages = TilePages<PG, PPT>;
+  auto pages = [&](int ib) __attribute__((always_inline)) {
+    return tile_pages<PG, PPT>(a, trow, kBlock * min(ib, last), wave >> 2, 2, srun);
+  };
+  auto load_codes = [&](const uint8_t* head, const Pages& bp, u32x4_t (&r)[PPT]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PPT; ++i)
+      r[i] = *reinterpret_cast<const u32x4_t*>(head + bp.at[PG == 1 ? 0 : i] + off[i]);
+  };
+  auto load_scales = [&](const Pages& bp) __attribute__((always_inline)) {
+    skr = kshead[bp.sat];
+    svr = vshead[bp.sat];
+  };
+  unsigned char* const kput = smem + tk0 * S::KROW + 32 * jb;
+  unsigned char* const vput = smem + S::V + tk0 * S::VROW + 32 * jb;
+  auto stage = [&](unsigned char* t, u32x4_t c) __attribute__((always_inline)) {
+    *reinterpret_cast<u32x4_t*>(t) = s8x8_exact(c.x, c.y);
+    *reinterpret_cast<u32x4_t*>(t + 16) = s8x8_exact(c.z, c.w);
+  };
+  float* const scl = reinterpret_cast<float*>(smem + S::SCALES);
+  auto stage_scales = [&]() __attribute__((always_inline)) {
+    const float v = f16_to_f32(svr);
+    scl[16 * srun + n16] = f16_to_f32(skr) * a.scale_log2;
+    scl[kBlock + 16 * srun + n16] = kept_scale(v);
+    scl[2 * kBlock + srun] = max_row16(fabsf(v) <= 65504.0f ? fabsf(v) : __builtin_huge_valf());
+  };
+
+  const unsigned char* const kget = smem + (32 * half + row) * S::KROW + 16 * grp;
+  const unsigned char* const vget = smem + S::V + (4 * grp + (n16 >> 2)) * S::VROW + 8 * (n16 & 3) +
+                                    32 * ((lane >> 4) & 1) + 256 * half;
+  unsigned char* const pput = smem + S::P + wave * 2048 + lane * 16;
+  const unsigned char* const pget = smem + S::P + (wave ^ 1) * 2048 + lane * 16;
+  float2* const state = reinterpret_cast<float2*>(smem + S::STATE);
+  const int own = 32 * half * S::VROW, other = 32 * (half ^ 1) * S::VROW;
+  RowState st;
+  Sum acc[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) acc[j] = Sum{};
+  u32x4_t w[4];  // of the half of this wave, of the other
+
+  // scores and weights of this wave's 32 tokens, and values into LDS
+  auto first = [&](int t0, uint32_t pages_ok) __attribute__((always_inline)) {
+    Sum sc = Sum{};
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      sc = tile_mfma(*reinterpret_cast<const u32x4_t*>(kget + 32 * kk), qb[kk], sc);
+      if (kk == 4 || kk == 8) stage(vput + (kk / 4 - 1) * 32 * S::VROW, vcr[kk / 4 - 1]);
+    }
+    const float* ks = scl + 32 * half + 4 * grp;
+    float s[N], vsc[N];
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const f32x4_t k4 = *reinterpret_cast<const f32x4_t*>(ks + G * i);
+      const f32x4_t v4 = *reinterpret_cast<const f32x4_t*>(ks + kBlock + G * i);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        vsc[i + r] = v4[r];
+        s[i + r] = sc[i + r] * k4[r];
+      }
+    }
+    const f32x4_t big = *reinterpret_cast<const f32x4_t*>(scl + 2 * kBlock);
+    float size = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+    if (__builtin_expect(t0 + kBlock > all || pages_ok != (1u << Q) - 1 || size > 65504.0f, 0)) {
+      uint32_t ok = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int t = 32 * half + 4 * G * (i >> 2) + 4 * grp + (i & 3);
+        ok |= (uint32_t)(t0 + t <= lim && ((pages_ok >> (t / 16)) & 1u)) << i;
+      }
+      size = hide<N, G>(__float_as_uint(pinned(__uint_as_float(ok))), s, vsc);
+    }
+    bool up;
+    const float alpha = row_block<N, G>(st, s, mul, vsc, size, w, up);
+    if (__builtin_expect(__ballot(up) != 0, 0)) {
+      const float f = pinned(up ? alpha : 1.0f);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[j] *= f;
+    }
+    *reinterpret_cast<u32x4_t*>(pput) = w[0];
+    *reinterpret_cast<u32x4_t*>(pput + 1024) = w[1];
+    state[32 * wave + row] = make_float2(st.m, st.e);
+  };
+  // the outputs of this wave's 128 dims, and the next keys into LDS
+  auto second = [&](int) __attribute__((always_inline)) {
+    w[2] = *reinterpret_cast<const u32x4_t*>(pget);
+    w[3] = *reinterpret_cast<const u32x4_t*>(pget + 1024);
+    const float2 o = state[32 * (wave ^ 1) + row];
+    typedef short s16x4_t __attribute__((ext_vector_type(4)));
+    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+    auto product = [&](int k, int j) __attribute__((always_inline)) {
+      const unsigned char* vp = vget + (k < 2 ? own : other) + 16 * (k & 1) * S::VROW + 64 * j;
+      const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4_t*)(vp)));
+      const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4_t*)(vp + 8 * S::VROW)));
+      acc[j] = tile_mfma(u32x4_t{lo.x, lo.y, hi.x, hi.y}, w[k], acc[j]);
+    };
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        product(k, j);
+        if (k == 1 && j < PPT) stage(kput + j * 32 * S::KROW, kcr[j]);
+      }
+    const float mine = unit(st), theirs = o.x + (o.y - 6.0f);
+    if (__builtin_expect(__ballot(mine != theirs) != 0, 0)) {
+      st.m = fmaxf(st.m, o.x);
+      st.e = fmaxf(st.e, o.y);
+      const float now = unit(st);
+      auto factor = [&](float u) { return u == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(u - now); };
+      const float fm = pinned(factor(mine)), ft = factor(theirs);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[j] *= fm;
+      st.z *= fm;
+#pragma unroll
+      for (int i = 2; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[i][k] = pack_f16(lo16<F16>(w[i][k]) * ft, hi16<F16>(w[i][k]) * ft);
+    }
+#pragma unroll
+    for (int k = 2; k < 4; ++k)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) product(k, j);
+  };
+
+  if (ib0 < ib1) {
+    Pages now = pages(ib0), next = pages(ib0 + 1);
+    load_codes(khead, now, kcr);
+    load_scales(now);
+#pragma unroll
+    for (int i = 0; i < PPT; ++i) stage(kput + i * 32 * S::KROW, kcr[i]);
+    stage_scales();
+    load_codes(vhead, now, vcr);
+    load_codes(khead, next, kcr);
+    load_scales(next);
+    __syncthreads();
+    auto block = [&](int ib, auto one, auto two) __attribute__((always_inline)) {
+      const Pages after = pages(ib + 2);
+      one();
+      load_codes(vhead, next, vcr);
+      __syncthreads();
+      two();
+      stage_scales();
+      load_codes(khead, after, kcr);
+      load_scales(after);
+      now = next;
+      next = after;
+      __syncthreads();
+    };
+    if (live) {
+      for (int ib = ib0; ib < ib1; ++ib)
+        block(ib, [&]() __attribute__((always_inline)) { first(kBlock * ib, now.ok); },
+              [&]() __attribute__((always_inline)) { second(ib); });
+    } else {
+      for (int ib = ib0; ib < ib1; ++ib)
+        block(ib,
+              [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < PPT; ++i) stage(vput + i * 32 * S::VROW, vcr[i]);
+              },
+              [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < PPT; ++i) stage(kput + i * 32 * S::KROW, kcr[i]);
+              });
+    }
+  }
+
+  // the halves' sums (every wave is past its last read of the states)
+  float z = sum_groups<G>(st.z);
+  state[32 * wave + row].x = z;
+  __syncthreads();
+  z += state[32 * (wave ^ 1) + row].x;
+  const int r = 32 * (wave >> 1) + row;
+  if (r >= rows) return;
+  if (it.parts == 1) {
+    const int64_t at = out_row(a, it, kh, rw0 + r, gqa) * D + 128 * half;
+    const float inv = z != 0.0f ? 1.0f / z : 1.0f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; v += 4)
+        store_row4(a, at + 32 * j + 2 * v + 4 * grp,
+                   f32x4_t{acc[j][v], acc[j][v + 1], acc[j][v + 2], acc[j][v + 3]} * inv);
+  } else {
+    const int64_t at = ((int64_t)kh * a.slots + it.slot + it.part) * R + r;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; v += 4)
+        *reinterpret_cast<f32x4_t*>(a.pacc + at * D + 128 * half + 32 * j + 2 * v + 4 * grp) =
+            f32x4_t{acc[j][v], acc[j][v + 1], acc[j][v + 2], acc[j][v + 3]};
+    if (grp == 0 && half == 0) {
       a.pm[at] = part_max(st, z);
       a.pz[at] = z;
     }
@@ -935,7 +1210,7 @@ struct PagedPlan {
   int rows;           // of a tile
   int64_t max_tiles;  // of the whole batch, at most
   int64_t target, slots, split;  // parts to aim at, parts and tiles of split contexts at most
-  int min_part;
+  int min_part, snake;
 };
 
 PagedPlan paged_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
@@ -944,13 +1219,25 @@ PagedPlan paged_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
   const int64_t gqa = Hq / Hkv;
   max_new = std::min(max_new, T);
   p.few = max_new * gqa <= 16;
-  p.rows = p.few ? 16 : D <= 128 ? TileShape<128>::ROWS : TileShape<256>::ROWS;
+  p.rows = p.few ? 16 : kTileRows;
   p.min_part = 128;
   p.max_tiles = std::min(T * gqa / p.rows + B, B * cdiv(max_new * gqa, p.rows));
   p.target = std::min<int64_t>(cdiv((p.few ? 4 : 2) * device_cus(), Hkv), kMaxParts);
   p.split = max_tokens > p.min_part ? std::min(p.max_tiles, p.target) : 0;
   p.slots = std::min(2 * p.target, p.split * cdiv(max_tokens, p.min_part));
+  // where the heads' items are dealt to the CUs evenly, and the grid holds the
+  // round that is reversed
+  p.snake = D <= 128 && device_cus() % Hkv == 0 && p.slots + p.max_tiles >= 2 * device_cus() / Hkv
+                ? (int)(device_cus() / Hkv) : 0;
   return p;
+}
+
+template <int D, int PG>
+void launch_tile(const PagedSdpaArgs& a, dim3 grid, hipStream_t st) {
+  if constexpr (D <= 128)
+    hipLaunchKernelGGL((paged_tile_kernel<D, PG>), grid, dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL(paged_pair_kernel<PG>, grid, dim3(512), 0, st, a);
 }
 
 template <int D>
@@ -959,13 +1246,17 @@ void launch_paged(const PagedSdpaArgs& a, const PagedPlan& p, hipStream_t st) {
   const dim3 merge((unsigned)(p.split * (p.rows / 16) * a.Hkv));
   if (p.few)
     hipLaunchKernelGGL(paged_few_kernel<D>, grid, dim3(256), 0, st, a);
+  else if (a.p.page_log2 >= 6)
+    launch_tile<D, 1>(a, grid, st);
+  else if (a.p.page_log2 == 5)
+    launch_tile<D, 2>(a, grid, st);
   else
-    hipLaunchKernelGGL(paged_tile_kernel<D>, grid, dim3(256), 0, st, a);
+    launch_tile<D, 4>(a, grid, st);
   if (merge.x == 0) return;
   if (p.few)
     hipLaunchKernelGGL((paged_merge_kernel<D, 16>), merge, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL((paged_merge_kernel<D, TileShape<D>::ROWS>), merge, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_merge_kernel<D, kTileRows>), merge, dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -994,7 +1285,8 @@ int paged_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, const Pag
                      (uint32_t)(ks.s_page / 8), (uint32_t)ks.c_tok};
   const PagedSdpaArgs a{p, (const uint16_t*)q, qst[0], qst[1], c, out, acc + n * D, acc + n * (D + 1), acc,
                         (int)Hq, (int)Hkv, (int)std::min<int64_t>(max_new, p.T), causal, qdt, odt,
-                        (int)plan.target, (int)plan.slots, plan.min_part, scale * 1.44269504088896340736f};
+                        (int)plan.target, (int)plan.slots, plan.min_part, plan.snake,
+                        scale * 1.44269504088896340736f};
   if (D == 64)
     launch_paged<64>(a, plan, st);
   else if (D == 128)
