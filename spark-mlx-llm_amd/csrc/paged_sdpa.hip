@@ -871,9 +871,9 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
 // 64 tokens over all dims, hands its weights to the other through LDS, and sums all
 // 64 tokens' values of its half of the dims. Eight waves a CU, every operand from
 // LDS is used for 32 rows, and a block's conversion is shared by 512 threads.
-// (24 sequences of up to 1000 new tokens, 166 GFLOP, 16 heads of 256: 296 us, 560
-// TFLOP/s; waves of 16 rows with all dims 346, waves of 32 rows alone on their SIMDs
-// 376.)
+// (24 sequences of up to 1000 new tokens, 166 GFLOP, 16 heads of 256: 271 us, 613
+// TFLOP/s. Before the contexts' split was tuned to it 296, where waves of 16 rows
+// with all dims took 346, and waves of 32 rows alone on their SIMDs 376.)
 //
 // Both waves weigh in the units of their own running maxima; where these differ
 // after a block (hardly ever: they move in steps of 2^8) both go on with the larger.
@@ -881,7 +881,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
 // A block has two phases. In the first its keys are read and its values are written
 // to LDS, in the second the values are read and the next keys are written: one buffer
 // of each and a barrier after each phase. (Half the waves a phase behind the others,
-// with two buffers, took 306 us.) Bound by the latency of a wave's own chain through
+// with two buffers, took 306 us for these 296.) Bound by the latency of a wave's own chain through
 // these phases.
 struct PairShape {
   static constexpr int D = 256, BLOCK = 64;
@@ -1222,7 +1222,10 @@ PagedPlan paged_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
   p.rows = p.few ? 16 : kTileRows;
   p.min_part = 128;
   p.max_tiles = std::min(T * gqa / p.rows + B, B * cdiv(max_new * gqa, p.rows));
-  p.target = std::min<int64_t>(cdiv((p.few ? 4 : 2) * device_cus(), Hkv), kMaxParts);
+  // a part for each workgroup that the chip holds at once, or a few more: decodes
+  // are bound by memory, where more in flight count (three workgroups a CU); a pair
+  // tile has a CU to itself (294 us with two parts a CU where one takes 271)
+  p.target = std::min<int64_t>(cdiv((p.few ? 4 : D <= 128 ? 2 : 1) * device_cus(), Hkv), kMaxParts);
   p.split = max_tokens > p.min_part ? std::min(p.max_tiles, p.target) : 0;
   p.slots = std::min(2 * p.target, p.split * cdiv(max_tokens, p.min_part));
   // where the heads' items are dealt to the CUs evenly, and the grid holds the
