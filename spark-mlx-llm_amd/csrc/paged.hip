@@ -235,7 +235,8 @@ __device__ __forceinline__ int write_page(const PageArgs& a, const RowPlan& r) {
 
 // Counters of a plan's pages, in LDS (up to kLdsPages) or, of larger pools, in
 // the workspace: there through device-scope atomics, which are coherent whatever
-// the vector cache holds.
+// the vector cache holds (a fork of 256 rows in 2048 pages 27.8 us, with counters in
+// the workspace 38.0; of 1024 rows in 16384 pages 37.3 and 62.3).
 constexpr int kLdsPages = 16384;
 template <bool LDS>
 struct Counters {
@@ -316,7 +317,8 @@ __device__ void count_held(const PageArgs& a, const Counters<LDS>& held, int (&s
   plan_sync<LDS>();
 }
 
-// One workgroup. Three passes over the pages' counters, two over the rows.
+// One workgroup. Three passes over the pages' counters, two over the rows: bound by
+// latency, 5.4 us for 8 rows of 512 pages, 7 us for 256 rows of 2048.
 template <bool LDS>
 __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PageArgs a) {
   extern __shared__ int s_pages[];
@@ -373,7 +375,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PageArgs 
 }
 
 // One workgroup. A page that moves keeps in held the (inverted) place of its new
-// number in the list.
+// number in the list. 3.5 us for 4 rows of 256 pages, 4.7 us for 96 of 2048.
 template <bool LDS>
 __global__ __launch_bounds__(kPlanThreads) void pages_compact_plan_kernel(PageArgs a) {
   extern __shared__ int s_pages[];

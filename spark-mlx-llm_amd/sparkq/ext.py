@@ -979,15 +979,19 @@ def qk_norm_rope(queries, keys, q_weight, k_weight, positions, *, dims: int, eps
     (the angle fp64) with one rounding at the end, where rms_norm and rope in
     turn round three times."""
     tensors = (queries, keys, q_weight, k_weight, positions)
-    if any(not isinstance(v, torch.Tensor) for v in tensors):
-        raise TypeError("queries, keys, weights and positions must be tensors")
+    for v in tensors:
+        if not isinstance(v, torch.Tensor):
+            raise TypeError("queries, keys, weights and positions must be tensors")
     qshape, kshape = queries.shape, keys.shape
-    if len(qshape) != 3 or len(kshape) != 3 or kshape[0] != qshape[0] or kshape[2] != qshape[2] \
-            or not qshape[1] or not kshape[1] or not qshape[2]:
+    if len(qshape) != 3 or len(kshape) != 3:
         raise ValueError("qk_norm_rope requires queries [T,Hq,D] and keys [T,Hkv,D]")
     t, hq, d = qshape
+    kt, hkv, kd = kshape
+    if kt != t or kd != d or not hq or not hkv or not d:
+        raise ValueError("qk_norm_rope requires queries [T,Hq,D] and keys [T,Hkv,D]")
     dtype = queries.dtype
-    if dtype not in _HALF or any(v.dtype is not dtype for v in (keys, q_weight, k_weight)):
+    if dtype not in _HALF or keys.dtype is not dtype or q_weight.dtype is not dtype \
+            or k_weight.dtype is not dtype:
         raise ValueError("qk_norm_rope requires BF16 or F16 queries, keys and weights of one dtype")
     if q_weight.shape != (d,) or k_weight.shape != (d,):
         raise ValueError(f"qk_norm_rope weights must have shape [{d}]")
@@ -996,10 +1000,13 @@ def qk_norm_rope(queries, keys, q_weight, k_weight, positions, *, dims: int, eps
         raise ValueError(f"qk_norm_rope positions must be int32 or int64 of shape [{t}]")
     if type(dims) is not int:
         raise ValueError("qk_norm_rope dims must be an int")
-    _require_device("qk_norm_rope", *tensors)
     index = queries.get_device()
-    if any(v.get_device() != index for v in tensors):
-        raise ValueError("qk_norm_rope tensors must live on one device")
+    for v in tensors:
+        i = v.get_device()
+        if i < 0:
+            raise ValueError("qk_norm_rope requires GPU execution")
+        if i != index:
+            raise ValueError("qk_norm_rope tensors must live on one device")
     qst, kst = queries.stride(), keys.stride()
     if qst[2] != 1:
         queries = queries.contiguous()
@@ -1007,14 +1014,13 @@ def qk_norm_rope(queries, keys, q_weight, k_weight, positions, *, dims: int, eps
     if kst[2] != 1:
         keys = keys.contiguous()
         kst = keys.stride()
-    dev = queries.device
-    q_out = torch.empty(qshape, dtype=dtype, device=dev)
-    k_out = torch.empty(kshape, dtype=dtype, device=dev)
+    q_out = torch.empty_like(queries, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(keys, memory_format=torch.contiguous_format)
     q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
     positions = positions.contiguous()
     _lib.launch("sparkq_qk_norm_rope", index, queries.data_ptr(), keys.data_ptr(),
                 q_weight.data_ptr(), k_weight.data_ptr(), positions.data_ptr(), 64 if wide else 32,
-                q_out.data_ptr(), k_out.data_ptr(), t, hq, kshape[1], d, dims,
+                q_out.data_ptr(), k_out.data_ptr(), t, hq, hkv, d, dims,
                 int(bool(traditional)), eps, base, scale, _lib.dtype_code(dtype),
                 (ctypes.c_int64 * 4)(qst[0], qst[1], kst[0], kst[1]))
     return q_out, k_out

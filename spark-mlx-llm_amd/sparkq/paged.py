@@ -32,6 +32,7 @@ __all__ = ["PagedKVCache", "kv_pages_compact", "kv_pages_fork", "paged_kv_append
            "paged_quantized_sdpa"]
 
 
+_CONTIGUOUS = torch.contiguous_format
 _I64x2, _I64x4, _I64x8, _I64x12 = (ctypes.c_int64 * n for n in (2, 4, 8, 12))
 _CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
@@ -162,7 +163,7 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
     _need_gpu(op, index)
     queries, qst = _rows16(queries)
     dev = kc.device
-    out = torch.empty(shape, dtype=out_dtype, device=dev) if out is None \
+    out = torch.empty_like(queries, dtype=out_dtype, memory_format=_CONTIGUOUS) if out is None \
         else _out_buffer(out, shape, out_dtype, dev)
     need = _lib.lib().sparkq_paged_sdpa_workspace_bytes(t, b, heads, hkv, d, max_new, width * page)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
@@ -186,7 +187,8 @@ def _pool(op, cache):
                            (ks, (page, 1), 2), (vs, (page, 1), 2)):
         s = t.stride()
         k = len(inner)
-        if any(x != y and n > 1 for x, y, n in zip(s[-k:], inner, t.shape[-k:])):
+        if s[-k:] != inner and any(x != y and n > 1
+                                   for x, y, n in zip(s[-k:], inner, t.shape[-k:])):
             raise ValueError(f"{op}: a page must be contiguous in every tensor of the cache")
         st += (s[0] * size if layered else 0, s[-k - 1] * size)
     return (kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr()), index, \
@@ -226,12 +228,14 @@ def kv_pages_fork(cache, page_table, lengths, parents=None, new_tokens=None):
     if new_tokens is not None:
         _check_ints(op, index, "new_tokens", new_tokens, (rows,))
     _need_gpu(op, index)
-    dev = page_table.device
-    table = torch.empty((rows, width), dtype=torch.int32, device=dev)
-    after = torch.empty(rows, dtype=torch.int32, device=dev)
-    missing = torch.empty(1, dtype=torch.int32, device=dev)
+    if rows == b:
+        table = torch.empty_like(page_table, memory_format=_CONTIGUOUS)
+        after = torch.empty_like(lengths)
+    else:
+        table, after = page_table.new_empty((rows, width)), lengths.new_empty(rows)
+    missing = lengths.new_empty(1)
     need = _lib.lib().sparkq_kv_pages_workspace_bytes(rows, pages)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=lengths.device)
     _lib.launch("sparkq_kv_pages_fork", index, *bufs, page_table.data_ptr(), lengths.data_ptr(),
                 _ptr(parents), _ptr(new_tokens), page_table.stride(0), table.data_ptr(),
                 after.data_ptr(), missing.data_ptr(), st, b, rows, width, pages, layers, page, cb,
@@ -247,11 +251,10 @@ def kv_pages_compact(cache, page_table, lengths):
     bufs, index, layers, pages, page, cb, sb, st = _pool(op, cache)
     b, width = _check_rows(op, index, page_table, lengths)
     _need_gpu(op, index)
-    dev = page_table.device
-    table = torch.empty((b, width), dtype=torch.int32, device=dev)
-    used = torch.empty(1, dtype=torch.int32, device=dev)
+    table = torch.empty_like(page_table, memory_format=_CONTIGUOUS)
+    used = lengths.new_empty(1)
     need = _lib.lib().sparkq_kv_pages_workspace_bytes(b, pages)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=lengths.device)
     _lib.launch("sparkq_kv_pages_compact", index, *bufs, page_table.data_ptr(), lengths.data_ptr(),
                 page_table.stride(0), table.data_ptr(), used.data_ptr(), st, b, width, pages,
                 layers, page, cb, sb, ws.data_ptr(), need)
