@@ -411,7 +411,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_compact_plan_kernel(PageAr
 
 // Copies page src[i] to dst[i] in every layer of the four tensors, in pieces
 // of 16 KB dealt over the workgroups, past the caches (read and written once).
-// Bound by HBM: 0.9 GB moved and written in 163 us, 5.5 TB/s; half the workgroups
+// Bound by HBM: 0.87 GB read and written in 161 us, 5.4 TB/s; half the workgroups
 // 205 us, cached accesses 171. No page is both a source and a
 // destination. The destination is dst[i], or list[dst[i]] where a list is given.
 __device__ void copy_pages(const PageArgs& a, const int* src, const int* dst, const int* list, int pairs,

@@ -623,12 +623,12 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
 //
 // Two workgroups a CU is what registers (240) and LDS (76 KB) allow; being at
 // different places of their blocks, one's products and LDS reads run beside the
-// other's softmax. 2048 new tokens of 8192, 32 heads of 128, 240 GFLOP: 304 us, 790
-// TFLOP/s. Bound by what a wave can issue: per block of 64 tokens 32 products (1024
-// cycles of the matrix cores), about 350 vector and 75 LDS instructions, 3200
-// cycles in all. Scores one block ahead, so that products and exponentials are
-// independent neighbours in one wave, saved 4% of the cycles and lost as much in
-// clock (2.34 -> 2.22 GHz).
+// other's softmax. 2048 new tokens of 8192, 32 heads of 128, 240 GFLOP: 298 us, 805
+// TFLOP/s. Bound by what a wave can issue and by the clock, which falls to 2.2 GHz:
+// per block of 64 tokens 32 products (1024 cycles of the matrix cores), about 350
+// vector and 75 LDS instructions, 2900 cycles in all. Scores one block ahead, so
+// that products and exponentials are independent neighbours in one wave, saved 4%
+// of the cycles and lost as much in clock.
 template <int D>
 struct TileShape {
   static constexpr int BLOCK = 64;                    // tokens
