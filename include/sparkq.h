@@ -612,12 +612,13 @@ int sparkq_paged_kv_append(const void* k, const void* v, void* k_codes, void* k_
  * tensors 16-byte aligned; pages lie less than 32 GiB apart and a head's tokens
  * within a page span less than 2 GiB (each SPARKQ_ERR_UNSUPPORTED). causal =
  * 1: row i of a sequence's n sees its tokens 0 .. length - n + i; 0: all of
- * them. Tokens without a page are hidden; a row that sees nothing is zero; rows
- * of out that fall to no sequence are left as they were. max_new bounds the new
- * tokens of one sequence: of longer ones the rows past it are left as they were
- * too. A chunk of one token per sequence is the decode step. Scores, normalizer
- * and sums are fp32; a weight times its value's scale is rounded to fp16 once
- * (from 2^-19 of the row's largest down, to 2^-29 of that).
+ * them. Tokens without a page are hidden; a row that sees nothing is zero, one
+ * that sees a value scale that is not finite has no finite values; rows of out
+ * that fall to no sequence are left as they were. max_new bounds the new tokens
+ * of one sequence: of longer ones the rows past it are left as they were too. A
+ * chunk of one token per sequence is the decode step. Scores, normalizer and
+ * sums are fp32; a weight times its value's scale is rounded to fp16 once (from
+ * 2^-19 of the row's largest down, to 2^-29 of that).
  * Workspace: sparkq_paged_sdpa_workspace_bytes (max_tokens = max_pages *
  * page_size), any initial value. */
 size_t sparkq_paged_sdpa_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv,

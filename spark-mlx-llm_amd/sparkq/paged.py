@@ -32,6 +32,7 @@ __all__ = ["PagedKVCache", "kv_pages_compact", "kv_pages_fork", "paged_kv_append
            "paged_quantized_sdpa"]
 
 
+_T = torch.Tensor
 _CONTIGUOUS = torch.contiguous_format
 _I64x2, _I64x4, _I64x8, _I64x12 = (ctypes.c_int64 * n for n in (2, 4, 8, 12))
 _CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -40,9 +41,9 @@ _CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.
 def _check_cache(op, cache, ndim):
     """((k_codes, k_scales, v_codes, v_scales), their GPU, codes' shape) of a
     cache with `ndim` axes in its codes."""
-    if len(cache) != 4 or any(not isinstance(t, torch.Tensor) for t in cache):
+    kc, ks, vc, vs = cache if len(cache) == 4 else (None,) * 4
+    if not (isinstance(kc, _T) and isinstance(ks, _T) and isinstance(vc, _T) and isinstance(vs, _T)):
         raise ValueError(f"{op}: the cache is (k_codes, k_scales, v_codes, v_scales)")
-    kc, ks, vc, vs = cache
     shape, scales = kc.shape, ks.shape
     if (len(shape) != ndim or vc.shape != shape or scales != shape[:-1] or vs.shape != scales
             or kc.dtype is not torch.int8 or vc.dtype is not torch.int8
@@ -69,22 +70,36 @@ def _check_ints(op, index, name, t, shape):
         raise ValueError(f"{op}: the last axis of {name} must be contiguous")
 
 
+def _check_rows(op, index, page_table, lengths):
+    """(sequences, pages per row) of a batch's table and lengths."""
+    shape = page_table.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"{op}: expected page_table [B,M] and lengths [B]")
+    b, width = shape
+    if not (page_table.dtype is torch.int32 and page_table.is_contiguous()
+            and page_table.get_device() == index and lengths.dtype is torch.int32
+            and lengths.shape == (b,) and lengths.is_contiguous()
+            and lengths.get_device() == index):  # (one test of what is nearly always so)
+        _check_ints(op, index, "page_table", page_table, shape)
+        _check_ints(op, index, "lengths", lengths, (b,))
+    return b, width
+
+
 def _check_batch(op, index, page_table, starts, lengths):
     """(sequences, pages per row) of a batch."""
-    if page_table.ndim != 2 or page_table.shape[1] < 1:
-        raise ValueError(f"{op}: expected page_table [B,M], lengths [B] and starts [B+1]")
-    b, width = shape = page_table.shape
-    _check_ints(op, index, "page_table", page_table, shape)
-    _check_ints(op, index, "lengths", lengths, (b,))
-    _check_ints(op, index, "starts", starts, (b + 1,))
+    b, width = _check_rows(op, index, page_table, lengths)
+    if not (starts.dtype is torch.int32 and starts.shape == (b + 1,) and starts.is_contiguous()
+            and starts.get_device() == index):
+        _check_ints(op, index, "starts", starts, (b + 1,))
     return b, width
 
 
 def _strides(op, kc, ks, vc, vs):
-    a, b = kc.stride(), vc.stride()
-    if a[3] != 1 or b[3] != 1:
+    a0, a1, a2, a3 = kc.stride()
+    b0, b1, b2, b3 = vc.stride()
+    if a3 != 1 or b3 != 1:
         raise ValueError(f"{op}: the codes' innermost axes must be contiguous")
-    return _I64x12(*a[:3], *ks.stride(), *b[:3], *vs.stride())
+    return _I64x12(a0, a1, a2, *ks.stride(), b0, b1, b2, *vs.stride())
 
 
 def _rows16(t):
@@ -130,8 +145,8 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
     """Attention of a batch's new tokens over their pages: queries [T,Hq,D]
     (float16 or bfloat16) -> [T,Hq,D]. With mask="causal" row i of a
     sequence's n new tokens sees its tokens 0 .. length - n + i, with None all
-    of them; tokens without a page are hidden, and a row that sees nothing is
-    zero. max_new is the most new tokens that a sequence has (1: a decode
+    of them; tokens without a page are hidden, a row that sees nothing is zero, and
+    one that sees a value scale that is not finite has no finite values. max_new is the most new tokens that a sequence has (1: a decode
     step). Rows that fall to no sequence, or to more than max_new of one, are
     left as they are in `out`, and hold anything in a new tensor. Codes and
     scales of keys lie as those of values do (the same strides), a page's scales
@@ -162,11 +177,10 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
     strides = _strides(op, kc, ks, vc, vs)
     _need_gpu(op, index)
     queries, qst = _rows16(queries)
-    dev = kc.device
     out = torch.empty_like(queries, dtype=out_dtype, memory_format=_CONTIGUOUS) if out is None \
-        else _out_buffer(out, shape, out_dtype, dev)
+        else _out_buffer(out, shape, out_dtype, kc.device)
     need = _lib.lib().sparkq_paged_sdpa_workspace_bytes(t, b, heads, hkv, d, max_new, width * page)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = kc.new_empty(need) if need else None  # (int8: bytes)
     _lib.launch("sparkq_paged_sdpa", index, queries.data_ptr(), kc.data_ptr(), ks.data_ptr(),
                 vc.data_ptr(), vs.data_ptr(), page_table.data_ptr(), starts.data_ptr(),
                 lengths.data_ptr(), out.data_ptr(), t, b, heads, hkv, d, pages, width,
@@ -182,26 +196,21 @@ def _pool(op, cache):
     layered = len(cache) == 4 and getattr(cache[0], "ndim", 0) == 5
     kc, ks, vc, vs, index, shape = _check_cache(op, cache, 5 if layered else 4)
     pages, hkv, page, d = shape[-4:]
+    layers = shape[0] if layered else 1
+    cb, sb = hkv * page * d, hkv * page * 2
+    bufs = kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr()
+    if kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous():
+        return bufs, index, layers, pages, page, cb, sb, \
+            _I64x8(pages * cb, cb, pages * cb, cb, pages * sb, sb, pages * sb, sb)
     st = []
     for t, inner, size in ((kc, (page * d, d, 1), 1), (vc, (page * d, d, 1), 1),
                            (ks, (page, 1), 2), (vs, (page, 1), 2)):
         s = t.stride()
         k = len(inner)
-        if s[-k:] != inner and any(x != y and n > 1
-                                   for x, y, n in zip(s[-k:], inner, t.shape[-k:])):
+        if any(x != y and n > 1 for x, y, n in zip(s[-k:], inner, t.shape[-k:])):
             raise ValueError(f"{op}: a page must be contiguous in every tensor of the cache")
         st += (s[0] * size if layered else 0, s[-k - 1] * size)
-    return (kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr()), index, \
-        shape[0] if layered else 1, pages, page, hkv * page * d, hkv * page * 2, _I64x8(*st)
-
-
-def _check_rows(op, index, page_table, lengths):
-    if page_table.ndim != 2 or page_table.shape[1] < 1:
-        raise ValueError(f"{op}: expected page_table [B,M] and lengths [B]")
-    b, width = shape = page_table.shape
-    _check_ints(op, index, "page_table", page_table, shape)
-    _check_ints(op, index, "lengths", lengths, (b,))
-    return b, width
+    return bufs, index, layers, pages, page, cb, sb, _I64x8(*st)
 
 
 def kv_pages_fork(cache, page_table, lengths, parents=None, new_tokens=None):
@@ -235,7 +244,7 @@ def kv_pages_fork(cache, page_table, lengths, parents=None, new_tokens=None):
         table, after = page_table.new_empty((rows, width)), lengths.new_empty(rows)
     missing = lengths.new_empty(1)
     need = _lib.lib().sparkq_kv_pages_workspace_bytes(rows, pages)
-    ws = torch.empty(need, dtype=torch.uint8, device=lengths.device)
+    ws = cache[0].new_empty(need)  # (int8: bytes)
     _lib.launch("sparkq_kv_pages_fork", index, *bufs, page_table.data_ptr(), lengths.data_ptr(),
                 _ptr(parents), _ptr(new_tokens), page_table.stride(0), table.data_ptr(),
                 after.data_ptr(), missing.data_ptr(), st, b, rows, width, pages, layers, page, cb,
@@ -254,7 +263,7 @@ def kv_pages_compact(cache, page_table, lengths):
     table = torch.empty_like(page_table, memory_format=_CONTIGUOUS)
     used = lengths.new_empty(1)
     need = _lib.lib().sparkq_kv_pages_workspace_bytes(b, pages)
-    ws = torch.empty(need, dtype=torch.uint8, device=lengths.device)
+    ws = cache[0].new_empty(need)  # (int8: bytes)
     _lib.launch("sparkq_kv_pages_compact", index, *bufs, page_table.data_ptr(), lengths.data_ptr(),
                 page_table.stride(0), table.data_ptr(), used.data_ptr(), st, b, width, pages,
                 layers, page, cb, sb, ws.data_ptr(), need)

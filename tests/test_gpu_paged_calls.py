@@ -221,16 +221,17 @@ def test_scales(gpu, new, scale):
     check(out, q, cache, table, starts, lengths, scale)
 
 
+@pytest.mark.parametrize("d", [128, 256])
 @pytest.mark.parametrize("new", [1, 64])
-def test_descending_starts_stay_in_bounds(gpu, new):
+def test_descending_starts_stay_in_bounds(gpu, new, d):
     """Sequences whose rows overlap are more work than the call's scratch is
     for: the others have their results, and what lies behind is left alone."""
     lengths = [3000] * 12 + [90]
-    q, _, _, cache, table, _ = ref.batch(7, lengths, [0] * 12 + [new], HQ, HKV, D, PAGE, extra_rows=70)
+    q, _, _, cache, table, _ = ref.batch(7, lengths, [0] * 12 + [new], HQ, HKV, d, PAGE, extra_rows=70)
     t = q.shape[0]
     q = q.to(BF)
     starts = [0 if i % 2 == 0 else new for i in range(13)] + [new]
-    out = torch.full((t + 64, HQ, D), 7.0, dtype=BF, device=gpu)
+    out = torch.full((t + 64, HQ, d), 7.0, dtype=BF, device=gpu)
     run(gpu, q, cache, table, starts, lengths, new, out=out[:t])
     assert (out[new:] == 7.0).all()
     assert out[:new].isfinite().all()
@@ -307,3 +308,98 @@ def test_a_step_that_runs_short_is_taken_back(gpu):
     assert cache.starts.tolist() == [0, 30, 46] and cache.max_new == 30
     cache.step([20], [0])
     assert cache.missing.item() == 0 and cache.lengths.tolist() == [50]
+
+
+# --- what head dims and halves of blocks see differently --------------------------
+
+@pytest.mark.parametrize("hkv,gqa,d", [(4, 4, 256), (2, 8, 128), (2, 16, 64)])
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("scale", [0.06, 1.0, 4.0])
+def test_sharp_and_flat_weights_over_long_chunks(gpu, hkv, gqa, d, page, scale):
+    """Scores of some hundred, where the running maximum moves from block to block
+    and differently in the halves of a block, and the contexts are split."""
+    import sparkq
+
+    lengths, news = [900, 130, 31], [70, 130, 31]
+    q, _, _, cache, table, starts = ref.batch(20, lengths, news, hkv * gqa, hkv, d, page)
+    q = q.to(BF)
+    out = sparkq.paged_quantized_sdpa(q.to(gpu), tuple(t.to(gpu) for t in cache), _ints(table, gpu),
+                                      _ints(starts, gpu), _ints(lengths, gpu), scale=scale,
+                                      max_new=130, out_dtype=torch.float32)
+    assert check(out, q, cache, table, starts, lengths, scale).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 100])
+def test_value_scales_in_any_order(gpu, d, new):
+    """Value scales over fp16's range, growing, falling and shuffled: the largest
+    so far decides the unit of a row's weights."""
+    lengths, news = [300, 280, 260], [new] * 3
+    q, _, _, cache, table, starts = ref.batch(21, lengths, news, 8, 2, d, 32)
+    order = torch.randperm(260, generator=torch.Generator().manual_seed(1)).tolist()
+    for b, n in enumerate(lengths):
+        for pos in range(n):
+            k = (pos, n - 1 - pos, order[min(pos, 259)])[b]
+            cache[3][table[b][pos // 32], :, pos % 32] = 2.0 ** (-24 + k * 39 / n)
+    q = q.to(BF)
+    out = run(gpu, q, cache, table, starts, lengths, new, out_dtype=torch.float32)
+    check(out, q, cache, table, starts, lengths, d ** -0.5)
+
+
+@pytest.mark.parametrize("new", [1, 24, 90])
+def test_hidden_values_at_head_dim_256(gpu, new):
+    """NaN and infinite scales behind each sequence's end and in pages that no
+    table names; a visible infinite one (p c inf: infinite, NaN where the code c
+    is 0) leaves just the rows that see it without finite values."""
+    lengths, news = [150, 97], [min(new, 150), min(new, 97)]
+    q, _, _, cache, table, starts = ref.batch(22, lengths, news, 8, 2, 256, 32)
+    _, ks, _, vs = cache
+    named = {p for r, n in zip(table, lengths) for p in r[: -(-n // 32)]}
+    for p in range(ks.shape[0]):
+        if p not in named:
+            ks[p], vs[p] = math.nan, math.inf
+    for r, n in zip(table, lengths):
+        if n % 32:
+            ks[r[n // 32], :, n % 32:] = math.inf
+            vs[r[n // 32], :, n % 32:] = math.nan
+    q = q.to(torch.float16)
+    check(run(gpu, q, cache, table, starts, lengths, new), q, cache, table, starts, lengths, 1 / 16)
+    vs[table[0][149 // 32], 1, 149 % 32] = math.inf  # the last token, of one KV head
+    out = run(gpu, q, cache, table, starts, lengths, new).cpu()
+    last = starts[1] - 1
+    assert not out[last, 4:].isfinite().any() and out[last, :4].isfinite().all()
+    assert out[:last].isfinite().all() and out[last + 1:].isfinite().all()
+
+
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("page", [16, 32, 128])
+def test_absent_pages_inside_a_context(gpu, d, page):
+    """Holes of every page size in the middle of the blocks of a chunk, and rows
+    whose every token is hidden."""
+    lengths, news = [700, 200], [60, 200]
+    q, _, _, cache, table, starts = ref.batch(23, lengths, news, 8, 2, d, page)
+    for j in range(0, len(table[0]) - 2, 3):
+        table[0][j] = -1
+    for j in range(0, 64 // page + 1):
+        table[1][j] = 10 ** 9
+    q = q.to(torch.float16)
+    out = run(gpu, q, cache, table, starts, lengths, 200)
+    assert check(out, q, cache, table, starts, lengths, d ** -0.5).all()
+    assert (out[starts[1]:starts[1] + 64] == 0).all()
+
+
+@pytest.mark.parametrize("d,hkv", [(256, 4), (128, 8), (64, 2)])
+def test_more_tiles_than_the_chip_holds(gpu, d, hkv):
+    """Several rounds of workgroups, the second of them dealt in reverse."""
+    n = 128 * 40 // 4
+    lengths, news = [n] * 3, [n, n - 5, 700]
+    q, _, _, cache, table, starts = ref.batch(24, lengths, news, 4 * hkv, hkv, d, 64)
+    q = q.to(BF)
+    out = run(gpu, q, cache, table, starts, lengths, n)
+    pick = torch.randperm(q.shape[0], generator=torch.Generator().manual_seed(2))[:60].sort().values
+    assert out.isfinite().all()
+    # some rows, each as a sequence of one new token of its own
+    seq = torch.bucketize(pick, torch.tensor(starts), right=True) - 1
+    own = [lengths[b] - news[b] + int(t) - starts[b] + 1 for b, t in zip(seq.tolist(), pick)]
+    check(out[pick.to(gpu)], q[pick], cache, [table[b] for b in seq.tolist()], list(range(61)), own,
+          d ** -0.5)
