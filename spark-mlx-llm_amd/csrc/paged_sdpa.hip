@@ -644,8 +644,8 @@ struct TileShape {
 // of 16 tokens, and of the run srun whose scales it takes. A lane's own offset
 // counts from the block's first token where PG is 1, else from its page's.
 // `ok` says which runs have a page; page 0 stands in for the others, whose tokens
-// are hidden. (2048 new tokens of 8192, 32 heads of 128: one page to a block 325 us,
-// two 352, four 382, with the lookups in scalar registers.)
+// are hidden. (2048 new tokens of 8192, 32 heads of 128: one page to a block 323 us,
+// two 350, four 384; a scalar load for each lookup 324, 354 and 393.)
 template <int PG, int PPT>
 struct TilePages {
   uint64_t at[PG == 1 ? 1 : PPT], sat;
@@ -654,23 +654,41 @@ struct TilePages {
 template <int PG, int PPT>
 __device__ __forceinline__ TilePages<PG, PPT> tile_pages(const PagedSdpaArgs& a, TableRow row, int t0, int run0,
                                                          int step, int srun) {
-  const int mask = (1 << a.p.page_log2) - 1;
-  auto look = [&](int run) { return row[min((t0 + 16 * run) >> a.p.page_log2, a.p.width - 1)]; };
-  auto valid = [&](int id) { return (unsigned)id < (unsigned)a.p.pages; };
-  auto keep = [&](int id) { return valid(id) ? id : 0; };
-  TilePages<PG, PPT> r;
-  if constexpr (PG == 1) {
-    const int id = look(0);
-    r.ok = valid(id) ? 15 : 0;
-    r.at[0] = code_at(a.c, keep(id), t0 & mask);
-    r.sat = scale_at(a.c, keep(id), (t0 & mask) + 16 * srun);
+  // the block's entries in one load; those past the table's row stand behind every
+  // length, and are the last one
+  typedef int entries_t __attribute__((ext_vector_type(PG), aligned(4)));
+  typedef const __attribute__((address_space(4))) entries_t* Entries;
+  const int mask = (1 << a.p.page_log2) - 1, j0 = t0 >> a.p.page_log2;
+  entries_t id;
+  if (PG == 1 || j0 + PG <= a.p.width) {
+    id = *(Entries)(row + (PG == 1 ? min(j0, a.p.width - 1) : j0));
   } else {
-    r.ok = 0;
 #pragma unroll
-    for (int h = 0; h < PG; ++h) r.ok |= (valid(look(4 / PG * h)) ? (1u << 4 / PG) - 1 : 0) << (4 / PG * h);
+    for (int h = 0; h < PG; ++h) id[h] = row[min(j0 + h, a.p.width - 1)];
+  }
+  constexpr uint32_t runs = (1u << 4 / PG) - 1;
+  TilePages<PG, PPT> r;
+  r.ok = 0;
 #pragma unroll
-    for (int i = 0; i < PPT; ++i) r.at[i] = code_at(a.c, keep(look(run0 + i * step)), 0);
-    r.sat = scale_at(a.c, keep(look(srun)), 16 * srun & mask);
+  for (int h = 0; h < PG; ++h) {
+    const bool valid = (unsigned)id[h] < (unsigned)a.p.pages;
+    r.ok |= (valid ? runs : 0) << (4 / PG * h);
+    id[h] = valid ? id[h] : 0;
+  }
+  auto of = [&](int run) __attribute__((always_inline)) {
+    const int h = run * PG / 4;
+    int v = id[0];
+#pragma unroll
+    for (int k = 1; k < PG; ++k) v = h == k ? id[k] : v;
+    return v;
+  };
+  if constexpr (PG == 1) {
+    r.at[0] = code_at(a.c, id[0], t0 & mask);
+    r.sat = scale_at(a.c, id[0], (t0 & mask) + 16 * srun);
+  } else {
+#pragma unroll
+    for (int i = 0; i < PPT; ++i) r.at[i] = code_at(a.c, of(run0 + i * step), 0);
+    r.sat = scale_at(a.c, of(srun), 16 * srun & mask);
   }
   return r;
 }
