@@ -1055,7 +1055,7 @@ int sparkq_kv_pages_fork(void* k_codes, void* v_codes, void* k_scales, void* v_s
   void* const bufs[4] = {k_codes, v_codes, k_scales, v_scales};
   REQUIRE((B == 0 || (page_table && lengths)) && (rows == 0 || (out_table && out_lengths)) && out_missing,
           "kv_pages_fork: null tensor pointer");
-  REQUIRE(parents || rows == B, "kv_pages_fork: without parents there is a row for each sequence");
+  REQUIRE(parents || rows == B || rows == 0, "kv_pages_fork: without parents there is a row for each sequence");
   if (int rc = kv_pages_check("kv_pages_fork", bufs, buf_strides, B, rows, max_pages, pages, layers,
                               table_stride, page_size, code_bytes, scale_bytes, workspace,
                               workspace_bytes))

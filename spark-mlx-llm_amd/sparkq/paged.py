@@ -323,9 +323,10 @@ class PagedKVCache:
         ints = torch.tensor(host, dtype=torch.int32, device=dev)
         if parents is not None:
             parents = ints[2 * rows + 1:]
-        self._last = self.page_table, self.lengths, self.starts, self.max_new
+        last = self.page_table, self.lengths, self.starts, self.max_new
         self.page_table, self.lengths, self.missing = kv_pages_fork(
             self.cache, self.page_table, self.lengths, parents, ints[:rows])
+        self._last = last
         self.starts, self.max_new = ints[rows:2 * rows + 1], max(new_tokens, default=0)
         return self.starts
 

@@ -195,6 +195,24 @@ def test_nothing_in_the_batch(gpu):
         assert torch.equal(a.cpu(), c)
 
 
+def test_a_batch_that_starts_empty_and_ends_empty(gpu):
+    import sparkq
+
+    cache = sparkq.PagedKVCache(2, 9, HKV, D, page_size=16, max_pages=3, device=gpu)
+    assert cache.step([]).tolist() == [0]
+    cache.step([20, 0, 48], [-1, -1, -1])
+    assert cache.lengths.tolist() == [20, 0, 48] and cache.missing.item() == 0
+    assert cache.page_table.tolist() == [[0, 1, -1], [-1] * 3, [2, 3, 4]]
+    x = torch.randn((68, HKV, D), device=gpu).to(BF)
+    cache.append(1, x, x)
+    out = cache.attend(1, x, scale=0.1)
+    assert out.isfinite().all() and out.shape == x.shape
+    cache.step([], [])
+    assert cache.compact().item() == 0
+    cache.step([1], [-1])
+    assert cache.page_table.tolist() == [[0, -1, -1]] and cache.lengths.tolist() == [1]
+
+
 @pytest.mark.parametrize("hkv,gqa,d", [(1, 4, 64), (1, 16, 128), (2, 1, 256)])
 @pytest.mark.parametrize("new", [1, 24])
 def test_long_contexts_among_many_sequences(gpu, hkv, gqa, d, new):
