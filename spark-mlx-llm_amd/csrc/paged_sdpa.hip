@@ -66,6 +66,8 @@ struct PagedSdpaArgs {
   float scale_log2;
 };
 
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+
 constexpr int kFewBlock = 32;    // tokens of a block
 constexpr int kTileRows = 128;  // rows of a tile
 
@@ -236,7 +238,6 @@ __device__ __forceinline__ float load_query(const PagedSdpaArgs& a, const uint16
     if (!live) qb[c] = u32x4_t{0, 0, 0, 0};
   }
   if (a.q_dtype == SPARKQ_F16) return 1.0f;
-  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
   u16x2_t most = {0, 0};
 #pragma unroll
   for (int c = 0; c < NK; ++c)
@@ -275,10 +276,10 @@ constexpr float kRoom = 8.0f;
 
 __device__ __forceinline__ float unit(const RowState& st) { return st.m + (st.e - 6.0f); }
 
-// |scale|, 0 where it does not count or is not finite
-__device__ __forceinline__ float scale_size(float v, bool counts) {
+// |scale|, 0 where it is not finite
+__device__ __forceinline__ float scale_size(float v) {
   v = fabsf(v);
-  return counts && v <= 65504.0f ? v : 0.0f;
+  return v <= 65504.0f ? v : 0.0f;
 }
 
 // What a part of a row's context hands on: its M, or -inf where it saw nothing
@@ -418,8 +419,9 @@ __device__ __forceinline__ BlockPages<Q> block_pages(const PagedSdpaArgs& a, Tab
 // The waves of a workgroup take turns at blocks of 32 tokens, each with the next
 // block's loads in flight and no barrier until they join; keys and values, read
 // once, go past the caches. Bound by HBM where there is much: 64 sequences of up to
-// 8192 tokens, 8 heads of 128, 304 MB in 61.5 us, 4.9 TB/s (two workgroups a CU 68,
-// cached loads 64); by the latency of its steps where there is little: one of 4095
+// 8192 tokens, 8 heads of 128, 304 MB in 60 us, 5.0 TB/s (before the blocks that all
+// rows see whole were spared the masks 61.5: two workgroups a CU 68, four, which
+// spill, 99, cached loads 64); by the latency of its steps where there is little: one of 4095
 // tokens 7 us, of which find_item and the first loads are half.
 //
 // Up to 16 rows: 16 sequences of 8192 tokens with 4 new ones (4 heads to each of 8
@@ -450,6 +452,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
   const int rr = 16 * it.tile + min(n16, rows - 1);
   const int lim = last_seen(a, it, rr, gqa);
   const int seen = last_seen(a, it, 16 * it.tile + rows - 1, gqa) + 1;  // by the last row: the most
+  const int all = last_seen(a, it, 16 * it.tile, gqa) + 1;              // by every row
   const int nblocks = (seen + kBlock - 1) / kBlock;
   const int ib0 = (int)((int64_t)it.part * nblocks / it.parts);
   const int ib1 = (int)((int64_t)(it.part + 1) * nblocks / it.parts);
@@ -516,29 +519,36 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
       }
     }
     float s[8], vsc[8];
+    u16x2_t most = {0, 0};  // the largest scale's bits: finite below those of infinity
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t kw = skr[i >> 1], vw = svr[i >> 1];
       s[i] = sc[i >> 2][i & 3] * (((i & 1) ? hi16<F16>(kw) : lo16<F16>(kw)) * a.scale_log2);
       vsc[i] = (i & 1) ? hi16<F16>(vw) : lo16<F16>(vw);
+      if (i & 1) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, vw & 0x7FFF7FFFu));
     }
-    uint32_t ok = 0;
+    const uint16_t top16 = most[0] > most[1] ? most[0] : most[1];
+    float size = f16_to_f32(top16);
+    if (__builtin_expect(t0 + kBlock > all || pages_ok != 3 || __ballot(top16 >= 0x7C00) != 0, 0)) {
+      uint32_t ok = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ok |= (uint32_t)(t0 + 8 * grp + i <= lim) << i;
-    if (!((pages_ok >> (grp >> 1)) & 1u)) ok = 0;
+      for (int i = 0; i < 8; ++i) ok |= (uint32_t)(t0 + 8 * grp + i <= lim) << i;
+      if (!((pages_ok >> (grp >> 1)) & 1u)) ok = 0;
+      ok = __float_as_uint(pinned(__uint_as_float(ok)));
+      size = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool live = (ok >> i) & 1u;
+        s[i] = live ? s[i] : kNegInf;
+        vsc[i] = live ? vsc[i] : 0.0f;
+        size = fmaxf(size, scale_size(vsc[i]));
+      }
+    }
+    size = max_groups<4>(size);
     load(ib + 4, next);
     next = block_pages<2>(a, trow, kBlock * min(ib + 8, last));
     u32x4_t w;
     bool up;
-    float size = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const bool live = (ok >> i) & 1u;
-      s[i] = live ? s[i] : kNegInf;
-      vsc[i] = live ? vsc[i] : 0.0f;
-      size = fmaxf(size, scale_size(vsc[i], true));
-    }
-    size = max_groups<4>(size);
     const float alpha = row_block<8, 4>(st, s, mul, vsc, size, &w, up);
     if (__ballot(up)) {
       const float f = pinned(up ? alpha : 1.0f);
