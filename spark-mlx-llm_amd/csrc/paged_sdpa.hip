@@ -26,11 +26,15 @@
 // Numerics. Both products are fp16 MFMAs with fp32 sums. Codes are exact in
 // fp16; a query row is shifted by a power of two to be exact too. The weight
 // of a value, p_n times its scale, is rounded to fp16 once (at most 2^-11 of it,
-// what an fp16 output's own rounding is and an eighth of a bf16 output's), under
-// a power of two that puts the largest one near 2^7: 2^8 of room for the running
-// maximum, which moves only when a block exceeds it by that much, and full
-// precision down to 2^-19 of the largest. The running maximum, the normalizer and the
-// sums are fp32.
+// what an fp16 output's own rounding is and an eighth of a bf16 output's), in a
+// unit that puts the largest one near 2^7: 2^8 of room for the running maximum,
+// which tiles move only when a block exceeds it by that much, and full precision
+// down to 2^-19 of the largest. The unit is a power of two beside the maximum
+// itself, so that the weight of the token that it comes from is its value's scale,
+// which fp16 holds: where one token outweighs the rest nothing is lost (fp16 outputs
+// of sharp rows: 1.07 times the error of rounding the exact ones with few rows, where
+// a power of two above the maximum had 1.41). The running maximum, the normalizer and
+// the sums are fp32.
 #include <algorithm>
 #include <type_traits>
 
@@ -264,15 +268,14 @@ __device__ __forceinline__ float pinned(float v) {
 // ---------------------------------------------------------------------------
 // online softmax of one block for one row per lane
 // ---------------------------------------------------------------------------
-// The state counts in units of 2^-M, M = m + e - 6: m the running maximum of
-// the scores (log2 units) and 2^e .. 2^(e+1) the largest finite value scale that
-// the row has seen, so that exp2(s - M) * v_scale < 2^7 at s = m.
+// The state counts in units of 2^M, M = m + e - 6: m the maximum of the scores
+// (log2 units) when it last moved, 2^e .. 2^(e+1) the largest finite value scale
+// that the row has seen, so that exp2(s - M) * v_scale < 2^7 at s = m.
 struct RowState {
   float m = kNegInf;  // -inf: nothing seen
   float z = 0.0f;
   float e = -24.0f;  // of the smallest fp16
 };
-constexpr float kRoom = 8.0f;
 
 __device__ __forceinline__ float unit(const RowState& st) { return st.m + (st.e - 6.0f); }
 
@@ -289,11 +292,12 @@ __device__ __forceinline__ float part_max(const RowState& st, float z) {
 }
 
 // A block's N scores of this lane's row (raw sums times the key scales times
-// the softmax scale: s * mul is in log2 units), of which those in `ok` are
-// visible where MASK; `size` is the block's largest finite value scale, used
-// where all of it is visible. Writes the packed fp16 weights of the lane's N
-// values; returns the factor for what is summed so far (up: it is not 1).
-template <int N, int G>
+// the softmax scale: s * mul is in log2 units; -inf where hidden), `size` the
+// largest finite value scale of those that are visible. The maximum moves where a
+// score exceeds it by more than ROOM: 0 with few rows; in tiles, whose sums are dear
+// to scale, 8. Writes the packed fp16 weights of the lane's N values; returns the
+// factor for what is summed so far (up: it is not 1).
+template <int N, int G, int ROOM>
 __device__ __forceinline__ float row_block(RowState& st, const float s[N], float mul, const float vsc[N],
                                            float size, u32x4_t w[N / 8], bool& up) {
   float top = s[0];
@@ -301,10 +305,10 @@ __device__ __forceinline__ float row_block(RowState& st, const float s[N], float
   for (int i = 1; i < N; ++i) top = fmaxf(top, s[i]);
   top = max_groups<G>(top) * mul;
   const float e = fmaxf(st.e, (float)((int)(__float_as_uint(size) >> 23) - 127));
-  const bool raise = top > st.m + kRoom;
+  const bool raise = top > st.m + ROOM;
   up = raise || e != st.e;
   const float old = unit(st);
-  if (raise) st.m = ceilf(top);
+  if (raise) st.m = top;
   st.e = e;
   const float M = st.m == kNegInf ? 0.0f : unit(st);
   const float alpha = old == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(old - M);
@@ -549,7 +553,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
     next = block_pages<2>(a, trow, kBlock * min(ib + 8, last));
     u32x4_t w;
     bool up;
-    const float alpha = row_block<8, 4>(st, s, mul, vsc, size, &w, up);
+    const float alpha = row_block<8, 4, 0>(st, s, mul, vsc, size, &w, up);
     if (__ballot(up)) {
       const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
@@ -830,7 +834,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
     }
     u32x4_t w[N / 8];
     bool up;
-    const float alpha = row_block<N, G>(st, s, mul, vsc, size, w, up);
+    const float alpha = row_block<N, G, 8>(st, s, mul, vsc, size, w, up);
     if (__builtin_expect(__ballot(up) != 0, 0)) {
       const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
@@ -912,12 +916,14 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
 // 64 tokens over all dims, hands its weights to the other through LDS, and sums all
 // 64 tokens' values of its half of the dims. Eight waves a CU, every operand from
 // LDS is used for 32 rows, and a block's conversion is shared by 512 threads.
-// (24 sequences of up to 1000 new tokens, 166 GFLOP, 16 heads of 256: 271 us, 613
-// TFLOP/s. Before the contexts' split was tuned to it 296, where waves of 16 rows
-// with all dims took 346, and waves of 32 rows alone on their SIMDs 376.)
+// (24 sequences of up to 1000 new tokens, 166 GFLOP, 16 heads of 256: 280 us, 593
+// TFLOP/s; 271 with maxima rounded up to whole numbers, which need no second pass
+// over the sums below. Before the contexts' split was tuned to it 296, where waves of
+// 16 rows with all dims took 346, and waves of 32 rows alone on their SIMDs 376.)
 //
 // Both waves weigh in the units of their own running maxima; where these differ
-// after a block (hardly ever: they move in steps of 2^8) both go on with the larger.
+// after a block (its first, and hardly ever later: they move by 2^8 or more) both go
+// on with the larger.
 //
 // A block has two phases. In the first its keys are read and its values are written
 // to LDS, in the second the values are read and the next keys are written: one buffer
@@ -1046,7 +1052,7 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
       size = hide<N, G>(__float_as_uint(pinned(__uint_as_float(ok))), s, vsc);
     }
     bool up;
-    const float alpha = row_block<N, G>(st, s, mul, vsc, size, w, up);
+    const float alpha = row_block<N, G, 8>(st, s, mul, vsc, size, w, up);
     if (__builtin_expect(__ballot(up) != 0, 0)) {
       const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
@@ -1079,24 +1085,33 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
         if (k == 1 && j < PPT) stage(kput + j * 32 * S::KROW, kcr[j]);
       }
     const float mine = unit(st), theirs = o.x + (o.y - 6.0f);
-    if (__builtin_expect(__ballot(mine != theirs) != 0, 0)) {
+    const bool differ = __ballot(mine != theirs) != 0;
+    float after = 1.0f;
+    if (__builtin_expect(differ, 0)) {
+      // The sums go into the other's unit while its weights are added, so that these
+      // stay as they were rounded; weights whose unit is 2^-60 of the row's own do not
+      // count. (A half that has seen nothing has the unit 2^-inf.)
       st.m = fmaxf(st.m, o.x);
       st.e = fmaxf(st.e, o.y);
-      const float now = unit(st);
-      auto factor = [&](float u) { return u == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(u - now); };
-      const float fm = pinned(factor(mine)), ft = factor(theirs);
+      const float now = unit(st), gap = mine - theirs;
+      const bool near = gap <= 60.0f;
+      const float rest = mine == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mine - now);
+      const float before = pinned(near ? __builtin_amdgcn_exp2f(gap) : 1.0f);
+      after = near ? __builtin_amdgcn_exp2f(theirs - now) : rest;
+      if (!near) w[2] = w[3] = u32x4_t{0, 0, 0, 0};
+      st.z *= rest;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[j] *= fm;
-      st.z *= fm;
-#pragma unroll
-      for (int i = 2; i < 4; ++i)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[i][k] = pack_f16(lo16<F16>(w[i][k]) * ft, hi16<F16>(w[i][k]) * ft);
+      for (int j = 0; j < NJ; ++j) acc[j] *= before;
     }
 #pragma unroll
     for (int k = 2; k < 4; ++k)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) product(k, j);
+    if (__builtin_expect(differ, 0)) {
+      const float f = pinned(after);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[j] *= f;
+    }
   };
 
   if (ib0 < ib1) {

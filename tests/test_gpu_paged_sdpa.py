@@ -9,7 +9,7 @@ Tolerance of an output o = sum p v / sum p, with mass = sum p|v| / sum p:
  - weights under fp16's normal range, which are rounded to its step of 2^-24
    instead, by 2^-25 of the unit at most. With s the largest score (log2) and V
    the largest value scale a row has seen, the unit is 2^(m + e - 6) with m <=
-   ceil(s) < s + 1 and 2^e <= V, so under 2^-5 V 2^s, and all these roundings
+   s and 2^e <= V, so under 2^-5 V 2^s, and all these roundings
    together add up to less than 2^-30 V 2^s sum |code| / sum p, sum p in units of
    1: 2^-30 of `steps`. (A sharp softmax needs it: where the code of the one
    token that counts is 0, the rest is all there is of want and mass.)
