@@ -916,7 +916,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
 // 64 tokens over all dims, hands its weights to the other through LDS, and sums all
 // 64 tokens' values of its half of the dims. Eight waves a CU, every operand from
 // LDS is used for 32 rows, and a block's conversion is shared by 512 threads.
-// (24 sequences of up to 1000 new tokens, 166 GFLOP, 16 heads of 256: 280 us, 593
+// (24 sequences of up to 1000 new tokens, 166 GFLOP, 16 heads of 256: 282 us, 588
 // TFLOP/s; 271 with maxima rounded up to whole numbers, which need no second pass
 // over the sums below. Before the contexts' split was tuned to it 296, where waves of
 // 16 rows with all dims took 346, and waves of 32 rows alone on their SIMDs 376.)
