@@ -649,6 +649,10 @@ int sparkq_paged_sdpa(const void* q, const void* k_codes, const void* k_scales,
  * writers where all its holders are writers. out_missing[0] = pages short;
  * when it is not 0 the entries that got none are -1 and no page is copied, so
  * the batch before the call still stands. Dropping a sequence frees its pages.
+ * A row whose tokens its max_pages have no room for stops at max_pages *
+ * page_size: appending all of them would write over tokens that are there, of
+ * other rows too. After the call the workspace's int32 [1] is the number of such
+ * rows, to be read like out_missing.
  *
  * compact: with U pages in use (out_used[0]), the pages numbered U or higher
  * move, in order, to the free numbers below U. out_table [B,max_pages].

@@ -158,8 +158,8 @@ void launch_append(const PagedAppendArgs& a, hipStream_t st) {
 constexpr int kPlanThreads = 1024;
 
 // Workspace, in ints: head, then arrays of P (held, first, list) and of rows
-// (base, src, dst).
-enum { kPairs = 0, kShort = 1, kFree = 2, kUsed = 3, kHead = 16 };
+// (base, src, dst). kOverfull is the caller's to read.
+enum { kPairs = 0, kOverfull = 1, kFree = 2, kHead = 16 };
 struct PageScratch {
   int* head;
   int *held, *first, *list;
@@ -204,6 +204,7 @@ struct RowPlan {
   int src;            // sequence that the row continues, or -1
   int before, after;  // tokens before and after the step
   int held, need;     // pages before and after
+  bool over;          // more tokens than its pages have room for
 };
 
 __device__ __forceinline__ RowPlan row_plan(const PageArgs& a, int i) {
@@ -211,13 +212,14 @@ __device__ __forceinline__ RowPlan row_plan(const PageArgs& a, int i) {
   r.src = a.parents ? a.parents[i] : i;
   if ((unsigned)r.src >= (unsigned)a.B) r.src = -1;
   const int64_t room = (int64_t)a.width << a.page_log2;
-  const int64_t n = r.src < 0 ? 0 : min((int64_t)max(a.lengths[r.src], 0), room);
-  const int64_t m = min(n + (a.fresh ? max(a.fresh[i], 0) : 0), room);
+  const int64_t was = r.src < 0 ? 0 : max(a.lengths[r.src], 0), n = min(was, room);
+  const int64_t more = a.fresh ? max(a.fresh[i], 0) : 0, m = min(n + more, room);
   r.before = (int)n;
   r.after = (int)m;
   const int64_t up = (1 << a.page_log2) - 1;
   r.held = (int)((n + up) >> a.page_log2);
   r.need = (int)((m + up) >> a.page_log2);
+  r.over = was + more > room;
   return r;
 }
 
@@ -353,16 +355,19 @@ __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PageArgs 
     }
   }
   plan_sync<LDS>();
-  int wanted = 0, pairs = 0;
+  int wanted = 0, pairs = 0, overfull = 0;
   for (int i0 = 0; i0 < a.rows; i0 += kPlanThreads) {
     const int i = i0 + tid;
     int copy = 0, w = -1, want = 0;
+    bool over = false;
     if (i < a.rows) {
       const RowPlan r = i0 == 0 ? mine : row_plan(a, i);
       w = i0 == 0 ? mine_w : write_page(a, r);
       copy = w >= 0 && (held.get(w) > 0 || first.get(w) != i);
       want = copy + (r.need - r.held);
+      over = r.over;
     }
+    overfull += __syncthreads_count(over);
     int t_want, t_copy;
     const int base = wanted + block_prefix(want, s_wave, t_want);
     const int pair = pairs + block_prefix(copy, s_wave, t_copy);
@@ -377,6 +382,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PageArgs 
   if (tid == 0) {
     const int missing = max(wanted - nfree, 0);
     a.s.head[kPairs] = missing ? 0 : pairs;
+    a.s.head[kOverfull] = overfull;
     a.s.head[kFree] = nfree;
     *a.out_count = missing;
   }

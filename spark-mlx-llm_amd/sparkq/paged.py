@@ -9,7 +9,8 @@ device that no call reads back:
 
   page_table [B,M]  the pages of each sequence; an entry outside the pool is
                     no page
-  lengths    [B]    tokens of each sequence, the new ones included
+  lengths    [B]    tokens of each sequence, the new ones included: at most
+                    M * page_size (and taken as that where they are more)
   starts     [B+1]  the packed rows of each sequence's new tokens are
                     starts[b] .. starts[b+1] - 1, its last token the last one
 
@@ -213,11 +214,19 @@ def _pool(op, cache):
     return bufs, index, layers, pages, page, cb, sb, _I64x8(*st)
 
 
-def kv_pages_fork(cache, page_table, lengths, parents=None, new_tokens=None):
+def kv_pages_fork(cache, page_table, lengths, parents=None, new_tokens=None, *,
+                  return_overfull: bool = False):
     """One step of a batch's pages, in every layer of the pool: row i of the
     new batch continues sequence parents[i] (itself without parents; -1 starts
     empty) and gets pages for new_tokens[i] more tokens. Returns (page_table
     [rows,M], lengths [rows] with the new tokens, missing [1]).
+
+    A row has room for M * page_size tokens, and its length stops there: were
+    more of them appended, they would land on tokens that are there already, of
+    other rows too. So a row must have the room. PagedKVCache sees to that; who
+    does not know the lengths on the host asks for `overfull` [1] with
+    return_overfull (a fourth result): the number of rows that have not, on the
+    device, to be read like `missing` before anything is appended.
 
     Pages that no new row holds are free: dropping a sequence frees its own,
     and sequences may share all pages of a prefix. Free pages go in ascending
@@ -249,6 +258,8 @@ def kv_pages_fork(cache, page_table, lengths, parents=None, new_tokens=None):
                 _ptr(parents), _ptr(new_tokens), page_table.stride(0), table.data_ptr(),
                 after.data_ptr(), missing.data_ptr(), st, b, rows, width, pages, layers, page, cb,
                 sb, ws.data_ptr(), need)
+    if return_overfull:
+        return table, after, missing, ws[4:8].view(torch.int32)
     return table, after, missing
 
 
@@ -280,7 +291,13 @@ class PagedKVCache:
             cache.append(l, keys, values)            # packed rows [T,Hkv,D]
             out = cache.attend(l, queries, scale=...)
 
-    and compact() moves the pages in use to the front of the pool."""
+    and compact() moves the pages in use to the front of the pool.
+
+    No row may hold more than max_pages * page_size tokens. The host counts each
+    row's: a step that would exceed it is short of pages like one that the pool
+    has none for (`missing`), and until undo() has taken it back the cache refuses
+    to append, attend, compact or step. `lengths` may be lowered in place (tokens
+    that are taken back) or set, not raised in place."""
 
     def __init__(self, layers: int, pages: int, kv_heads: int, head_dim: int, *,
                  page_size: int = 64, max_pages: int = 128, batch: int = 0, device="cuda"):
@@ -301,14 +318,43 @@ class PagedKVCache:
         self.starts = torch.zeros((batch + 1,), dtype=torch.int32, device=dev)
         self.missing = torch.zeros((1,), dtype=torch.int32, device=dev)
         self.max_new = 0
-        self._last = None
+        self._last, self._full, self._counts = None, False, [0] * batch
+
+    @property
+    def lengths(self):
+        """Tokens of each row, the new ones included (int32, on the device)."""
+        return self._lengths
+
+    @lengths.setter
+    def lengths(self, value):
+        self._lengths, self._counts = value, None  # (counted when a step needs it)
+
+    def _after(self, new_tokens, parents):
+        """Tokens of each row after a step. Lengths are read from the device only
+        where they are not known, or may have been lowered and that matters."""
+        rows, read = self.page_table.shape[0], self._counts is None
+        while True:
+            counts = self._lengths.tolist() if read else self._counts
+            before = counts if parents is None else \
+                [counts[p] if 0 <= p < rows else 0 for p in parents]
+            after = [n + k for n, k in zip(before, new_tokens)]
+            if read or max(after, default=0) <= self.max_pages * self.page_size:
+                return after
+            read = True
+
+    def _ready(self):
+        if self._full:
+            raise ValueError("the last step would fill rows past max_pages * page_size tokens: "
+                             "take it back with undo()")
 
     def step(self, new_tokens, parents=None):
         """Start a step: the batch's rows continue `parents` (itself without)
         and get new_tokens[i] tokens each (a list of Python ints). Returns the
-        packed rows' starts. `missing` then counts the pages that the pool was
-        short of (on the device): a caller that may run short reads it before
-        the step's first append, and takes the step back with undo()."""
+        packed rows' starts. `missing` then counts the pages that the pool, or
+        rows of max_pages, were short of (on the device): a caller that may run
+        short reads it before the step's first append, and takes the step back
+        with undo()."""
+        self._ready()
         new_tokens = [int(n) for n in new_tokens]
         if any(n < 0 for n in new_tokens):
             raise ValueError("new_tokens must not be negative")
@@ -319,14 +365,23 @@ class PagedKVCache:
         for n in new_tokens:
             ends.append(ends[-1] + n)
         dev = self.page_table.device
-        host = new_tokens + ends + ([] if parents is None else [int(p) for p in parents])
+        parents = None if parents is None else [int(p) for p in parents]
+        after = self._after(new_tokens, parents)
+        host = new_tokens + ends + (parents or [])
         ints = torch.tensor(host, dtype=torch.int32, device=dev)
         if parents is not None:
             parents = ints[2 * rows + 1:]
-        last = self.page_table, self.lengths, self.starts, self.max_new
-        self.page_table, self.lengths, self.missing = kv_pages_fork(
-            self.cache, self.page_table, self.lengths, parents, ints[:rows])
-        self._last = last
+        last = self.page_table, self._lengths, self._counts, self.starts, self.max_new
+        short = sum(max(0, -(-n // self.page_size) - self.max_pages) for n in after)
+        if short:  # no page is touched: the tokens without a place would fall on others
+            room = self.max_pages * self.page_size
+            self.page_table = self.page_table.new_full((rows, self.max_pages), -1)
+            self._lengths = ints.new_tensor([min(n, room) for n in after])
+            self.missing, self._full = self.missing.new_full((1,), short), True
+        else:
+            self.page_table, self._lengths, self.missing = kv_pages_fork(
+                self.cache, self.page_table, self._lengths, parents, ints[:rows])
+        self._last, self._counts = last, after
         self.starts, self.max_new = ints[rows:2 * rows + 1], max(new_tokens, default=0)
         return self.starts
 
@@ -335,17 +390,19 @@ class PagedKVCache:
         appended: the batch is what it was, and a smaller step can follow."""
         if self._last is None:
             raise ValueError("there is no step to take back")
-        self.page_table, self.lengths, self.starts, self.max_new = self._last
-        self._last = None
+        self.page_table, self._lengths, self._counts, self.starts, self.max_new = self._last
+        self._last, self._full = None, False
 
     def layer(self, index: int):
         return tuple(t[index] for t in self.cache)
 
     def append(self, index: int, keys, values):
+        self._ready()
         paged_kv_append(keys, values, self.layer(index), self.page_table, self.starts,
                         self.lengths)
 
     def attend(self, index: int, queries, *, scale, mask="causal", out_dtype=None, out=None):
+        self._ready()
         return paged_quantized_sdpa(queries, self.layer(index), self.page_table, self.starts,
                                     self.lengths, scale=scale, max_new=max(self.max_new, 1),
                                     mask=mask, out_dtype=out_dtype, out=out)
@@ -353,6 +410,7 @@ class PagedKVCache:
     def compact(self):
         """Returns the number of pages in use (on the device): the pages from
         it on are free."""
+        self._ready()
         self._last = None
         self.page_table, used = kv_pages_compact(self.cache, self.page_table, self.lengths)
         return used
