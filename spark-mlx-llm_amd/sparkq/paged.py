@@ -387,9 +387,13 @@ class PagedKVCache:
 
     def undo(self):
         """Take back a step that was short of pages, before anything of it was
-        appended: the batch is what it was, and a smaller step can follow."""
+        appended: the batch is what it was, and a smaller step can follow. Reads
+        `missing`. A step that was not short may have copied pages over those of
+        sequences that it dropped, and stands."""
         if self._last is None:
             raise ValueError("there is no step to take back")
+        if self.missing.item() == 0:
+            raise ValueError("the last step was not short of pages")
         self.page_table, self._lengths, self._counts, self.starts, self.max_new = self._last
         self._last, self._full = None, False
 
@@ -398,6 +402,7 @@ class PagedKVCache:
 
     def append(self, index: int, keys, values):
         self._ready()
+        self._last = None  # what is appended cannot be taken back
         paged_kv_append(keys, values, self.layer(index), self.page_table, self.starts,
                         self.lengths)
 

@@ -132,3 +132,33 @@ def test_random_steps_keep_every_token(make, seed):
         told.step(news, parents)
         assert cache.missing.item() == 0
         told.check()
+
+
+def test_undo_takes_back_only_what_it_can(make):
+    """A step that had its pages may have copied them over those of a sequence
+    that it dropped, and what was appended may lie in pages held before."""
+    cache = make(4, 2, 2)
+    told = Told(cache)
+    told.step([20, 16])
+    with pytest.raises(ValueError, match="no step"):  # appended to
+        cache.undo()
+    told.check()
+    dropped = cache.page_table[1, 0].item()
+    cache.step([1, 1], [0, 0])
+    assert cache.missing.item() == 0 and (cache.page_table == dropped).any()
+    state = [t.clone() for t in (cache.page_table, cache.lengths, cache.starts)]
+    with pytest.raises(ValueError, match="was not short"):
+        cache.undo()
+    assert all(torch.equal(a, b) for a, b in
+               zip((cache.page_table, cache.lengths, cache.starts), state))
+    cache.append(0, torch.ones((2, 1, 64)), torch.ones((2, 1, 64)))
+    cache.step([11, 11])  # 32 each
+    cache.step([0, 0, 0], [0, 1, 1])
+    cache.step([16, 0, 16], [-1, 0, -1])  # two pages are held, two free: not short
+    with pytest.raises(ValueError, match="was not short"):
+        cache.undo()
+    cache.step([32, 32, 16], [-1, -1, -1])
+    assert cache.missing.item() == 1
+    cache.append(0, torch.ones((80, 1, 64)), torch.ones((80, 1, 64)))
+    with pytest.raises(ValueError, match="no step"):
+        cache.undo()
