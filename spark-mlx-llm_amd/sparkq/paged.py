@@ -350,7 +350,8 @@ class PagedKVCache:
     def step(self, new_tokens, parents=None):
         """Start a step: the batch's rows continue `parents` (itself without)
         and get new_tokens[i] tokens each (a list of Python ints). Returns the
-        packed rows' starts. `missing` then counts the pages that the pool, or
+        packed rows' starts. Enqueued without waiting for the device, but not in a
+        graph's capture: its numbers come from the host. `missing` then counts the pages that the pool, or
         rows of max_pages, were short of (on the device): a caller that may run
         short reads it before the step's first append, and takes the step back
         with undo()."""
@@ -368,7 +369,14 @@ class PagedKVCache:
         parents = None if parents is None else [int(p) for p in parents]
         after = self._after(new_tokens, parents)
         host = new_tokens + ends + (parents or [])
-        ints = torch.tensor(host, dtype=torch.int32, device=dev)
+        if dev.type == "cuda":
+            # from pinned memory, which torch keeps until the copy is done: a copy from
+            # pageable memory would wait for all that the stream has still to do
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a step takes its numbers from the host and cannot be captured")
+            ints = torch.tensor(host, dtype=torch.int32, pin_memory=True).to(dev, non_blocking=True)
+        else:
+            ints = torch.tensor(host, dtype=torch.int32, device=dev)
         if parents is not None:
             parents = ints[2 * rows + 1:]
         last = self.page_table, self._lengths, self._counts, self.starts, self.max_new
