@@ -27,14 +27,16 @@
 // fp16; a query row is shifted by a power of two to be exact too. The weight
 // of a value, p_n times its scale, is rounded to fp16 once (at most 2^-11 of it,
 // what an fp16 output's own rounding is and an eighth of a bf16 output's), in a
-// unit that puts the largest one near 2^7: 2^8 of room for the running maximum,
-// which tiles move only when a block exceeds it by that much, and full precision
-// down to 2^-19 of the largest. The unit is a power of two beside the maximum
-// itself, so that the weight of the token that it comes from is its value's scale,
-// which fp16 holds: where one token outweighs the rest nothing is lost (fp16 outputs
-// of sharp rows: 1.07 times the error of rounding the exact ones with few rows, where
-// a power of two above the maximum had 1.41). The running maximum, the normalizer and
-// the sums are fp32.
+// unit that the largest of these weights sets, so that neither tokens of small
+// values and much weight nor those of large values and little cost the others their
+// bits: near 2^14 with few rows, near 2^7 in tiles, which move their unit only when
+// a block exceeds it by 2^8. In the products the scales' exponents stand for the
+// scales. So the unit is a power of two beside the score of the token that it comes
+// from, whose weight is then its value's scale times a power of two, which fp16
+// holds: where one token outweighs the rest nothing is lost (fp16 outputs of sharp
+// rows: 1.07 times the error of rounding the exact ones with few rows, where a power
+// of two above the maximum had 1.41). The running maximum, the normalizer and the
+// sums are fp32.
 #include <algorithm>
 #include <type_traits>
 
@@ -268,49 +270,46 @@ __device__ __forceinline__ float pinned(float v) {
 // ---------------------------------------------------------------------------
 // online softmax of one block for one row per lane
 // ---------------------------------------------------------------------------
-// The state counts in units of 2^M, M = m + e - 6: m the maximum of the scores
-// (log2 units) when it last moved, 2^e .. 2^(e+1) the largest finite value scale
-// that the row has seen, so that exp2(s - M) * v_scale < 2^7 at s = m.
+// The state counts in units of 2^(t - TOP), t the largest score (log2 units) plus
+// exponent of the value's scale (2^e <= scale < 2^(e+1)) when it last moved: with
+// TOP = kTopFew or kTopTile, and ROOM for t to be exceeded by, weights stay under
+// 2^15.
 struct RowState {
-  float m = kNegInf;  // -inf: nothing seen
+  float t = kNegInf;  // -inf: nothing seen
   float z = 0.0f;
-  float e = -24.0f;  // of the smallest fp16
 };
+constexpr int kTopFew = 13, kTopTile = 6;
 
-__device__ __forceinline__ float unit(const RowState& st) { return st.m + (st.e - 6.0f); }
+template <int TOP>
+__device__ __forceinline__ float unit(const RowState& st) { return st.t - (float)TOP; }
 
-// |scale|, 0 where it is not finite
-__device__ __forceinline__ float scale_size(float v) {
-  v = fabsf(v);
-  return v <= 65504.0f ? v : 0.0f;
+// The exponent of a value scale's size; no less than -60 (fp16 ends at -24: 0 is
+// meant), so that a row whose best token has no value keeps a finite normalizer.
+__device__ __forceinline__ float scale_exp(float v) {
+  return (float)max((int)(__float_as_uint(v) >> 23 & 255u), 127 - 60) - 127.0f;
 }
 
-// What a part of a row's context hands on: its M, or -inf where it saw nothing
+// What a part of a row's context hands on: its unit, or -inf where it saw nothing
 // (scores that are all NaN leave no maximum, but a sum that is not 0).
+template <int TOP>
 __device__ __forceinline__ float part_max(const RowState& st, float z) {
-  return st.m != kNegInf ? unit(st) : (z != 0.0f ? 0.0f : kNegInf);
+  return st.t != kNegInf ? unit<TOP>(st) : (z != 0.0f ? 0.0f : kNegInf);
 }
 
 // A block's N scores of this lane's row (raw sums times the key scales times
-// the softmax scale: s * mul is in log2 units; -inf where hidden), `size` the
-// largest finite value scale of those that are visible. The maximum moves where a
-// score exceeds it by more than ROOM: 0 with few rows; in tiles, whose sums are dear
-// to scale, 8. Writes the packed fp16 weights of the lane's N values; returns the
-// factor for what is summed so far (up: it is not 1).
-template <int N, int G, int ROOM>
-__device__ __forceinline__ float row_block(RowState& st, const float s[N], float mul, const float vsc[N],
-                                           float size, u32x4_t w[N / 8], bool& up) {
-  float top = s[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) top = fmaxf(top, s[i]);
-  top = max_groups<G>(top) * mul;
-  const float e = fmaxf(st.e, (float)((int)(__float_as_uint(size) >> 23) - 127));
-  const bool raise = top > st.m + ROOM;
-  up = raise || e != st.e;
-  const float old = unit(st);
-  if (raise) st.m = top;
-  st.e = e;
-  const float M = st.m == kNegInf ? 0.0f : unit(st);
+// the softmax scale: s * mul is in log2 units; -inf where hidden), `t` the largest
+// score plus scale exponent of those that are visible, or up to log2(kSpread) more.
+// The state's moves where it is exceeded by more than ROOM: 0 with
+// few rows; in tiles, whose sums are dear to scale, 8. Writes the packed fp16 weights
+// of the lane's N values; returns the factor for what is summed so far (up: it is
+// not 1).
+template <int N, int TOP, int ROOM>
+__device__ __forceinline__ float row_block(RowState& st, const float s[N], float mul, const float vsc[N], float t,
+                                           u32x4_t w[N / 8], bool& up) {
+  up = t > st.t + ROOM;
+  const float old = unit<TOP>(st);
+  if (up) st.t = t;
+  const float M = st.t == kNegInf ? 0.0f : unit<TOP>(st);
   const float alpha = old == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(old - M);
   float p[N], sum = 0.0f;
 #pragma unroll
@@ -331,18 +330,27 @@ __device__ __forceinline__ float kept_scale(float v) {
   return fabsf(v) <= 65504.0f ? v + 0.0f : -0.0f;
 }
 
+// The largest and least value scale of 16 tokens, for blocks that are taken whole
+// (no row hides any of them, and one exponent stands for all). A scale that is not
+// finite makes the largest infinite and the least 0.
+__device__ __forceinline__ float most_of(float v) {
+  return max_row16(fabsf(v) <= 65504.0f ? fabsf(v) : __builtin_huge_valf());
+}
+__device__ __forceinline__ float least_of(float v) { return -max_row16(-fabsf(kept_scale(v))); }
+constexpr float kSpread = 16.0f;  // of the largest to the least that one exponent stands for
+
 // Hides the scores that are not in `ok` and turns those of values that are not
-// finite to NaN; returns the largest value scale of the others.
+// finite to NaN; returns the largest score plus scale exponent of the others.
 template <int N, int G>
-__device__ __forceinline__ float hide(uint32_t ok, float s[N], const float vsc[N]) {
-  float size = 0.0f;
+__device__ __forceinline__ float hide(uint32_t ok, float s[N], float mul, const float vsc[N]) {
+  float t = kNegInf;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const bool live = (ok >> i) & 1u;
     s[i] = live ? (__float_as_uint(vsc[i]) == 0x80000000u ? __builtin_nanf("") : s[i]) : kNegInf;
-    size = fmaxf(size, live ? fabsf(vsc[i]) : 0.0f);
+    t = fmaxf(t, fmaf(s[i], mul, scale_exp(vsc[i])));
   }
-  return max_groups<G>(size);
+  return max_groups<G>(t);
 }
 
 // Four outputs (dims d .. d + 3) of a row.
@@ -409,6 +417,30 @@ __device__ __forceinline__ BlockPages<Q> block_pages(const PagedSdpaArgs& a, Tab
     for (int h = 0; h < Q; ++h) keep(h, look(h));
   }
   return r;
+}
+
+// Which of the TOK (16 or 32) tokens from t0 on have value codes of nothing but 0,
+// a bit each. Such a row is stored with scale 1, which says nothing of its size: it
+// would take the unit away from values that are small beside 1, so its scale is
+// taken for 0. Called where a scale is 1, which is rare: the codes are read again,
+// 64 / TOK lanes a token.
+template <int D, int TOK>
+__device__ __forceinline__ uint32_t zero_values(const PagedSdpaArgs& a, TableRow row, const uint8_t* vhead, int t0) {
+  constexpr int LPT = 64 / TOK, PIECES = D / 16 / LPT;
+  const int lane = threadIdx.x & 63, t = t0 + lane % TOK;
+  const int id = row[min(t >> a.p.page_log2, a.p.width - 1)];
+  const uint8_t* p = vhead + code_at(a.c, (unsigned)id < (unsigned)a.p.pages ? id : 0, t & ((1 << a.p.page_log2) - 1)) +
+                     16 * PIECES * (lane / TOK);
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i) {
+    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(p + 16 * i);
+    any |= x.x | x.y | x.z | x.w;
+  }
+  uint64_t zero = __ballot(any == 0);
+#pragma unroll
+  for (int n = 32; n >= TOK; n /= 2) zero &= zero >> n;
+  return (uint32_t)zero & (uint32_t)((1ull << TOK) - 1);
 }
 
 // ---------------------------------------------------------------------------
@@ -524,36 +556,42 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
     }
     float s[8], vsc[8];
     u16x2_t most = {0, 0};  // the largest scale's bits: finite below those of infinity
+    u16x2_t one = {1, 1};   // 0 where a scale is 1
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t kw = skr[i >> 1], vw = svr[i >> 1];
       s[i] = sc[i >> 2][i & 3] * (((i & 1) ? hi16<F16>(kw) : lo16<F16>(kw)) * a.scale_log2);
       vsc[i] = (i & 1) ? hi16<F16>(vw) : lo16<F16>(vw);
-      if (i & 1) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, vw & 0x7FFF7FFFu));
+      if (i & 1) {
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, vw & 0x7FFF7FFFu));
+        one = __builtin_elementwise_min(one, __builtin_bit_cast(u16x2_t, vw ^ 0x3C003C00u));
+      }
     }
-    const uint16_t top16 = most[0] > most[1] ? most[0] : most[1];
-    float size = f16_to_f32(top16);
-    if (__builtin_expect(t0 + kBlock > all || pages_ok != 3 || __ballot(top16 >= 0x7C00) != 0, 0)) {
+    const bool odd = most[0] >= 0x7C00 || most[1] >= 0x7C00 || one[0] == 0 || one[1] == 0;
+    if (__builtin_expect(t0 + kBlock > all || pages_ok != 3 || __ballot(odd) != 0, 0)) {
       uint32_t ok = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ok |= (uint32_t)(t0 + 8 * grp + i <= lim) << i;
       if (!((pages_ok >> (grp >> 1)) & 1u)) ok = 0;
       ok = __float_as_uint(pinned(__uint_as_float(ok)));
-      size = 0.0f;
+      uint32_t zero = 0;
+      if (__ballot(one[0] == 0 || one[1] == 0)) zero = zero_values<D, 32>(a, trow, vhead, t0) >> (8 * grp);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const bool live = (ok >> i) & 1u;
         s[i] = live ? s[i] : kNegInf;
-        vsc[i] = live ? vsc[i] : 0.0f;
-        size = fmaxf(size, scale_size(vsc[i]));
+        vsc[i] = live && !(((zero >> i) & 1u) && vsc[i] == 1.0f) ? vsc[i] : 0.0f;
       }
     }
-    size = max_groups<4>(size);
+    float t = kNegInf;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t = fmaxf(t, fmaf(s[i], mul, scale_exp(vsc[i])));
+    t = max_groups<4>(t);
     load(ib + 4, next);
     next = block_pages<2>(a, trow, kBlock * min(ib + 8, last));
     u32x4_t w;
     bool up;
-    const float alpha = row_block<8, 4, 0>(st, s, mul, vsc, size, &w, up);
+    const float alpha = row_block<8, kTopFew, 0>(st, s, mul, vsc, t, &w, up);
     if (__ballot(up)) {
       const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
@@ -584,7 +622,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
   float* wacc = wz + 64;                       // [4][16][D]
   if (n16 < rows) {
     if (grp == 0) {
-      wm[wave * 16 + n16] = part_max(st, z);
+      wm[wave * 16 + n16] = part_max<kTopFew>(st, z);
       wz[wave * 16 + n16] = z;
     }
 #pragma unroll
@@ -648,8 +686,8 @@ struct TileShape {
   static constexpr int BLOCK = 64;                    // tokens
   static constexpr int KROW = 2 * D + 16, VROW = 2 * D + 64;
   static constexpr int V = BLOCK * KROW;
-  static constexpr int SCALES = V + BLOCK * VROW;     // of keys, of values, the largest of each 16 of these
-  static constexpr int BUF = SCALES + 2 * BLOCK * 4 + 32;  // (as many again that are not read)
+  static constexpr int SCALES = V + BLOCK * VROW;     // of keys, of values, the largest and least of each 16 of these
+  static constexpr int BUF = SCALES + 2 * BLOCK * 4 + 64;  // (as many again that are not read)
   static constexpr int BYTES = 2 * BUF;
 };
 
@@ -773,7 +811,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
   unsigned char* const vput = smem + S::V + tk0 * S::VROW + 32 * jb;
   float* const sput = reinterpret_cast<float*>(smem + S::SCALES) + (ks_lane ? 0 : kBlock) + 16 * wave + n16;
   float* const bput = reinterpret_cast<float*>(smem + S::SCALES) + 2 * kBlock + (ks_lane ? 4 : 0) + wave;
-  auto stage = [&](auto bufc) {
+  auto stage = [&](auto bufc, int ib) {  // block ib, no further than the last
     constexpr int at = decltype(bufc)::value * S::BUF;
 #pragma unroll
     for (int i = 0; i < PPT; ++i) {
@@ -783,9 +821,14 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
       *reinterpret_cast<u32x4_t*>(vt) = s8x8_exact(vcr[i].x, vcr[i].y);
       *reinterpret_cast<u32x4_t*>(vt + 16) = s8x8_exact(vcr[i].z, vcr[i].w);
     }
-    const float v = f16_to_f32(sr);
+    float v = f16_to_f32(sr);
+    if (__builtin_expect(__ballot(!ks_lane && v == 1.0f) != 0, 0)) {
+      const uint32_t zero = zero_values<D, 16>(a, trow, vhead, kBlock * min(ib, last) + 16 * wave);
+      if (!ks_lane && v == 1.0f && ((zero >> n16) & 1u)) v = 0.0f;
+    }
     sput[at / 4] = ks_lane ? v * a.scale_log2 : kept_scale(v);
-    bput[at / 4] = max_row16(fabsf(v) <= 65504.0f ? fabsf(v) : __builtin_huge_valf());
+    bput[at / 4] = most_of(v);
+    bput[at / 4 + 8] = least_of(v);
   };
 
   const unsigned char* const kget = smem + row * S::KROW + 16 * grp;  // chunk 2 kk + g of token `row`
@@ -820,21 +863,30 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
       }
     }
     const float* big = reinterpret_cast<const float*>(smem + at + S::SCALES) + 2 * kBlock;
-    float size = big[0];
+    float size = big[0], least = big[8];
 #pragma unroll
-    for (int i = 1; i < Q; ++i) size = fmaxf(size, big[i]);
-    if (__builtin_expect(t0 + kBlock > all || pages_ok != (1u << Q) - 1 || size > 65504.0f, 0)) {
+    for (int i = 1; i < Q; ++i) {
+      size = fmaxf(size, big[i]);
+      least = fminf(least, big[8 + i]);
+    }
+    float t;
+    if (__builtin_expect(t0 + kBlock > all || pages_ok != (1u << Q) - 1 || size > kSpread * least, 0)) {
       uint32_t ok = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int t = 4 * G * (i >> 2) + 4 * grp + (i & 3);
-        ok |= (uint32_t)(t0 + t <= lim && ((pages_ok >> (t / 16)) & 1u)) << i;
+        const int j = 4 * G * (i >> 2) + 4 * grp + (i & 3);
+        ok |= (uint32_t)(t0 + j <= lim && ((pages_ok >> (j / 16)) & 1u)) << i;
       }
-      size = hide<N, G>(__float_as_uint(pinned(__uint_as_float(ok))), s, vsc);
+      t = hide<N, G>(__float_as_uint(pinned(__uint_as_float(ok))), s, mul, vsc);
+    } else {
+      t = s[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) t = fmaxf(t, s[i]);
+      t = fmaf(max_groups<G>(t), mul, scale_exp(size));
     }
     u32x4_t w[N / 8];
     bool up;
-    const float alpha = row_block<N, G, 8>(st, s, mul, vsc, size, w, up);
+    const float alpha = row_block<N, kTopTile, 8>(st, s, mul, vsc, t, w, up);
     if (__builtin_expect(__ballot(up) != 0, 0)) {
       const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
@@ -860,14 +912,14 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
     uint32_t ok_now = bp.ok, ok_next;
     load(bp);
     bp = pages(ib0 + 1);
-    stage(std::integral_constant<int, 0>{});
+    stage(std::integral_constant<int, 0>{}, ib0);
     load(bp);
     ok_next = bp.ok;
     __syncthreads();
     auto step = [&](int ib, auto cur) {
       const Pages after = pages(ib + 2);
       if (wr0 < it.rows) compute(cur, kBlock * ib, ok_now);
-      stage(std::integral_constant<int, 1 - decltype(cur)::value>{});
+      stage(std::integral_constant<int, 1 - decltype(cur)::value>{}, ib + 1);
       load(after);
       ok_now = ok_next;
       ok_next = after.ok;
@@ -902,7 +954,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
         *reinterpret_cast<f32x4_t*>(a.pacc + at * D + 32 * j + 2 * v + 4 * grp) =
             f32x4_t{acc[j][v], acc[j][v + 1], acc[j][v + 2], acc[j][v + 3]};
     if (grp == 0) {
-      a.pm[at] = part_max(st, z);
+      a.pm[at] = part_max<kTopTile>(st, z);
       a.pz[at] = z;
     }
   }
@@ -934,9 +986,9 @@ struct PairShape {
   static constexpr int D = 256, BLOCK = 64;
   static constexpr int KROW = 2 * D + 16, VROW = 2 * D + 64;
   static constexpr int V = BLOCK * KROW, P = V + BLOCK * VROW;
-  static constexpr int STATE = P + 8 * 2 * 1024;      // of each wave's rows: maximum, scale exponent
-  static constexpr int SCALES = STATE + 8 * 32 * 8;   // of keys, of values, the largest of each 16 of these
-  static constexpr int BYTES = SCALES + 2 * BLOCK * 4 + 16;
+  static constexpr int STATE = P + 8 * 2 * 1024;      // of each wave's rows: t
+  static constexpr int SCALES = STATE + 8 * 32 * 4;   // of keys, of values, the largest and least of each 16 of these
+  static constexpr int BYTES = SCALES + 2 * BLOCK * 4 + 32;
 };
 
 template <int PG>  // pages that a block lies in: 1, 2 or 4
@@ -1000,11 +1052,16 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
     *reinterpret_cast<u32x4_t*>(t + 16) = s8x8_exact(c.z, c.w);
   };
   float* const scl = reinterpret_cast<float*>(smem + S::SCALES);
-  auto stage_scales = [&]() __attribute__((always_inline)) {
-    const float v = f16_to_f32(svr);
+  auto stage_scales = [&](int ib) __attribute__((always_inline)) {  // block ib, no further than the last
+    float v = f16_to_f32(svr);
+    if (__builtin_expect(__ballot(v == 1.0f) != 0, 0)) {
+      const uint32_t zero = zero_values<D, 16>(a, trow, vhead, kBlock * min(ib, last) + 16 * srun);
+      if (v == 1.0f && ((zero >> n16) & 1u)) v = 0.0f;
+    }
     scl[16 * srun + n16] = f16_to_f32(skr) * a.scale_log2;
     scl[kBlock + 16 * srun + n16] = kept_scale(v);
-    scl[2 * kBlock + srun] = max_row16(fabsf(v) <= 65504.0f ? fabsf(v) : __builtin_huge_valf());
+    scl[2 * kBlock + srun] = most_of(v);
+    scl[2 * kBlock + 4 + srun] = least_of(v);
   };
 
   const unsigned char* const kget = smem + (32 * half + row) * S::KROW + 16 * grp;
@@ -1012,7 +1069,7 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
                                     32 * ((lane >> 4) & 1) + 256 * half;
   unsigned char* const pput = smem + S::P + wave * 2048 + lane * 16;
   const unsigned char* const pget = smem + S::P + (wave ^ 1) * 2048 + lane * 16;
-  float2* const state = reinterpret_cast<float2*>(smem + S::STATE);
+  float* const state = reinterpret_cast<float*>(smem + S::STATE);
   const int own = 32 * half * S::VROW, other = 32 * (half ^ 1) * S::VROW;
   RowState st;
   Sum acc[NJ];
@@ -1041,18 +1098,26 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
       }
     }
     const f32x4_t big = *reinterpret_cast<const f32x4_t*>(scl + 2 * kBlock);
-    float size = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
-    if (__builtin_expect(t0 + kBlock > all || pages_ok != (1u << Q) - 1 || size > 65504.0f, 0)) {
+    const f32x4_t low = *reinterpret_cast<const f32x4_t*>(scl + 2 * kBlock + 4);
+    const float size = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3]));
+    const float least = fminf(fminf(low[0], low[1]), fminf(low[2], low[3]));
+    float t;
+    if (__builtin_expect(t0 + kBlock > all || pages_ok != (1u << Q) - 1 || size > kSpread * least, 0)) {
       uint32_t ok = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int t = 32 * half + 4 * G * (i >> 2) + 4 * grp + (i & 3);
-        ok |= (uint32_t)(t0 + t <= lim && ((pages_ok >> (t / 16)) & 1u)) << i;
+        const int j = 32 * half + 4 * G * (i >> 2) + 4 * grp + (i & 3);
+        ok |= (uint32_t)(t0 + j <= lim && ((pages_ok >> (j / 16)) & 1u)) << i;
       }
-      size = hide<N, G>(__float_as_uint(pinned(__uint_as_float(ok))), s, vsc);
+      t = hide<N, G>(__float_as_uint(pinned(__uint_as_float(ok))), s, mul, vsc);
+    } else {
+      t = s[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) t = fmaxf(t, s[i]);
+      t = fmaf(max_groups<G>(t), mul, scale_exp(size));
     }
     bool up;
-    const float alpha = row_block<N, G, 8>(st, s, mul, vsc, size, w, up);
+    const float alpha = row_block<N, kTopTile, 8>(st, s, mul, vsc, t, w, up);
     if (__builtin_expect(__ballot(up) != 0, 0)) {
       const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
@@ -1060,13 +1125,13 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
     }
     *reinterpret_cast<u32x4_t*>(pput) = w[0];
     *reinterpret_cast<u32x4_t*>(pput + 1024) = w[1];
-    state[32 * wave + row] = make_float2(st.m, st.e);
+    state[32 * wave + row] = st.t;
   };
   // the outputs of this wave's 128 dims, and the next keys into LDS
   auto second = [&](int) __attribute__((always_inline)) {
     w[2] = *reinterpret_cast<const u32x4_t*>(pget);
     w[3] = *reinterpret_cast<const u32x4_t*>(pget + 1024);
-    const float2 o = state[32 * (wave ^ 1) + row];
+    const float o = state[32 * (wave ^ 1) + row];
     typedef short s16x4_t __attribute__((ext_vector_type(4)));
     typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
     auto product = [&](int k, int j) __attribute__((always_inline)) {
@@ -1084,16 +1149,15 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
         product(k, j);
         if (k == 1 && j < PPT) stage(kput + j * 32 * S::KROW, kcr[j]);
       }
-    const float mine = unit(st), theirs = o.x + (o.y - 6.0f);
+    const float mine = st.t, theirs = o;
     const bool differ = __ballot(mine != theirs) != 0;
     float after = 1.0f;
     if (__builtin_expect(differ, 0)) {
       // The sums go into the other's unit while its weights are added, so that these
       // stay as they were rounded; weights whose unit is 2^-60 of the row's own do not
       // count. (A half that has seen nothing has the unit 2^-inf.)
-      st.m = fmaxf(st.m, o.x);
-      st.e = fmaxf(st.e, o.y);
-      const float now = unit(st), gap = mine - theirs;
+      st.t = fmaxf(mine, theirs);
+      const float now = st.t, gap = mine - theirs;
       const bool near = gap <= 60.0f;
       const float rest = mine == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mine - now);
       const float before = pinned(near ? __builtin_amdgcn_exp2f(gap) : 1.0f);
@@ -1120,7 +1184,7 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
     load_scales(now);
 #pragma unroll
     for (int i = 0; i < PPT; ++i) stage(kput + i * 32 * S::KROW, kcr[i]);
-    stage_scales();
+    stage_scales(ib0);
     load_codes(vhead, now, vcr);
     load_codes(khead, next, kcr);
     load_scales(next);
@@ -1131,7 +1195,7 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
       load_codes(vhead, next, vcr);
       __syncthreads();
       two();
-      stage_scales();
+      stage_scales(ib + 1);
       load_codes(khead, after, kcr);
       load_scales(after);
       now = next;
@@ -1158,9 +1222,9 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
 
   // the halves' sums (every wave is past its last read of the states)
   float z = sum_groups<G>(st.z);
-  state[32 * wave + row].x = z;
+  state[32 * wave + row] = z;
   __syncthreads();
-  z += state[32 * (wave ^ 1) + row].x;
+  z += state[32 * (wave ^ 1) + row];
   const int r = 32 * (wave >> 1) + row;
   if (r >= rows) return;
   if (it.parts == 1) {
@@ -1181,7 +1245,7 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
         *reinterpret_cast<f32x4_t*>(a.pacc + at * D + 128 * half + 32 * j + 2 * v + 4 * grp) =
             f32x4_t{acc[j][v], acc[j][v + 1], acc[j][v + 2], acc[j][v + 3]};
     if (grp == 0 && half == 0) {
-      a.pm[at] = part_max(st, z);
+      a.pm[at] = part_max<kTopTile>(st, z);
       a.pz[at] = z;
     }
   }

@@ -146,14 +146,15 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
     """Attention of a batch's new tokens over their pages: queries [T,Hq,D]
     (float16 or bfloat16) -> [T,Hq,D]. With mask="causal" row i of a
     sequence's n new tokens sees its tokens 0 .. length - n + i, with None all
-    of them; tokens without a page are hidden, a row that sees nothing is zero, and
-    one that sees a value scale that is not finite has no finite values. max_new is the most new tokens that a sequence has (1: a decode
+    of them; tokens without a page are hidden, a row that sees nothing is zero,
+    and one that sees a value scale that is not finite has no finite values. max_new is the most new tokens that a sequence has (1: a decode
     step). Rows that fall to no sequence, or to more than max_new of one, are
     left as they are in `out`, and hold anything in a new tensor. Codes and
     scales of keys lie as those of values do (the same strides), a page's scales
     of a head together. A weight times its value's scale is rounded to float16
-    once (from 2^-19 of the row's largest down, to 2^-29 of that); scores,
-    normalizer and sums are fp32."""
+    once (11 bits; below 2^-16 of the row's largest such product, of a value
+    that is not all zeros, to 2^-27 of that); scores, normalizer and sums are
+    fp32."""
     op = "paged_quantized_sdpa"
     kc, ks, vc, vs, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
     if queries.ndim != 3 or queries.shape[2] != d or not queries.shape[1] \
