@@ -25,16 +25,20 @@
 //
 // Numerics. Both products are fp16 MFMAs with fp32 sums. Codes are exact in
 // fp16; a query row is shifted by a power of two to be exact too. The weight
-// of a value, p_n times its scale, is rounded to fp16 once (at most 2^-11 of it,
-// what an fp16 output's own rounding is and an eighth of a bf16 output's), in a
+// of a value, p_n times its scale, goes in as two fp16 operands, what the first's
+// rounding leaves being the second (22 bits), with few rows, where the matrix cores
+// idle (64 sequences 66.9 -> 67.5 us), and in tiles with fp32 outputs. With 16-bit
+// outputs tiles take one, off by at most 2^-11, what an fp16 output's own rounding is
+// and an eighth of a bf16 output's: the second product costs a quarter of the time
+// (2048 new tokens 315 -> 392 us, 24 sequences at D = 256 290 -> 343). All of them in a
 // unit that the largest of these weights sets, so that neither tokens of small
 // values and much weight nor those of large values and little cost the others their
 // bits: near 2^14 with few rows, near 2^7 in tiles, which move their unit only when
 // a block exceeds it by 2^8. In the products the scales' exponents stand for the
 // scales. So the unit is a power of two beside the score of the token that it comes
-// from, whose weight is then its value's scale times a power of two, which fp16
+// from, whose weight is then its value's scale times a power of two, which one fp16
 // holds: where one token outweighs the rest nothing is lost (fp16 outputs of sharp
-// rows: 1.07 times the error of rounding the exact ones with few rows, where a power
+// rows in tiles: 1.07 to 1.13 times the error of rounding the exact ones, where a power
 // of two above the maximum had 1.41). The running maximum, the normalizer and the
 // sums are fp32.
 #include <algorithm>
@@ -301,11 +305,11 @@ __device__ __forceinline__ float part_max(const RowState& st, float z) {
 // score plus scale exponent of those that are visible, or up to log2(kSpread) more.
 // The state's moves where it is exceeded by more than ROOM: 0 with
 // few rows; in tiles, whose sums are dear to scale, 8. Writes the packed fp16 weights
-// of the lane's N values; returns the factor for what is summed so far (up: it is
-// not 1).
-template <int N, int TOP, int ROOM>
+// of the lane's N values (with TWO also what their rounding left of them); returns
+// the factor for what is summed so far (up: it is not 1).
+template <int N, int TOP, int ROOM, bool TWO>
 __device__ __forceinline__ float row_block(RowState& st, const float s[N], float mul, const float vsc[N], float t,
-                                           u32x4_t w[N / 8], bool& up) {
+                                           u32x4_t w[N / 8], u32x4_t rest[N / 8], bool& up) {
   up = t > st.t + ROOM;
   const float old = unit<TOP>(st);
   if (up) st.t = t;
@@ -320,7 +324,11 @@ __device__ __forceinline__ float row_block(RowState& st, const float s[N], float
   }
   st.z = fmaf(st.z, up ? alpha : 1.0f, sum);
 #pragma unroll
-  for (int i = 0; i < N; i += 2) w[i / 8][i / 2 % 4] = pack_f16(p[i], p[i + 1]);
+  for (int i = 0; i < N; i += 2) {
+    const uint32_t h = pack_f16(p[i], p[i + 1]);
+    w[i / 8][i / 2 % 4] = h;
+    if (TWO) rest[i / 8][i / 2 % 4] = pack_f16(p[i] - lo16<F16>(h), p[i + 1] - hi16<F16>(h));
+  }
   return alpha;
 }
 
@@ -589,9 +597,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
     t = max_groups<4>(t);
     load(ib + 4, next);
     next = block_pages<2>(a, trow, kBlock * min(ib + 8, last));
-    u32x4_t w;
+    u32x4_t w, rest;
     bool up;
-    const float alpha = row_block<8, kTopFew, 0>(st, s, mul, vsc, t, &w, up);
+    const float alpha = row_block<8, kTopFew, 0, true>(st, s, mul, vsc, t, &w, &rest, up);
     if (__ballot(up)) {
       const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
@@ -603,7 +611,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
       typedef int v2i_t __attribute__((ext_vector_type(2)));
       const v2i_t t8 = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
           (__attribute__((address_space(3))) v2i_t*)(vaddr + 16 * j));
-      acc[j] = mfma16x16x32_f16(s8x8_exact((uint32_t)t8.x, (uint32_t)t8.y), w, acc[j]);
+      const u32x4_t v8 = s8x8_exact((uint32_t)t8.x, (uint32_t)t8.y);
+      acc[j] = mfma16x16x32_f16(v8, w, acc[j]);
+      acc[j] = mfma16x16x32_f16(v8, rest, acc[j]);
     }
   };
 
@@ -747,7 +757,7 @@ __device__ __forceinline__ TilePages<PG, PPT> tile_pages(const PagedSdpaArgs& a,
 
 __device__ __forceinline__ f32x16_t tile_mfma(u32x4_t x, u32x4_t y, f32x16_t c) { return mfma32x32x16<F16>(x, y, c); }
 
-template <int D, int PG>
+template <int D, int PG, bool TWO>
 __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
   using S = TileShape<D>;
   constexpr int R = kTileRows, kBlock = S::BLOCK, G = 2, N = kBlock / G, Q = kBlock / 16;
@@ -884,9 +894,9 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
       for (int i = 1; i < N; ++i) t = fmaxf(t, s[i]);
       t = fmaf(max_groups<G>(t), mul, scale_exp(size));
     }
-    u32x4_t w[N / 8];
+    u32x4_t w[N / 8], rest[N / 8];
     bool up;
-    const float alpha = row_block<N, kTopTile, 8>(st, s, mul, vsc, t, w, up);
+    const float alpha = row_block<N, kTopTile, 8, TWO>(st, s, mul, vsc, t, w, rest, up);
     if (__builtin_expect(__ballot(up) != 0, 0)) {
       const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
@@ -904,6 +914,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
         const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
             (__attribute__((address_space(3))) s16x4_t*)(vp + 8 * S::VROW)));
         acc[j] = tile_mfma(u32x4_t{lo.x, lo.y, hi.x, hi.y}, w[k], acc[j]);
+        if (TWO) acc[j] = tile_mfma(u32x4_t{lo.x, lo.y, hi.x, hi.y}, rest[k], acc[j]);
       }
   };
 
@@ -982,18 +993,19 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
 // of each and a barrier after each phase. (Half the waves a phase behind the others,
 // with two buffers, took 306 us for these 296.) Bound by the latency of a wave's own chain through
 // these phases.
+template <bool TWO>
 struct PairShape {
   static constexpr int D = 256, BLOCK = 64;
   static constexpr int KROW = 2 * D + 16, VROW = 2 * D + 64;
   static constexpr int V = BLOCK * KROW, P = V + BLOCK * VROW;
-  static constexpr int STATE = P + 8 * 2 * 1024;      // of each wave's rows: t
+  static constexpr int STATE = P + 8 * 2 * 1024 * (TWO ? 2 : 1);  // of each wave's rows: t
   static constexpr int SCALES = STATE + 8 * 32 * 4;   // of keys, of values, the largest and least of each 16 of these
   static constexpr int BYTES = SCALES + 2 * BLOCK * 4 + 32;
 };
 
-template <int PG>  // pages that a block lies in: 1, 2 or 4
+template <int PG, bool TWO>  // pages that a block lies in: 1, 2 or 4
 __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
-  using S = PairShape;
+  using S = PairShape<TWO>;
   constexpr int D = S::D, R = kTileRows, kBlock = S::BLOCK, N = 16, Q = kBlock / 16, G = 2;
   constexpr int NK = D / 16, NJ = 4, PPT = 2;
   using Sum = f32x16_t;
@@ -1067,15 +1079,16 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
   const unsigned char* const kget = smem + (32 * half + row) * S::KROW + 16 * grp;
   const unsigned char* const vget = smem + S::V + (4 * grp + (n16 >> 2)) * S::VROW + 8 * (n16 & 3) +
                                     32 * ((lane >> 4) & 1) + 256 * half;
-  unsigned char* const pput = smem + S::P + wave * 2048 + lane * 16;
-  const unsigned char* const pget = smem + S::P + (wave ^ 1) * 2048 + lane * 16;
+  constexpr int WAVE = TWO ? 4096 : 2048;
+  unsigned char* const pput = smem + S::P + wave * WAVE + lane * 16;
+  const unsigned char* const pget = smem + S::P + (wave ^ 1) * WAVE + lane * 16;
   float* const state = reinterpret_cast<float*>(smem + S::STATE);
   const int own = 32 * half * S::VROW, other = 32 * (half ^ 1) * S::VROW;
   RowState st;
   Sum acc[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) acc[j] = Sum{};
-  u32x4_t w[4];  // of the half of this wave, of the other
+  u32x4_t w[4], rest[4];  // of the half of this wave, of the other
 
   // scores and weights of this wave's 32 tokens, and values into LDS
   auto first = [&](int t0, uint32_t pages_ok) __attribute__((always_inline)) {
@@ -1117,7 +1130,7 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
       t = fmaf(max_groups<G>(t), mul, scale_exp(size));
     }
     bool up;
-    const float alpha = row_block<N, kTopTile, 8>(st, s, mul, vsc, t, w, up);
+    const float alpha = row_block<N, kTopTile, 8, TWO>(st, s, mul, vsc, t, w, rest, up);
     if (__builtin_expect(__ballot(up) != 0, 0)) {
       const float f = pinned(up ? alpha : 1.0f);
 #pragma unroll
@@ -1125,12 +1138,20 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
     }
     *reinterpret_cast<u32x4_t*>(pput) = w[0];
     *reinterpret_cast<u32x4_t*>(pput + 1024) = w[1];
+    if (TWO) {
+      *reinterpret_cast<u32x4_t*>(pput + 2048) = rest[0];
+      *reinterpret_cast<u32x4_t*>(pput + 3072) = rest[1];
+    }
     state[32 * wave + row] = st.t;
   };
   // the outputs of this wave's 128 dims, and the next keys into LDS
   auto second = [&](int) __attribute__((always_inline)) {
     w[2] = *reinterpret_cast<const u32x4_t*>(pget);
     w[3] = *reinterpret_cast<const u32x4_t*>(pget + 1024);
+    if (TWO) {
+      rest[2] = *reinterpret_cast<const u32x4_t*>(pget + 2048);
+      rest[3] = *reinterpret_cast<const u32x4_t*>(pget + 3072);
+    }
     const float o = state[32 * (wave ^ 1) + row];
     typedef short s16x4_t __attribute__((ext_vector_type(4)));
     typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
@@ -1141,6 +1162,7 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
       const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4_t*)(vp + 8 * S::VROW)));
       acc[j] = tile_mfma(u32x4_t{lo.x, lo.y, hi.x, hi.y}, w[k], acc[j]);
+      if (TWO) acc[j] = tile_mfma(u32x4_t{lo.x, lo.y, hi.x, hi.y}, rest[k], acc[j]);
     };
 #pragma unroll
     for (int k = 0; k < 2; ++k)
@@ -1159,11 +1181,11 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
       st.t = fmaxf(mine, theirs);
       const float now = st.t, gap = mine - theirs;
       const bool near = gap <= 60.0f;
-      const float rest = mine == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mine - now);
+      const float own_factor = mine == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(mine - now);
       const float before = pinned(near ? __builtin_amdgcn_exp2f(gap) : 1.0f);
-      after = near ? __builtin_amdgcn_exp2f(theirs - now) : rest;
-      if (!near) w[2] = w[3] = u32x4_t{0, 0, 0, 0};
-      st.z *= rest;
+      after = near ? __builtin_amdgcn_exp2f(theirs - now) : own_factor;
+      if (!near) w[2] = w[3] = rest[2] = rest[3] = u32x4_t{0, 0, 0, 0};
+      st.z *= own_factor;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) acc[j] *= before;
     }
@@ -1357,12 +1379,22 @@ PagedPlan paged_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
   return p;
 }
 
-template <int D, int PG>
+template <int D, int PG, bool TWO>
 void launch_tile(const PagedSdpaArgs& a, dim3 grid, hipStream_t st) {
   if constexpr (D <= 128)
-    hipLaunchKernelGGL((paged_tile_kernel<D, PG>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((paged_tile_kernel<D, PG, TWO>), grid, dim3(256), 0, st, a);
   else
-    hipLaunchKernelGGL(paged_pair_kernel<PG>, grid, dim3(512), 0, st, a);
+    hipLaunchKernelGGL((paged_pair_kernel<PG, TWO>), grid, dim3(512), 0, st, a);
+}
+
+template <int D, bool TWO>
+void launch_tiles(const PagedSdpaArgs& a, dim3 grid, hipStream_t st) {
+  if (a.p.page_log2 >= 6)
+    launch_tile<D, 1, TWO>(a, grid, st);
+  else if (a.p.page_log2 == 5)
+    launch_tile<D, 2, TWO>(a, grid, st);
+  else
+    launch_tile<D, 4, TWO>(a, grid, st);
 }
 
 template <int D>
@@ -1371,12 +1403,10 @@ void launch_paged(const PagedSdpaArgs& a, const PagedPlan& p, hipStream_t st) {
   const dim3 merge((unsigned)(p.split * (p.rows / 16) * a.Hkv));
   if (p.few)
     hipLaunchKernelGGL(paged_few_kernel<D>, grid, dim3(256), 0, st, a);
-  else if (a.p.page_log2 >= 6)
-    launch_tile<D, 1>(a, grid, st);
-  else if (a.p.page_log2 == 5)
-    launch_tile<D, 2>(a, grid, st);
+  else if (a.out_dtype == SPARKQ_F32)
+    launch_tiles<D, true>(a, grid, st);
   else
-    launch_tile<D, 4>(a, grid, st);
+    launch_tiles<D, false>(a, grid, st);
   if (merge.x == 0) return;
   if (p.few)
     hipLaunchKernelGGL((paged_merge_kernel<D, 16>), merge, dim3(256), 0, st, a);

@@ -151,10 +151,12 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
     step). Rows that fall to no sequence, or to more than max_new of one, are
     left as they are in `out`, and hold anything in a new tensor. Codes and
     scales of keys lie as those of values do (the same strides), a page's scales
-    of a head together. A weight times its value's scale is rounded to float16
-    once (11 bits; below 2^-16 of the row's largest such product, of a value
-    that is not all zeros, to 2^-27 of that); scores, normalizer and sums are
-    fp32."""
+    of a head together. A weight times its value's scale
+    is held in 22 bits in calls of up to 16 rows a sequence and KV head (max_new *
+    Hq / Hkv: decode steps, a few drafted tokens) and wherever out_dtype is
+    float32; in others, with 16-bit outputs, in float16's 11, which their own
+    rounding is near (float32 outputs cost up to a quarter more time there). Scores,
+    normalizer and sums are fp32."""
     op = "paged_quantized_sdpa"
     kc, ks, vc, vs, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
     if queries.ndim != 3 or queries.shape[2] != d or not queries.shape[1] \

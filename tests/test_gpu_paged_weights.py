@@ -4,7 +4,9 @@ large values and next to no weight, tokens of small values and all the weight.
 
 Tolerance of an output o = sum p v / sum p, v = scale * code, P the largest p *
 scale of a token that has a code other than 0:
- - each weight's rounding to fp16: `bits` of it (2^-11: half a step of 11 bits);
+ - each weight's rounding: `bits` of it. 2^-11, half a step of fp16's 11 bits, in
+   tiles with a 16-bit output. Else what fp16 leaves, 2^-11 of the weight at most, is
+   a second operand and rounded by 2^-11 in turn: 2^-22;
  - weights under fp16's normal range, rounded to half of 2^-24: with few rows the
    unit puts P at 2^13 or above, so 2^-38 of P each; in tiles at 2^6, less 2^4 by
    which the scales of a block that is taken whole may differ: 2^-27 of P. In all
@@ -44,7 +46,7 @@ def _case(kind, amp, n, new, hq, hkv, d, page, seed):
 
     first, last = 0, n - new  # the last one that every row sees
     special = {"zero low": [3, last], "zero": [0, n // 2], "zero high": [n // 3],
-               "zero block": list(range(64, min(192, last))), "far": [2, last], "sink": [first]}[kind]
+               "zero block": list(range(64, min(192, last))), "far": [2, last], "sink": [first], "plain": []}[kind]
     for at in special:
         if kind.startswith("zero"):
             vc[at], vs[at] = 0, 1.0
@@ -124,7 +126,47 @@ def test_no_token_costs_the_others_their_bits(gpu, kind, amp, n, new, hq, hkv, d
         out = sparkq.paged_quantized_sdpa(q.to(gpu), cache, table, _ints([0, new], gpu),
                                           _ints([n], gpu), scale=d ** -0.5, max_new=new,
                                           out_dtype=dtype)
-        _check(out, q, kc, ks, vc, vs, 2.0 ** -11, 2.0 ** (-38 if few else -27))
+        bits = 2.0 ** (-22 if few or dtype == torch.float32 else -11)
+        _check(out, q, kc, ks, vc, vs, bits, 2.0 ** (-38 if few else -27))
+
+
+@pytest.mark.parametrize("n,new,hq,hkv,d,page", [
+    (700, 1, 4, 1, 64, 64), (900, 1, 8, 2, 128, 16), (500, 4, 8, 2, 128, 64), (600, 1, 4, 1, 256, 32),
+    (900, 40, 8, 2, 128, 64), (300, 100, 4, 1, 64, 16), (400, 50, 4, 1, 256, 32)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_contiguous_caches_bars(gpu, n, new, hq, hkv, d, page, dtype):
+    """Weights of 22 bits: with few rows 16-bit outputs are within one unit of the
+    rounded float64 ones, where these are not small, and float32 ones have 2e-5 of
+    their norm whatever the rows. (A score of D products is off by some sqrt(D)
+    2^-24 of its partial sums, independently of the others, as each weight is by
+    2^-22, and the output, itself a sum of n terms of either sign, by about as much
+    of itself: 16 * 2^-24 * 8 = 8e-6. Weights of 11 bits leave 1.5e-4.)"""
+    import sparkq
+
+    import oracle as o
+    from helpers import check_rounded16, rel_l2
+
+    q, kc, ks, vc, vs = _case("plain", 1.0, n, new, hq, hkv, d, page, seed=7)
+    q = q.to(dtype)
+    cache, table = _pool(gpu, kc, ks, vc, vs, page, 2)
+    want = torch.zeros((new, hq, d), dtype=torch.float64)
+    see = torch.ones((new, n), dtype=torch.bool).tril(n - new)
+    for h in range(hq):
+        k, v = (c[:, h * hkv // hq].double() * x[:, h * hkv // hq].double()[:, None]
+                for c, x in ((kc, ks), (vc, vs)))
+        sc = torch.where(see, q[:, h].double() @ k.T * d ** -0.5, -torch.inf)
+        want[:, h] = torch.softmax(sc, -1) @ v
+    for out_dtype in (torch.float32, dtype):
+        out = sparkq.paged_quantized_sdpa(q.to(gpu), cache, table, _ints([0, new], gpu),
+                                          _ints([n], gpu), scale=d ** -0.5, max_new=new,
+                                          out_dtype=out_dtype).cpu()
+        if out_dtype == torch.float32:
+            rel = rel_l2(out.numpy(), want.numpy())
+            print(f"[weights] relative L2 error {rel:.2e}", flush=True)
+            assert rel <= 2e-5
+        elif new * hq // hkv <= 16:
+            check_rounded16(out.view(torch.int16).numpy().view("uint16"), want.numpy(),
+                            o.BF16 if dtype == torch.bfloat16 else o.F16)
 
 
 @pytest.mark.parametrize("n,new,hq,hkv,d,page", [
