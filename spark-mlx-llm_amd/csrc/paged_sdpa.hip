@@ -1291,6 +1291,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedSdpaArgs a) {
   if (it.b < 0) return;
   const int r0 = 16 * (x % GROUPS);
   const int rows = min(it.rows - R * it.tile - r0, 16), parts = it.parts;
+  if (rows <= 0) return;
   const int64_t base = ((int64_t)kh * a.slots + it.slot) * R + r0;
   for (int r = wave; r < rows; r += 4) {
     float mm = kNegInf, z = 0.0f;
