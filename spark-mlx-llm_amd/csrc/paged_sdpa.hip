@@ -73,7 +73,7 @@ struct PagedSdpaArgs {
   int slots;       // parts of split contexts, at most, per KV head
   int min_part;    // tokens of a part, at least
   int snake;       // items that the chip's CUs take a round of, per KV head (0: in order)
-  float scale_log2;
+  float scale_log2, sign;  // size (log2 units) and sign of the softmax scale
 };
 
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
@@ -238,7 +238,10 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 
 // A row's query values as exact fp16: chunk c of this lane holds dims dim0(c) ..
 // +8. bf16 rows are shifted by a power of two for that; returns the factor that
-// undoes it. (What bf16 can hold below 2^-28 of the row's largest is rounded.)
+// undoes it, times the softmax scale: what takes the row's sums times the key scales
+// to log2 units. (Scaled sooner, rows of the smallest queries could pass fp32's
+// range; where it ends under 2^-126, every score is next to 0, and stays so. What
+// bf16 can hold below 2^-28 of the row's largest is rounded.)
 template <int NK, int G, typename F>
 __device__ __forceinline__ float load_query(const PagedSdpaArgs& a, const uint16_t* row, bool live, F dim0,
                                             u32x4_t qb[NK]) {
@@ -247,7 +250,7 @@ __device__ __forceinline__ float load_query(const PagedSdpaArgs& a, const uint16
     qb[c] = *reinterpret_cast<const u32x4_t*>(row + dim0(c));
     if (!live) qb[c] = u32x4_t{0, 0, 0, 0};
   }
-  if (a.q_dtype == SPARKQ_F16) return 1.0f;
+  if (a.q_dtype == SPARKQ_F16) return fmaxf(a.scale_log2, 0x1p-126f);
   u16x2_t most = {0, 0};
 #pragma unroll
   for (int c = 0; c < NK; ++c)
@@ -261,7 +264,7 @@ __device__ __forceinline__ float load_query(const PagedSdpaArgs& a, const uint16
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       qb[c][i] = pack_f16(ldexpf(lo16<BF16>(qb[c][i]), -e), ldexpf(hi16<BF16>(qb[c][i]), -e));
-  return ldexpf(1.0f, e);
+  return fmaxf(ldexpf(a.scale_log2, e), 0x1p-126f);
 }
 
 // v, in a way that what depends on it stays in its branch: the compiler would
@@ -300,8 +303,8 @@ __device__ __forceinline__ float part_max(const RowState& st, float z) {
   return st.t != kNegInf ? unit<TOP>(st) : (z != 0.0f ? 0.0f : kNegInf);
 }
 
-// A block's N scores of this lane's row (raw sums times the key scales times
-// the softmax scale: s * mul is in log2 units; -inf where hidden), `t` the largest
+// A block's N scores of this lane's row (raw sums times the key scales and the
+// softmax scale's sign: s * mul is in log2 units; -inf where hidden), `t` the largest
 // score plus scale exponent of those that are visible, or up to log2(kSpread) more.
 // The state's moves where it is exceeded by more than ROOM: 0 with
 // few rows; in tiles, whose sums are dear to scale, 8. Writes the packed fp16 weights
@@ -568,7 +571,7 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const uint32_t kw = skr[i >> 1], vw = svr[i >> 1];
-      s[i] = sc[i >> 2][i & 3] * (((i & 1) ? hi16<F16>(kw) : lo16<F16>(kw)) * a.scale_log2);
+      s[i] = sc[i >> 2][i & 3] * (((i & 1) ? hi16<F16>(kw) : lo16<F16>(kw)) * a.sign);
       vsc[i] = (i & 1) ? hi16<F16>(vw) : lo16<F16>(vw);
       if (i & 1) {
         most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, vw & 0x7FFF7FFFu));
@@ -836,7 +839,7 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
       const uint32_t zero = zero_values<D, 16>(a, trow, vhead, kBlock * min(ib, last) + 16 * wave);
       if (!ks_lane && v == 1.0f && ((zero >> n16) & 1u)) v = 0.0f;
     }
-    sput[at / 4] = ks_lane ? v * a.scale_log2 : kept_scale(v);
+    sput[at / 4] = ks_lane ? v * a.sign : kept_scale(v);
     bput[at / 4] = most_of(v);
     bput[at / 4 + 8] = least_of(v);
   };
@@ -1070,7 +1073,7 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
       const uint32_t zero = zero_values<D, 16>(a, trow, vhead, kBlock * min(ib, last) + 16 * srun);
       if (v == 1.0f && ((zero >> n16) & 1u)) v = 0.0f;
     }
-    scl[16 * srun + n16] = f16_to_f32(skr) * a.scale_log2;
+    scl[16 * srun + n16] = f16_to_f32(skr) * a.sign;
     scl[kBlock + 16 * srun + n16] = kept_scale(v);
     scl[2 * kBlock + srun] = most_of(v);
     scl[2 * kBlock + 4 + srun] = least_of(v);
@@ -1442,7 +1445,7 @@ int paged_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, const Pag
   const PagedSdpaArgs a{p, (const uint16_t*)q, qst[0], qst[1], c, out, acc + n * D, acc + n * (D + 1), acc,
                         (int)Hq, (int)Hkv, (int)std::min<int64_t>(max_new, p.T), causal, qdt, odt,
                         (int)plan.target, (int)plan.slots, plan.min_part, plan.snake,
-                        scale * 1.44269504088896340736f};
+                        fabsf(scale) * 1.44269504088896340736f, scale < 0.0f ? -1.0f : 1.0f};
   if (D == 64)
     launch_paged<64>(a, plan, st);
   else if (D == 128)
