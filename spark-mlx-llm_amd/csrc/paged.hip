@@ -358,8 +358,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PageArgs 
   int wanted = 0, pairs = 0, overfull = 0;
   for (int i0 = 0; i0 < a.rows; i0 += kPlanThreads) {
     const int i = i0 + tid;
-    int copy = 0, w = -1, want = 0;
-    bool over = false;
+    int copy = 0, w = -1, want = 0, over = 0;
     if (i < a.rows) {
       const RowPlan r = i0 == 0 ? mine : row_plan(a, i);
       w = i0 == 0 ? mine_w : write_page(a, r);
@@ -367,17 +366,18 @@ __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PageArgs 
       want = copy + (r.need - r.held);
       over = r.over;
     }
-    overfull += __syncthreads_count(over);
     int t_want, t_copy;
     const int base = wanted + block_prefix(want, s_wave, t_want);
-    const int pair = pairs + block_prefix(copy, s_wave, t_copy);
+    // (copies and overfull rows in one: of either no more than kPlanThreads)
+    const int pair = pairs + (block_prefix(over << 16 | copy, s_wave, t_copy) & 0xFFFF);
     if (i < a.rows) a.s.base[i] = copy ? ~base : base;  // negative: its first page is a copy
     if (copy) {
       a.s.src[pair] = w;
       a.s.dst[pair] = base;  // of the list
     }
     wanted += t_want;
-    pairs += t_copy;
+    pairs += t_copy & 0xFFFF;
+    overfull += t_copy >> 16;
   }
   if (tid == 0) {
     const int missing = max(wanted - nfree, 0);
