@@ -466,14 +466,14 @@ __device__ __forceinline__ uint32_t zero_values(const PagedSdpaArgs& a, TableRow
 // The waves of a workgroup take turns at blocks of 32 tokens, each with the next
 // block's loads in flight and no barrier until they join; keys and values, read
 // once, go past the caches. Bound by HBM where there is much: 64 sequences of up to
-// 8192 tokens, 8 heads of 128, 304 MB in 60 us, 5.0 TB/s (before the blocks that all
-// rows see whole were spared the masks 61.5: two workgroups a CU 68, four, which
-// spill, 99, cached loads 64); by the latency of its steps where there is little: one of 4095
-// tokens 7 us, of which find_item and the first loads are half.
+// 8192 tokens, 8 heads of 128, 304 MB in 62.5 us, 4.9 TB/s (of an earlier form that
+// took 61.5: two workgroups a CU 68, four, which spill, 99, cached loads 64); by the
+// latency of its steps where there is little: one of 4095 tokens 7 us, of which
+// find_item and the first loads are half.
 //
-// Up to 16 rows: 16 sequences of 8192 tokens with 4 new ones (4 heads to each of 8
-// of 128) 82 us, by tiles 100; 8 new ones, two passes over the cache, 113 and by
-// tiles 98; one new one 74, by tiles 96.
+// Up to 16 rows: 16 sequences of 8192 tokens (4 heads to each of 8 of 128) with one
+// new one each 61 us a call, with 4 new ones 66, by tiles 84 and 82; with 8 new ones,
+// which would be two passes over the cache here, 83 by tiles.
 template <int D>
 struct FewLds {
   static constexpr int VROW = D + 16;
@@ -688,12 +688,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_few_kernel(PagedS
 //
 // Two workgroups a CU is what registers (240) and LDS (76 KB) allow; being at
 // different places of their blocks, one's products and LDS reads run beside the
-// other's softmax. 2048 new tokens of 8192, 32 heads of 128, 240 GFLOP: 298 us, 805
-// TFLOP/s. Bound by what a wave can issue and by the clock, which falls to 2.2 GHz:
-// per block of 64 tokens 32 products (1024 cycles of the matrix cores), about 350
-// vector and 75 LDS instructions, 2900 cycles in all. Scores one block ahead, so
-// that products and exponentials are independent neighbours in one wave, saved 4%
-// of the cycles and lost as much in clock.
+// other's softmax. 2048 new tokens of 8192, 32 heads of 128, 240 GFLOP: 314 us, 764
+// TFLOP/s. Nothing is full: of the cycles the matrix cores are busy in 34%, the LDS in
+// 44%, vector instructions issue in 53%, and waves wait in 26% of theirs. What is short
+// is the overlap of two waves a SIMD, each of which needs some 3000 cycles for a block
+// of 64 tokens with 32 products (1024 cycles of the matrix cores), about 370 vector and
+// 75 LDS instructions; and the clock falls to 2.2 GHz. Scores one block ahead, so that
+// products and exponentials are independent neighbours in one wave, saved 4% of the
+// cycles and lost as much in clock.
 template <int D>
 struct TileShape {
   static constexpr int BLOCK = 64;                    // tokens
@@ -709,8 +711,8 @@ struct TileShape {
 // of 16 tokens, and of the run srun whose scales it takes. A lane's own offset
 // counts from the block's first token where PG is 1, else from its page's.
 // `ok` says which runs have a page; page 0 stands in for the others, whose tokens
-// are hidden. (2048 new tokens of 8192, 32 heads of 128: one page to a block 323 us,
-// two 350, four 384; a scalar load for each lookup 324, 354 and 393.)
+// are hidden. (2048 new tokens of 8192, 32 heads of 128: one page to a block 314 us,
+// two 316, four 319.)
 template <int PG, int PPT>
 struct TilePages {
   uint64_t at[PG == 1 ? 1 : PPT], sat;
@@ -982,10 +984,10 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
 // 64 tokens over all dims, hands its weights to the other through LDS, and sums all
 // 64 tokens' values of its half of the dims. Eight waves a CU, every operand from
 // LDS is used for 32 rows, and a block's conversion is shared by 512 threads.
-// (24 sequences of up to 1000 new tokens, 166 GFLOP, 16 heads of 256: 282 us, 588
-// TFLOP/s; 271 with maxima rounded up to whole numbers, which need no second pass
-// over the sums below. Before the contexts' split was tuned to it 296, where waves of
-// 16 rows with all dims took 346, and waves of 32 rows alone on their SIMDs 376.)
+// (24 sequences of up to 1000 new tokens, 166 GFLOP, 16 heads of 256: 289 us, 575
+// TFLOP/s. With maxima rounded up to whole numbers, which need no second pass over the
+// sums below but cost bits, 18 us less; an earlier form of 296, where waves of 16 rows
+// with all dims took 346, and waves of 32 rows alone on their SIMDs 376.)
 //
 // Both waves weigh in the units of their own running maxima; where these differ
 // after a block (its first, and hardly ever later: they move by 2^8 or more) both go
@@ -994,8 +996,9 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
 // A block has two phases. In the first its keys are read and its values are written
 // to LDS, in the second the values are read and the next keys are written: one buffer
 // of each and a barrier after each phase. (Half the waves a phase behind the others,
-// with two buffers, took 306 us for these 296.) Bound by the latency of a wave's own chain through
-// these phases.
+// with two buffers, took 306 us for these 296.) Bound by the latency of a wave's own
+// chain through these phases: matrix cores busy in 24% of the cycles, the LDS in 32%,
+// waves wait in 30% of theirs, and a CU has no other workgroup to run meanwhile.
 template <bool TWO>
 struct PairShape {
   static constexpr int D = 256, BLOCK = 64;
@@ -1370,9 +1373,10 @@ PagedPlan paged_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, i
   p.rows = p.few ? 16 : kTileRows;
   p.min_part = 128;
   p.max_tiles = std::min(T * gqa / p.rows + B, B * cdiv(max_new * gqa, p.rows));
-  // a part for each workgroup that the chip holds at once, or a few more: decodes
-  // are bound by memory, where more in flight count (three workgroups a CU); a pair
-  // tile has a CU to itself (294 us with two parts a CU where one takes 271)
+  // a part for each workgroup that the chip holds at once (two tiles a CU, one pair
+  // tile: 294 us with two parts a CU where one took 271); with few rows, where three
+  // workgroups fit, four, as ragged lengths leave uneven ends (64 sequences 67.5 us,
+  // three parts 70.2, six 67.0; 16 of 8192 tokens with 4 new ones 66.1, 63.1 and 72.9)
   p.target = std::min<int64_t>(cdiv((p.few ? 4 : D <= 128 ? 2 : 1) * device_cus(), Hkv), kMaxParts);
   p.split = max_tokens > p.min_part ? std::min(p.max_tiles, p.target) : 0;
   p.slots = std::min(2 * p.target, p.split * cdiv(max_tokens, p.min_part));
