@@ -617,11 +617,11 @@ int sparkq_paged_kv_append(const void* k, const void* v, void* k_codes, void* k_
  * that fall to no sequence are left as they were. max_new bounds the new tokens
  * of one sequence: of longer ones the rows past it are left as they were too. A
  * chunk of one token per sequence is the decode step. Scores, normalizer and
- * sums are fp32; a weight times its value's scale
- * is two fp16 operands, 22 bits, in calls of up to 16 rows a (sequence, KV head)
- * (max_new * Hq / Hkv) and wherever out_dtype is F32, else one of 11 bits: the
- * second costs a quarter of the time there. (That is down to 2^-16 of the row's
- * largest such product, of a value that is not all zeros, and below to 2^-27 of it.)
+ * sums are fp32. A weight times its value's scale goes in as two fp16 operands (22
+ * bits) in calls of up to 16 rows a sequence and KV head (max_new * Hq / Hkv) and
+ * wherever out_dtype is F32, else as one of 11 bits: there the second would cost a
+ * quarter of the time. (That holds down to 2^-16 of the row's largest such product,
+ * of a value that is not all zeros; below, to 2^-27 of it.)
  * Workspace: sparkq_paged_sdpa_workspace_bytes (max_tokens = max_pages *
  * page_size), any initial value. */
 size_t sparkq_paged_sdpa_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64_t Hkv,

@@ -147,16 +147,16 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
     (float16 or bfloat16) -> [T,Hq,D]. With mask="causal" row i of a
     sequence's n new tokens sees its tokens 0 .. length - n + i, with None all
     of them; tokens without a page are hidden, a row that sees nothing is zero,
-    and one that sees a value scale that is not finite has no finite values. max_new is the most new tokens that a sequence has (1: a decode
-    step). Rows that fall to no sequence, or to more than max_new of one, are
-    left as they are in `out`, and hold anything in a new tensor. Codes and
-    scales of keys lie as those of values do (the same strides), a page's scales
-    of a head together. A weight times its value's scale
-    is held in 22 bits in calls of up to 16 rows a sequence and KV head (max_new *
-    Hq / Hkv: decode steps, a few drafted tokens) and wherever out_dtype is
-    float32; in others, with 16-bit outputs, in float16's 11, which their own
-    rounding is near (float32 outputs cost up to a quarter more time there). Scores,
-    normalizer and sums are fp32."""
+    and one that sees a value scale that is not finite has no finite values.
+    max_new is the most new tokens that a sequence has (1: a decode step). Rows
+    that fall to no sequence, or to more than max_new of one, are left as they
+    are in `out`, and hold anything in a new tensor. Codes and scales of keys lie
+    as those of values do (the same strides), a page's scales of a head together.
+    A weight times its value's scale is held in 22 bits in calls of up to 16 rows
+    a sequence and KV head (max_new * Hq / Hkv: decode steps, a few drafted
+    tokens) and wherever out_dtype is float32; in others, with 16-bit outputs, in
+    float16's 11, which their own rounding is near (float32 outputs cost up to a
+    quarter more time there). Scores, normalizer and sums are fp32."""
     op = "paged_quantized_sdpa"
     kc, ks, vc, vs, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
     if queries.ndim != 3 or queries.shape[2] != d or not queries.shape[1] \
@@ -354,11 +354,14 @@ class PagedKVCache:
         """Start a step: the batch's rows continue `parents` (itself without)
         and get new_tokens[i] tokens each (a list of Python ints). Returns the
         packed rows' starts. Enqueued without waiting for the device, but not in a
-        graph's capture: its numbers come from the host. `missing` then counts the pages that the pool, or
-        rows of max_pages, were short of (on the device): a caller that may run
-        short reads it before the step's first append, and takes the step back
-        with undo()."""
+        graph's capture: its numbers come from the host. `missing` then counts the
+        pages that the pool, or rows of max_pages, were short of (on the device): a
+        caller that may run short reads it before the step's first append, and
+        takes the step back with undo()."""
         self._ready()
+        dev = self.page_table.device
+        if dev.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a step takes its numbers from the host and cannot be captured")
         new_tokens = [int(n) for n in new_tokens]
         if any(n < 0 for n in new_tokens):
             raise ValueError("new_tokens must not be negative")
@@ -368,15 +371,12 @@ class PagedKVCache:
         ends = [0]
         for n in new_tokens:
             ends.append(ends[-1] + n)
-        dev = self.page_table.device
         parents = None if parents is None else [int(p) for p in parents]
         after = self._after(new_tokens, parents)
         host = new_tokens + ends + (parents or [])
         if dev.type == "cuda":
             # from pinned memory, which torch keeps until the copy is done: a copy from
             # pageable memory would wait for all that the stream has still to do
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("a step takes its numbers from the host and cannot be captured")
             ints = torch.tensor(host, dtype=torch.int32, pin_memory=True).to(dev, non_blocking=True)
         else:
             ints = torch.tensor(host, dtype=torch.int32, device=dev)
@@ -413,9 +413,9 @@ class PagedKVCache:
 
     def append(self, index: int, keys, values):
         self._ready()
-        self._last = None  # what is appended cannot be taken back
         paged_kv_append(keys, values, self.layer(index), self.page_table, self.starts,
                         self.lengths)
+        self._last = None  # what is appended cannot be taken back
 
     def attend(self, index: int, queries, *, scale, mask="causal", out_dtype=None, out=None):
         self._ready()

@@ -33,7 +33,7 @@ Registered ops:
 and, writing the cache's four tensors in place:
   paged_kv_append(keys, values, k_codes, k_scales, v_codes, v_scales, page_table, starts, lengths)
   kv_pages_fork(k_codes, k_scales, v_codes, v_scales, page_table, lengths, parents, new_tokens)
-      -> (page_table, lengths, missing)
+      -> (page_table, lengths, missing); rows must have room for their new tokens
   kv_pages_compact(k_codes, k_scales, v_codes, v_scales, page_table, lengths)
       -> (page_table, used)
 """

@@ -162,3 +162,20 @@ def test_undo_takes_back_only_what_it_can(make):
     cache.append(0, torch.ones((80, 1, 64)), torch.ones((80, 1, 64)))
     with pytest.raises(ValueError, match="no step"):
         cache.undo()
+
+
+def test_undo_after_a_refused_append(make, monkeypatch):
+    cache = make(3, 2, 2)
+    cache.step([16, 16])
+    table = cache.page_table.clone()
+    cache.step([16, 16])
+    assert cache.missing.item() == 1
+
+    def refuse(*args):
+        raise ValueError("like the cache")
+
+    monkeypatch.setattr(paged, "paged_kv_append", refuse)
+    with pytest.raises(ValueError, match="like the cache"):
+        cache.append(0, torch.ones((32, 2, 64)), torch.ones((32, 2, 64)))
+    cache.undo()
+    assert torch.equal(cache.page_table, table) and cache.lengths.tolist() == [16, 16]
