@@ -680,6 +680,129 @@ int sparkq_kv_pages_compact(void* k_codes, void* v_codes, void* k_scales, void* 
                             int64_t scale_bytes, void* workspace, size_t workspace_bytes,
                             void* stream);
 
+/* sparkq_paged_sdpa that also returns lse [T,Hq] float32: the natural logarithm of
+ * the sum of each row's exp(scale * q . k) over the tokens that it sees, -inf where
+ * that is none. Rows of lse are written where rows of out are. */
+int sparkq_paged_sdpa_lse(const void* q, const void* k_codes, const void* k_scales,
+                          const void* v_codes, const void* v_scales,
+                          const int32_t* page_table, const int32_t* starts,
+                          const int32_t* lengths, void* out, float* lse, int64_t T, int64_t B,
+                          int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t max_pages,
+                          int64_t table_stride, int page_size, int64_t max_new, int causal,
+                          int q_dtype, int out_dtype, float scale, const int64_t* q_strides,
+                          const int64_t* strides, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/* ------------------------------------------------------------------------
+ * Long contexts over the paged cache (no counterpart in the reference): which
+ * pages a query attends, and which tokens a cache keeps. Conventions are those
+ * of the calls above; strides[0..5] are the keys' alone where a call reads no
+ * values.
+ * ---------------------------------------------------------------------- */
+
+/* Bounds of each page's keys: bounds bf16 [pages,Hkv,2,D], the least key of a
+ * channel rounded down, then the largest rounded up, with bounds_strides[0..1] =
+ * page, head in elements (multiples of 8, 16-byte aligned, [2][D] contiguous).
+ * Written for the pages that hold the batch's new tokens (the last starts[b+1] -
+ * starts[b] of sequence b, of at most max_new), from all tokens of the page that
+ * the sequence has. A page with a key scale that is not finite is bounded by
+ * bf16's largest numbers. Sequences with new tokens must not share the pages
+ * that these lie in. */
+int sparkq_paged_key_bounds(const void* k_codes, const void* k_scales, void* bounds,
+                            const int32_t* page_table, const int32_t* starts,
+                            const int32_t* lengths, int64_t B, int64_t Hkv, int64_t D,
+                            int64_t pages, int64_t max_pages, int64_t table_stride,
+                            int page_size, int64_t max_new, const int64_t* strides,
+                            const int64_t* bounds_strides, void* stream);
+
+/* Scores of a row's pages: scores[t,h,j] = max over the query heads g of KV head h
+ * of scale * sum_d max(q[t,g,d] lo[d], q[t,g,d] hi[d]) (min where scale < 0), no less
+ * than any of their logits with a key of page j of t's sequence; -inf where t sees
+ * nothing of the page (causal as in sparkq_paged_sdpa) or there is none. A head
+ * whose sum is NaN does not count. scores float32 [T,Hkv,max_pages] contiguous and
+ * 16-byte aligned, seen int32 [T]: how many of its pages t sees. Rows that fall to
+ * no sequence, or past max_new of one, are left as they were. Products of 16-bit
+ * values are exact, sums fp32. */
+int sparkq_paged_page_scores(const void* q, const void* bounds, const int32_t* page_table,
+                             const int32_t* starts, const int32_t* lengths, float* scores,
+                             int32_t* seen, int64_t T, int64_t B, int64_t Hq, int64_t Hkv,
+                             int64_t D, int64_t pages, int64_t max_pages,
+                             int64_t table_stride, int page_size, int64_t max_new, int causal,
+                             int q_dtype, float scale, const int64_t* q_strides,
+                             const int64_t* bounds_strides, void* stream);
+
+/* Places of the largest values of each row of x float32 [layers,rows,heads,n]
+ * (strides[0..2] in elements, n contiguous): out int32 [layers,rows,heads,count],
+ * in ascending order, -1 behind them where a row has fewer values. Of row r only
+ * the first lengths[r] values count (all n where lengths is NULL; clamped to
+ * [0,n]). Its first `first` and last `last` places are taken whatever their values
+ * are (first + last <= count). Equal values: the lowest place. NaN counts as
+ * -inf. n and count below 2^30, layers * rows * heads below 2^22. */
+int sparkq_select_top(const float* x, const int32_t* lengths, int32_t* out, int64_t layers,
+                      int64_t rows, int64_t heads, int64_t n, int64_t count, int64_t first,
+                      int64_t last, const int64_t* strides, void* stream);
+
+/* Attention of each new token over selected pages: sparkq_paged_sdpa where row t
+ * sees, of the tokens that it would see there, those of the pages selected[t,h,:]
+ * for KV head h: int32 [T,Hkv,count] places in its sequence's table row (what
+ * sparkq_select_top returns), selected_strides[0..1] = token, head in elements, the
+ * last axis contiguous. Entries outside the table row, or of pages that are absent
+ * or that t does not see, count for nothing; a page that is named twice counts
+ * twice. Weights times value scales are held in 22 bits. Workspace:
+ * sparkq_paged_sparse_workspace_bytes, any initial value. */
+size_t sparkq_paged_sparse_workspace_bytes(int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                           int64_t count, int page_size);
+int sparkq_paged_sparse_sdpa(const void* q, const void* k_codes, const void* k_scales,
+                             const void* v_codes, const void* v_scales,
+                             const int32_t* selected, const int32_t* page_table,
+                             const int32_t* starts, const int32_t* lengths, void* out,
+                             int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                             int64_t count, int64_t pages, int64_t max_pages,
+                             int64_t table_stride, int page_size, int64_t max_new, int causal,
+                             int q_dtype, int out_dtype, float scale,
+                             const int64_t* q_strides, const int64_t* selected_strides,
+                             const int64_t* strides, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
+/* Attention weight that the cached tokens gather: mass[b,h,n] += the sum of exp(scale
+ * * q[t,g] . k[n] - lse[t,g]) over sequence b's new tokens t (the first max_new of
+ * them) that see token n and the query heads g of KV head h, lse [T,Hq] as
+ * sparkq_paged_sdpa_lse returns it (a row of -inf adds nothing). The sequence's
+ * new tokens, its last starts[b+1] - starts[b], start from 0 instead of what mass
+ * holds. mass float32 [B,Hkv,max_pages * page_size], mass_strides[0..1] = sequence,
+ * head in elements (even, mass 16-byte aligned), the last axis contiguous; places
+ * from lengths[b] on and sequences without new tokens are left as they were. Sums
+ * are fp32, always in the same order. */
+int sparkq_paged_kv_mass(const void* q, const float* lse, const void* k_codes,
+                         const void* k_scales, float* mass, const int32_t* page_table,
+                         const int32_t* starts, const int32_t* lengths, int64_t T, int64_t B,
+                         int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t max_pages,
+                         int64_t table_stride, int page_size, int64_t max_new, int causal,
+                         int q_dtype, float scale, const int64_t* q_strides,
+                         const int64_t* mass_strides, const int64_t* strides, void* stream);
+
+/* Some tokens of each sequence alone: sequences of more than `count` tokens keep
+ * `count`, in every layer and KV head those that keep int32 [layers,B,Hkv,count]
+ * (contiguous) lists in ascending order (sparkq_select_top's). They move to the front
+ * of the sequence's pages in their order, and their mass with them (float32
+ * [layers,B,Hkv,max_pages * page_size] with mass_strides[0..2] = layer, sequence,
+ * head in elements, or NULL). An entry i below i, or not below the length, stands
+ * for i. Shorter sequences stay as they are. Pages that are written and that
+ * another sequence (or entry) holds too are replaced by free ones, in ascending
+ * order to the sequences in order; the rest are written in place. out_missing[0] =
+ * pages short: when it is not 0 nothing was moved, and out_table and out_lengths are
+ * the old ones. A kept token without a page comes as zeros. Pools, buf_strides and
+ * workspace (sparkq_kv_pages_workspace_bytes(B, pages)) as in sparkq_kv_pages_fork,
+ * with a page's codes [Hkv,page_size,D] and scales [Hkv,page_size] contiguous. */
+int sparkq_kv_pages_evict(void* k_codes, void* v_codes, void* k_scales, void* v_scales,
+                          const int32_t* keep, float* mass, const int32_t* page_table,
+                          const int32_t* lengths, int64_t table_stride, int32_t* out_table,
+                          int32_t* out_lengths, int32_t* out_missing,
+                          const int64_t* buf_strides, const int64_t* mass_strides, int64_t B,
+                          int64_t Hkv, int64_t D, int64_t count, int64_t max_pages,
+                          int64_t pages, int64_t layers, int page_size, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,7 @@ BUILD = os.path.join(HERE, "_build")
 SOURCES = ["w4a16.hip", "w4q.hip", "w4mr.hip", "w8a8.hip", "w8a16.hip", "w8aff.hip", "affgemm.hip", "sdpa.hip", "sdpa_affine.hip", "sdpa_gen.hip",
            "sdpa_stage.hip",
            "layer.hip", "qknorm.hip", "paged.hip", "paged_sdpa.hip",
+           "paged_pages.hip", "select.hip", "paged_sparse.hip", "paged_mass.hip",
            "abi.cpp"]
 ARCH = "gfx950"
 

@@ -62,8 +62,28 @@ int paged_kv_append(const PagedBatch& p, const void* k, const void* v, const int
 size_t paged_sdpa_workspace(int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                             int64_t max_new, int64_t max_tokens);
 int paged_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, const PagedSide& ks,
-               const PagedSide& vs, void* out, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
+               const PagedSide& vs, void* out, float* lse, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new,
                int causal, int qdt, int odt, float scale, void* ws, size_t wsb, hipStream_t st);
+// launchers (paged_pages.hip, select.hip, paged_sparse.hip, paged_mass.hip)
+int paged_key_bounds(const PagedBatch& p, const PagedSide& ks, void* bounds, const int64_t* bst, int64_t H, int64_t D,
+                     int64_t max_new, hipStream_t st);
+int paged_page_scores(const PagedBatch& p, const void* q, const int64_t* qst, const void* bounds, const int64_t* bst,
+                      float* scores, int32_t* seen, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int causal,
+                      int qdt, float scale, hipStream_t st);
+int select_top(const float* x, const int32_t* lengths, int32_t* out, int64_t layers, int64_t rows, int64_t heads,
+               int64_t n, int64_t count, int64_t first, int64_t last, const int64_t* st, hipStream_t stream);
+size_t paged_sparse_workspace(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t count, int64_t page);
+int paged_sparse_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, const PagedSide& ks, const PagedSide& vs,
+                      const int32_t* list, const int64_t* lst, int64_t count, void* out, int64_t Hq, int64_t Hkv,
+                      int64_t D, int64_t max_new, int causal, int qdt, int odt, float scale, void* ws, size_t wsb,
+                      hipStream_t st);
+int paged_kv_mass(const PagedBatch& p, const void* q, const int64_t* qst, const float* lse, const PagedSide& ks,
+                  float* mass, const int64_t* mst, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int causal,
+                  int qdt, float scale, hipStream_t st);
+int kv_pages_evict(const int32_t* table, int64_t table_stride, const int32_t* lengths, const int32_t* keep,
+                   int64_t count, float* mass, const int64_t* mst, int32_t* out_table, int32_t* out_lengths,
+                   int32_t* missing, int64_t B, int64_t width, int64_t pages, int page_size, int64_t layers, int64_t H,
+                   int64_t D, void* const* bufs, const int64_t* strides, void* ws, hipStream_t st);
 size_t kv_pages_workspace(int64_t rows, int64_t pages);
 int kv_pages_fork(const int32_t* table, int64_t table_stride, const int32_t* lengths,
                   const int32_t* parents, const int32_t* fresh, int32_t* out_table,
@@ -970,6 +990,60 @@ size_t sparkq_paged_sdpa_workspace_bytes(int64_t T, int64_t B, int64_t Hq, int64
   return paged_sdpa_workspace(T, B, Hq, Hkv, D, max_new, max_tokens);
 }
 
+// The checks that every attention over a paged cache shares.
+static int paged_attn_check(const char* op, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages,
+                            int64_t max_pages, int64_t table_stride, int page_size, int64_t max_new, const void* q,
+                            const void* out, const int32_t* page_table, const int32_t* starts, const int32_t* lengths,
+                            const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                            const int64_t* q_strides, const int64_t* strides, int q_dtype, int out_dtype, float scale) {
+  if (int rc = paged_check(op, T, B, Hkv, D, pages, max_pages, table_stride, page_size, k_codes, k_scales, v_codes,
+                           v_scales, strides))
+    return rc;
+  REQUIRE(Hq > 0 && Hq % Hkv == 0, "%s: query heads must be divisible by KV heads", op);
+  REQUIRE(max_new > 0 && max_new <= kI32Max, "%s: max_new must be positive", op);
+  REQUIRE(Hq <= 65535 && T <= kI32Max / Hq && B <= kI32Max / (4 * Hkv), "%s: shape too large", op);
+  REQUIRE_SUPPORTED(strides[3] % 8 == 0 && strides[4] % 8 == 0 && strides[5] == 1,
+                    "%s: scales must be contiguous over a page's tokens, pages and heads "
+                    "multiples of 8 scales apart", op);
+  REQUIRE_SUPPORTED(aligned(k_scales, 16) && aligned(v_scales, 16),
+                    "%s: scales must be 16-byte aligned", op);
+  for (int i = 0; i < 6; ++i)
+    REQUIRE_SUPPORTED(strides[i] == strides[6 + i], "%s: keys and values must have the same strides", op);
+  REQUIRE_SUPPORTED(strides[0] / 16 <= kI32Max && strides[3] / 8 <= kI32Max &&
+                        strides[2] <= kI32Max / page_size,
+                    "%s: pages must be less than 32 GiB apart and a head's tokens span less "
+                    "than 2 GiB", op);
+  REQUIRE((T == 0 || (q && out)) && q_strides && starts && (B == 0 || (page_table && lengths)),
+          "%s: null tensor pointer", op);
+  REQUIRE(is_half_dtype(q_dtype), "%s requires float16 or bfloat16 queries", op);
+  REQUIRE(out_dtype == q_dtype || out_dtype == SPARKQ_F32,
+          "%s: out dtype must be the query dtype or float32", op);
+  REQUIRE(std::isfinite(scale), "%s: scale must be finite", op);
+  REQUIRE(q_strides[0] >= 0 && q_strides[1] >= 0 && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0 &&
+              aligned(q, 16) && aligned(out, 16),
+          "%s: query rows must be 16-byte aligned", op);
+  return SPARKQ_OK;
+}
+
+static int paged_sdpa_call(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                           const void* v_scales, const int32_t* page_table, const int32_t* starts,
+                           const int32_t* lengths, void* out, float* lse, int64_t T, int64_t B, int64_t Hq,
+                           int64_t Hkv, int64_t D, int64_t pages, int64_t max_pages, int64_t table_stride,
+                           int page_size, int64_t max_new, int causal, int q_dtype, int out_dtype, float scale,
+                           const int64_t* q_strides, const int64_t* strides, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  if (int rc = paged_attn_check("paged_sdpa", T, B, Hq, Hkv, D, pages, max_pages, table_stride, page_size, max_new, q,
+                                out, page_table, starts, lengths, k_codes, k_scales, v_codes, v_scales, q_strides,
+                                strides, q_dtype, out_dtype, scale))
+    return rc;
+  DEVICE_OK();
+  return paged_sdpa(paged_batch(page_table, starts, lengths, T, B, pages, max_pages, table_stride,
+                                page_size),
+                    q, q_strides, paged_side(k_codes, k_scales, strides),
+                    paged_side(v_codes, v_scales, strides + 6), out, lse, Hq, Hkv, D, max_new, causal != 0,
+                    q_dtype, out_dtype, scale, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
 int sparkq_paged_sdpa(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
                       const void* v_scales, const int32_t* page_table, const int32_t* starts,
                       const int32_t* lengths, void* out, int64_t T, int64_t B, int64_t Hq,
@@ -977,38 +1051,154 @@ int sparkq_paged_sdpa(const void* q, const void* k_codes, const void* k_scales, 
                       int64_t table_stride, int page_size, int64_t max_new, int causal, int q_dtype,
                       int out_dtype, float scale, const int64_t* q_strides, const int64_t* strides,
                       void* workspace, size_t workspace_bytes, void* stream) {
-  if (int rc = paged_check("paged_sdpa", T, B, Hkv, D, pages, max_pages, table_stride, page_size,
-                           k_codes, k_scales, v_codes, v_scales, strides))
+  return paged_sdpa_call(q, k_codes, k_scales, v_codes, v_scales, page_table, starts, lengths, out, nullptr, T, B, Hq,
+                         Hkv, D, pages, max_pages, table_stride, page_size, max_new, causal, q_dtype, out_dtype, scale,
+                         q_strides, strides, workspace, workspace_bytes, stream);
+}
+
+int sparkq_paged_sdpa_lse(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                          const void* v_scales, const int32_t* page_table, const int32_t* starts,
+                          const int32_t* lengths, void* out, float* lse, int64_t T, int64_t B, int64_t Hq,
+                          int64_t Hkv, int64_t D, int64_t pages, int64_t max_pages, int64_t table_stride,
+                          int page_size, int64_t max_new, int causal, int q_dtype, int out_dtype, float scale,
+                          const int64_t* q_strides, const int64_t* strides, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  REQUIRE((T == 0 || lse) && aligned(lse, 4), "paged_sdpa: null tensor pointer");
+  return paged_sdpa_call(q, k_codes, k_scales, v_codes, v_scales, page_table, starts, lengths, out, lse, T, B, Hq, Hkv,
+                         D, pages, max_pages, table_stride, page_size, max_new, causal, q_dtype, out_dtype, scale,
+                         q_strides, strides, workspace, workspace_bytes, stream);
+}
+
+// Keys alone are checked as both sides of a cache.
+static int paged_keys_check(const char* op, int64_t T, int64_t B, int64_t Hkv, int64_t D, int64_t pages,
+                            int64_t max_pages, int64_t table_stride, int page_size, const void* kc, const void* ks,
+                            const int64_t* st) {
+  REQUIRE(st, "%s: null tensor pointer", op);
+  int64_t both[12];
+  for (int i = 0; i < 12; ++i) both[i] = st[i % 6];
+  return paged_check(op, T, B, Hkv, D, pages, max_pages, table_stride, page_size, kc, ks, kc, ks, both);
+}
+
+static int bounds_check(const char* op, const void* bounds, const int64_t* st, int64_t D, int64_t Hkv) {
+  REQUIRE(bounds && st, "%s: null tensor pointer", op);
+  REQUIRE(st[0] >= 0 && st[1] >= 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && aligned(bounds, 16),
+          "%s: bounds must be 16-byte aligned", op);
+  REQUIRE(st[1] >= 2 * D || Hkv == 1, "%s: bounds overlap", op);
+  return SPARKQ_OK;
+}
+
+int sparkq_paged_key_bounds(const void* k_codes, const void* k_scales, void* bounds, const int32_t* page_table,
+                            const int32_t* starts, const int32_t* lengths, int64_t B, int64_t Hkv, int64_t D,
+                            int64_t pages, int64_t max_pages, int64_t table_stride, int page_size, int64_t max_new,
+                            const int64_t* strides, const int64_t* bounds_strides, void* stream) {
+  if (int rc = paged_keys_check("paged_key_bounds", 0, B, Hkv, D, pages, max_pages, table_stride, page_size, k_codes,
+                                k_scales, strides))
     return rc;
-  REQUIRE(Hq > 0 && Hq % Hkv == 0, "paged_sdpa: query heads must be divisible by KV heads");
-  REQUIRE(max_new > 0 && max_new <= kI32Max, "paged_sdpa: max_new must be positive");
-  REQUIRE(Hq <= 65535 && T <= kI32Max / Hq && B <= kI32Max / (4 * Hkv), "paged_sdpa: shape too large");
-  REQUIRE_SUPPORTED(strides[3] % 8 == 0 && strides[4] % 8 == 0 && strides[5] == 1,
-                    "paged_sdpa: scales must be contiguous over a page's tokens, pages and heads "
-                    "multiples of 8 scales apart");
-  REQUIRE_SUPPORTED(aligned(k_scales, 16) && aligned(v_scales, 16),
-                    "paged_sdpa: scales must be 16-byte aligned");
-  for (int i = 0; i < 6; ++i)
-    REQUIRE_SUPPORTED(strides[i] == strides[6 + i], "paged_sdpa: keys and values must have the same strides");
-  REQUIRE_SUPPORTED(strides[0] / 16 <= kI32Max && strides[3] / 8 <= kI32Max &&
-                        strides[2] <= kI32Max / page_size,
-                    "paged_sdpa: pages must be less than 32 GiB apart and a head's tokens span less "
-                    "than 2 GiB");
-  REQUIRE((T == 0 || (q && out)) && q_strides && starts && (B == 0 || (page_table && lengths)),
-          "paged_sdpa: null tensor pointer");
-  REQUIRE(is_half_dtype(q_dtype), "paged_sdpa requires float16 or bfloat16 queries");
-  REQUIRE(out_dtype == q_dtype || out_dtype == SPARKQ_F32,
-          "paged_sdpa: out dtype must be the query dtype or float32");
-  REQUIRE(std::isfinite(scale), "paged_sdpa: scale must be finite");
-  REQUIRE(q_strides[0] >= 0 && q_strides[1] >= 0 && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0 &&
-              aligned(q, 16) && aligned(out, 16),
-          "paged_sdpa: query rows must be 16-byte aligned");
+  if (int rc = bounds_check("paged_key_bounds", bounds, bounds_strides, D, Hkv)) return rc;
+  REQUIRE(starts && (B == 0 || (page_table && lengths)), "paged_key_bounds: null tensor pointer");
+  REQUIRE(max_new > 0 && max_new <= kI32Max, "paged_key_bounds: max_new must be positive");
   DEVICE_OK();
-  return paged_sdpa(paged_batch(page_table, starts, lengths, T, B, pages, max_pages, table_stride,
-                                page_size),
-                    q, q_strides, paged_side(k_codes, k_scales, strides),
-                    paged_side(v_codes, v_scales, strides + 6), out, Hq, Hkv, D, max_new, causal != 0,
-                    q_dtype, out_dtype, scale, workspace, workspace_bytes, (hipStream_t)stream);
+  return paged_key_bounds(paged_batch(page_table, starts, lengths, kI32Max, B, pages, max_pages, table_stride, page_size),
+                          paged_side(k_codes, k_scales, strides), bounds, bounds_strides, Hkv, D, max_new,
+                          (hipStream_t)stream);
+}
+
+int sparkq_paged_page_scores(const void* q, const void* bounds, const int32_t* page_table, const int32_t* starts,
+                             const int32_t* lengths, float* scores, int32_t* seen, int64_t T, int64_t B, int64_t Hq,
+                             int64_t Hkv, int64_t D, int64_t pages, int64_t max_pages, int64_t table_stride,
+                             int page_size, int64_t max_new, int causal, int q_dtype, float scale,
+                             const int64_t* q_strides, const int64_t* bounds_strides, void* stream) {
+  static const int64_t none[6] = {0, 0, 0, 0, 0, 0};
+  if (int rc = paged_keys_check("paged_page_scores", T, B, Hkv, D, pages, max_pages, table_stride, page_size, bounds,
+                                bounds, none))
+    return rc;
+  if (int rc = bounds_check("paged_page_scores", bounds, bounds_strides, D, Hkv)) return rc;
+  REQUIRE(Hq > 0 && Hq % Hkv == 0, "paged_page_scores: query heads must be divisible by KV heads");
+  REQUIRE(max_new > 0 && max_new <= kI32Max, "paged_page_scores: max_new must be positive");
+  REQUIRE(Hq <= 65535 && T <= kI32Max / Hq, "paged_page_scores: shape too large");
+  REQUIRE((T == 0 || (q && scores && seen)) && q_strides && starts && (B == 0 || (page_table && lengths)),
+          "paged_page_scores: null tensor pointer");
+  REQUIRE(is_half_dtype(q_dtype), "paged_page_scores requires float16 or bfloat16 queries");
+  REQUIRE(std::isfinite(scale), "paged_page_scores: scale must be finite");
+  REQUIRE(q_strides[0] >= 0 && q_strides[1] >= 0 && q_strides[0] % 8 == 0 && q_strides[1] % 8 == 0 &&
+              aligned(q, 16) && aligned(scores, 16) && aligned(seen, 4),
+          "paged_page_scores: query rows and scores must be 16-byte aligned");
+  DEVICE_OK();
+  return paged_page_scores(paged_batch(page_table, starts, lengths, T, B, pages, max_pages, table_stride, page_size), q,
+                           q_strides, bounds, bounds_strides, scores, seen, Hq, Hkv, D, max_new, causal != 0, q_dtype,
+                           scale, (hipStream_t)stream);
+}
+
+int sparkq_select_top(const float* x, const int32_t* lengths, int32_t* out, int64_t layers, int64_t rows,
+                      int64_t heads, int64_t n, int64_t count, int64_t first, int64_t last, const int64_t* strides,
+                      void* stream) {
+  REQUIRE(layers >= 0 && rows >= 0 && heads > 0 && n > 0 && count > 0, "select_top: bad shape");
+  REQUIRE(layers <= kI32Max && rows <= kI32Max && heads <= kI32Max && n <= kI32Max / 2 && count <= kI32Max / 2,
+          "select_top: shape too large");
+  // (a workgroup of 1024 threads a row, fewer than 2^32 threads)
+  REQUIRE(layers == 0 || rows == 0 || layers * rows <= 0x3FFFFF / heads, "select_top: shape too large");
+  REQUIRE(first >= 0 && last >= 0 && first <= count && last <= count - first,
+          "select_top: first and last must not be negative and together no more than count");
+  REQUIRE(strides && (layers * rows == 0 || (x && out)), "select_top: null tensor pointer");
+  REQUIRE(strides[0] >= 0 && strides[1] >= 0 && strides[2] >= 0, "select_top: negative stride");
+  REQUIRE(aligned(x, 4) && aligned(out, 4) && aligned(lengths, 4), "select_top: tensors must be 4-byte aligned");
+  DEVICE_OK();
+  return select_top(x, lengths, out, layers, rows, heads, n, count, first, last, strides, (hipStream_t)stream);
+}
+
+size_t sparkq_paged_sparse_workspace_bytes(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t count,
+                                           int page_size) {
+  if (T <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D <= 0 || count <= 0 || page_size <= 0) return 0;
+  return paged_sparse_workspace(T, Hq, Hkv, D, count, page_size);
+}
+
+int sparkq_paged_sparse_sdpa(const void* q, const void* k_codes, const void* k_scales, const void* v_codes,
+                             const void* v_scales, const int32_t* selected, const int32_t* page_table,
+                             const int32_t* starts, const int32_t* lengths, void* out, int64_t T, int64_t B,
+                             int64_t Hq, int64_t Hkv, int64_t D, int64_t count, int64_t pages, int64_t max_pages,
+                             int64_t table_stride, int page_size, int64_t max_new, int causal, int q_dtype,
+                             int out_dtype, float scale, const int64_t* q_strides, const int64_t* selected_strides,
+                             const int64_t* strides, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = paged_attn_check("paged_sparse_sdpa", T, B, Hq, Hkv, D, pages, max_pages, table_stride, page_size,
+                                max_new, q, out, page_table, starts, lengths, k_codes, k_scales, v_codes, v_scales,
+                                q_strides, strides, q_dtype, out_dtype, scale))
+    return rc;
+  REQUIRE(count > 0 && count <= kI32Max / page_size, "paged_sparse_sdpa: bad count of selected pages");
+  REQUIRE((T == 0 || selected) && selected_strides, "paged_sparse_sdpa: null tensor pointer");
+  REQUIRE(selected_strides[0] >= 0 && selected_strides[1] >= 0 && aligned(selected, 4),
+          "paged_sparse_sdpa: negative stride");
+  DEVICE_OK();
+  return paged_sparse_sdpa(paged_batch(page_table, starts, lengths, T, B, pages, max_pages, table_stride, page_size), q,
+                           q_strides, paged_side(k_codes, k_scales, strides), paged_side(v_codes, v_scales, strides + 6),
+                           selected, selected_strides, count, out, Hq, Hkv, D, max_new, causal != 0, q_dtype, out_dtype,
+                           scale, workspace, workspace_bytes, (hipStream_t)stream);
+}
+
+int sparkq_paged_kv_mass(const void* q, const float* lse, const void* k_codes, const void* k_scales, float* mass,
+                         const int32_t* page_table, const int32_t* starts, const int32_t* lengths, int64_t T,
+                         int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pages, int64_t max_pages,
+                         int64_t table_stride, int page_size, int64_t max_new, int causal, int q_dtype, float scale,
+                         const int64_t* q_strides, const int64_t* mass_strides, const int64_t* strides,
+                         void* stream) {
+  REQUIRE(strides, "paged_kv_mass: null tensor pointer");
+  int64_t both[12];
+  for (int i = 0; i < 12; ++i) both[i] = strides[i % 6];
+  // (mass in the outputs' place: aligned like them)
+  if (int rc = paged_attn_check("paged_kv_mass", T, B, Hq, Hkv, D, pages, max_pages, table_stride, page_size, max_new, q,
+                                mass, page_table, starts, lengths, k_codes, k_scales, k_codes, k_scales, q_strides, both,
+                                q_dtype, q_dtype, scale))
+    return rc;
+  REQUIRE((T == 0 || lse) && mass_strides && aligned(lse, 4), "paged_kv_mass: null tensor pointer");
+  const int64_t tokens = max_pages * page_size;
+  REQUIRE(mass_strides[0] % 2 == 0 && mass_strides[1] % 2 == 0 && mass_strides[0] >= 0 && mass_strides[1] >= 0,
+          "paged_kv_mass: rows of mass must be 8-byte aligned");
+  REQUIRE((mass_strides[1] >= tokens || Hkv == 1) && (mass_strides[0] >= tokens || B <= 1),
+          "paged_kv_mass: rows of mass overlap");
+  REQUIRE(T <= kI32Max / 2 / Hq, "paged_kv_mass: shape too large");
+  DEVICE_OK();
+  return paged_kv_mass(paged_batch(page_table, starts, lengths, T, B, pages, max_pages, table_stride, page_size), q,
+                       q_strides, lse, paged_side(k_codes, k_scales, strides), mass, mass_strides, Hq, Hkv, D, max_new,
+                       causal != 0, q_dtype, scale, (hipStream_t)stream);
 }
 
 size_t sparkq_kv_pages_workspace_bytes(int64_t rows, int64_t pages) {
@@ -1083,6 +1273,37 @@ int sparkq_kv_pages_compact(void* k_codes, void* v_codes, void* k_scales, void* 
   return kv_pages_compact(page_table, table_stride, lengths, out_table, out_used, B, max_pages, pages,
                           page_size, layers, bufs, buf_strides, code_bytes, scale_bytes, workspace,
                           (hipStream_t)stream);
+}
+
+int sparkq_kv_pages_evict(void* k_codes, void* v_codes, void* k_scales, void* v_scales, const int32_t* keep,
+                          float* mass, const int32_t* page_table, const int32_t* lengths, int64_t table_stride,
+                          int32_t* out_table, int32_t* out_lengths, int32_t* out_missing, const int64_t* buf_strides,
+                          const int64_t* mass_strides, int64_t B, int64_t Hkv, int64_t D, int64_t count,
+                          int64_t max_pages, int64_t pages, int64_t layers, int page_size, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  void* const bufs[4] = {k_codes, v_codes, k_scales, v_scales};
+  REQUIRE((B == 0 || (page_table && lengths && out_table && out_lengths && keep)) && out_missing,
+          "kv_pages_evict: null tensor pointer");
+  REQUIRE(Hkv > 0 && Hkv <= 65535 && count > 0 && count <= kI32Max / 2, "kv_pages_evict: bad shape");
+  REQUIRE_SUPPORTED(D == 64 || D == 128 || D == 256, "kv_pages_evict: head dim must be 64, 128 or 256 (got %lld)",
+                    (long long)D);
+  REQUIRE(page_size >= 16 && page_size <= 1024, "kv_pages_evict: page_size must be a power of two from 16 to 1024 (got %d)",
+          page_size);
+  if (int rc = kv_pages_check("kv_pages_evict", bufs, buf_strides, B, B, max_pages, pages, layers, table_stride,
+                              page_size, Hkv * page_size * D, 2 * Hkv * page_size, workspace, workspace_bytes))
+    return rc;
+  REQUIRE(B == 0 || layers <= kI32Max / 2 / (B * Hkv), "kv_pages_evict: shape too large");
+  if (mass) {
+    const int64_t tokens = max_pages * page_size;
+    REQUIRE(mass_strides && aligned(mass, 4), "kv_pages_evict: null tensor pointer");
+    REQUIRE((mass_strides[2] >= tokens || Hkv == 1) && (mass_strides[1] >= tokens || B <= 1) &&
+                (mass_strides[0] >= tokens || layers == 1),
+            "kv_pages_evict: rows of mass overlap");
+  }
+  DEVICE_OK();
+  return kv_pages_evict(page_table, table_stride, lengths, keep, count, mass, mass_strides, out_table, out_lengths,
+                        out_missing, B, max_pages, pages, page_size, layers, Hkv, D, bufs, buf_strides, workspace,
+                        (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -30,6 +30,8 @@ struct PagedSide {
   int64_t s_page, s_head, s_tok;
 };
 
+constexpr int64_t kMaxGrid = 0x7FFFFFFF / 256;  // workgroups of 256 threads: fewer than 2^31 threads
+
 struct SeqRows {
   int first, count;  // packed rows [first, first + count)
   int length;        // tokens in the cache, the new ones included
@@ -48,6 +50,35 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedBatch& p, int b) {
 __device__ __forceinline__ int page_of(const PagedBatch& p, int b, int pos) {
   const int id = p.table[b * p.table_stride + (pos >> p.page_log2)];
   return (unsigned)id < (unsigned)p.pages ? id : -1;
+}
+
+// the sequence whose rows hold packed row t, or -1
+__device__ __forceinline__ int seq_of_row(const PagedBatch& p, int t) {
+  int lo = 0, hi = p.B;  // the first b with starts[b + 1] > t
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (p.starts[mid + 1] > t)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo < p.B ? lo : -1;
+}
+
+// the same in one round trip for every 64 sequences: all lanes of a wave ask for the
+// same row
+__device__ __forceinline__ int wave_seq_of_row(const PagedBatch& p, int t) {
+  const int lane = threadIdx.x & 63;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const unsigned long long past = __ballot(b0 + lane < p.B && p.starts[min(b0 + lane, p.B - 1) + 1] > t);
+    if (past) return b0 + __builtin_ctzll(past);
+  }
+  return -1;
+}
+
+// last token that row i of a sequence's new tokens sees (-1: none)
+__device__ __forceinline__ int last_seen_by(const SeqRows& s, int i, int causal) {
+  return causal ? min(max(s.length - s.count + i, -1), s.length - 1) : s.length - 1;
 }
 
 }  // namespace sparkq

@@ -25,19 +25,6 @@ struct PagedAppendArgs {
   int H, D, x_dtype;
 };
 
-// the sequence whose rows hold packed row t, or -1
-__device__ __forceinline__ int seq_of_row(const PagedBatch& p, int t) {
-  int lo = 0, hi = p.B;  // the first b with starts[b + 1] > t
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (p.starts[mid + 1] > t)
-      hi = mid;
-    else
-      lo = mid + 1;
-  }
-  return lo < p.B ? lo : -1;
-}
-
 // v / s for rounding to a whole number, with inv = 1 / s to a unit of fp32 or so:
 // the quotient's error (2^-22) after one correction is far below what matters.
 // A quotient of a 16-bit v (11 bits) and an fp16 s that is not half-way between
@@ -498,6 +485,184 @@ __global__ __launch_bounds__(256) void pages_compact_kernel(PageArgs a) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// eviction: some of each row's tokens to the front of its pages
+// ---------------------------------------------------------------------------
+// Token i < count of a row of more than `count` becomes its token keep[i] >= i, in
+// every layer and head by a list of its own. Pages that are written and that another
+// row holds too are replaced by free ones; all others are written in place.
+struct EvictArgs {
+  PageArgs p;           // (table, lengths, out_table, out_lengths, out_count)
+  const int32_t* keep;  // [layers, B, H, count]
+  float* mass;          // [layers, B, H, tokens], or null
+  int64_t m_layer, m_row, m_head;
+  int H, D, count, slices;  // slices: of a token's codes, a workgroup each
+};
+
+// pages that a row of more than `count` tokens keeps
+__device__ __forceinline__ int kept_pages(const EvictArgs& e) {
+  return (int)(((int64_t)e.count + (1 << e.p.page_log2) - 1) >> e.p.page_log2);
+}
+
+// One workgroup: holders of each page, free pages in order, and where each row's
+// replacements start among these (a wave a row).
+template <bool LDS>
+__global__ __launch_bounds__(kPlanThreads) void pages_evict_plan_kernel(EvictArgs e) {
+  extern __shared__ int s_pages[];
+  __shared__ int s_wave[kPlanThreads / 64], s_src[kPlanThreads], s_held[kPlanThreads];
+  const PageArgs& a = e.p;
+  const Counters<LDS> held{LDS ? s_pages : a.s.held};
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  count_held<LDS>(a, held, tid < a.rows ? row_plan(a, tid) : RowPlan{}, s_src, s_held);
+  const int per = (a.pages + kPlanThreads - 1) / kPlanThreads;
+  const int p0 = min(tid * per, a.pages), p1 = min(p0 + per, a.pages);
+  int n = 0, nfree;
+  for (int p = p0; p < p1; ++p) n += held.get(p) == 0;
+  int at = block_prefix(n, s_wave, nfree);
+  for (int p = p0; p < p1; ++p) {
+    const int holders = held.get(p);
+    if (holders == 0) a.s.list[at++] = p;
+    if (LDS) a.s.held[p] = holders;
+  }
+  const int kept = kept_pages(e);
+  int wanted = 0;
+  for (int i0 = 0; i0 < a.rows; i0 += kPlanThreads) {
+    __syncthreads();  // s_held is done with
+    for (int k = wave; k < min(a.rows - i0, kPlanThreads); k += kPlanThreads / 64) {
+      const RowPlan r = row_plan(a, i0 + k);
+      int c = 0;
+      for (int j0 = 0; r.before > e.count && j0 < kept; j0 += 64) {
+        const int id = j0 + lane < kept ? held_page(a, r, j0 + lane) : -1;
+        c += __builtin_popcountll(__ballot(id >= 0 && held.get(max(id, 0)) > 1));
+      }
+      if (lane == 0) s_held[k] = c;
+    }
+    __syncthreads();
+    const int i = i0 + tid;
+    int total;
+    const int base = wanted + block_prefix(i < a.rows ? s_held[tid] : 0, s_wave, total);
+    if (i < a.rows) a.s.base[i] = base;
+    wanted += total;
+  }
+  if (tid == 0) {
+    const int missing = max(wanted - nfree, 0);
+    a.s.head[kPairs] = missing;
+    *a.out_count = missing;
+  }
+}
+
+// The tables and lengths after it: a wave a row.
+__global__ __launch_bounds__(256) void pages_evict_table_kernel(EvictArgs e) {
+  const PageArgs& a = e.p;
+  const int lane = threadIdx.x & 63, i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= a.rows) return;
+  const RowPlan r = row_plan(a, i);
+  const bool less = r.before > e.count && a.s.head[kPairs] == 0;
+  const int n = less ? kept_pages(e) : r.held;
+  int at = a.s.base[i];
+  if (lane == 0) a.out_lengths[i] = less ? e.count : r.before;
+  for (int j0 = 0; j0 < a.width; j0 += 64) {
+    const int j = j0 + lane;
+    int id = j < n ? held_page(a, r, j) : -1;
+    const bool other = less && id >= 0 && a.s.held[id] > 1;
+    const unsigned long long m = __ballot(other);
+    if (other)
+      id = a.s.list[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))];
+    at += __builtin_popcountll(m);
+    if (j < a.width) a.out_table[(int64_t)i * a.width + j] = id;
+  }
+}
+
+// A workgroup per (layer, row, head, keys or values, slice of the codes) takes the
+// kept tokens in order, a chunk at a time: every load of a chunk is done before its
+// first store. What a chunk writes lies before all that later chunks read (keep[i] >=
+// i), so their loads need not wait for it.
+template <int LPT>  // 16-byte pieces of a token in a slice
+__global__ __launch_bounds__(256) void pages_evict_kernel(EvictArgs e) {
+  constexpr int TPP = 256 / LPT, U = 8, C = U * TPP, S = (C + 255) / 256;
+  const PageArgs& a = e.p;
+  const int tid = threadIdx.x;
+  int x = blockIdx.x;
+  const int slice = x % e.slices;
+  x /= e.slices;
+  const int side = x & 1;
+  x >>= 1;
+  const int h = x % e.H;
+  x /= e.H;
+  const int b = x % a.rows, layer = x / a.rows;
+  const RowPlan r = row_plan(a, b);
+  if (r.before <= e.count || a.s.head[kPairs] != 0) return;
+  const int mask = (1 << a.page_log2) - 1;
+  const int32_t* keep = e.keep + (((int64_t)layer * a.rows + b) * e.H + h) * e.count;
+  const int32_t* now = a.out_table + (int64_t)b * a.width;
+  uint8_t* const codes = a.buf[side].p + layer * a.buf[side].layer + ((int64_t)h << a.page_log2) * e.D + 16 * LPT * slice;
+  uint8_t* const scales = a.buf[2 + side].p + layer * a.buf[2 + side].layer + 2 * ((int64_t)h << a.page_log2);
+  const int64_t c_page = a.buf[side].page, s_page = a.buf[2 + side].page;
+  float* const mass = e.mass && side == 0 ? e.mass + layer * e.m_layer + b * e.m_row + h * e.m_head : nullptr;
+  struct Move {
+    int src, from, to, slot;  // token, its page or -1, the page that it goes to or -1, slot there
+  };
+  auto find = [&](int i) {
+    Move m;
+    const int k = keep[min(i, e.count - 1)];
+    m.src = k < i || k >= r.before ? i : k;
+    m.from = held_page(a, r, m.src >> a.page_log2);
+    m.to = now[i >> a.page_log2];
+    m.slot = i & mask;
+    if (m.src == i && m.from == m.to) m.to = -1;  // it stays where it is
+    return m;
+  };
+  for (int i0 = 0; i0 < e.count; i0 += C) {
+    u32x4_t v[U];
+    Move mv[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * TPP + tid / LPT;
+      mv[u] = find(min(i, e.count - 1));
+      if (i >= e.count) mv[u].to = -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      v[u] = u32x4_t{0, 0, 0, 0};
+      if (mv[u].from >= 0 && mv[u].to >= 0)
+        v[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(
+            codes + mv[u].from * c_page + (int64_t)(mv[u].src & mask) * e.D + 16 * (tid % LPT)));
+    }
+    Move sm[S];
+    uint16_t sc[S];
+    float w[S];
+#pragma unroll
+    for (int u = 0; u < S; ++u) {
+      const int k = tid + 256 * u, i = i0 + k;
+      sm[u].to = -1;
+      if (slice == 0 && k < C && i < e.count) {
+        sm[u] = find(i);
+        sc[u] = 0x3C00u;  // a token without a page comes as zeros with scale 1
+        if (sm[u].from >= 0)
+          sc[u] = *reinterpret_cast<const uint16_t*>(scales + sm[u].from * s_page + 2 * (sm[u].src & mask));
+        if (mass) w[u] = mass[sm[u].src];
+      }
+    }
+    // (a load in flight still reads memory that another thread may write)
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (mv[u].to >= 0)
+        __builtin_nontemporal_store(v[u], reinterpret_cast<u32x4_t*>(codes + mv[u].to * c_page +
+                                                                     (int64_t)mv[u].slot * e.D + 16 * (tid % LPT)));
+#pragma unroll
+    for (int u = 0; u < S; ++u) {
+      const int k = tid + 256 * u, i = i0 + k;
+      if (slice != 0 || k >= C || i >= e.count) continue;
+      if (mass) mass[i] = w[u];
+      if (sm[u].to >= 0) *reinterpret_cast<uint16_t*>(scales + sm[u].to * s_page + 2 * sm[u].slot) = sc[u];
+    }
+  }
+}
+
 }  // namespace
 
 int paged_kv_append(const PagedBatch& p, const void* k, const void* v, const int64_t* xst,
@@ -579,6 +744,49 @@ int kv_pages_compact(const int32_t* table, int64_t table_stride, const int32_t* 
     hipLaunchKernelGGL(pages_compact_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, st, a);
   hipLaunchKernelGGL(pages_compact_kernel, page_grid(a), dim3(256), 0, st, a);
   return check_launch("pages_compact_kernel");
+}
+
+int kv_pages_evict(const int32_t* table, int64_t table_stride, const int32_t* lengths, const int32_t* keep,
+                   int64_t count, float* mass, const int64_t* mst, int32_t* out_table, int32_t* out_lengths,
+                   int32_t* missing, int64_t B, int64_t width, int64_t pages, int page_size, int64_t layers, int64_t H,
+                   int64_t D, void* const* bufs, const int64_t* strides, void* ws, hipStream_t st) {
+  const int64_t code_bytes = H * page_size * D, scale_bytes = 2 * H * page_size;
+  EvictArgs e{};
+  e.p = page_args(table, table_stride, lengths, B, B, width, pages, page_size, layers, bufs, strides, code_bytes,
+                  scale_bytes, ws);
+  e.p.out_table = out_table;
+  e.p.out_lengths = out_lengths;
+  e.p.out_count = missing;
+  e.keep = keep;
+  e.mass = mass;
+  if (mass) {
+    e.m_layer = mst[0];
+    e.m_row = mst[1];
+    e.m_head = mst[2];
+  }
+  e.H = (int)H;
+  e.D = (int)D;
+  e.count = (int)count;
+  // tokens in slices of 64 bytes where whole ones would not fill the chip
+  const int64_t groups = layers * B * H * 2;
+  const bool sliced = groups < 4 * device_cus();
+  const int pieces = sliced ? 4 : (int)(D / 16);
+  e.slices = (int)(D / 16 / pieces);
+  if (groups > kMaxGrid / e.slices) return set_error(SPARKQ_ERR_INVALID, "kv_pages_evict: shape too large");
+  if (pages <= kLdsPages)
+    hipLaunchKernelGGL(pages_evict_plan_kernel<true>, dim3(1), dim3(kPlanThreads), pages * sizeof(int), st, e);
+  else
+    hipLaunchKernelGGL(pages_evict_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, st, e);
+  if (B == 0) return check_launch("pages_evict_kernel");
+  hipLaunchKernelGGL(pages_evict_table_kernel, dim3((unsigned)cdiv(B, 4)), dim3(256), 0, st, e);
+  const dim3 grid((unsigned)(groups * e.slices));
+  if (pieces == 4)
+    hipLaunchKernelGGL(pages_evict_kernel<4>, grid, dim3(256), 0, st, e);
+  else if (pieces == 8)
+    hipLaunchKernelGGL(pages_evict_kernel<8>, grid, dim3(256), 0, st, e);
+  else
+    hipLaunchKernelGGL(pages_evict_kernel<16>, grid, dim3(256), 0, st, e);
+  return check_launch("pages_evict_kernel");
 }
 
 }  // namespace sparkq

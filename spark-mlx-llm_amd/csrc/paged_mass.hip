@@ -1,0 +1,398 @@
+// paged_mass.hip -- the attention weight that the cached tokens of a paged INT8 KV
+// cache gather from a batch's new tokens (gfx950):
+//
+//   mass[b,h,n] += sum_t sum_g exp(scale * q[t,g] . k[h,n] - lse[t,g])
+//
+// over sequence b's new tokens t that see token n and the query heads g of KV head
+// h, with the logarithms of the rows' sums that the attention returned. A batch's
+// new tokens start from 0. One workgroup has all rows that see its tokens: every sum
+// has one order, and there are no atomics.
+#include <algorithm>
+
+#include "paged_attn.h"
+
+namespace sparkq {
+namespace {
+
+struct MassArgs {
+  PagedSdpaArgs a;   // (no values, no outputs)
+  const float* lse;  // [T, Hq]
+  float* mass;       // [B, Hkv, tokens], tokens contiguous
+  int64_t m_row, m_head;
+  int tokens;        // of a row of it
+  float scale;       // the softmax scale in log2 units, signed
+};
+
+// What a row's logarithm is in log2 units; a row that sees nothing weighs nothing.
+__device__ __forceinline__ float row_base(float lse) {
+  return lse == kNegInf ? __builtin_huge_valf() : lse * 1.44269504088896340736f;
+}
+
+// ---------------------------------------------------------------------------
+// at most 16 rows a (sequence, KV head)
+// ---------------------------------------------------------------------------
+// S^T (16 tokens x 16 rows) = K . Q^T twice a block of 32 tokens, the lane with a
+// row's scores of tokens 8g .. 8g+7; the rows' weights are summed over 16 lanes. The
+// waves of a workgroup take turns at blocks, each with the next one's loads in
+// flight. Contexts are split like the attention's.
+template <int D>
+__global__ __launch_bounds__(256) void paged_mass_few_kernel(MassArgs s) {
+  constexpr int NK = D / 32, PL = D / 64, kBlock = kFewBlock;
+  const PagedSdpaArgs& a = s.a;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n16 = lane & 15, grp = lane >> 4;
+  const int kh = blockIdx.x % a.Hkv, gqa = a.Hq / a.Hkv;
+  const Item it = find_item<16, false>(a, blockIdx.x / a.Hkv);
+  if (it.b < 0) return;
+  const int rows = it.rows, rr = min(n16, rows - 1);
+  const bool live = n16 < rows;
+  const int lim = last_seen(a, it, rr, gqa);
+  const int all = last_seen(a, it, 0, gqa) + 1;  // seen by every row
+  const int nblocks = (it.length + kBlock - 1) / kBlock;
+  const int ib0 = (int)((int64_t)it.part * nblocks / it.parts);
+  const int ib1 = (int)((int64_t)(it.part + 1) * nblocks / it.parts);
+  const TableRow trow = table_row(a, it.b);
+
+  u32x4_t qb[NK];
+  const int64_t t = it.first + rr / gqa;
+  const int head = kh * gqa + rr % gqa;
+  const float mul = load_query<NK, 4>(a, a.q + t * a.q_tok + head * a.q_head, true,
+                                      [&](int c) { return 16 * (grp + 4 * (c >> 1)) + 8 * (c & 1); }, qb);
+  const float base = row_base(s.lse[t * a.Hq + head]);
+
+  u32x4_t kr[2][PL], skr;
+  float2 old;
+  BlockPages<2> next;
+  uint32_t pages_ok;
+  const int ktok = 8 * (n16 >> 2) + (n16 & 3);
+  const uint32_t koff = (ktok & 15) * a.c.c_tok + 16 * grp;
+  const uint8_t* const khead = a.c.k + kh * a.c.c_head;
+  const uint16_t* const kshead = a.c.ks + kh * a.c.s_head;
+  const int slot_mask = (1 << a.p.page_log2) - 1;
+  const int last = ib1 - 1;
+  // lane q < 4 of a group has the sums of tokens 8 grp + 2 q, + 1 of a block
+  const int off = 8 * grp + 2 * (n16 & 3);
+  float* const mine = s.mass + it.b * s.m_row + kh * s.m_head + off;
+  const int fresh = it.length - it.count;  // tokens from it on start from 0
+  auto load = [&](int ib, const BlockPages<2>& bp) {
+    const int t0 = kBlock * min(ib, last);
+    const int s0 = t0 & slot_mask, s1 = (t0 + 16) & slot_mask;
+    const uint64_t o0 = code_at(a.c, bp.id[0], s0), o1 = code_at(a.c, bp.id[1], s1);
+    const uint8_t* kp = khead + (n16 < 8 ? o0 : o1) + koff;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < PL; ++i)
+        kr[h][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kp + (4 * h * a.c.c_tok + 64 * i)));
+    const bool h = grp >= 2;
+    skr = *reinterpret_cast<const u32x4_t*>(kshead + scale_at(a.c, h ? bp.id[1] : bp.id[0], (h ? s1 : s0) + 8 * (grp & 1)));
+    old = *reinterpret_cast<const float2*>(mine + (min(t0 + off, s.tokens - 2) - off));
+    pages_ok = bp.ok;
+  };
+
+  auto block = [&](int ib) {
+    const int t0 = kBlock * ib;
+    f32x4_t sc[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      sc[h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < NK; ++c) {
+        const u32x4_t kp = kr[h][c >> 1];
+        sc[h] = mfma16x16x32_f16((c & 1) ? s8x8_exact(kp.z, kp.w) : s8x8_exact(kp.x, kp.y), qb[c], sc[h]);
+      }
+    }
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t kw = skr[i >> 1];
+      const float v = sc[i >> 2][i & 3] * (((i & 1) ? hi16<F16>(kw) : lo16<F16>(kw)) * a.sign);
+      const float e = __builtin_amdgcn_exp2f(fmaf(v, mul, -base));
+      p[i] = live ? e : 0.0f;
+    }
+    if (__builtin_expect(t0 + kBlock > all || pages_ok != 3, 0)) {
+      const bool in = (pages_ok >> (grp >> 1)) & 1u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = in && t0 + 8 * grp + i <= lim ? p[i] : 0.0f;
+    }
+    const float2 was = old;
+    load(ib + 4, next);
+    next = block_pages<2>(a, trow, kBlock * min(ib + 8, last));
+    // sums over the 16 lanes: lanes 4k + q end with tokens 2q, 2q + 1
+    float h4[4], h2[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // lanes with bit 1 keep tokens 4 .. 7
+      const bool up = n16 & 2;
+      const float keep = up ? p[4 + i] : p[i], give = up ? p[i] : p[4 + i];
+      h4[i] = keep + dpp_row<0x4E>(give);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {  // bit 0: the upper two of these
+      const bool up = n16 & 1;
+      const float keep = up ? h4[2 + i] : h4[i], give = up ? h4[i] : h4[2 + i];
+      h2[i] = keep + dpp_row<0xB1>(give);
+      h2[i] += dpp_row<0x124>(h2[i]);
+      h2[i] += dpp_row<0x128>(h2[i]);
+    }
+    const int at = t0 + 8 * grp + 2 * n16;
+    if (n16 < 4) {
+      if (at + 1 < it.length) {
+        *reinterpret_cast<float2*>(mine + t0) =
+            make_float2((at < fresh ? was.x : 0.0f) + h2[0], (at + 1 < fresh ? was.y : 0.0f) + h2[1]);
+      } else if (at < it.length) {
+        mine[t0] = (at < fresh ? was.x : 0.0f) + h2[0];
+      }
+    }
+  };
+
+  int ib = ib0 + wave;
+  if (ib < ib1) {
+    load(ib, block_pages<2>(a, trow, kBlock * ib));
+    next = block_pages<2>(a, trow, kBlock * min(ib + 4, last));
+    for (; ib < ib1; ib += 4) block(ib);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// more rows
+// ---------------------------------------------------------------------------
+// A workgroup has 64 tokens (32 at D = 256) of one KV head, whose keys stay in its waves' registers
+// as the first operand of the 32 x 32 products; the waves take turns at tiles of 32
+// rows, whose queries come straight from memory in the operand's layout, the next
+// tile's in flight. A lane has one row's scores of half the tokens and sums its
+// rows' weights in registers; lanes and waves are joined at the end through LDS.
+// Codes are exact in either 16-bit type, so queries stay as they are.
+template <typename T>
+__device__ __forceinline__ u32x4_t codes_as(uint32_t lo, uint32_t hi);
+template <>
+__device__ __forceinline__ u32x4_t codes_as<F16>(uint32_t lo, uint32_t hi) {
+  return s8x8_exact(lo, hi);
+}
+template <>
+__device__ __forceinline__ u32x4_t codes_as<BF16>(uint32_t lo, uint32_t hi) {
+  auto pair = [](uint32_t w, int i) {
+    return pack_round<BF16>((float)(int8_t)(w >> (8 * i)), (float)(int8_t)(w >> (8 * i + 8)));
+  };
+  return u32x4_t{pair(lo, 0), pair(lo, 2), pair(hi, 0), pair(hi, 2)};
+}
+
+// tokens of a workgroup: what the registers hold
+constexpr int mass_tokens(int D) { return D <= 128 ? 64 : 32; }
+
+// The block of `size` tokens that is number x of the batch's sequences with new tokens
+struct TokenBlock {
+  int b, t0;
+  SeqRows s;
+};
+__device__ __forceinline__ TokenBlock find_block(const PagedBatch& p, int size, int x) {
+  const int lane = threadIdx.x & 63;
+  TokenBlock r{-1, 0, {0, 0, 0}};
+  int before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    int n = 0;
+    if (b0 + lane < p.B) {
+      const SeqRows s = seq_rows(p, b0 + lane);
+      n = s.count > 0 ? (s.length + size - 1) / size : 0;
+    }
+    const int end = before + wave_prefix(n);
+    const unsigned long long hit = __ballot(x < end);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      r.b = b0 + l;
+      r.t0 = size * (x - __builtin_amdgcn_readlane(end - n, l));
+      r.s = seq_rows(p, r.b);
+      break;
+    }
+    before = __builtin_amdgcn_readlane(end, 63);
+  }
+  for (int* f : {&r.b, &r.t0, &r.s.first, &r.s.count, &r.s.length}) *f = __builtin_amdgcn_readfirstlane(*f);
+  return r;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void paged_mass_many_kernel(MassArgs s, int blocks) {
+  constexpr int NK = D / 16, N = mass_tokens(D), H = N / 32;
+  const PagedSdpaArgs& a = s.a;
+  __shared__ float s_sum[4][N][33];
+  __shared__ __attribute__((aligned(16))) float s_scale[N];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, grp = lane >> 5;
+  const int gqa = a.Hq / a.Hkv, kh = blockIdx.x % a.Hkv;
+  for (int x = blockIdx.x / a.Hkv; x < blocks; x += gridDim.x / a.Hkv) {
+    const TokenBlock tb = find_block(a.p, N, x);
+    if (tb.b < 0) return;
+    const int t0 = tb.t0, rows = min(tb.s.count, a.max_new) * gqa;
+    // the first row that sees the block's first token
+    const int skip = a.causal ? max(t0 - (tb.s.length - tb.s.count), 0) : 0;
+    const int row0 = (int)min((int64_t)skip * gqa, (int64_t)rows) & ~31;
+
+    u32x4_t kf[H][NK];
+    uint64_t present[H];  // tokens that have a page (a bit a lane)
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      const int pos = t0 + 32 * h + col;
+      const int id = pos < tb.s.length ? page_of(a.p, tb.b, pos) : -1;
+      present[h] = __ballot(id >= 0);
+      const int at = max(id, 0), slot = pos & ((1 << a.p.page_log2) - 1);
+      const uint8_t* kp = a.c.k + kh * a.c.c_head + code_at(a.c, at, slot) + 8 * grp;
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        const uint2 w = *reinterpret_cast<const uint2*>(kp + 16 * k);
+        kf[h][k] = codes_as<T>(w.x, w.y);
+      }
+      if (wave == 0 && grp == 0)
+        s_scale[32 * h + col] = f16_to_f32(a.c.ks[kh * a.c.s_head + scale_at(a.c, at, slot)]) * s.scale;
+    }
+    __syncthreads();
+    float sum[H][16];
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) sum[h][v] = 0.0f;
+
+    auto place = [&](int r0, int64_t& t, int& head) {
+      const int rr = min(r0 + col, rows - 1), i = rr / gqa;
+      t = tb.s.first + i;
+      head = kh * gqa + rr - i * gqa;
+    };
+    u32x4_t qn[NK];
+    float base_n;
+    auto load = [&](int r0) {
+      int64_t t;
+      int head;
+      place(r0, t, head);
+      const uint16_t* q = a.q + t * a.q_tok + head * a.q_head + 8 * grp;
+#pragma unroll
+      for (int k = 0; k < NK; ++k) qn[k] = *reinterpret_cast<const u32x4_t*>(q + 16 * k);
+      base_n = s.lse[t * a.Hq + head];
+    };
+    int r0 = row0 + 32 * wave;
+    if (r0 < rows) load(r0);
+    for (; r0 < rows; r0 += 128) {
+      u32x4_t q[NK];
+#pragma unroll
+      for (int k = 0; k < NK; ++k) q[k] = qn[k];
+      const float base = row_base(base_n);
+      if (r0 + 128 < rows) load(r0 + 128);
+      // what the tile's first row sees
+      const int least = last_seen_by(tb.s, r0 / gqa, a.causal);
+      const bool whole = least >= t0 + N - 1 && r0 + 32 <= rows;
+      const int lim = whole || r0 + col >= rows ? -1 : last_seen_by(tb.s, (r0 + col) / gqa, a.causal);
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        f32x16_t sc = f32x16_t{};
+#pragma unroll
+        for (int k = 0; k < NK; ++k) sc = mfma32x32x16<T>(kf[h][k], q[k], sc);
+        float e[16];
+#pragma unroll
+        for (int v = 0; v < 16; v += 4) {
+          const f32x4_t k4 = *reinterpret_cast<const f32x4_t*>(s_scale + 32 * h + 2 * v + 4 * grp);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) e[v + r] = __builtin_amdgcn_exp2f(fmaf(sc[v + r], k4[r], -base));
+        }
+        if (__builtin_expect(!whole, 0)) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) e[v] = t0 + 32 * h + mfma32_row(lane, v) <= lim ? e[v] : 0.0f;
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sum[h][v] += e[v];
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) s_sum[wave][32 * h + mfma32_row(lane, v)][col] = sum[h][v];
+    __syncthreads();
+    // four threads a token, a wave's sums each
+    const int tok = tid >> 2;
+    if (tok < N) {
+      float v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v += s_sum[tid & 3][tok][i];
+      v += dpp_row<0xB1>(v);
+      v += dpp_row<0x4E>(v);
+      if ((tid & 3) == 0 && t0 + tok < tb.s.length) {
+        float* m = s.mass + tb.b * s.m_row + kh * s.m_head + t0 + tok;
+        uint64_t have = present[0];
+        if (H == 2 && tok >= 32) have = present[H - 1];
+        *m = (t0 + tok < tb.s.length - tb.s.count ? *m : 0.0f) + ((have >> (tok & 31)) & 1 ? v : 0.0f);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <int D>
+void launch_few(const MassArgs& s, int64_t items, hipStream_t st) {
+  hipLaunchKernelGGL(paged_mass_few_kernel<D>, dim3((unsigned)(items * s.a.Hkv)), dim3(256), 0, st, s);
+}
+template <typename T, int D>
+void launch_many(const MassArgs& s, int64_t items, int64_t blocks, hipStream_t st) {
+  hipLaunchKernelGGL((paged_mass_many_kernel<T, D>), dim3((unsigned)(items * s.a.Hkv)), dim3(256), 0, st, s, (int)blocks);
+}
+
+}  // namespace
+
+int paged_kv_mass(const PagedBatch& p, const void* q, const int64_t* qst, const float* lse, const PagedSide& ks,
+                  float* mass, const int64_t* mst, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, int causal,
+                  int qdt, float scale, hipStream_t st) {
+  if (p.T == 0 || p.B == 0) return SPARKQ_OK;
+  max_new = std::min<int64_t>(max_new, p.T);
+  const int64_t gqa = Hq / Hkv, max_tokens = (int64_t)p.width << p.page_log2;
+  MassArgs s{};
+  s.a.p = p;
+  s.a.q = (const uint16_t*)q;
+  s.a.q_tok = qst[0];
+  s.a.q_head = qst[1];
+  s.a.c = CodeLayout{ks.codes, nullptr, ks.scales, nullptr, ks.c_head, ks.s_head, (uint32_t)(ks.c_page / 16),
+                     (uint32_t)(ks.s_page / 8), (uint32_t)ks.c_tok};
+  s.a.Hq = (int)Hq;
+  s.a.Hkv = (int)Hkv;
+  s.a.max_new = (int)max_new;
+  s.a.causal = causal;
+  s.a.q_dtype = qdt;
+  s.a.scale_log2 = fabsf(scale) * 1.44269504088896340736f;
+  s.a.sign = scale < 0.0f ? -1.0f : 1.0f;
+  s.lse = lse;
+  s.mass = mass;
+  s.m_row = mst[0];
+  s.m_head = mst[1];
+  s.tokens = (int)max_tokens;
+  s.scale = scale * 1.44269504088896340736f;
+  if (max_new * gqa <= 16) {
+    // (as the attention's plan: B sequences of one tile, and the parts of split contexts)
+    s.a.min_part = 128;
+    s.a.target = (int)std::min<int64_t>(cdiv(4 * device_cus(), Hkv), 512);
+    const int64_t split = max_tokens > 128 ? std::min<int64_t>(p.B, s.a.target) : 0;
+    s.a.slots = (int)std::min<int64_t>(2 * s.a.target, split * cdiv(max_tokens, 128));
+    const int64_t items = s.a.slots + p.B;
+    if (items > kMaxGrid / Hkv) return set_error(SPARKQ_ERR_INVALID, "paged_kv_mass: shape too large");
+    if (D == 64)
+      launch_few<64>(s, items, st);
+    else if (D == 128)
+      launch_few<128>(s, items, st);
+    else
+      launch_few<256>(s, items, st);
+    return check_launch("paged_mass_few_kernel");
+  }
+  const int64_t blocks = p.B * cdiv(max_tokens, mass_tokens((int)D));
+  if (blocks > 0x7FFFFFFF) return set_error(SPARKQ_ERR_INVALID, "paged_kv_mass: shape too large");
+  // no more workgroups than the chip holds eight times over; they take further blocks
+  const int64_t items = std::min(blocks, cdiv(16 * device_cus(), Hkv));
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    if (D == 64)
+      launch_many<T, 64>(s, items, blocks, st);
+    else if (D == 128)
+      launch_many<T, 128>(s, items, blocks, st);
+    else
+      launch_many<T, 256>(s, items, blocks, st);
+  };
+  if (qdt == SPARKQ_BF16)
+    go(BF16{});
+  else
+    go(F16{});
+  return check_launch("paged_mass_many_kernel");
+}
+
+}  // namespace sparkq

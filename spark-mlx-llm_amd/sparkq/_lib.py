@@ -89,6 +89,20 @@ SIGNATURES = {
     "sparkq_quantized_sdpa_call_workspace_bytes": (SZ, [I64, I64, I64, I64, I64, I64, I64, I]),
     "sparkq_quantized_sdpa": (I, [P, P, P, P, P, P, P, P, I, I, P, P, I64, I64, I64, I64, I64,
                                   I64, I64, I, I, I, I, F, P, P, SZ, P]),
+    "sparkq_paged_sdpa_lse": (I, [P, P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64,
+                                  I64, I, I64, I, I, I, F, P, P, P, SZ, P]),
+    "sparkq_paged_key_bounds": (I, [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I, I64, P, P,
+                                    P]),
+    "sparkq_paged_page_scores": (I, [P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I,
+                                     I64, I, I, F, P, P, P]),
+    "sparkq_select_top": (I, [P, P, P, I64, I64, I64, I64, I64, I64, I64, P, P]),
+    "sparkq_paged_sparse_workspace_bytes": (SZ, [I64, I64, I64, I64, I64, I]),
+    "sparkq_paged_sparse_sdpa": (I, [P, P, P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64,
+                                     I64, I64, I64, I, I64, I, I, I, F, P, P, P, P, SZ, P]),
+    "sparkq_paged_kv_mass": (I, [P, P, P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I,
+                                 I64, I, I, F, P, P, P, P]),
+    "sparkq_kv_pages_evict": (I, [P, P, P, P, P, P, P, P, I64, P, P, P, P, P, I64, I64, I64, I64,
+                                  I64, I64, I64, I, P, SZ, P]),
 }
 
 

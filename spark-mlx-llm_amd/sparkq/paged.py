@@ -29,13 +29,14 @@ import torch
 from . import _lib
 from .ext import _HALF, _out_buffer, _ptr
 
-__all__ = ["PagedKVCache", "kv_pages_compact", "kv_pages_fork", "paged_kv_append",
-           "paged_quantized_sdpa"]
+__all__ = ["PagedKVCache", "kv_pages_compact", "kv_pages_evict", "kv_pages_fork",
+           "paged_key_bounds", "paged_kv_append", "paged_kv_mass", "paged_page_scores",
+           "paged_quantized_sdpa", "paged_sparse_sdpa", "select_top"]
 
 
 _T = torch.Tensor
 _CONTIGUOUS = torch.contiguous_format
-_I64x2, _I64x4, _I64x8, _I64x12 = (ctypes.c_int64 * n for n in (2, 4, 8, 12))
+_I64x2, _I64x3, _I64x4, _I64x6, _I64x8, _I64x12 = (ctypes.c_int64 * n for n in (2, 3, 4, 6, 8, 12))
 _CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
@@ -113,6 +114,33 @@ def _rows16(t):
     return t, t.stride()
 
 
+def _check_attention(op, queries, hkv, d, index, mask, scale, max_new):
+    if queries.ndim != 3 or queries.shape[2] != d or not queries.shape[1] \
+            or queries.shape[1] % hkv:
+        raise ValueError(f"{op}: queries must be [T,Hq,{d}] with Hq divisible by {hkv}")
+    if queries.dtype not in _HALF:
+        raise ValueError(f"{op} requires float16 or bfloat16 queries")
+    if queries.get_device() != index:
+        raise ValueError(f"{op}: queries must live on the cache's device")
+    if mask is not None and mask != "causal":
+        raise ValueError(f"{op} takes mask=None or mask='causal'")
+    if not isinstance(scale, (float, int)) or not math.isfinite(scale):
+        raise ValueError("scale must be a finite Python number")
+    _check_max_new(op, max_new)
+
+
+def _check_max_new(op, max_new):
+    if type(max_new) is not int or max_new < 1:
+        raise ValueError(f"{op}: max_new must be a positive Python int")
+
+
+def _out_dtype(queries, out_dtype):
+    out_dtype = queries.dtype if out_dtype is None else out_dtype
+    if out_dtype is not queries.dtype and out_dtype is not torch.float32:
+        raise ValueError("out_dtype must be the query dtype or torch.float32")
+    return out_dtype
+
+
 def paged_kv_append(keys, values, cache, page_table, starts, lengths):
     """Quantize a batch's new tokens into their pages, in place: keys and
     values [T,Hkv,D] (float16, bfloat16 or float32; views of a packed
@@ -142,7 +170,7 @@ def paged_kv_append(keys, values, cache, page_table, starts, lengths):
 
 
 def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, max_new: int,
-                         mask="causal", out_dtype=None, out=None):
+                         mask="causal", out_dtype=None, out=None, return_lse: bool = False):
     """Attention of a batch's new tokens over their pages: queries [T,Hq,D]
     (float16 or bfloat16) -> [T,Hq,D]. With mask="causal" row i of a
     sequence's n new tokens sees its tokens 0 .. length - n + i, with None all
@@ -156,27 +184,15 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
     a sequence and KV head (max_new * Hq / Hkv: decode steps, a few drafted
     tokens) and wherever out_dtype is float32; in others, with 16-bit outputs, in
     float16's 11, which their own rounding is near (float32 outputs cost up to a
-    quarter more time there). Scores, normalizer and sums are fp32."""
+    quarter more time there). Scores, normalizer and sums are fp32.
+
+    With return_lse the result is (out, lse [T,Hq] float32): the natural logarithm of
+    the sum of each row's exponentiated scores, -inf where it sees nothing."""
     op = "paged_quantized_sdpa"
     kc, ks, vc, vs, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
-    if queries.ndim != 3 or queries.shape[2] != d or not queries.shape[1] \
-            or queries.shape[1] % hkv:
-        raise ValueError(f"{op}: queries must be [T,Hq,{d}] with Hq divisible by {hkv}")
+    _check_attention(op, queries, hkv, d, index, mask, scale, max_new)
     t, heads, _ = shape = queries.shape
-    dtype = queries.dtype
-    if dtype not in _HALF:
-        raise ValueError(f"{op} requires float16 or bfloat16 queries")
-    if queries.get_device() != index:
-        raise ValueError(f"{op}: queries must live on the cache's device")
-    if mask is not None and mask != "causal":
-        raise ValueError(f"{op} takes mask=None or mask='causal'")
-    if not isinstance(scale, (float, int)) or not math.isfinite(scale):
-        raise ValueError("scale must be a finite Python number")
-    if type(max_new) is not int or max_new < 1:
-        raise ValueError(f"{op}: max_new must be a positive Python int")
-    out_dtype = dtype if out_dtype is None else out_dtype
-    if out_dtype is not dtype and out_dtype is not torch.float32:
-        raise ValueError("out_dtype must be the query dtype or torch.float32")
+    dtype, out_dtype = queries.dtype, _out_dtype(queries, out_dtype)
     b, width = _check_batch(op, index, page_table, starts, lengths)
     strides = _strides(op, kc, ks, vc, vs)
     _need_gpu(op, index)
@@ -185,12 +201,205 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
         else _out_buffer(out, shape, out_dtype, kc.device)
     need = _lib.lib().sparkq_paged_sdpa_workspace_bytes(t, b, heads, hkv, d, max_new, width * page)
     ws = kc.new_empty(need) if need else None  # (int8: bytes)
-    _lib.launch("sparkq_paged_sdpa", index, queries.data_ptr(), kc.data_ptr(), ks.data_ptr(),
-                vc.data_ptr(), vs.data_ptr(), page_table.data_ptr(), starts.data_ptr(),
-                lengths.data_ptr(), out.data_ptr(), t, b, heads, hkv, d, pages, width,
-                page_table.stride(0), page, max_new, 1 if mask is not None else 0, _CODE[dtype],
-                _CODE[out_dtype], scale, _I64x2(qst[0], qst[1]), strides, _ptr(ws), need)
+    head = (queries.data_ptr(), kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr(),
+            page_table.data_ptr(), starts.data_ptr(), lengths.data_ptr(), out.data_ptr())
+    tail = (t, b, heads, hkv, d, pages, width, page_table.stride(0), page, max_new,
+            1 if mask is not None else 0, _CODE[dtype], _CODE[out_dtype], scale,
+            _I64x2(qst[0], qst[1]), strides, _ptr(ws), need)
+    if not return_lse:
+        _lib.launch("sparkq_paged_sdpa", index, *head, *tail)
+        return out
+    lse = kc.new_empty((t, heads), dtype=torch.float32)
+    _lib.launch("sparkq_paged_sdpa_lse", index, *head, lse.data_ptr(), *tail)
+    return out, lse
+
+
+# --- long contexts: which pages a query attends, which tokens a cache keeps -------
+
+def _key_strides(op, kc, ks):
+    a0, a1, a2, a3 = kc.stride()
+    if a3 != 1:
+        raise ValueError(f"{op}: the codes' innermost axes must be contiguous")
+    return _I64x6(a0, a1, a2, *ks.stride())
+
+
+def _check_bounds(op, bounds, index, shape):
+    """Strides of bounds [pages,Hkv,2,D]."""
+    if not isinstance(bounds, _T) or bounds.dtype is not torch.bfloat16 or bounds.shape != shape:
+        raise ValueError(f"{op}: bounds must be a bfloat16 tensor of shape {list(shape)}")
+    if bounds.get_device() != index:
+        raise ValueError(f"{op}: bounds must live on the cache's device")
+    st = bounds.stride()
+    if st[3] != 1 or st[2] != shape[3]:
+        raise ValueError(f"{op}: the last two axes of bounds must be contiguous")
+    return _I64x2(st[0], st[1])
+
+
+def paged_key_bounds(cache, bounds, page_table, starts, lengths, *, max_new: int):
+    """Bounds of the keys of the pages that a batch's new tokens lie in, in place:
+    bounds [pages,Hkv,2,D] bfloat16, in each channel the least key of the page's
+    tokens rounded down, and the largest rounded up. Called after paged_kv_append
+    with its batch, it keeps the bounds of one layer's cache; each page is read as a
+    whole, so copies of pages (kv_pages_fork) need no bounds of their own before.
+    max_new is the most new tokens that a sequence has. A page with a key scale that
+    is not finite is bounded by bfloat16's largest numbers. Sequences with new tokens
+    must not share the pages that these lie in."""
+    op = "paged_key_bounds"
+    kc, ks, _, _, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
+    bst = _check_bounds(op, bounds, index, (pages, hkv, 2, d))
+    _check_max_new(op, max_new)
+    b, width = _check_batch(op, index, page_table, starts, lengths)
+    strides = _key_strides(op, kc, ks)
+    _need_gpu(op, index)
+    _lib.launch("sparkq_paged_key_bounds", index, kc.data_ptr(), ks.data_ptr(), bounds.data_ptr(),
+                page_table.data_ptr(), starts.data_ptr(), lengths.data_ptr(), b, hkv, d, pages,
+                width, page_table.stride(0), page, max_new, strides, bst)
+
+
+def paged_page_scores(queries, bounds, page_table, starts, lengths, *, page_size: int, scale,
+                      max_new: int, mask="causal"):
+    """Scores of the pages that a batch's new tokens see, (scores [T,Hkv,M] float32,
+    seen [T] int32): for row t, KV head h and entry j of its sequence's table row
+
+        max over the head's query heads g of  scale * sum_d max(q[t,g,d] lo, q[t,g,d] hi)
+
+    with the bounds of that page [pages,Hkv,2,D]: no logit of the row with a key of
+    the page is larger. (scale < 0: with min for max.) -inf where the row sees
+    nothing of the page, or there is none; a head whose sum is NaN does not count.
+    seen counts the pages that each row sees, for select_top:
+
+        scores, seen = paged_page_scores(...)
+        pages = select_top(scores, count, lengths=seen, first=1, last=2)
+        out = paged_sparse_sdpa(queries, cache, pages, ...)
+
+    Rows that fall to no sequence, or to more than max_new of one, hold anything."""
+    op = "paged_page_scores"
+    if not isinstance(bounds, _T) or bounds.ndim != 4 or bounds.shape[2] != 2:
+        raise ValueError(f"{op}: bounds must be a bfloat16 tensor of shape [pages,Hkv,2,D]")
+    (pages, hkv, _, d), index = bounds.shape, bounds.get_device()
+    bst = _check_bounds(op, bounds, index, bounds.shape)
+    _check_attention(op, queries, hkv, d, index, mask, scale, max_new)
+    if type(page_size) is not int or page_size < 16 or page_size > 1024 or page_size & (page_size - 1):
+        raise ValueError(f"{op}: page_size must be a power of two from 16 to 1024")
+    b, width = _check_batch(op, index, page_table, starts, lengths)
+    _need_gpu(op, index)
+    queries, qst = _rows16(queries)
+    t, heads, _ = queries.shape
+    scores = bounds.new_empty((t, hkv, width), dtype=torch.float32)
+    seen = bounds.new_empty(t, dtype=torch.int32)
+    _lib.launch("sparkq_paged_page_scores", index, queries.data_ptr(), bounds.data_ptr(),
+                page_table.data_ptr(), starts.data_ptr(), lengths.data_ptr(), scores.data_ptr(),
+                seen.data_ptr(), t, b, heads, hkv, d, pages, width, page_table.stride(0), page_size,
+                max_new, 1 if mask is not None else 0, _CODE[queries.dtype], scale,
+                _I64x2(qst[0], qst[1]), bst)
+    return scores, seen
+
+
+def select_top(x, count: int, *, lengths=None, first: int = 0, last: int = 0):
+    """Places of the `count` largest values of each row of x [...,R,H,N] (float32, 3
+    or 4 axes): [...,R,H,count] int32 in ascending order, -1 behind them where a row
+    has fewer values. Of row r only the first lengths[r] values count (int32 [R], the
+    same for all layers; N without). The first `first` and the last `last` of these
+    are taken whatever they are, and among equal values those at the lowest places;
+    NaN counts as -inf. first + last is at most count."""
+    op = "select_top"
+    if not isinstance(x, _T) or x.dtype is not torch.float32 or x.ndim not in (3, 4):
+        raise ValueError(f"{op} takes a float32 tensor [R,H,N] or [layers,R,H,N]")
+    for name, v, least in (("count", count, 1), ("first", first, 0), ("last", last, 0)):
+        if type(v) is not int or v < least:
+            raise ValueError(f"{op}: {name} must be a Python int of at least {least}")
+    if first + last > count:
+        raise ValueError(f"{op}: first and last together must be no more than count")
+    (rows, heads, n), index = x.shape[-3:], x.get_device()
+    if not n or not heads:
+        raise ValueError(f"{op}: rows must not be empty")
+    if n > 1 and x.stride(-1) != 1:
+        raise ValueError(f"{op}: the last axis of x must be contiguous")
+    if lengths is not None:
+        _check_ints(op, index, "lengths", lengths, (rows,))
+    _need_gpu(op, index)
+    layers, st = (x.shape[0], x.stride()) if x.ndim == 4 else (1, (0, *x.stride()))
+    out = x.new_empty((*x.shape[:-1], count), dtype=torch.int32)
+    _lib.launch("sparkq_select_top", index, x.data_ptr(), _ptr(lengths), out.data_ptr(), layers,
+                rows, heads, n, count, first, last, _I64x3(*st[:3]))
     return out
+
+
+def paged_sparse_sdpa(queries, cache, selected, page_table, starts, lengths, *, scale,
+                      max_new: int, mask="causal", out_dtype=None, out=None):
+    """paged_quantized_sdpa over selected pages: row t sees, of the tokens that it
+    sees there, those of the pages selected[t,h] for KV head h: selected [T,Hkv,count]
+    int32, places in its sequence's row of page_table, as select_top returns them.
+    Places outside the row (-1), and pages that are absent or that t does not see,
+    count for nothing, and a page that is named twice counts twice. Weights times
+    value scales are held in 22 bits; scores, normalizer and sums are fp32."""
+    op = "paged_sparse_sdpa"
+    kc, ks, vc, vs, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
+    _check_attention(op, queries, hkv, d, index, mask, scale, max_new)
+    t, heads, _ = shape = queries.shape
+    out_dtype = _out_dtype(queries, out_dtype)
+    if not isinstance(selected, _T) or selected.ndim != 3 or not selected.shape[2]:
+        raise ValueError(f"{op}: selected must be an int32 tensor [T,Hkv,count]")
+    count = selected.shape[2]
+    _check_ints(op, index, "selected", selected, (t, hkv, count))
+    b, width = _check_batch(op, index, page_table, starts, lengths)
+    strides = _strides(op, kc, ks, vc, vs)
+    _need_gpu(op, index)
+    queries, qst = _rows16(queries)
+    out = torch.empty_like(queries, dtype=out_dtype, memory_format=_CONTIGUOUS) if out is None \
+        else _out_buffer(out, shape, out_dtype, kc.device)
+    need = _lib.lib().sparkq_paged_sparse_workspace_bytes(t, heads, hkv, d, count, page)
+    ws = kc.new_empty(need) if need else None  # (int8: bytes)
+    _lib.launch("sparkq_paged_sparse_sdpa", index, queries.data_ptr(), kc.data_ptr(),
+                ks.data_ptr(), vc.data_ptr(), vs.data_ptr(), selected.data_ptr(),
+                page_table.data_ptr(), starts.data_ptr(), lengths.data_ptr(), out.data_ptr(), t, b,
+                heads, hkv, d, count, pages, width, page_table.stride(0), page, max_new,
+                1 if mask is not None else 0, _CODE[queries.dtype], _CODE[out_dtype], scale,
+                _I64x2(qst[0], qst[1]), _I64x2(selected.stride(0), selected.stride(1)), strides,
+                _ptr(ws), need)
+    return out
+
+
+def _check_mass(op, mass, index, shape):
+    if not isinstance(mass, _T) or mass.dtype is not torch.float32 or mass.shape != shape:
+        raise ValueError(f"{op}: mass must be a float32 tensor of shape {list(shape)}")
+    if mass.get_device() != index:
+        raise ValueError(f"{op}: mass must live on the cache's device")
+    if mass.stride(-1) != 1:
+        raise ValueError(f"{op}: the last axis of mass must be contiguous")
+
+
+def paged_kv_mass(queries, lse, cache, mass, page_table, starts, lengths, *, scale, max_new: int,
+                  mask="causal"):
+    """The attention weight that each cached token gathers, in place: mass
+    [B,Hkv,M*page_size] float32 grows by the sum of
+
+        exp(scale * q[t,g] . k - lse[t,g])
+
+    over a sequence's new tokens t that see the token and the query heads g of the KV
+    head, with queries, cache, scale and mask of the attention and the lse [T,Hq]
+    that paged_quantized_sdpa(return_lse=True) returned for them. A batch's new tokens
+    start from 0, whatever mass holds there. Sums are fp32, in one order. max_new is
+    the most new tokens that a sequence has; those of one past it add nothing."""
+    op = "paged_kv_mass"
+    kc, ks, _, _, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
+    _check_attention(op, queries, hkv, d, index, mask, scale, max_new)
+    t, heads, _ = queries.shape
+    if not isinstance(lse, _T) or lse.dtype is not torch.float32 or lse.shape != (t, heads):
+        raise ValueError(f"{op}: lse must be a float32 tensor of shape {[t, heads]}")
+    if lse.get_device() != index:
+        raise ValueError(f"{op}: lse must live on the cache's device")
+    b, width = _check_batch(op, index, page_table, starts, lengths)
+    _check_mass(op, mass, index, (b, hkv, width * page))
+    strides = _key_strides(op, kc, ks)
+    _need_gpu(op, index)
+    queries, qst = _rows16(queries)
+    lse = lse.contiguous()
+    _lib.launch("sparkq_paged_kv_mass", index, queries.data_ptr(), lse.data_ptr(), kc.data_ptr(),
+                ks.data_ptr(), mass.data_ptr(), page_table.data_ptr(), starts.data_ptr(),
+                lengths.data_ptr(), t, b, heads, hkv, d, pages, width, page_table.stride(0), page,
+                max_new, 1 if mask is not None else 0, _CODE[queries.dtype], scale,
+                _I64x2(qst[0], qst[1]), _I64x2(mass.stride(0), mass.stride(1)), strides)
 
 
 def _pool(op, cache):
@@ -282,6 +491,49 @@ def kv_pages_compact(cache, page_table, lengths):
                 page_table.stride(0), table.data_ptr(), used.data_ptr(), st, b, width, pages,
                 layers, page, cb, sb, ws.data_ptr(), need)
     return table, used
+
+
+def kv_pages_evict(cache, keep, page_table, lengths, *, mass=None):
+    """Sequences of more than `count` tokens keep `count` of them: those that keep
+    [layers,B,Hkv,count] int32 (of one layer's cache [B,Hkv,count]) lists in ascending
+    order for each layer and KV head, as select_top(mass, count, lengths=lengths)
+    returns them. They move to the front of the sequence's pages, in their order, and
+    their mass ([layers,B,Hkv,M*page_size] float32) with them. Returns (page_table
+    [B,M], lengths [B], missing [1]).
+
+    Shorter sequences stay as they are. A page that is written and that another
+    sequence holds too is replaced by a free one, in ascending order to the sequences
+    in order, as kv_pages_fork deals them; the rest are written in place. `missing`
+    counts the pages that the pool was short of; when it is not 0 nothing was moved,
+    and table and lengths are the old ones. An entry i of keep that is below i, or not
+    below the length, stands for token i. Positions of tokens in a cache are then no
+    longer those of the text, which matters to who rotates later tokens (keys are
+    rotated before they are appended), and bounds of written pages have to be taken
+    again."""
+    op = "kv_pages_evict"
+    bufs, index, layers, pages, page, cb, _, st = _pool(op, cache)
+    hkv, d = cache[0].shape[-3], cache[0].shape[-1]
+    b, width = _check_rows(op, index, page_table, lengths)
+    lead = (layers,) if cache[0].ndim == 5 else ()
+    if not isinstance(keep, _T) or not keep.ndim or not keep.shape[-1]:
+        raise ValueError(f"{op}: keep must be an int32 tensor {[*lead, b, hkv]} + [count]")
+    count = keep.shape[-1]
+    _check_ints(op, index, "keep", keep, (*lead, b, hkv, count))
+    mst = None
+    if mass is not None:
+        _check_mass(op, mass, index, (*lead, b, hkv, width * page))
+        mst = _I64x3(*(mass.stride() if lead else (0, *mass.stride()))[:3])
+    _need_gpu(op, index)
+    keep = keep.contiguous()
+    table = torch.empty_like(page_table, memory_format=_CONTIGUOUS)
+    after, missing = torch.empty_like(lengths), lengths.new_empty(1)
+    need = _lib.lib().sparkq_kv_pages_workspace_bytes(b, pages)
+    ws = cache[0].new_empty(need)  # (int8: bytes)
+    _lib.launch("sparkq_kv_pages_evict", index, *bufs, keep.data_ptr(), _ptr(mass),
+                page_table.data_ptr(), lengths.data_ptr(), page_table.stride(0), table.data_ptr(),
+                after.data_ptr(), missing.data_ptr(), st, mst, b, hkv, d, count, width, pages,
+                layers, page, ws.data_ptr(), need)
+    return table, after, missing
 
 
 class PagedKVCache:
