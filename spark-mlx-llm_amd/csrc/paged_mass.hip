@@ -156,12 +156,14 @@ __global__ __launch_bounds__(256) void paged_mass_few_kernel(MassArgs s) {
 // ---------------------------------------------------------------------------
 // more rows
 // ---------------------------------------------------------------------------
-// A workgroup has 64 tokens (32 at D = 256) of one KV head, whose keys stay in its waves' registers
-// as the first operand of the 32 x 32 products; the waves take turns at tiles of 32
-// rows, whose queries come straight from memory in the operand's layout, the next
-// tile's in flight. A lane has one row's scores of half the tokens and sums its
-// rows' weights in registers; lanes and waves are joined at the end through LDS.
-// Codes are exact in either 16-bit type, so queries stay as they are.
+// A wave has 32 tokens of one KV head, their codes in registers as the first operand
+// of the 32 x 32 products. The workgroup goes over the rows that see its tokens, kRows
+// at a time: it brings their queries into LDS, the next ones' loads in flight, and a
+// wave takes tiles of 32 of them as second operands. A lane then has one row's scores of 16
+// tokens, and sums its rows' weights in registers; lanes (and waves) are joined at the
+// end through LDS. Codes are exact in either 16-bit type, so queries stay as they are.
+// WAYS waves share 32 tokens and take turns at the tiles: four where the chip would
+// otherwise have less than a workgroup a CU, else one.
 template <typename T>
 __device__ __forceinline__ u32x4_t codes_as(uint32_t lo, uint32_t hi);
 template <>
@@ -176,9 +178,6 @@ __device__ __forceinline__ u32x4_t codes_as<BF16>(uint32_t lo, uint32_t hi) {
   return u32x4_t{pair(lo, 0), pair(lo, 2), pair(hi, 0), pair(hi, 2)};
 }
 
-// tokens of a workgroup: what the registers hold
-constexpr int mass_tokens(int D) { return D <= 128 ? 64 : 32; }
-
 // The block of `size` tokens that is number x of the batch's sequences with new tokens
 struct TokenBlock {
   int b, t0;
@@ -189,18 +188,18 @@ __device__ __forceinline__ TokenBlock find_block(const PagedBatch& p, int size, 
   TokenBlock r{-1, 0, {0, 0, 0}};
   int before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    int n = 0;
-    if (b0 + lane < p.B) {
-      const SeqRows s = seq_rows(p, b0 + lane);
-      n = s.count > 0 ? (s.length + size - 1) / size : 0;
-    }
+    SeqRows s{0, 0, 0};
+    if (b0 + lane < p.B) s = seq_rows(p, b0 + lane);
+    const int n = s.count > 0 ? (s.length + size - 1) / size : 0;
     const int end = before + wave_prefix(n);
     const unsigned long long hit = __ballot(x < end);
     if (hit) {
       const int l = __builtin_ctzll(hit);
       r.b = b0 + l;
       r.t0 = size * (x - __builtin_amdgcn_readlane(end - n, l));
-      r.s = seq_rows(p, r.b);
+      r.s.first = __builtin_amdgcn_readlane(s.first, l);
+      r.s.count = __builtin_amdgcn_readlane(s.count, l);
+      r.s.length = __builtin_amdgcn_readlane(s.length, l);
       break;
     }
     before = __builtin_amdgcn_readlane(end, 63);
@@ -209,15 +208,37 @@ __device__ __forceinline__ TokenBlock find_block(const PagedBatch& p, int size, 
   return r;
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void paged_mass_many_kernel(MassArgs s, int blocks) {
-  constexpr int NK = D / 16, N = mass_tokens(D), H = N / 32;
+constexpr int mass_tokens(int ways) { return 128 / ways; }  // of a workgroup
+
+template <int D, int WAYS>
+struct MassShape {
+  static constexpr int ROWS = 32 * (WAYS == 1 ? 2 : WAYS);  // queries in LDS at a time
+  static constexpr int QROW = 2 * D + 16;                   // any 16 lanes' reads hit different banks
+  static constexpr int BUF = ROWS * QROW;
+  static constexpr int JOIN = 4 * 32 * 33 * 4;
+  static constexpr int BYTES = 2 * BUF > JOIN ? 2 * BUF : JOIN;
+};
+
+// rr / gqa with inv = 1 / gqa, for quotients up to 2^22
+__device__ __forceinline__ int row_of(int rr, int gqa, float inv) {
+  const int t = (int)((float)rr * inv), r = rr - t * gqa;
+  return t + (r >= gqa) - (r < 0);
+}
+
+template <typename T, int D, int WAYS>
+__global__ __launch_bounds__(256, D == 256 && WAYS == 4 ? 1 : 2) void paged_mass_many_kernel(MassArgs s, int blocks) {
+  using S = MassShape<D, WAYS>;
+  constexpr int NK = D / 16, N = mass_tokens(WAYS), kRows = S::ROWS;
+  constexpr int PPR = D / 8, PPT = kRows * PPR / 256;  // 16-byte pieces of a row, of a thread
   const PagedSdpaArgs& a = s.a;
-  __shared__ float s_sum[4][N][33];
+  __shared__ __attribute__((aligned(16))) unsigned char smem[S::BYTES];
+  __shared__ float s_base[2][kRows];
+  __shared__ int s_lim[2][kRows];
   __shared__ __attribute__((aligned(16))) float s_scale[N];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 31, grp = lane >> 5;
+  const int col = lane & 31, grp = lane >> 5, group = wave / WAYS, way = wave % WAYS;
   const int gqa = a.Hq / a.Hkv, kh = blockIdx.x % a.Hkv;
+  const float inv = 1.0f / (float)gqa;
   for (int x = blockIdx.x / a.Hkv; x < blocks; x += gridDim.x / a.Hkv) {
     const TokenBlock tb = find_block(a.p, N, x);
     if (tb.b < 0) return;
@@ -226,97 +247,112 @@ __global__ __launch_bounds__(256, 2) void paged_mass_many_kernel(MassArgs s, int
     const int skip = a.causal ? max(t0 - (tb.s.length - tb.s.count), 0) : 0;
     const int row0 = (int)min((int64_t)skip * gqa, (int64_t)rows) & ~31;
 
-    u32x4_t kf[H][NK];
-    uint64_t present[H];  // tokens that have a page (a bit a lane)
-#pragma unroll
-    for (int h = 0; h < H; ++h) {
-      const int pos = t0 + 32 * h + col;
-      const int id = pos < tb.s.length ? page_of(a.p, tb.b, pos) : -1;
-      present[h] = __ballot(id >= 0);
+    u32x4_t kf[NK];
+    const int w0 = t0 + 32 * group, pos = w0 + col;
+    const int id = pos < tb.s.length ? page_of(a.p, tb.b, pos) : -1;
+    const uint64_t present = __ballot(id >= 0);  // tokens that have a page
+    {
       const int at = max(id, 0), slot = pos & ((1 << a.p.page_log2) - 1);
       const uint8_t* kp = a.c.k + kh * a.c.c_head + code_at(a.c, at, slot) + 8 * grp;
 #pragma unroll
       for (int k = 0; k < NK; ++k) {
         const uint2 w = *reinterpret_cast<const uint2*>(kp + 16 * k);
-        kf[h][k] = codes_as<T>(w.x, w.y);
+        kf[k] = codes_as<T>(w.x, w.y);
       }
-      if (wave == 0 && grp == 0)
-        s_scale[32 * h + col] = f16_to_f32(a.c.ks[kh * a.c.s_head + scale_at(a.c, at, slot)]) * s.scale;
+      if (way == 0 && grp == 0)
+        s_scale[32 * group + col] = f16_to_f32(a.c.ks[kh * a.c.s_head + scale_at(a.c, at, slot)]) * s.scale;
     }
-    __syncthreads();
-    float sum[H][16];
-#pragma unroll
-    for (int h = 0; h < H; ++h)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) sum[h][v] = 0.0f;
 
-    auto place = [&](int r0, int64_t& t, int& head) {
-      const int rr = min(r0 + col, rows - 1), i = rr / gqa;
-      t = tb.s.first + i;
-      head = kh * gqa + rr - i * gqa;
-    };
-    u32x4_t qn[NK];
-    float base_n;
+    // Piece i of a round of rows: row tid / PPR + i TPP, values 8 (tid % PPR) ..; a
+    // row's first piece brings its logarithm and what it sees.
+    constexpr int TPP = 256 / PPR;
+    u32x4_t qr[PPT];
+    float base_r;
+    int lim_r;
     auto load = [&](int r0) {
-      int64_t t;
-      int head;
-      place(r0, t, head);
-      const uint16_t* q = a.q + t * a.q_tok + head * a.q_head + 8 * grp;
 #pragma unroll
-      for (int k = 0; k < NK; ++k) qn[k] = *reinterpret_cast<const u32x4_t*>(q + 16 * k);
-      base_n = s.lse[t * a.Hq + head];
+      for (int i = 0; i < PPT; ++i) {
+        const int rr = min(r0 + tid / PPR + i * TPP, rows - 1), t = row_of(rr, gqa, inv);
+        qr[i] = *reinterpret_cast<const u32x4_t*>(a.q + (tb.s.first + t) * a.q_tok + (kh * gqa + rr - t * gqa) * a.q_head +
+                                                  8 * (tid % PPR));
+      }
+      if (tid < kRows) {
+        const int rr = min(r0 + tid, rows - 1), t = row_of(rr, gqa, inv);
+        base_r = row_base(s.lse[(int64_t)(tb.s.first + t) * a.Hq + kh * gqa + rr - t * gqa]);
+        lim_r = r0 + tid < rows ? last_seen_by(tb.s, t, a.causal) : -1;
+      }
     };
-    int r0 = row0 + 32 * wave;
-    if (r0 < rows) load(r0);
-    for (; r0 < rows; r0 += 128) {
-      u32x4_t q[NK];
+    auto stage = [&](int buf) {
 #pragma unroll
-      for (int k = 0; k < NK; ++k) q[k] = qn[k];
-      const float base = row_base(base_n);
-      if (r0 + 128 < rows) load(r0 + 128);
-      // what the tile's first row sees
-      const int least = last_seen_by(tb.s, r0 / gqa, a.causal);
-      const bool whole = least >= t0 + N - 1 && r0 + 32 <= rows;
-      const int lim = whole || r0 + col >= rows ? -1 : last_seen_by(tb.s, (r0 + col) / gqa, a.causal);
+      for (int i = 0; i < PPT; ++i)
+        *reinterpret_cast<u32x4_t*>(smem + buf * S::BUF + (tid / PPR + i * TPP) * S::QROW + 16 * (tid % PPR)) = qr[i];
+      if (tid < kRows) {
+        s_base[buf][tid] = base_r;
+        s_lim[buf][tid] = lim_r;
+      }
+    };
+    float sum[16];
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        f32x16_t sc = f32x16_t{};
+    for (int v = 0; v < 16; ++v) sum[v] = 0.0f;
+    auto tile = [&](int buf, int r) {  // rows r .. r + 31 of a buffer
+      const unsigned char* q = smem + buf * S::BUF + (r + col) * S::QROW + 16 * grp;
+      f32x16_t sc = f32x16_t{};
 #pragma unroll
-        for (int k = 0; k < NK; ++k) sc = mfma32x32x16<T>(kf[h][k], q[k], sc);
-        float e[16];
+      for (int k = 0; k < NK; ++k) sc = mfma32x32x16<T>(kf[k], *reinterpret_cast<const u32x4_t*>(q + 32 * k), sc);
+      const float base = s_base[buf][r + col];
+      const int lim = s_lim[buf][r + col];
+      float e[16];
 #pragma unroll
-        for (int v = 0; v < 16; v += 4) {
-          const f32x4_t k4 = *reinterpret_cast<const f32x4_t*>(s_scale + 32 * h + 2 * v + 4 * grp);
+      for (int v = 0; v < 16; v += 4) {
+        const f32x4_t k4 = *reinterpret_cast<const f32x4_t*>(s_scale + 32 * group + 2 * v + 4 * grp);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) e[v + r] = __builtin_amdgcn_exp2f(fmaf(sc[v + r], k4[r], -base));
-        }
-        if (__builtin_expect(!whole, 0)) {
+        for (int i = 0; i < 4; ++i) e[v + i] = __builtin_amdgcn_exp2f(fmaf(sc[v + i], k4[i], -base));
+      }
+      if (__builtin_expect(__ballot(lim < w0 + 31) != 0, 0)) {
 #pragma unroll
-          for (int v = 0; v < 16; ++v) e[v] = t0 + 32 * h + mfma32_row(lane, v) <= lim ? e[v] : 0.0f;
-        }
+        for (int v = 0; v < 16; ++v) e[v] = w0 + mfma32_row(lane, v) <= lim ? e[v] : 0.0f;
+      }
 #pragma unroll
-        for (int v = 0; v < 16; ++v) sum[h][v] += e[v];
+      for (int v = 0; v < 16; ++v) sum[v] += e[v];
+    };
+    auto round = [&](int buf) {
+      if constexpr (WAYS == 1) {
+        tile(buf, 0);
+        tile(buf, 32);
+      } else {
+        tile(buf, 32 * way);
+      }
+    };
+    if (row0 < rows) {
+      load(row0);
+      stage(0);
+      load(row0 + kRows);
+      __syncthreads();
+      for (int r0 = row0, buf = 0; r0 < rows; r0 += kRows, buf ^= 1) {
+        round(buf);
+        stage(buf ^ 1);
+        load(r0 + 2 * kRows);
+        __syncthreads();
       }
     }
+    float(*join)[32][33] = reinterpret_cast<float(*)[32][33]>(smem);
 #pragma unroll
-    for (int h = 0; h < H; ++h)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) s_sum[wave][32 * h + mfma32_row(lane, v)][col] = sum[h][v];
+    for (int v = 0; v < 16; ++v) join[wave][mfma32_row(lane, v)][col] = sum[v];
     __syncthreads();
-    // four threads a token, a wave's sums each
-    const int tok = tid >> 2;
-    if (tok < N) {
-      float v = 0.0f;
+    // 256 / N threads a token: half of a wave's sums each
+    const int tok = tid / (256 / N), h = tid % (256 / N);
+    float v = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v += s_sum[tid & 3][tok][i];
-      v += dpp_row<0xB1>(v);
+    for (int i = 0; i < 16; ++i) v += join[tok / 32 * WAYS + h / 2][tok % 32][16 * (h & 1) + i];
+    v += dpp_row<0xB1>(v);
+    if (WAYS == 4) {
       v += dpp_row<0x4E>(v);
-      if ((tid & 3) == 0 && t0 + tok < tb.s.length) {
-        float* m = s.mass + tb.b * s.m_row + kh * s.m_head + t0 + tok;
-        uint64_t have = present[0];
-        if (H == 2 && tok >= 32) have = present[H - 1];
-        *m = (t0 + tok < tb.s.length - tb.s.count ? *m : 0.0f) + ((have >> (tok & 31)) & 1 ? v : 0.0f);
-      }
+      v += dpp_row<0x141>(v);
+    }
+    if (h == 0 && t0 + tok < tb.s.length) {
+      float* m = s.mass + tb.b * s.m_row + kh * s.m_head + t0 + tok;
+      const bool in = WAYS == 4 ? (present >> (tok & 31)) & 1 : page_of(a.p, tb.b, t0 + tok) >= 0;
+      *m = (t0 + tok < tb.s.length - tb.s.count ? *m : 0.0f) + (in ? v : 0.0f);
     }
     __syncthreads();
   }
@@ -327,8 +363,12 @@ void launch_few(const MassArgs& s, int64_t items, hipStream_t st) {
   hipLaunchKernelGGL(paged_mass_few_kernel<D>, dim3((unsigned)(items * s.a.Hkv)), dim3(256), 0, st, s);
 }
 template <typename T, int D>
-void launch_many(const MassArgs& s, int64_t items, int64_t blocks, hipStream_t st) {
-  hipLaunchKernelGGL((paged_mass_many_kernel<T, D>), dim3((unsigned)(items * s.a.Hkv)), dim3(256), 0, st, s, (int)blocks);
+void launch_many(const MassArgs& s, bool share, int64_t items, int64_t blocks, hipStream_t st) {
+  const dim3 grid((unsigned)(items * s.a.Hkv));
+  if (share)
+    hipLaunchKernelGGL((paged_mass_many_kernel<T, D, 4>), grid, dim3(256), 0, st, s, (int)blocks);
+  else
+    hipLaunchKernelGGL((paged_mass_many_kernel<T, D, 1>), grid, dim3(256), 0, st, s, (int)blocks);
 }
 
 }  // namespace
@@ -375,18 +415,19 @@ int paged_kv_mass(const PagedBatch& p, const void* q, const int64_t* qst, const 
       launch_few<256>(s, items, st);
     return check_launch("paged_mass_few_kernel");
   }
-  const int64_t blocks = p.B * cdiv(max_tokens, mass_tokens((int)D));
+  const bool share = p.B * cdiv(max_tokens, mass_tokens(1)) * Hkv < 2 * device_cus();
+  const int64_t blocks = p.B * cdiv(max_tokens, mass_tokens(share ? 4 : 1));
   if (blocks > 0x7FFFFFFF) return set_error(SPARKQ_ERR_INVALID, "paged_kv_mass: shape too large");
-  // no more workgroups than the chip holds eight times over; they take further blocks
+  // no more workgroups than the chip holds a few times over; they take further blocks
   const int64_t items = std::min(blocks, cdiv(16 * device_cus(), Hkv));
   auto go = [&](auto t) {
     using T = decltype(t);
     if (D == 64)
-      launch_many<T, 64>(s, items, blocks, st);
+      launch_many<T, 64>(s, share, items, blocks, st);
     else if (D == 128)
-      launch_many<T, 128>(s, items, blocks, st);
+      launch_many<T, 128>(s, share, items, blocks, st);
     else
-      launch_many<T, 256>(s, items, blocks, st);
+      launch_many<T, 256>(s, share, items, blocks, st);
   };
   if (qdt == SPARKQ_BF16)
     go(BF16{});

@@ -135,81 +135,82 @@ struct ScoreArgs {
   uint32_t flip;   // bits that give a packed pair the scale's sign
 };
 
-__device__ __forceinline__ f32x4_t mfma16x16x32_bf16(u32x4_t x, u32x4_t y, f32x4_t c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c,
-                                                 0, 0, 0);
-}
-
-// A packed pair of query values as bf16 operands: parts of the positive ones for
-// the upper bounds, of the negative ones for the lower. A bf16 value is its own
-// part; one of fp16 is the sum of two of its sign, of 8 and of up to 3 bits.
 template <typename T>
-struct Parts {
-  static constexpr int N = T::code == SPARKQ_BF16 ? 1 : 2;
+__device__ __forceinline__ f32x4_t mfma16(u32x4_t x, u32x4_t y, f32x4_t c) {
+  if constexpr (T::code == SPARKQ_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c,
+                                                   0, 0, 0);
+  else
+    return mfma16x16x32_f16(x, y, c);
+}
+
+// A lane's share of the bounds of a page: dims 32 c + 8 grp .. + 8, and what the
+// scores have to be multiplied by. For fp16 queries the bounds are turned to fp16,
+// shifted by a power of two for that: exact but for what bf16 holds below 2^-28 of
+// the page's largest, which is rounded.
+template <typename T, int D>
+struct PageOperand {
+  u32x4_t lo[D / 32], hi[D / 32];
+  float mul;
 };
-template <typename T>
-__device__ __forceinline__ void query_parts(uint32_t q, uint32_t hi[Parts<T>::N], uint32_t lo[Parts<T>::N]) {
-  const s16x2_t v = __builtin_bit_cast(s16x2_t, q), zero = {0, 0};
-  if constexpr (T::code == SPARKQ_BF16) {  // (their bits sort as whole numbers do)
-    hi[0] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(v, zero));
-    lo[0] = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(v, zero));
-  } else {
-    const uint32_t pos = __builtin_bit_cast(uint32_t, v > zero) & q, neg = __builtin_bit_cast(uint32_t, v < zero) & q;
-    auto split = [](uint32_t w, uint32_t& first, uint32_t& rest) {
-      const float x = lo16<F16>(w), y = hi16<F16>(w);
-      first = __float_as_uint(x) >> 16 | (__float_as_uint(y) & 0xFFFF0000u);  // cut: the rest has its sign
-      const float rx = x - lo16<BF16>(first), ry = y - hi16<BF16>(first);
-      rest = pack_round<BF16>(rx == rx ? rx : 0.0f, ry == ry ? ry : 0.0f);  // (of an infinite one nothing)
-    };
-    split(pos, hi[0], hi[1]);
-    split(neg, lo[0], lo[1]);
-  }
-}
-
 template <typename T, int D>
-struct QueryOperand {
-  u32x4_t hi[D / 32][Parts<T>::N], lo[D / 32][Parts<T>::N];
-};
-// dims 32 c + 8 grp .. + 8 of a row, or nothing
-template <typename T, int D>
-__device__ __forceinline__ void split_query(const u32x4_t (&raw)[D / 32], bool live, uint32_t flip,
-                                            QueryOperand<T, D>& q) {
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t hi[Parts<T>::N], lo[Parts<T>::N];
-      query_parts<T>(live ? raw[c][i] ^ flip : 0, hi, lo);
-#pragma unroll
-      for (int k = 0; k < Parts<T>::N; ++k) {
-        q.hi[c][k][i] = hi[k];
-        q.lo[c][k][i] = lo[k];
-      }
-    }
-}
-
-// scores of 16 pages (4 grp + r in a lane's result) for the operand's 16 rows
-template <typename T, int D>
-__device__ __forceinline__ f32x4_t page_scores(const u32x4_t (&lo)[D / 32], const u32x4_t (&hi)[D / 32],
-                                               const QueryOperand<T, D>& q) {
-  f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int c = 0; c < D / 32; ++c)
-#pragma unroll
-    for (int k = 0; k < Parts<T>::N; ++k) {
-      s = mfma16x16x32_bf16(lo[c], q.lo[c][k], s);
-      s = mfma16x16x32_bf16(hi[c], q.hi[c][k], s);
-    }
-  return s;
-}
-
-template <int D>
-__device__ __forceinline__ void load_bounds(const uint16_t* at, u32x4_t (&lo)[D / 32], u32x4_t (&hi)[D / 32]) {
+__device__ __forceinline__ void load_bounds(const uint16_t* at, PageOperand<T, D>& b) {
 #pragma unroll
   for (int c = 0; c < D / 32; ++c) {
-    lo[c] = *reinterpret_cast<const u32x4_t*>(at + 32 * c);
-    hi[c] = *reinterpret_cast<const u32x4_t*>(at + D + 32 * c);
+    b.lo[c] = *reinterpret_cast<const u32x4_t*>(at + 32 * c);
+    b.hi[c] = *reinterpret_cast<const u32x4_t*>(at + D + 32 * c);
   }
+}
+template <typename T, int D>
+__device__ __forceinline__ void turn_bounds(PageOperand<T, D>& b) {
+  b.mul = 1.0f;
+  if constexpr (T::code == SPARKQ_F16) {
+    typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+    u16x2_t most = {0, 0};
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, b.lo[c][i] & 0x7FFF7FFFu));
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, b.hi[c][i] & 0x7FFF7FFFu));
+      }
+    uint32_t top = max((uint32_t)most[0], (uint32_t)most[1]);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    // 2^e <= the largest < 2^(e + 1); 0, and infinities, stay as they are
+    const int e = (int)(top >> 7) - 127, shift = top >= 0x80u && top < 0x7F80u ? 14 - e : 0;
+    auto turn = [&](uint32_t w) {
+      return (uint32_t)f32_to_f16(ldexpf(lo16<BF16>(w), shift)) | (uint32_t)f32_to_f16(ldexpf(hi16<BF16>(w), shift)) << 16;
+    };
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        b.lo[c][i] = turn(b.lo[c][i]);
+        b.hi[c][i] = turn(b.hi[c][i]);
+      }
+    b.mul = ldexpf(1.0f, -shift);
+  }
+}
+
+// scores of 16 pages (4 grp + r in a lane's result) for 16 rows of query values, raw
+template <typename T, int D>
+__device__ __forceinline__ f32x4_t page_scores(const PageOperand<T, D>& b, const u32x4_t (&raw)[D / 32],
+                                               uint32_t flip) {
+  f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) {
+    u32x4_t pos, neg;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // (16-bit floats' bits have the sign of whole numbers)
+      const s16x2_t v = __builtin_bit_cast(s16x2_t, raw[c][i] ^ flip), zero = {0, 0};
+      pos[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(v, zero));
+      neg[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(v, zero));
+    }
+    s = mfma16<T>(b.lo[c], neg, s);
+    s = mfma16<T>(b.hi[c], pos, s);
+  }
+  return s;
 }
 
 // One new token a sequence: a group's query heads are the product's 16 columns, and
@@ -223,37 +224,44 @@ __global__ __launch_bounds__(256) void paged_scores_one_kernel(ScoreArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kh = blockIdx.x % a.Hkv, x = blockIdx.x / a.Hkv, b = x / a.chunks, chunk = x - b * a.chunks;
   const int gqa = a.Hq / a.Hkv;
+  const int j0 = chunk * kOnePages + 16 * wave;
+  // (asked for before the lengths are known, which say whether it is a page)
+  int id[kOneTiles];
+#pragma unroll
+  for (int i = 0; i < kOneTiles; ++i) id[i] = a.p.table[b * a.p.table_stride + min(j0 + 64 * i + n16, a.p.width - 1)];
   const SeqRows s = seq_rows(a.p, b);
   if (s.count == 0) return;
   const int t = s.first, lim = last_seen_by(s, 0, a.causal);
   const int pages = lim < 0 ? 0 : (lim >> a.p.page_log2) + 1;
   if (kh == 0 && chunk == 0 && tid == 0) a.seen[t] = pages;
   float* out = a.scores + ((int64_t)t * a.Hkv + kh) * a.p.width;
-  const int j0 = chunk * kOnePages + 16 * wave;
-  u32x4_t lo[kOneTiles][NK], hi[kOneTiles][NK];
+  if (j0 >= pages) {  // (a wave's tiles lie 64 pages apart)
+#pragma unroll
+    for (int i = 0; i < kOneTiles; ++i)
+      if (grp == 0 && j0 + 64 * i + n16 < a.p.width) out[j0 + 64 * i + n16] = kNegInf;
+    return;
+  }
+  PageOperand<T, D> page[kOneTiles];
   uint64_t present[kOneTiles];
 #pragma unroll
   for (int i = 0; i < kOneTiles; ++i) {
-    const int j = j0 + 64 * i + n16;
-    int id = j < pages ? a.p.table[b * a.p.table_stride + j] : -1;
-    const bool in = (unsigned)id < (unsigned)a.p.pages;
+    const bool in = j0 + 64 * i + n16 < pages && (unsigned)id[i] < (unsigned)a.p.pages;
     present[i] = __ballot(in);
-    load_bounds<D>(a.bounds + (in ? id : 0) * a.b_page + kh * a.b_head + 8 * grp, lo[i], hi[i]);
+    load_bounds<T, D>(a.bounds + (in ? id[i] : 0) * a.b_page + kh * a.b_head + 8 * grp, page[i]);
   }
   f32x4_t most[kOneTiles];
 #pragma unroll
   for (int i = 0; i < kOneTiles; ++i) most[i] = f32x4_t{kNegInf, kNegInf, kNegInf, kNegInf};
   for (int g0 = 0; g0 < gqa; g0 += 16) {
-    const int g = min(g0 + n16, gqa - 1);
+    const int g = min(g0 + n16, gqa - 1);  // (the last head again for what is past it)
     const uint16_t* row = a.q + t * a.q_tok + (kh * gqa + g) * a.q_head + 8 * grp;
     u32x4_t raw[NK];
 #pragma unroll
     for (int c = 0; c < NK; ++c) raw[c] = *reinterpret_cast<const u32x4_t*>(row + 32 * c);
-    QueryOperand<T, D> q;
-    split_query<T, D>(raw, true, a.flip, q);  // (the last head again for what is past it)
 #pragma unroll
     for (int i = 0; i < kOneTiles; ++i) {
-      const f32x4_t v = page_scores<T, D>(lo[i], hi[i], q);
+      if (g0 == 0) turn_bounds<T, D>(page[i]);
+      const f32x4_t v = page_scores<T, D>(page[i], raw, a.flip);
 #pragma unroll
       for (int r = 0; r < 4; ++r) most[i][r] = fmaxf(most[i][r], v[r]);
     }
@@ -263,10 +271,11 @@ __global__ __launch_bounds__(256) void paged_scores_one_kernel(ScoreArgs a) {
     float v[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = max_row16(most[i][r]);
-    const int j = j0 + 64 * i + 4 * grp + n16;  // lane n16 < 4 of a group stores score n16
+    const int k = 4 * grp + n16, j = j0 + 64 * i + k;  // lane n16 < 4 of a group stores score n16
+    const float mul = __shfl(page[i].mul, k & 63) * a.scale;
     if (n16 < 4 && j < a.p.width) {
       const float m = n16 == 0 ? v[0] : n16 == 1 ? v[1] : n16 == 2 ? v[2] : v[3];
-      out[j] = ((present[i] >> (4 * grp + n16)) & 1) && m != kNegInf ? m * a.scale : kNegInf;
+      out[j] = ((present[i] >> k) & 1) && m != kNegInf ? m * mul : kNegInf;
     }
   }
 }
@@ -327,34 +336,43 @@ __global__ __launch_bounds__(256) void paged_scores_many_kernel(ScoreArgs a) {
   f32x4_t most[TILES];
 #pragma unroll
   for (int i = 0; i < TILES; ++i) most[i] = f32x4_t{kNegInf, kNegInf, kNegInf, kNegInf};
+  float mul[TILES][4] = {};
   uint64_t present[TILES] = {0, 0};
   if (j0 < most_pages) {
-    u32x4_t lo[TILES][NK], hi[TILES][NK];
+    PageOperand<T, D> page[TILES];
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       const int j = j0 + 16 * i + n16;
       const int id = j < most_pages ? a.p.table[tt.b * a.p.table_stride + j] : -1;
       const bool in = (unsigned)id < (unsigned)a.p.pages;
       present[i] = __ballot(in);
-      load_bounds<D>(a.bounds + (in ? id : 0) * a.b_page + kh * a.b_head + 8 * grp, lo[i], hi[i]);
+      load_bounds<T, D>(a.bounds + (in ? id : 0) * a.b_page + kh * a.b_head + 8 * grp, page[i]);
     }
     const uint16_t* row = a.q + t * a.q_tok + kh * gqa * a.q_head + 8 * grp;
-    u32x4_t raw[NK];
+    u32x4_t next[NK];
+    auto load = [&](int g) {
 #pragma unroll
-    for (int c = 0; c < NK; ++c) raw[c] = *reinterpret_cast<const u32x4_t*>(row + 32 * c);
+      for (int c = 0; c < NK; ++c) next[c] = *reinterpret_cast<const u32x4_t*>(row + g * a.q_head + 32 * c);
+    };
+    load(0);
+#pragma unroll
+    for (int i = 0; i < TILES; ++i) turn_bounds<T, D>(page[i]);
     for (int g = 0; g < gqa; ++g) {
-      QueryOperand<T, D> q;
-      split_query<T, D>(raw, true, a.flip, q);
-      row += g + 1 < gqa ? a.q_head : 0;
+      u32x4_t raw[NK];
 #pragma unroll
-      for (int c = 0; c < NK; ++c) raw[c] = *reinterpret_cast<const u32x4_t*>(row + 32 * c);
+      for (int c = 0; c < NK; ++c) raw[c] = next[c];
+      load(min(g + 1, gqa - 1));
 #pragma unroll
       for (int i = 0; i < TILES; ++i) {
-        const f32x4_t v = page_scores<T, D>(lo[i], hi[i], q);
+        const f32x4_t v = page_scores<T, D>(page[i], raw, a.flip);
 #pragma unroll
         for (int r = 0; r < 4; ++r) most[i][r] = fmaxf(most[i][r], v[r]);
       }
     }
+#pragma unroll
+    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mul[i][r] = __shfl(page[i].mul, 4 * grp + r) * a.scale;
   }
   if (n16 >= rows) return;
   float* out = a.scores + ((int64_t)t * a.Hkv + kh) * a.p.width;
@@ -364,7 +382,7 @@ __global__ __launch_bounds__(256) void paged_scores_many_kernel(ScoreArgs a) {
     f32x4_t v;
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      v[r] = j + r < pages && ((present[i] >> (4 * grp + r)) & 1) && most[i][r] != kNegInf ? most[i][r] * a.scale : kNegInf;
+      v[r] = j + r < pages && ((present[i] >> (4 * grp + r)) & 1) && most[i][r] != kNegInf ? most[i][r] * mul[i][r] : kNegInf;
     if ((a.p.width & 3) == 0) {
       if (j < a.p.width) *reinterpret_cast<f32x4_t*>(out + j) = v;
     } else {

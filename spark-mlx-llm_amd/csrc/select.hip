@@ -2,10 +2,9 @@
 // (gfx950): pages for a query to attend, tokens for a cache to keep.
 //
 // A row's values are ordered as whole numbers (`key`), and the k-th largest key is
-// found by its bits: of the keys with the bits found so far the next one is set in
-// if that leaves k of them. What is larger than that key is taken, and of what is
-// equal to it the first that there is room for, so ties go to the lowest place.
-// Counts are whole numbers: nothing depends on an order of additions.
+// found from its leading bits on, by counting. What is larger than that key is taken,
+// and of what is equal to it the first that there is room for, so ties go to the
+// lowest place. Counts are whole numbers: nothing depends on an order of additions.
 #include <algorithm>
 
 #include "common.h"
@@ -57,6 +56,7 @@ __device__ __forceinline__ int lanes_below(unsigned long long mask) {
 // ---------------------------------------------------------------------------
 // a wave a row: rows of up to 64 * KPT values, which stay in registers
 // ---------------------------------------------------------------------------
+// A bit at a time: it is set in the k-th key if k keys have it and the bits so far.
 template <int KPT>
 __global__ __launch_bounds__(256) void select_wave_kernel(SelectArgs a) {
   const int lane = threadIdx.x & 63;
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void select_wave_kernel(SelectArgs a) {
 // ---------------------------------------------------------------------------
 // Wave w has the places [w per, (w + 1) per), 64 KPT of them at a time: rows of up to
 // 1024 KPT values stay in registers, longer ones are read again for every pass.
-constexpr int kSelectWaves = 16;
+constexpr int kSelectWaves = 16, kBins = 2048;
 template <int KPT, bool HELD>
 struct SelectKeys {
   uint32_t key[KPT];
@@ -145,7 +145,7 @@ struct SelectKeys {
 
 template <int KPT, bool HELD>
 __global__ __launch_bounds__(64 * kSelectWaves) void select_group_kernel(SelectArgs a) {
-  __shared__ int s_count[2][2 * kSelectWaves];
+  __shared__ int s_bins[kBins], s_pick[3], s_count[2][kSelectWaves];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const SelectRow s = select_row(a, blockIdx.x);
@@ -158,23 +158,52 @@ __global__ __launch_bounds__(64 * kSelectWaves) void select_group_kernel(SelectA
   keys.w0 = min(wave * per, s.n);
   keys.w1 = min(keys.w0 + per, s.n);
   if (HELD) keys.load(a, s, keys.w0, lane);
-  uint32_t theta = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t cand = theta | 1u << bit;
-    int c = 0;
+  // The k-th largest key by digits of 11, 11 and 10 bits: how many of the keys with
+  // the digits found so far have each next one, and down from the largest which digit
+  // the k-th has.
+  uint32_t prefix = 0, theta = 0;
+  int need = s.k;  // its place among the keys with the digits so far
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int above = 32 - 11 * pass, shift = max(above - 11, 0);
+    for (int d = tid; d < kBins; d += 64 * kSelectWaves) s_bins[d] = 0;
+    __syncthreads();
     keys.each(a, s, lane, [&](int) {
 #pragma unroll
-      for (int u = 0; u < KPT; ++u) c += __builtin_popcountll(__ballot(keys.key[u] >= cand));
+      for (int u = 0; u < KPT; ++u) {
+        const uint32_t key = keys.key[u];
+        const bool in = pass == 0 ? key != 0 : key >> above == prefix;
+        if (in) atomicAdd(&s_bins[(key >> shift) & ((1u << (above - shift)) - 1)], 1);
+      }
     });
-    int* box = s_count[bit & 1];
-    if (lane == 0) box[wave] = c;
     __syncthreads();
-    c = 0;
+    // two digits a thread, from the largest down
+    const int d = kBins - 1 - 2 * tid;
+    const int c0 = s_bins[d], c1 = s_bins[d - 1];
+    int before = c0 + c1;
 #pragma unroll
-    for (int w = 0; w < kSelectWaves; ++w) c += box[w];
-    if (c >= s.k) {
-      theta = cand;
-      if (c == s.k) break;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(before, o);
+      if (lane >= o) before += y;
+    }
+    if (lane == 63) s_count[0][wave] = before;
+    __syncthreads();
+    before -= c0 + c1;
+#pragma unroll
+    for (int w = 0; w < kSelectWaves; ++w) before += w < wave ? s_count[0][w] : 0;
+    if (before < need && need <= before + c0 + c1) {
+      const bool second = need > before + c0;
+      s_pick[0] = d - second;
+      s_pick[1] = need - before - (second ? c0 : 0);
+      s_pick[2] = second ? c1 : c0;
+    }
+    __syncthreads();
+    prefix = pass == 0 ? s_pick[0] : prefix << (above - shift) | s_pick[0];
+    need = s_pick[1];
+    theta = prefix << shift;
+    if (need == s_pick[2]) {  // all keys with these digits are taken
+      --theta;
+      break;
     }
   }
   // what each wave has that is larger, and equal
@@ -189,13 +218,13 @@ __global__ __launch_bounds__(64 * kSelectWaves) void select_group_kernel(SelectA
   __syncthreads();
   if (lane == 0) {
     s_count[0][wave] = more;
-    s_count[0][kSelectWaves + wave] = same;
+    s_count[1][wave] = same;
   }
   __syncthreads();
   int all_more = 0, more_before = 0, same_before = 0;
 #pragma unroll
   for (int w = 0; w < kSelectWaves; ++w) {
-    const int m = s_count[0][w], e = s_count[0][kSelectWaves + w];
+    const int m = s_count[0][w], e = s_count[1][w];
     all_more += m;
     more_before += w < wave ? m : 0;
     same_before += w < wave ? e : 0;
