@@ -1194,7 +1194,8 @@ int sparkq_paged_kv_mass(const void* q, const float* lse, const void* k_codes, c
           "paged_kv_mass: rows of mass must be 8-byte aligned");
   REQUIRE((mass_strides[1] >= tokens || Hkv == 1) && (mass_strides[0] >= tokens || B <= 1),
           "paged_kv_mass: rows of mass overlap");
-  REQUIRE(T <= kI32Max / 2 / Hq && T <= 1 << 22, "paged_kv_mass: shape too large");
+  REQUIRE(T <= kI32Max / 2 / Hq && q_strides[0] <= kI32Max && q_strides[1] <= kI32Max / Hq / 2,
+          "paged_kv_mass: shape too large");
   DEVICE_OK();
   return paged_kv_mass(paged_batch(page_table, starts, lengths, T, B, pages, max_pages, table_stride, page_size), q,
                        q_strides, lse, paged_side(k_codes, k_scales, strides), mass, mass_strides, Hq, Hkv, D, max_new,

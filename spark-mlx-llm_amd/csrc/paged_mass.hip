@@ -8,6 +8,7 @@
 // new tokens start from 0. One workgroup has all rows that see its tokens: every sum
 // has one order, and there are no atomics.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged_attn.h"
 
@@ -208,28 +209,32 @@ __device__ __forceinline__ TokenBlock find_block(const PagedBatch& p, int size, 
   return r;
 }
 
-constexpr int mass_tokens(int ways) { return 128 / ways; }  // of a workgroup
+constexpr int kMassHeads = 128;  // rows of a new token, at most: a round of them
+constexpr int mass_tokens(int ways) { return 256 / ways; }  // of a workgroup
 
 template <int D, int WAYS>
 struct MassShape {
-  static constexpr int ROWS = 32 * (WAYS == 1 ? 2 : WAYS);  // queries in LDS at a time
-  static constexpr int QROW = 2 * D + 16;                   // any 16 lanes' reads hit different banks
-  static constexpr int BUF = ROWS * QROW;
-  static constexpr int JOIN = 4 * 32 * 33 * 4;
+  static constexpr int ROWS = 128;         // queries in LDS at a time
+  static constexpr int BUF = ROWS * 2 * D;
+  static constexpr int JOIN = 8 * 32 * 33 * 4;
   static constexpr int BYTES = 2 * BUF > JOIN ? 2 * BUF : JOIN;
+  // 16-byte piece p of row r lies at place p ^ turn(r) of its row: any 16 rows' pieces p
+  // hit different banks
+  static __device__ __forceinline__ int turn(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
 };
 
-// rr / gqa with inv = 1 / gqa, for quotients up to 2^22
-__device__ __forceinline__ int row_of(int rr, int gqa, float inv) {
-  const int t = (int)((float)rr * inv), r = rr - t * gqa;
-  return t + (r >= gqa) - (r < 0);
+// Wait for this thread's loads into LDS.
+__device__ __forceinline__ void wait_loads() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
 template <typename T, int D, int WAYS>
-__global__ __launch_bounds__(256, D == 256 && WAYS == 4 ? 1 : 2) void paged_mass_many_kernel(MassArgs s, int blocks) {
+__global__ __launch_bounds__(512, D <= 128 ? 4 : 2) void paged_mass_many_kernel(MassArgs s, int blocks) {
   using S = MassShape<D, WAYS>;
   constexpr int NK = D / 16, N = mass_tokens(WAYS), kRows = S::ROWS;
-  constexpr int PPR = D / 8, PPT = kRows * PPR / 256;  // 16-byte pieces of a row, of a thread
+  constexpr int PPR = D / 8, PPT = kRows * PPR / 512;  // 16-byte pieces of a row, of a thread
   const PagedSdpaArgs& a = s.a;
   __shared__ __attribute__((aligned(16))) unsigned char smem[S::BYTES];
   __shared__ float s_base[2][kRows];
@@ -238,20 +243,18 @@ __global__ __launch_bounds__(256, D == 256 && WAYS == 4 ? 1 : 2) void paged_mass
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, grp = lane >> 5, group = wave / WAYS, way = wave % WAYS;
   const int gqa = a.Hq / a.Hkv, kh = blockIdx.x % a.Hkv;
-  const float inv = 1.0f / (float)gqa;
+  const int per = kRows / gqa;  // new tokens of a round
   for (int x = blockIdx.x / a.Hkv; x < blocks; x += gridDim.x / a.Hkv) {
     const TokenBlock tb = find_block(a.p, N, x);
     if (tb.b < 0) return;
-    const int t0 = tb.t0, rows = min(tb.s.count, a.max_new) * gqa;
-    // the first row that sees the block's first token
-    const int skip = a.causal ? max(t0 - (tb.s.length - tb.s.count), 0) : 0;
-    const int row0 = (int)min((int64_t)skip * gqa, (int64_t)rows) & ~31;
+    const int t0 = tb.t0, count = min(tb.s.count, a.max_new);
+    // the first new token that sees the block's first token
+    const int first = min(a.causal ? max(t0 - (tb.s.length - tb.s.count), 0) : 0, count);
 
     u32x4_t kf[NK];
     const int w0 = t0 + 32 * group, pos = w0 + col;
-    const int id = pos < tb.s.length ? page_of(a.p, tb.b, pos) : -1;
-    const uint64_t present = __ballot(id >= 0);  // tokens that have a page
     {
+      const int id = pos < tb.s.length ? page_of(a.p, tb.b, pos) : -1;
       const int at = max(id, 0), slot = pos & ((1 << a.p.page_log2) - 1);
       const uint8_t* kp = a.c.k + kh * a.c.c_head + code_at(a.c, at, slot) + 8 * grp;
 #pragma unroll
@@ -263,75 +266,90 @@ __global__ __launch_bounds__(256, D == 256 && WAYS == 4 ? 1 : 2) void paged_mass
         s_scale[32 * group + col] = f16_to_f32(a.c.ks[kh * a.c.s_head + scale_at(a.c, at, slot)]) * s.scale;
     }
 
-    // Piece i of a round of rows: row tid / PPR + i TPP, values 8 (tid % PPR) ..; a
-    // row's first piece brings its logarithm and what it sees.
-    constexpr int TPP = 256 / PPR;
-    u32x4_t qr[PPT];
+    // A round is of whole new tokens: `per` of them, all heads of each. Piece i of a
+    // thread lies at place tid + 512 i of a buffer. The first kRows threads also bring a
+    // row's logarithm and what it sees; rows past a round's own, and past the last new
+    // token, see nothing.
+    int qt[PPT], qo[PPT];
+#pragma unroll
+    for (int i = 0; i < PPT; ++i) {
+      const int r = (tid + 512 * i) / PPR, rr = min(r, per * gqa - 1);
+      qt[i] = rr / gqa;
+      qo[i] = (rr - qt[i] * gqa) * (int)a.q_head + 8 * ((tid % PPR) ^ S::turn(r));
+    }
+    const uint16_t* const qbase = a.q + tb.s.first * a.q_tok + (int64_t)kh * gqa * a.q_head;
+    const int q_tok = (int)a.q_tok, lt = tid / gqa;
+    const float* const lp = s.lse + (int64_t)tb.s.first * a.Hq + kh * gqa + tid - lt * gqa;
     float base_r;
     int lim_r;
-    auto load = [&](int r0) {
+    auto load = [&](int i0, int buf) {  // new tokens i0 .. i0 + per - 1
 #pragma unroll
-      for (int i = 0; i < PPT; ++i) {
-        const int rr = min(r0 + tid / PPR + i * TPP, rows - 1), t = row_of(rr, gqa, inv);
-        qr[i] = *reinterpret_cast<const u32x4_t*>(a.q + (tb.s.first + t) * a.q_tok + (kh * gqa + rr - t * gqa) * a.q_head +
-                                                  8 * (tid % PPR));
-      }
+      for (int i = 0; i < PPT; ++i)
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(qbase + ((int64_t)min(i0 + qt[i], count - 1) * q_tok + qo[i])),
+            (__attribute__((address_space(3))) void*)(smem + buf * S::BUF + 8192 * i + 1024 * wave), 16, 0, 0);
       if (tid < kRows) {
-        const int rr = min(r0 + tid, rows - 1), t = row_of(rr, gqa, inv);
-        base_r = row_base(s.lse[(int64_t)(tb.s.first + t) * a.Hq + kh * gqa + rr - t * gqa]);
-        lim_r = r0 + tid < rows ? last_seen_by(tb.s, t, a.causal) : -1;
+        const bool live = lt < per && i0 + lt < count;
+        base_r = live ? row_base(lp[(int64_t)(i0 + lt) * a.Hq]) : __builtin_huge_valf();
+        lim_r = live ? last_seen_by(tb.s, i0 + lt, a.causal) : -1;
       }
     };
     auto stage = [&](int buf) {
-#pragma unroll
-      for (int i = 0; i < PPT; ++i)
-        *reinterpret_cast<u32x4_t*>(smem + buf * S::BUF + (tid / PPR + i * TPP) * S::QROW + 16 * (tid % PPR)) = qr[i];
       if (tid < kRows) {
         s_base[buf][tid] = base_r;
         s_lim[buf][tid] = lim_r;
       }
+      wait_loads();
     };
     float sum[16];
 #pragma unroll
     for (int v = 0; v < 16; ++v) sum[v] = 0.0f;
-    auto tile = [&](int buf, int r) {  // rows r .. r + 31 of a buffer
-      const unsigned char* q = smem + buf * S::BUF + (r + col) * S::QROW + 16 * grp;
+    auto tile = [&](int buf, int r, bool whole) {  // rows r .. r + 31 of a buffer
+      // (16 ((2 k + grp) ^ turn) is 32 k ^ 16 (grp ^ turn): one address, where the compiler
+      // would keep one for each k)
+      uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem + buf * S::BUF +
+                    (r + col) * 2 * D + 16 * (grp ^ S::turn(r + col));
+      asm volatile("" : "+v"(at));
+      constexpr int AHEAD = 4;  // operands on the way
+      u32x4_t q[AHEAD];
+      auto read = [&](int k) { return *(__attribute__((address_space(3))) const u32x4_t*)(uintptr_t)(at ^ (32 * k)); };
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) q[k] = read(k);
+      const float base = s_base[buf][r + col];
+      // (in the compiler's own order every product waits for its operand)
+      __builtin_amdgcn_sched_barrier(0);
       f32x16_t sc = f32x16_t{};
 #pragma unroll
-      for (int k = 0; k < NK; ++k) sc = mfma32x32x16<T>(kf[k], *reinterpret_cast<const u32x4_t*>(q + 32 * k), sc);
-      const float base = s_base[buf][r + col];
-      const int lim = s_lim[buf][r + col];
-      float e[16];
+      for (int k = 0; k < NK; ++k) {
+        sc = mfma32x32x16<T>(kf[k], q[k % AHEAD], sc);
+        if (k + AHEAD < NK) q[k % AHEAD] = read(k + AHEAD);
+        __builtin_amdgcn_sched_barrier(0);
+      }
 #pragma unroll
       for (int v = 0; v < 16; v += 4) {
         const f32x4_t k4 = *reinterpret_cast<const f32x4_t*>(s_scale + 32 * group + 2 * v + 4 * grp);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e[v + i] = __builtin_amdgcn_exp2f(fmaf(sc[v + i], k4[i], -base));
+        for (int i = 0; i < 4; ++i) sc[v + i] = __builtin_amdgcn_exp2f(fmaf(sc[v + i], k4[i], -base));
       }
-      if (__builtin_expect(__ballot(lim < w0 + 31) != 0, 0)) {
+      if (__builtin_expect(!whole, 0)) {
+        const int rel = s_lim[buf][r + col] - w0 - 4 * grp;  // of this lane's tokens (mfma32_row)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) e[v] = w0 + mfma32_row(lane, v) <= lim ? e[v] : 0.0f;
+        for (int v = 0; v < 16; ++v) sc[v] = 8 * (v >> 2) + (v & 3) <= rel ? sc[v] : 0.0f;
       }
 #pragma unroll
-      for (int v = 0; v < 16; ++v) sum[v] += e[v];
+      for (int v = 0; v < 16; ++v) sum[v] += sc[v];
     };
-    auto round = [&](int buf) {
-      if constexpr (WAYS == 1) {
-        tile(buf, 0);
-        tile(buf, 32);
-      } else {
-        tile(buf, 32 * way);
-      }
-    };
-    if (row0 < rows) {
-      load(row0);
+    if (first < count) {
+      load(first, 0);
       stage(0);
-      load(row0 + kRows);
       __syncthreads();
-      for (int r0 = row0, buf = 0; r0 < rows; r0 += kRows, buf ^= 1) {
-        round(buf);
+      for (int i0 = first, buf = 0; i0 < count; i0 += per, buf ^= 1) {
+        load(i0 + per, buf ^ 1);
+        // whether these rows see all of this wave's tokens: the first sees the least
+        const bool whole = i0 + per <= count && last_seen_by(tb.s, i0, a.causal) >= w0 + 31;
+#pragma unroll 1
+        for (int r = 32 * way; r < kRows; r += 32 * WAYS) tile(buf, r, whole);
         stage(buf ^ 1);
-        load(r0 + 2 * kRows);
         __syncthreads();
       }
     }
@@ -339,19 +357,17 @@ __global__ __launch_bounds__(256, D == 256 && WAYS == 4 ? 1 : 2) void paged_mass
 #pragma unroll
     for (int v = 0; v < 16; ++v) join[wave][mfma32_row(lane, v)][col] = sum[v];
     __syncthreads();
-    // 256 / N threads a token: half of a wave's sums each
-    const int tok = tid / (256 / N), h = tid % (256 / N);
+    // 512 / N threads a token: half of a wave's sums each
+    const int tok = tid / (512 / N), h = tid % (512 / N);
     float v = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) v += join[tok / 32 * WAYS + h / 2][tok % 32][16 * (h & 1) + i];
     v += dpp_row<0xB1>(v);
-    if (WAYS == 4) {
-      v += dpp_row<0x4E>(v);
-      v += dpp_row<0x141>(v);
-    }
+    v += dpp_row<0x4E>(v);
+    if (WAYS == 4) v += dpp_row<0x141>(v);
     if (h == 0 && t0 + tok < tb.s.length) {
       float* m = s.mass + tb.b * s.m_row + kh * s.m_head + t0 + tok;
-      const bool in = WAYS == 4 ? (present >> (tok & 31)) & 1 : page_of(a.p, tb.b, t0 + tok) >= 0;
+      const bool in = page_of(a.p, tb.b, t0 + tok) >= 0;
       *m = (t0 + tok < tb.s.length - tb.s.count ? *m : 0.0f) + (in ? v : 0.0f);
     }
     __syncthreads();
@@ -366,9 +382,9 @@ template <typename T, int D>
 void launch_many(const MassArgs& s, bool share, int64_t items, int64_t blocks, hipStream_t st) {
   const dim3 grid((unsigned)(items * s.a.Hkv));
   if (share)
-    hipLaunchKernelGGL((paged_mass_many_kernel<T, D, 4>), grid, dim3(256), 0, st, s, (int)blocks);
+    hipLaunchKernelGGL((paged_mass_many_kernel<T, D, 4>), grid, dim3(512), 0, st, s, (int)blocks);
   else
-    hipLaunchKernelGGL((paged_mass_many_kernel<T, D, 1>), grid, dim3(256), 0, st, s, (int)blocks);
+    hipLaunchKernelGGL((paged_mass_many_kernel<T, D, 2>), grid, dim3(512), 0, st, s, (int)blocks);
 }
 
 }  // namespace
@@ -379,6 +395,9 @@ int paged_kv_mass(const PagedBatch& p, const void* q, const int64_t* qst, const 
   if (p.T == 0 || p.B == 0) return SPARKQ_OK;
   max_new = std::min<int64_t>(max_new, p.T);
   const int64_t gqa = Hq / Hkv, max_tokens = (int64_t)p.width << p.page_log2;
+  if (gqa > kMassHeads)
+    return set_error(SPARKQ_ERR_UNSUPPORTED, "paged_kv_mass: at most %d query heads to a KV head (got %lld)", kMassHeads,
+                     (long long)gqa);
   MassArgs s{};
   s.a.p = p;
   s.a.q = (const uint16_t*)q;
@@ -415,11 +434,11 @@ int paged_kv_mass(const PagedBatch& p, const void* q, const int64_t* qst, const 
       launch_few<256>(s, items, st);
     return check_launch("paged_mass_few_kernel");
   }
-  const bool share = p.B * cdiv(max_tokens, mass_tokens(1)) * Hkv < 2 * device_cus();
-  const int64_t blocks = p.B * cdiv(max_tokens, mass_tokens(share ? 4 : 1));
+  const bool share = p.B * cdiv(max_tokens, mass_tokens(2)) * Hkv < 2 * device_cus();
+  const int64_t blocks = p.B * cdiv(max_tokens, mass_tokens(share ? 4 : 2));
   if (blocks > 0x7FFFFFFF) return set_error(SPARKQ_ERR_INVALID, "paged_kv_mass: shape too large");
   // no more workgroups than the chip holds a few times over; they take further blocks
-  const int64_t items = std::min(blocks, cdiv(16 * device_cus(), Hkv));
+  const int64_t items = std::min(blocks, cdiv(8 * device_cus(), Hkv));
   auto go = [&](auto t) {
     using T = decltype(t);
     if (D == 64)
