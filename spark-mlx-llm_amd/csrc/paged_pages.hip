@@ -214,9 +214,10 @@ __device__ __forceinline__ f32x4_t page_scores(const PageOperand<T, D>& b, const
 }
 
 // One new token a sequence: a group's query heads are the product's 16 columns, and
-// the largest of their scores is taken over a row of 16 lanes. A workgroup takes
-// kOnePages pages of one KV head, a wave 16 at a time.
-constexpr int kOneTiles = 2, kOnePages = 64 * kOneTiles;
+// the largest of their scores is taken over a row of 16 lanes. A wave has 16 pages of
+// one KV head, a workgroup 64. A chain of three round trips: one sequence of 512 pages
+// takes 4.2 us, 64 of up to 512 (39 MB) 14.5 (with 32 pages a wave 5.3 and 15.9).
+constexpr int kOnePages = 64;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_scores_one_kernel(ScoreArgs a) {
   constexpr int NK = D / 32;
@@ -224,59 +225,43 @@ __global__ __launch_bounds__(256) void paged_scores_one_kernel(ScoreArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kh = blockIdx.x % a.Hkv, x = blockIdx.x / a.Hkv, b = x / a.chunks, chunk = x - b * a.chunks;
   const int gqa = a.Hq / a.Hkv;
-  const int j0 = chunk * kOnePages + 16 * wave;
+  const int j0 = chunk * kOnePages + 16 * wave, j = j0 + n16;
   // (asked for before the lengths are known, which say whether it is a page)
-  int id[kOneTiles];
-#pragma unroll
-  for (int i = 0; i < kOneTiles; ++i) id[i] = a.p.table[b * a.p.table_stride + min(j0 + 64 * i + n16, a.p.width - 1)];
+  const int id = a.p.table[b * a.p.table_stride + min(j, a.p.width - 1)];
   const SeqRows s = seq_rows(a.p, b);
   if (s.count == 0) return;
   const int t = s.first, lim = last_seen_by(s, 0, a.causal);
   const int pages = lim < 0 ? 0 : (lim >> a.p.page_log2) + 1;
   if (kh == 0 && chunk == 0 && tid == 0) a.seen[t] = pages;
   float* out = a.scores + ((int64_t)t * a.Hkv + kh) * a.p.width;
-  if (j0 >= pages) {  // (a wave's tiles lie 64 pages apart)
-#pragma unroll
-    for (int i = 0; i < kOneTiles; ++i)
-      if (grp == 0 && j0 + 64 * i + n16 < a.p.width) out[j0 + 64 * i + n16] = kNegInf;
+  if (j0 >= pages) {
+    if (grp == 0 && j < a.p.width) out[j] = kNegInf;
     return;
   }
-  PageOperand<T, D> page[kOneTiles];
-  uint64_t present[kOneTiles];
-#pragma unroll
-  for (int i = 0; i < kOneTiles; ++i) {
-    const bool in = j0 + 64 * i + n16 < pages && (unsigned)id[i] < (unsigned)a.p.pages;
-    present[i] = __ballot(in);
-    load_bounds<T, D>(a.bounds + (in ? id[i] : 0) * a.b_page + kh * a.b_head + 8 * grp, page[i]);
-  }
-  f32x4_t most[kOneTiles];
-#pragma unroll
-  for (int i = 0; i < kOneTiles; ++i) most[i] = f32x4_t{kNegInf, kNegInf, kNegInf, kNegInf};
+  const bool in = j < pages && (unsigned)id < (unsigned)a.p.pages;
+  PageOperand<T, D> page;
+  load_bounds<T, D>(a.bounds + (in ? id : 0) * a.b_page + kh * a.b_head + 8 * grp, page);
+  f32x4_t most = {kNegInf, kNegInf, kNegInf, kNegInf};
   for (int g0 = 0; g0 < gqa; g0 += 16) {
     const int g = min(g0 + n16, gqa - 1);  // (the last head again for what is past it)
     const uint16_t* row = a.q + t * a.q_tok + (kh * gqa + g) * a.q_head + 8 * grp;
     u32x4_t raw[NK];
 #pragma unroll
     for (int c = 0; c < NK; ++c) raw[c] = *reinterpret_cast<const u32x4_t*>(row + 32 * c);
+    if (g0 == 0) turn_bounds<T, D>(page);
+    const f32x4_t v = page_scores<T, D>(page, raw, a.flip);
 #pragma unroll
-    for (int i = 0; i < kOneTiles; ++i) {
-      if (g0 == 0) turn_bounds<T, D>(page[i]);
-      const f32x4_t v = page_scores<T, D>(page[i], raw, a.flip);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) most[i][r] = fmaxf(most[i][r], v[r]);
-    }
+    for (int r = 0; r < 4; ++r) most[r] = fmaxf(most[r], v[r]);
   }
+  float v[4];
 #pragma unroll
-  for (int i = 0; i < kOneTiles; ++i) {
-    float v[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = max_row16(most[i][r]);
-    const int k = 4 * grp + n16, j = j0 + 64 * i + k;  // lane n16 < 4 of a group stores score n16
-    const float mul = __shfl(page[i].mul, k & 63) * a.scale;
-    if (n16 < 4 && j < a.p.width) {
-      const float m = n16 == 0 ? v[0] : n16 == 1 ? v[1] : n16 == 2 ? v[2] : v[3];
-      out[j] = ((present[i] >> k) & 1) && m != kNegInf ? m * mul : kNegInf;
-    }
+  for (int r = 0; r < 4; ++r) v[r] = max_row16(most[r]);
+  const int k = 4 * grp + n16;  // lane n16 < 4 of a group stores score n16
+  const float mul = __shfl(page.mul, k & 63) * a.scale;
+  const uint64_t present = __ballot(in);
+  if (n16 < 4 && j0 + k < a.p.width) {
+    const float m = n16 == 0 ? v[0] : n16 == 1 ? v[1] : n16 == 2 ? v[2] : v[3];
+    out[j0 + k] = ((present >> k) & 1) && m != kNegInf ? m * mul : kNegInf;
   }
 }
 
@@ -290,8 +275,9 @@ __device__ __forceinline__ TokenTile find_tokens(const PagedBatch& p, int max_ne
   TokenTile t{-1, 0, {0, 0, 0}};
   int before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    int tiles = 0;
-    if (b0 + lane < p.B) tiles = (min(seq_rows(p, b0 + lane).count, max_new) + 15) / 16;
+    SeqRows s{0, 0, 0};
+    if (b0 + lane < p.B) s = seq_rows(p, b0 + lane);
+    const int tiles = (min(s.count, max_new) + 15) / 16;
     int end = tiles;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -301,13 +287,17 @@ __device__ __forceinline__ TokenTile find_tokens(const PagedBatch& p, int max_ne
     const unsigned long long hit = __ballot(x < before + end);
     if (hit) {
       const int l = __builtin_ctzll(hit);
-      t.b = __builtin_amdgcn_readfirstlane(b0 + l);
-      t.row0 = 16 * __builtin_amdgcn_readfirstlane(x - before - __shfl(end - tiles, l));
-      t.s = seq_rows(p, t.b);
-      return t;
+      t.b = b0 + l;
+      t.row0 = 16 * (x - before - __builtin_amdgcn_readlane(end - tiles, l));
+      t.s.first = __builtin_amdgcn_readlane(s.first, l);
+      t.s.count = __builtin_amdgcn_readlane(s.count, l);
+      t.s.length = __builtin_amdgcn_readlane(s.length, l);
+      break;
     }
     before += __builtin_amdgcn_readlane(end, 63);
   }
+  // (the compiler does not see that a loop left on a ballot leaves scalars)
+  for (int* f : {&t.b, &t.row0, &t.s.first, &t.s.count, &t.s.length}) *f = __builtin_amdgcn_readfirstlane(*f);
   return t;
 }
 

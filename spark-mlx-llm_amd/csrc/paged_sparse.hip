@@ -355,10 +355,12 @@ SparsePlan sparse_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t count, int64_
   const int64_t gqa = Hq / Hkv;
   p.tiles = cdiv(gqa, 16);
   p.rows_held = std::min<int64_t>(gqa, 16);
-  // lists are split where there are too few of them for the chip, into parts of no
-  // less than 128 tokens (a block for each wave)
+  // Lists are split where there are fewer of them than CUs, into parts of no less than
+  // 128 tokens (a block for each wave). More parts fill the chip better, but joining
+  // them costs 4 us: 224 lists of 77 pages of 32 tokens at D = 256 take 51 us whole, 53
+  // + 5 in two parts; 56 lists of 32 pages of 64 at D = 128 15 + 4 in four, 17 + 4 in ten.
   const int64_t most = std::min(cdiv(count * page, 128), count);
-  p.parts = std::max<int64_t>(std::min(cdiv(3 * device_cus(), T * Hkv * p.tiles), most), 1);
+  p.parts = std::max<int64_t>(std::min(device_cus() / std::max<int64_t>(T * Hkv * p.tiles, 1), most), 1);
   return p;
 }
 
