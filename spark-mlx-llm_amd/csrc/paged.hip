@@ -497,6 +497,7 @@ struct EvictArgs {
   float* mass;          // [layers, B, H, tokens], or null
   int64_t m_layer, m_row, m_head;
   int H, D, count, slices;  // slices: of a token's codes, a workgroup each
+  bool tables;              // written by the plan
 };
 
 // pages that a row of more than `count` tokens keeps
@@ -504,8 +505,32 @@ __device__ __forceinline__ int kept_pages(const EvictArgs& e) {
   return (int)(((int64_t)e.count + (1 << e.p.page_log2) - 1) >> e.p.page_log2);
 }
 
+// Row i's table and length after it, by a wave: `room` says that the pool has the
+// pages, held(p) who holds page p.
+template <typename F>
+__device__ __forceinline__ void evict_row(const EvictArgs& e, int i, bool room, F held) {
+  const PageArgs& a = e.p;
+  const int lane = threadIdx.x & 63;
+  const RowPlan r = row_plan(a, i);
+  const bool less = r.before > e.count && room;
+  const int n = less ? kept_pages(e) : r.held;
+  int at = a.s.base[i];
+  if (lane == 0) a.out_lengths[i] = less ? e.count : r.before;
+  for (int j0 = 0; j0 < a.width; j0 += 64) {
+    const int j = j0 + lane;
+    int id = j < n ? held_page(a, r, j) : -1;
+    const bool other = less && id >= 0 && held(max(id, 0)) > 1;
+    const unsigned long long m = __ballot(other);
+    if (other)
+      id = a.s.list[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))];
+    at += __builtin_popcountll(m);
+    if (j < a.width) a.out_table[(int64_t)i * a.width + j] = id;
+  }
+}
+
 // One workgroup: holders of each page, free pages in order, and where each row's
-// replacements start among these (a wave a row).
+// replacements start among these (a wave a row); the rows' tables too where they are
+// so few that another launch would take longer (`tables`).
 template <bool LDS>
 __global__ __launch_bounds__(kPlanThreads) void pages_evict_plan_kernel(EvictArgs e) {
   extern __shared__ int s_pages[];
@@ -544,33 +569,23 @@ __global__ __launch_bounds__(kPlanThreads) void pages_evict_plan_kernel(EvictArg
     if (i < a.rows) a.s.base[i] = base;
     wanted += total;
   }
+  const int missing = max(wanted - nfree, 0);
   if (tid == 0) {
-    const int missing = max(wanted - nfree, 0);
     a.s.head[kPairs] = missing;
     *a.out_count = missing;
   }
+  if (e.tables) {
+    __syncthreads();  // base, and the list
+    for (int i = wave; i < a.rows; i += kPlanThreads / 64)
+      evict_row(e, i, missing == 0, [&](int p) { return held.get(p); });
+  }
 }
 
-// The tables and lengths after it: a wave a row.
+// The tables and lengths after it, of many rows: a wave a row.
 __global__ __launch_bounds__(256) void pages_evict_table_kernel(EvictArgs e) {
-  const PageArgs& a = e.p;
-  const int lane = threadIdx.x & 63, i = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (i >= a.rows) return;
-  const RowPlan r = row_plan(a, i);
-  const bool less = r.before > e.count && a.s.head[kPairs] == 0;
-  const int n = less ? kept_pages(e) : r.held;
-  int at = a.s.base[i];
-  if (lane == 0) a.out_lengths[i] = less ? e.count : r.before;
-  for (int j0 = 0; j0 < a.width; j0 += 64) {
-    const int j = j0 + lane;
-    int id = j < n ? held_page(a, r, j) : -1;
-    const bool other = less && id >= 0 && a.s.held[id] > 1;
-    const unsigned long long m = __ballot(other);
-    if (other)
-      id = a.s.list[at + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))];
-    at += __builtin_popcountll(m);
-    if (j < a.width) a.out_table[(int64_t)i * a.width + j] = id;
-  }
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= e.p.rows) return;
+  evict_row(e, i, e.p.s.head[kPairs] == 0, [&](int p) { return e.p.s.held[p]; });
 }
 
 // A workgroup per (layer, row, head, keys or values, slice of the codes) takes the
@@ -773,12 +788,13 @@ int kv_pages_evict(const int32_t* table, int64_t table_stride, const int32_t* le
   const int pieces = sliced ? 4 : (int)(D / 16);
   e.slices = (int)(D / 16 / pieces);
   if (groups > kMaxGrid / e.slices) return set_error(SPARKQ_ERR_INVALID, "kv_pages_evict: shape too large");
+  e.tables = B * cdiv(width, 64) <= 128;  // (no more than 8 rounds a wave: 0.5 us each)
   if (pages <= kLdsPages)
     hipLaunchKernelGGL(pages_evict_plan_kernel<true>, dim3(1), dim3(kPlanThreads), pages * sizeof(int), st, e);
   else
     hipLaunchKernelGGL(pages_evict_plan_kernel<false>, dim3(1), dim3(kPlanThreads), 0, st, e);
   if (B == 0) return check_launch("pages_evict_kernel");
-  hipLaunchKernelGGL(pages_evict_table_kernel, dim3((unsigned)cdiv(B, 4)), dim3(256), 0, st, e);
+  if (!e.tables) hipLaunchKernelGGL(pages_evict_table_kernel, dim3((unsigned)cdiv(B, 4)), dim3(256), 0, st, e);
   const dim3 grid((unsigned)(groups * e.slices));
   if (pieces == 4)
     hipLaunchKernelGGL(pages_evict_kernel<4>, grid, dim3(256), 0, st, e);
