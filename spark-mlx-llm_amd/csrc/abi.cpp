@@ -1183,9 +1183,9 @@ int sparkq_paged_kv_mass(const void* q, const float* lse, const void* k_codes, c
   REQUIRE(strides, "paged_kv_mass: null tensor pointer");
   int64_t both[12];
   for (int i = 0; i < 12; ++i) both[i] = strides[i % 6];
-  // (mass in the outputs' place: aligned like them)
+  // (mass in the outputs' place: aligned like them, and none of no sequences)
   if (int rc = paged_attn_check("paged_kv_mass", T, B, Hq, Hkv, D, pages, max_pages, table_stride, page_size, max_new, q,
-                                mass, page_table, starts, lengths, k_codes, k_scales, k_codes, k_scales, q_strides, both,
+                                B == 0 ? q : (const void*)mass, page_table, starts, lengths, k_codes, k_scales, k_codes, k_scales, q_strides, both,
                                 q_dtype, q_dtype, scale))
     return rc;
   REQUIRE((T == 0 || lse) && mass_strides && aligned(lse, 4), "paged_kv_mass: null tensor pointer");

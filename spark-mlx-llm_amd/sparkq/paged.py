@@ -536,6 +536,21 @@ def kv_pages_evict(cache, keep, page_table, lengths, *, mass=None):
     return table, after, missing
 
 
+def _compact_bounds(bounds, page_table, lengths, page_size):
+    """Moves the bounds [layers,pages,Hkv,2,D] of pages as kv_pages_compact moves these: a
+    page's bounds in four pieces, in the place of its codes and scales."""
+    layers, pages, hkv, _, d = bounds.shape
+    index, (b, width) = bounds.get_device(), page_table.shape
+    piece = hkv * d  # bytes: a quarter of a page's
+    table, used = torch.empty_like(page_table), lengths.new_empty(1)
+    need = _lib.lib().sparkq_kv_pages_workspace_bytes(b, pages)
+    ws = bounds.new_empty(need, dtype=torch.int8)
+    _lib.launch("sparkq_kv_pages_compact", index, *(bounds.data_ptr() + i * piece for i in range(4)),
+                page_table.data_ptr(), lengths.data_ptr(), page_table.stride(0), table.data_ptr(),
+                used.data_ptr(), _I64x8(*(4 * piece * pages, 4 * piece) * 4), b, width, pages, layers,
+                page_size, piece, piece, ws.data_ptr(), need)
+
+
 class PagedKVCache:
     """A pool of pages for the layers of a model, and the batch that holds
     them: `pages` pages of `page_size` tokens, at most `max_pages` of them to a
@@ -552,10 +567,23 @@ class PagedKVCache:
     row's: a step that would exceed it is short of pages like one that the pool
     has none for (`missing`), and until undo() has taken it back the cache refuses
     to append, attend, compact or step. `lengths` may be lowered in place (tokens
-    that are taken back) or set, not raised in place."""
+    that are taken back) or set, not raised in place.
+
+    With bounds=True append() keeps the bounds of each page's keys, and
+
+        out = cache.attend_pages(l, queries, scale=..., count=32)
+
+    attends the `count` pages of each KV head that score highest instead of all. With
+    mass=True attend() adds up the attention weight that each token gathers, and
+
+        cache.evict(count)                           # between steps
+
+    leaves each row the `count` tokens that gathered most. (After it lengths are no
+    longer positions: count these apart.)"""
 
     def __init__(self, layers: int, pages: int, kv_heads: int, head_dim: int, *,
-                 page_size: int = 64, max_pages: int = 128, batch: int = 0, device="cuda"):
+                 page_size: int = 64, max_pages: int = 128, batch: int = 0, device="cuda",
+                 bounds: bool = False, mass: bool = False):
         if min(layers, pages, kv_heads, max_pages) < 1 or batch < 0:
             raise ValueError("layers, pages, kv_heads and max_pages must be positive")
         if head_dim not in (64, 128, 256):
@@ -568,6 +596,10 @@ class PagedKVCache:
             torch.zeros(shape, dtype=torch.float16, device=device) for codes in (1, 0, 1, 0))
         self.page_size, self.max_pages = page_size, max_pages
         dev = self.cache[0].device
+        self.bounds = torch.zeros((layers, pages, kv_heads, 2, head_dim), dtype=torch.bfloat16,
+                                  device=dev) if bounds else None
+        self.mass = torch.zeros((layers, batch, kv_heads, max_pages * page_size),
+                                device=dev) if mass else None
         self.page_table = torch.full((batch, max_pages), -1, dtype=torch.int32, device=dev)
         self.lengths = torch.zeros((batch,), dtype=torch.int32, device=dev)
         self.starts = torch.zeros((batch + 1,), dtype=torch.int32, device=dev)
@@ -634,7 +666,7 @@ class PagedKVCache:
             ints = torch.tensor(host, dtype=torch.int32, device=dev)
         if parents is not None:
             parents = ints[2 * rows + 1:]
-        last = self.page_table, self._lengths, self._counts, self.starts, self.max_new
+        last = (self.page_table, self._lengths, self._counts, self.starts, self.max_new, self.mass)
         short = sum(max(0, -(-n // self.page_size) - self.max_pages) for n in after)
         if short:  # no page is touched: the tokens without a place would fall on others
             room = self.max_pages * self.page_size
@@ -644,9 +676,19 @@ class PagedKVCache:
         else:
             self.page_table, self._lengths, self.missing = kv_pages_fork(
                 self.cache, self.page_table, self._lengths, parents, ints[:rows])
+            if self.mass is not None and parents is not None:
+                self.mass = self._mass_of(parents)
         self._last, self._counts = last, after
         self.starts, self.max_new = ints[rows:2 * rows + 1], max(new_tokens, default=0)
         return self.starts
+
+    def _mass_of(self, parents):
+        """Mass of rows that continue `parents`; what starts empty has only new tokens, which
+        start from 0."""
+        layers, rows, *shape = self.mass.shape
+        if rows == 0:
+            return self.mass.new_zeros((layers, parents.shape[0], *shape))
+        return self.mass.index_select(1, parents.clamp(0, rows - 1))
 
     def undo(self):
         """Take back a step that was short of pages, before anything of it was
@@ -657,7 +699,8 @@ class PagedKVCache:
             raise ValueError("there is no step to take back")
         if self.missing.item() == 0:
             raise ValueError("the last step was not short of pages")
-        self.page_table, self._lengths, self._counts, self.starts, self.max_new = self._last
+        (self.page_table, self._lengths, self._counts, self.starts, self.max_new,
+         self.mass) = self._last
         self._last, self._full = None, False
 
     def layer(self, index: int):
@@ -667,18 +710,74 @@ class PagedKVCache:
         self._ready()
         paged_kv_append(keys, values, self.layer(index), self.page_table, self.starts,
                         self.lengths)
+        if self.bounds is not None:
+            paged_key_bounds(self.layer(index), self.bounds[index], self.page_table, self.starts,
+                             self.lengths, max_new=max(self.max_new, 1))
         self._last = None  # what is appended cannot be taken back
 
     def attend(self, index: int, queries, *, scale, mask="causal", out_dtype=None, out=None):
         self._ready()
-        return paged_quantized_sdpa(queries, self.layer(index), self.page_table, self.starts,
-                                    self.lengths, scale=scale, max_new=max(self.max_new, 1),
-                                    mask=mask, out_dtype=out_dtype, out=out)
+        batch = self.page_table, self.starts, self.lengths
+        kw = {"scale": scale, "max_new": max(self.max_new, 1), "mask": mask}
+        if self.mass is None:
+            return paged_quantized_sdpa(queries, self.layer(index), *batch, out_dtype=out_dtype,
+                                        out=out, **kw)
+        out, lse = paged_quantized_sdpa(queries, self.layer(index), *batch, out_dtype=out_dtype,
+                                        out=out, return_lse=True, **kw)
+        paged_kv_mass(queries, lse, self.layer(index), self.mass[index], *batch, **kw)
+        return out
+
+    def attend_pages(self, index: int, queries, *, scale, count: int, first: int = 1, last: int = 2,
+                     mask="causal", out_dtype=None, out=None):
+        """Attention over `count` pages of each KV head for each new token: the first
+        `first` and last `last` that it sees, and those whose bounds allow the largest
+        logits."""
+        self._ready()
+        if self.bounds is None:
+            raise ValueError("attend_pages needs a cache with bounds=True")
+        if self.mass is not None:
+            raise ValueError("a cache with mass=True attends all tokens: attention over selected "
+                             "pages does not say what the others gather")
+        batch = self.page_table, self.starts, self.lengths
+        kw = {"scale": scale, "max_new": max(self.max_new, 1), "mask": mask}
+        scores, seen = paged_page_scores(queries, self.bounds[index], *batch,
+                                         page_size=self.page_size, **kw)
+        pages = select_top(scores, count, lengths=seen, first=first, last=last)
+        return paged_sparse_sdpa(queries, self.layer(index), pages, *batch, out_dtype=out_dtype,
+                                 out=out, **kw)
+
+    def evict(self, count: int, *, first: int = 0, last: int = 0):
+        """Rows of more than `count` tokens keep `count` of them, in each layer and KV head
+        its own: the first `first`, the last `last`, and those of the rest that gathered
+        the most attention weight. To be called between steps: the tokens of the last one
+        are then old ones. Returns `missing` (on the device, like step's): pages that the
+        pool was short of, as what is written must not be shared; when it is not 0 all is
+        as it was."""
+        self._ready()
+        if self.mass is None:
+            raise ValueError("evict needs a cache with mass=True")
+        keep = select_top(self.mass, count, lengths=self._lengths, first=first, last=last)
+        before = self._lengths
+        self.page_table, self._lengths, self.missing = kv_pages_evict(
+            self.cache, keep, self.page_table, before, mass=self.mass)
+        self._last = None  # (the host's counts stay: they are no less than the tokens)
+        self.starts, self.max_new = torch.zeros_like(self.starts), 0
+        if self.bounds is not None and self.page_table.shape[0]:
+            # all tokens of the rows that changed as new ones
+            ends = torch.where(self._lengths < before, self._lengths, 0).cumsum(0, dtype=torch.int32)
+            starts = torch.cat([ends.new_zeros(1), ends])
+            for index in range(self.cache[0].shape[0]):
+                paged_key_bounds(self.layer(index), self.bounds[index], self.page_table, starts,
+                                 self._lengths, max_new=count)
+        return self.missing
 
     def compact(self):
         """Returns the number of pages in use (on the device): the pages from
         it on are free."""
         self._ready()
         self._last = None
-        self.page_table, used = kv_pages_compact(self.cache, self.page_table, self.lengths)
+        before = self.page_table
+        self.page_table, used = kv_pages_compact(self.cache, before, self.lengths)
+        if self.bounds is not None:
+            _compact_bounds(self.bounds, before, self.lengths, self.page_size)
         return used

@@ -295,9 +295,114 @@ def _(k_codes, k_scales, v_codes, v_scales, page_table, lengths):
     return page_table.new_empty(page_table.shape), lengths.new_empty((1,))
 
 
+# --- long contexts over a paged cache -----------------------------------------------
+
+@custom_op(f"{_NS}::paged_sdpa_lse", mutates_args=())
+def paged_sdpa_lse(queries: Tensor, k_codes: Tensor, k_scales: Tensor, v_codes: Tensor,
+                   v_scales: Tensor, page_table: Tensor, starts: Tensor, lengths: Tensor,
+                   scale: float, max_new: int, causal: bool,
+                   out_dtype: Optional[torch.dtype]) -> Tuple[Tensor, Tensor]:
+    return paged.paged_quantized_sdpa(queries, (k_codes, k_scales, v_codes, v_scales), page_table,
+                                      starts, lengths, scale=scale, max_new=max_new,
+                                      mask="causal" if causal else None, out_dtype=out_dtype,
+                                      return_lse=True)
+
+
+@paged_sdpa_lse.register_fake
+def _(queries, k_codes, k_scales, v_codes, v_scales, page_table, starts, lengths, scale, max_new,
+      causal, out_dtype):
+    return (queries.new_empty(queries.shape, dtype=out_dtype or queries.dtype),
+            queries.new_empty(queries.shape[:2], dtype=torch.float32))
+
+
+@custom_op(f"{_NS}::paged_key_bounds", mutates_args=("bounds",))
+def paged_key_bounds(k_codes: Tensor, k_scales: Tensor, v_codes: Tensor, v_scales: Tensor,
+                     bounds: Tensor, page_table: Tensor, starts: Tensor, lengths: Tensor,
+                     max_new: int) -> None:
+    paged.paged_key_bounds((k_codes, k_scales, v_codes, v_scales), bounds, page_table, starts,
+                           lengths, max_new=max_new)
+
+
+@paged_key_bounds.register_fake
+def _(k_codes, k_scales, v_codes, v_scales, bounds, page_table, starts, lengths, max_new):
+    return None
+
+
+@custom_op(f"{_NS}::paged_page_scores", mutates_args=())
+def paged_page_scores(queries: Tensor, bounds: Tensor, page_table: Tensor, starts: Tensor,
+                      lengths: Tensor, page_size: int, scale: float, max_new: int,
+                      causal: bool) -> Tuple[Tensor, Tensor]:
+    return paged.paged_page_scores(queries, bounds, page_table, starts, lengths,
+                                   page_size=page_size, scale=scale, max_new=max_new,
+                                   mask="causal" if causal else None)
+
+
+@paged_page_scores.register_fake
+def _(queries, bounds, page_table, starts, lengths, page_size, scale, max_new, causal):
+    t = queries.shape[0]
+    return (queries.new_empty((t, bounds.shape[1], page_table.shape[1]), dtype=torch.float32),
+            queries.new_empty((t,), dtype=torch.int32))
+
+
+@custom_op(f"{_NS}::select_top", mutates_args=())
+def select_top(x: Tensor, count: int, lengths: Optional[Tensor], first: int, last: int) -> Tensor:
+    return paged.select_top(x, count, lengths=lengths, first=first, last=last)
+
+
+@select_top.register_fake
+def _(x, count, lengths, first, last):
+    return x.new_empty((*x.shape[:-1], count), dtype=torch.int32)
+
+
+@custom_op(f"{_NS}::paged_sparse_sdpa", mutates_args=())
+def paged_sparse_sdpa(queries: Tensor, k_codes: Tensor, k_scales: Tensor, v_codes: Tensor,
+                      v_scales: Tensor, selected: Tensor, page_table: Tensor, starts: Tensor,
+                      lengths: Tensor, scale: float, max_new: int, causal: bool,
+                      out_dtype: Optional[torch.dtype]) -> Tensor:
+    return paged.paged_sparse_sdpa(queries, (k_codes, k_scales, v_codes, v_scales), selected,
+                                   page_table, starts, lengths, scale=scale, max_new=max_new,
+                                   mask="causal" if causal else None, out_dtype=out_dtype)
+
+
+@paged_sparse_sdpa.register_fake
+def _(queries, k_codes, k_scales, v_codes, v_scales, selected, page_table, starts, lengths, scale,
+      max_new, causal, out_dtype):
+    return queries.new_empty(queries.shape, dtype=out_dtype or queries.dtype)
+
+
+@custom_op(f"{_NS}::paged_kv_mass", mutates_args=("mass",))
+def paged_kv_mass(queries: Tensor, lse: Tensor, k_codes: Tensor, k_scales: Tensor, v_codes: Tensor,
+                  v_scales: Tensor, mass: Tensor, page_table: Tensor, starts: Tensor,
+                  lengths: Tensor, scale: float, max_new: int, causal: bool) -> None:
+    paged.paged_kv_mass(queries, lse, (k_codes, k_scales, v_codes, v_scales), mass, page_table,
+                        starts, lengths, scale=scale, max_new=max_new,
+                        mask="causal" if causal else None)
+
+
+@paged_kv_mass.register_fake
+def _(queries, lse, k_codes, k_scales, v_codes, v_scales, mass, page_table, starts, lengths, scale,
+      max_new, causal):
+    return None
+
+
+@custom_op(f"{_NS}::kv_pages_evict", mutates_args=(*_CACHE, "mass"))
+def kv_pages_evict(k_codes: Tensor, k_scales: Tensor, v_codes: Tensor, v_scales: Tensor,
+                   keep: Tensor, page_table: Tensor, lengths: Tensor,
+                   mass: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+    return paged.kv_pages_evict((k_codes, k_scales, v_codes, v_scales), keep, page_table, lengths,
+                                mass=mass)
+
+
+@kv_pages_evict.register_fake
+def _(k_codes, k_scales, v_codes, v_scales, keep, page_table, lengths, mass):
+    return (page_table.new_empty(page_table.shape), lengths.new_empty(lengths.shape),
+            lengths.new_empty((1,)))
+
+
 __all__ = [
     "affine_quantized_matmul", "w8a8_linear", "w8a16_per_channel", "quantize_per_token",
     "int8_matmul_int32", "int8_sdpa_s8", "int8_sdpa_affine", "rms_norm", "rope", "qkv_rope",
     "fused_ffn", "attention_gate", "qk_norm_rope", "paged_sdpa", "paged_kv_append",
-    "kv_pages_fork", "kv_pages_compact",
+    "kv_pages_fork", "kv_pages_compact", "paged_sdpa_lse", "paged_key_bounds", "paged_page_scores",
+    "select_top", "paged_sparse_sdpa", "paged_kv_mass", "kv_pages_evict",
 ]
