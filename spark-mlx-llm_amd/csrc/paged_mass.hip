@@ -30,36 +30,50 @@ __device__ __forceinline__ float row_base(float lse) {
 }
 
 // ---------------------------------------------------------------------------
-// at most 16 rows a (sequence, KV head)
+// at most 64 rows a (sequence, KV head)
 // ---------------------------------------------------------------------------
-// S^T (16 tokens x 16 rows) = K . Q^T twice a block of 32 tokens, the lane with a
-// row's scores of tokens 8g .. 8g+7; the rows' weights are summed over 16 lanes. The
-// waves of a workgroup take turns at blocks, each with the next one's loads in
-// flight. Contexts are split like the attention's.
-template <int D>
+// S^T (16 tokens x 16 rows) = K . Q^T twice a block of 32 tokens and once for each of
+// the TILES of 16 rows, the lane with a row's scores of tokens 8g .. 8g+7; the rows'
+// weights are summed over the tiles and then over 16 lanes. The waves of a workgroup
+// take turns at blocks, each with the next one's loads in flight. Contexts are split
+// like the attention's.
+// It reads the keys once, D + 2 bytes a token and KV head, and the sums it adds to: of
+// one new token each of 64 sequences of up to 8192 (8 KV heads of 128) 103 MB in 28 us,
+// where latency and the first blocks' table lookups are what is left. More tiles take
+// more products and exponentials a key, and the bytes cease to bind: 48 sequences of 8 new
+// tokens and up to 12000 (32 rows) 33 us, the kernel for more rows 93. At 64 rows the two
+// meet: 2 sequences of 16 new tokens and up to 12000 17.3 us, there 19.8; with 4 KV heads
+// of 256 18.4 and 18.8.
+template <int D, int TILES>
 __global__ __launch_bounds__(256) void paged_mass_few_kernel(MassArgs s) {
   constexpr int NK = D / 32, PL = D / 64, kBlock = kFewBlock;
   const PagedSdpaArgs& a = s.a;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, grp = lane >> 4;
   const int kh = blockIdx.x % a.Hkv, gqa = a.Hq / a.Hkv;
-  const Item it = find_item<16, false>(a, blockIdx.x / a.Hkv);
+  const Item it = find_item<16 * TILES, false>(a, blockIdx.x / a.Hkv);
   if (it.b < 0) return;
-  const int rows = it.rows, rr = min(n16, rows - 1);
-  const bool live = n16 < rows;
-  const int lim = last_seen(a, it, rr, gqa);
+  const int rows = it.rows;
   const int all = last_seen(a, it, 0, gqa) + 1;  // seen by every row
   const int nblocks = (it.length + kBlock - 1) / kBlock;
   const int ib0 = (int)((int64_t)it.part * nblocks / it.parts);
   const int ib1 = (int)((int64_t)(it.part + 1) * nblocks / it.parts);
   const TableRow trow = table_row(a, it.b);
 
-  u32x4_t qb[NK];
-  const int64_t t = it.first + rr / gqa;
-  const int head = kh * gqa + rr % gqa;
-  const float mul = load_query<NK, 4>(a, a.q + t * a.q_tok + head * a.q_head, true,
-                                      [&](int c) { return 16 * (grp + 4 * (c >> 1)) + 8 * (c & 1); }, qb);
-  const float base = row_base(s.lse[t * a.Hq + head]);
+  u32x4_t qb[TILES][NK];
+  float mul[TILES], base[TILES];
+  int lim[TILES];  // (of a row that is none: -1)
+#pragma unroll
+  for (int i = 0; i < TILES; ++i) {
+    const int r = 16 * i + n16, rr = min(r, rows - 1), rt = rr / gqa;
+    const int64_t t = it.first + rt;
+    const int head = kh * gqa + rr - rt * gqa;
+    mul[i] = load_query<NK, 4>(a, a.q + t * a.q_tok + head * a.q_head, true,
+                               [&](int c) { return 16 * (grp + 4 * (c >> 1)) + 8 * (c & 1); }, qb[i]);
+    base[i] = row_base(s.lse[t * a.Hq + head]);
+    lim[i] = r < rows ? last_seen(a, it, rr, gqa) : -1;
+  }
+  const bool full = rows == 16 * TILES;
 
   u32x4_t kr[2][PL], skr;
   float2 old;
@@ -93,32 +107,51 @@ __global__ __launch_bounds__(256) void paged_mass_few_kernel(MassArgs s) {
 
   auto block = [&](int ib) {
     const int t0 = kBlock * ib;
-    f32x4_t sc[2];
+    // (one tile's products take the keys as they come, several of them converted once)
+    u32x4_t kf[2][NK];
+    auto key = [&](int h, int c) {
+      const u32x4_t kp = kr[h][c >> 1];
+      return (c & 1) ? s8x8_exact(kp.z, kp.w) : s8x8_exact(kp.x, kp.y);
+    };
+    float ksc[8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      sc[h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < 8; ++i) ksc[i] = ((i & 1) ? hi16<F16>(skr[i >> 1]) : lo16<F16>(skr[i >> 1])) * a.sign;
+    const uint32_t ok = pages_ok;
+    const float2 was = old;
+    auto ahead = [&]() {
+      load(ib + 4, next);
+      next = block_pages<2>(a, trow, kBlock * min(ib + 8, last));
+    };
+    if constexpr (TILES > 1) {
 #pragma unroll
-      for (int c = 0; c < NK; ++c) {
-        const u32x4_t kp = kr[h][c >> 1];
-        sc[h] = mfma16x16x32_f16((c & 1) ? s8x8_exact(kp.z, kp.w) : s8x8_exact(kp.x, kp.y), qb[c], sc[h]);
-      }
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < NK; ++c) kf[h][c] = key(h, c);
+      ahead();
     }
+    const bool hidden = t0 + kBlock > all || ok != 3 || !full;
     float p[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t kw = skr[i >> 1];
-      const float v = sc[i >> 2][i & 3] * (((i & 1) ? hi16<F16>(kw) : lo16<F16>(kw)) * a.sign);
-      const float e = __builtin_amdgcn_exp2f(fmaf(v, mul, -base));
-      p[i] = live ? e : 0.0f;
-    }
-    if (__builtin_expect(t0 + kBlock > all || pages_ok != 3, 0)) {
-      const bool in = (pages_ok >> (grp >> 1)) & 1u;
+    for (int r = 0; r < TILES; ++r) {
+      f32x4_t sc[2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) p[i] = in && t0 + 8 * grp + i <= lim ? p[i] : 0.0f;
+      for (int h = 0; h < 2; ++h) {
+        sc[h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < NK; ++c) sc[h] = mfma16x16x32_f16(TILES > 1 ? kf[h][c] : key(h, c), qb[r][c], sc[h]);
+      }
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(sc[i >> 2][i & 3] * ksc[i], mul[r], -base[r]));
+      if (hidden) {
+        const int rel = (ok >> (grp >> 1)) & 1u ? lim[r] - t0 - 8 * grp : -1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = i <= rel ? e[i] : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = r == 0 ? e[i] : p[i] + e[i];
     }
-    const float2 was = old;
-    load(ib + 4, next);
-    next = block_pages<2>(a, trow, kBlock * min(ib + 8, last));
+    if constexpr (TILES == 1) ahead();
     // sums over the 16 lanes: lanes 4k + q end with tokens 2q, 2q + 1
     float h4[4], h2[2];
 #pragma unroll
@@ -163,8 +196,14 @@ __global__ __launch_bounds__(256) void paged_mass_few_kernel(MassArgs s) {
 // wave takes tiles of 32 of them as second operands. A lane then has one row's scores of 16
 // tokens, and sums its rows' weights in registers; lanes (and waves) are joined at the
 // end through LDS. Codes are exact in either 16-bit type, so queries stay as they are.
-// WAYS waves share 32 tokens and take turns at the tiles: four where the chip would
-// otherwise have less than a workgroup a CU, else one.
+// WAYS waves share 32 tokens and take turns at the tiles: two, or four where that gives
+// less than two workgroups a CU (500 new tokens of 1000, 8 KV heads: four 22 us, two 28;
+// 3 sequences of 300 and 6000, 4 KV heads of 256: two 33, four 49).
+// What it has to do is the product and an exponential a score: 2048 new tokens of 8192, 32
+// heads of 128 on 8, take 155 us, 780 TFLOP/s. The vector units bound it (66 % busy, the
+// matrix units 42 %): a multiply-add, an exponential and an addition a score, and what
+// hides the loads. Queries go straight into LDS: through registers the same tiles take
+// 164 us, as 11 of them spill.
 template <typename T>
 __device__ __forceinline__ u32x4_t codes_as(uint32_t lo, uint32_t hi);
 template <>
@@ -347,8 +386,9 @@ __global__ __launch_bounds__(512, D <= 128 ? 4 : 2) void paged_mass_many_kernel(
         load(i0 + per, buf ^ 1);
         // whether these rows see all of this wave's tokens: the first sees the least
         const bool whole = i0 + per <= count && last_seen_by(tb.s, i0, a.causal) >= w0 + 31;
+        const int live = min(per, count - i0) * gqa;
 #pragma unroll 1
-        for (int r = 32 * way; r < kRows; r += 32 * WAYS) tile(buf, r, whole);
+        for (int r = 32 * way; r < live; r += 32 * WAYS) tile(buf, r, whole);
         stage(buf ^ 1);
         __syncthreads();
       }
@@ -375,8 +415,14 @@ __global__ __launch_bounds__(512, D <= 128 ? 4 : 2) void paged_mass_many_kernel(
 }
 
 template <int D>
-void launch_few(const MassArgs& s, int64_t items, hipStream_t st) {
-  hipLaunchKernelGGL(paged_mass_few_kernel<D>, dim3((unsigned)(items * s.a.Hkv)), dim3(256), 0, st, s);
+void launch_few(const MassArgs& s, int tiles, int64_t items, hipStream_t st) {
+  const dim3 grid((unsigned)(items * s.a.Hkv));
+  if (tiles == 1)
+    hipLaunchKernelGGL((paged_mass_few_kernel<D, 1>), grid, dim3(256), 0, st, s);
+  else if (tiles == 2)
+    hipLaunchKernelGGL((paged_mass_few_kernel<D, 2>), grid, dim3(256), 0, st, s);
+  else
+    hipLaunchKernelGGL((paged_mass_few_kernel<D, 4>), grid, dim3(256), 0, st, s);
 }
 template <typename T, int D>
 void launch_many(const MassArgs& s, bool share, int64_t items, int64_t blocks, hipStream_t st) {
@@ -418,20 +464,22 @@ int paged_kv_mass(const PagedBatch& p, const void* q, const int64_t* qst, const 
   s.m_head = mst[1];
   s.tokens = (int)max_tokens;
   s.scale = scale * 1.44269504088896340736f;
-  if (max_new * gqa <= 16) {
-    // (as the attention's plan: B sequences of one tile, and the parts of split contexts)
+  if (max_new * gqa <= 64) {
+    const int tiles = max_new * gqa <= 16 ? 1 : max_new * gqa <= 32 ? 2 : 4;
+    // (as the attention's plan: B sequences of one tile, and the parts of split contexts,
+    // about as many as the chip holds at once)
     s.a.min_part = 128;
-    s.a.target = (int)std::min<int64_t>(cdiv(4 * device_cus(), Hkv), 512);
+    s.a.target = (int)std::min<int64_t>(cdiv((tiles == 1 ? 4 : 2) * device_cus(), Hkv), 512);
     const int64_t split = max_tokens > 128 ? std::min<int64_t>(p.B, s.a.target) : 0;
     s.a.slots = (int)std::min<int64_t>(2 * s.a.target, split * cdiv(max_tokens, 128));
     const int64_t items = s.a.slots + p.B;
     if (items > kMaxGrid / Hkv) return set_error(SPARKQ_ERR_INVALID, "paged_kv_mass: shape too large");
     if (D == 64)
-      launch_few<64>(s, items, st);
+      launch_few<64>(s, tiles, items, st);
     else if (D == 128)
-      launch_few<128>(s, items, st);
+      launch_few<128>(s, tiles, items, st);
     else
-      launch_few<256>(s, items, st);
+      launch_few<256>(s, tiles, items, st);
     return check_launch("paged_mass_few_kernel");
   }
   const bool share = p.B * cdiv(max_tokens, mass_tokens(2)) * Hkv < 2 * device_cus();
