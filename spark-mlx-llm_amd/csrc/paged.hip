@@ -592,9 +592,15 @@ __global__ __launch_bounds__(256) void pages_evict_table_kernel(EvictArgs e) {
 // kept tokens in order, a chunk at a time: every load of a chunk is done before its
 // first store. What a chunk writes lies before all that later chunks read (keep[i] >=
 // i), so their loads need not wait for it.
+// A slice is 128 bytes, a line of the cache (halves of one make the writes twice: 225 us
+// where these take 124), and a chunk a token a thread, as each is a chain of keep, table,
+// load, store. 16 rows of up to 6000 tokens that keep 1500, 8 layers
+// of 8 heads of 128, take 119 us with 1024 threads, 121 with 512, 124 with 256; 4 rows in
+// one layer 12, 14 and 21. 24 such rows move 868 MB in 167 us, 5.2 TB/s.
+constexpr int kEvictThreads = 1024;
 template <int LPT>  // 16-byte pieces of a token in a slice
-__global__ __launch_bounds__(256) void pages_evict_kernel(EvictArgs e) {
-  constexpr int TPP = 256 / LPT, U = 8, C = U * TPP, S = (C + 255) / 256;
+__global__ __launch_bounds__(kEvictThreads) void pages_evict_kernel(EvictArgs e) {
+  constexpr int C = kEvictThreads, U = LPT, TPP = C / U;  // tokens of a chunk, loads of a thread, tokens between them
   const PageArgs& a = e.p;
   const int tid = threadIdx.x;
   int x = blockIdx.x;
@@ -643,20 +649,15 @@ __global__ __launch_bounds__(256) void pages_evict_kernel(EvictArgs e) {
         v[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(
             codes + mv[u].from * c_page + (int64_t)(mv[u].src & mask) * e.D + 16 * (tid % LPT)));
     }
-    Move sm[S];
-    uint16_t sc[S];
-    float w[S];
-#pragma unroll
-    for (int u = 0; u < S; ++u) {
-      const int k = tid + 256 * u, i = i0 + k;
-      sm[u].to = -1;
-      if (slice == 0 && k < C && i < e.count) {
-        sm[u] = find(i);
-        sc[u] = 0x3C00u;  // a token without a page comes as zeros with scale 1
-        if (sm[u].from >= 0)
-          sc[u] = *reinterpret_cast<const uint16_t*>(scales + sm[u].from * s_page + 2 * (sm[u].src & mask));
-        if (mass) w[u] = mass[sm[u].src];
-      }
+    Move sm;
+    uint16_t sc;
+    float w;
+    const bool mine = slice == 0 && i0 + tid < e.count;
+    if (mine) {
+      sm = find(i0 + tid);
+      sc = 0x3C00u;  // a token without a page comes as zeros with scale 1
+      if (sm.from >= 0) sc = *reinterpret_cast<const uint16_t*>(scales + sm.from * s_page + 2 * (sm.src & mask));
+      if (mass) w = mass[sm.src];
     }
     // (a load in flight still reads memory that another thread may write)
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -668,12 +669,9 @@ __global__ __launch_bounds__(256) void pages_evict_kernel(EvictArgs e) {
       if (mv[u].to >= 0)
         __builtin_nontemporal_store(v[u], reinterpret_cast<u32x4_t*>(codes + mv[u].to * c_page +
                                                                      (int64_t)mv[u].slot * e.D + 16 * (tid % LPT)));
-#pragma unroll
-    for (int u = 0; u < S; ++u) {
-      const int k = tid + 256 * u, i = i0 + k;
-      if (slice != 0 || k >= C || i >= e.count) continue;
-      if (mass) mass[i] = w[u];
-      if (sm[u].to >= 0) *reinterpret_cast<uint16_t*>(scales + sm[u].to * s_page + 2 * sm[u].slot) = sc[u];
+    if (mine) {
+      if (mass) mass[i0 + tid] = w;
+      if (sm.to >= 0) *reinterpret_cast<uint16_t*>(scales + sm.to * s_page + 2 * sm.slot) = sc;
     }
   }
 }
@@ -782,11 +780,8 @@ int kv_pages_evict(const int32_t* table, int64_t table_stride, const int32_t* le
   e.H = (int)H;
   e.D = (int)D;
   e.count = (int)count;
-  // tokens in slices of 64 bytes where whole ones would not fill the chip
+  e.slices = (int)cdiv(D, 128);
   const int64_t groups = layers * B * H * 2;
-  const bool sliced = groups < 4 * device_cus();
-  const int pieces = sliced ? 4 : (int)(D / 16);
-  e.slices = (int)(D / 16 / pieces);
   if (groups > kMaxGrid / e.slices) return set_error(SPARKQ_ERR_INVALID, "kv_pages_evict: shape too large");
   e.tables = B * cdiv(width, 64) <= 128;  // (no more than 8 rounds a wave: 0.5 us each)
   if (pages <= kLdsPages)
@@ -796,12 +791,10 @@ int kv_pages_evict(const int32_t* table, int64_t table_stride, const int32_t* le
   if (B == 0) return check_launch("pages_evict_kernel");
   if (!e.tables) hipLaunchKernelGGL(pages_evict_table_kernel, dim3((unsigned)cdiv(B, 4)), dim3(256), 0, st, e);
   const dim3 grid((unsigned)(groups * e.slices));
-  if (pieces == 4)
-    hipLaunchKernelGGL(pages_evict_kernel<4>, grid, dim3(256), 0, st, e);
-  else if (pieces == 8)
-    hipLaunchKernelGGL(pages_evict_kernel<8>, grid, dim3(256), 0, st, e);
+  if (D == 64)
+    hipLaunchKernelGGL(pages_evict_kernel<4>, grid, dim3(kEvictThreads), 0, st, e);
   else
-    hipLaunchKernelGGL(pages_evict_kernel<16>, grid, dim3(256), 0, st, e);
+    hipLaunchKernelGGL(pages_evict_kernel<8>, grid, dim3(kEvictThreads), 0, st, e);
   return check_launch("pages_evict_kernel");
 }
 

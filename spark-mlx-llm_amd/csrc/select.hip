@@ -74,6 +74,8 @@ __device__ __forceinline__ uint32_t kth_key(const uint32_t (&key)[KPT], int k, u
 // ---------------------------------------------------------------------------
 // a wave a row: rows of up to 64 * KPT values, which stay in registers
 // ---------------------------------------------------------------------------
+// A chain of at most 32 counts, each KPT ballots: 128 rows of up to 512 (0.1 MB) take
+// 5.8 us, about 3 of them a launch's and the load's latency.
 template <int KPT>
 __global__ __launch_bounds__(256) void select_wave_kernel(SelectArgs a) {
   const int lane = threadIdx.x & 63;
@@ -121,6 +123,9 @@ __global__ __launch_bounds__(256) void select_wave_kernel(SelectArgs a) {
 // with the digits found so far have each next one, and down from the largest which
 // digit the k-th has. Where few enough keys share its first digit they are listed, and
 // one wave finds it among them.
+// 1024 rows of up to 8192 values (30 MB) take 20.5 us, where a copy of them takes 6: four
+// workgroups a CU go through one chain of barriers each, the counting in LDS first among
+// what they wait for.
 constexpr int kBins = 2048, kListed = 512, kPerThread = 16;
 
 template <int W, bool HELD>
@@ -315,6 +320,10 @@ int select_top(const float* x, const int32_t* lengths, int32_t* out, int64_t lay
   if (total == 0) return SPARKQ_OK;
   const SelectArgs a{x, lengths, out, st[0], st[1], st[2], (uint32_t)total, (int)rows, (int)heads, (int)n, (int)count,
                      (int)first, (int)last};
+  // Up to 1024 values a wave a row: 2048 rows of 1000 take 10.7 us, with a workgroup each
+  // 12.6 or more; rows of 2000 13.4 with a workgroup, 17.4 with a wave. The smallest
+  // workgroup that holds the keys of longer ones; without (rows of 16000) 2048 rows take
+  // 83 us, with them 64.
   if (n <= 256)
     launch_wave<4>(a, stream);
   else if (n <= 512)
