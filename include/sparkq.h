@@ -772,7 +772,8 @@ int sparkq_paged_sparse_sdpa(const void* q, const void* k_codes, const void* k_s
  * holds. mass float32 [B,Hkv,max_pages * page_size], mass_strides[0..1] = sequence,
  * head in elements (even, mass 16-byte aligned), the last axis contiguous; places
  * from lengths[b] on and sequences without new tokens are left as they were. Sums
- * are fp32, always in the same order. */
+ * are fp32, always in the same order. At most 128 query heads to a KV head; a row's
+ * query heads lie within 2^30 elements, rows less than 2^31 apart. */
 int sparkq_paged_kv_mass(const void* q, const float* lse, const void* k_codes,
                          const void* k_scales, float* mass, const int32_t* page_table,
                          const int32_t* starts, const int32_t* lengths, int64_t T, int64_t B,

@@ -1294,6 +1294,8 @@ int sparkq_kv_pages_evict(void* k_codes, void* v_codes, void* k_scales, void* v_
                               page_size, Hkv * page_size * D, 2 * Hkv * page_size, workspace, workspace_bytes))
     return rc;
   REQUIRE(B == 0 || layers <= kI32Max / 2 / (B * Hkv), "kv_pages_evict: shape too large");
+  for (int i = 0; i < 4; ++i)  // (what moves in place must not be another layer's too)
+    REQUIRE(layers == 1 || buf_strides[2 * i] >= Hkv * page_size * (i < 2 ? D : 2), "kv_pages_evict: layers overlap");
   if (mass) {
     const int64_t tokens = max_pages * page_size;
     REQUIRE(mass_strides && aligned(mass, 4), "kv_pages_evict: null tensor pointer");

@@ -379,8 +379,10 @@ def paged_kv_mass(queries, lse, cache, mass, page_table, starts, lengths, *, sca
     over a sequence's new tokens t that see the token and the query heads g of the KV
     head, with queries, cache, scale and mask of the attention and the lse [T,Hq]
     that paged_quantized_sdpa(return_lse=True) returned for them. A batch's new tokens
-    start from 0, whatever mass holds there. Sums are fp32, in one order. max_new is
-    the most new tokens that a sequence has; those of one past it add nothing."""
+    start from 0, whatever mass holds there, so a step's tokens are weighed once. Sums
+    are fp32, in one order. max_new is the most new tokens that a sequence has; those of
+    one past it add nothing. What is seen by a row whose lse is NaN, or has a key
+    scale that is not finite, has no finite sum. At most 128 query heads to a KV head."""
     op = "paged_kv_mass"
     kc, ks, _, _, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
     _check_attention(op, queries, hkv, d, index, mask, scale, max_new)
@@ -574,7 +576,8 @@ class PagedKVCache:
         out = cache.attend_pages(l, queries, scale=..., count=32)
 
     attends the `count` pages of each KV head that score highest instead of all. With
-    mass=True attend() adds up the attention weight that each token gathers, and
+    mass=True attend(), called once for a step and layer, adds up the attention weight
+    that each token gathers, and
 
         cache.evict(count)                           # between steps
 

@@ -615,3 +615,16 @@ def test_evict_of_one_layer(gpu):
     for a, b in zip(dev, cache):
         assert torch.equal(a.cpu(), b[0])
     assert torch.equal(m.cpu(), after[0])
+
+
+@pytest.mark.parametrize("hkv,d", [(2, 64), (1, 128), (1, 256)])
+def test_evict_in_chunks(gpu, hkv, d):
+    """More tokens than a workgroup takes at a time, from all over the row."""
+    rng, gen = random.Random(d), torch.Generator().manual_seed(d)
+    page, lengths, count = 64, [5000, 2500, 2301, 900], 2300
+    width = 80
+    pages = sum(-(-n // page) for n in lengths) + 1
+    pool = ref.pool(gen, pages, hkv, page, d, layers=2)
+    table = ref.tables(rng, lengths, page, pages, width)
+    mass = torch.rand((2, len(lengths), hkv, width * page), generator=gen)
+    run_evict(gpu, pool, _keeps(rng, lengths, 2, hkv, count), table, lengths, mass)
