@@ -794,7 +794,9 @@ int sparkq_paged_kv_mass(const void* q, const float* lse, const void* k_codes,
  * pages short: when it is not 0 nothing was moved, and out_table and out_lengths are
  * the old ones. A kept token without a page comes as zeros. Pools, buf_strides and
  * workspace (sparkq_kv_pages_workspace_bytes(B, pages)) as in sparkq_kv_pages_fork,
- * with a page's codes [Hkv,page_size,D] and scales [Hkv,page_size] contiguous. */
+ * with a page's codes [Hkv,page_size,D] and scales [Hkv,page_size] contiguous and
+ * layers that do not overlap; 2 layers * B * Hkv at most 2^22 - 1 (half of it at D =
+ * 256). */
 int sparkq_kv_pages_evict(void* k_codes, void* v_codes, void* k_scales, void* v_scales,
                           const int32_t* keep, float* mass, const int32_t* page_table,
                           const int32_t* lengths, int64_t table_stride, int32_t* out_table,

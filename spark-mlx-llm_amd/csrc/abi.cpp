@@ -1185,8 +1185,8 @@ int sparkq_paged_kv_mass(const void* q, const float* lse, const void* k_codes, c
   for (int i = 0; i < 12; ++i) both[i] = strides[i % 6];
   // (mass in the outputs' place: aligned like them, and none of no sequences)
   if (int rc = paged_attn_check("paged_kv_mass", T, B, Hq, Hkv, D, pages, max_pages, table_stride, page_size, max_new, q,
-                                B == 0 ? q : (const void*)mass, page_table, starts, lengths, k_codes, k_scales, k_codes, k_scales, q_strides, both,
-                                q_dtype, q_dtype, scale))
+                                B == 0 ? q : (const void*)mass, page_table, starts, lengths, k_codes, k_scales,
+                                k_codes, k_scales, q_strides, both, q_dtype, q_dtype, scale))
     return rc;
   REQUIRE((T == 0 || lse) && mass_strides && aligned(lse, 4), "paged_kv_mass: null tensor pointer");
   const int64_t tokens = max_pages * page_size;
@@ -1293,7 +1293,9 @@ int sparkq_kv_pages_evict(void* k_codes, void* v_codes, void* k_scales, void* v_
   if (int rc = kv_pages_check("kv_pages_evict", bufs, buf_strides, B, B, max_pages, pages, layers, table_stride,
                               page_size, Hkv * page_size * D, 2 * Hkv * page_size, workspace, workspace_bytes))
     return rc;
-  REQUIRE(B == 0 || layers <= kI32Max / 2 / (B * Hkv), "kv_pages_evict: shape too large");
+  // (a workgroup of 1024 threads for 128 bytes of each list's keys and of its values, fewer
+  // than 2^32 threads)
+  REQUIRE(B == 0 || layers <= 0x3FFFFF / (D > 128 ? 4 : 2) / Hkv / B, "kv_pages_evict: shape too large");
   for (int i = 0; i < 4; ++i)  // (what moves in place must not be another layer's too)
     REQUIRE(layers == 1 || buf_strides[2 * i] >= Hkv * page_size * (i < 2 ? D : 2), "kv_pages_evict: layers overlap");
   if (mass) {

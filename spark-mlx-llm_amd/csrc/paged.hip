@@ -782,7 +782,6 @@ int kv_pages_evict(const int32_t* table, int64_t table_stride, const int32_t* le
   e.count = (int)count;
   e.slices = (int)cdiv(D, 128);
   const int64_t groups = layers * B * H * 2;
-  if (groups > kMaxGrid / e.slices) return set_error(SPARKQ_ERR_INVALID, "kv_pages_evict: shape too large");
   e.tables = B * cdiv(width, 64) <= 128;  // (no more than 8 rounds a wave: 0.5 us each)
   if (pages <= kLdsPages)
     hipLaunchKernelGGL(pages_evict_plan_kernel<true>, dim3(1), dim3(kPlanThreads), pages * sizeof(int), st, e);

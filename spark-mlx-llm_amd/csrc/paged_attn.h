@@ -56,7 +56,7 @@ struct SeqWork {
   int first, count, length, rows, tiles;
 };
 
-template <int R>  // rows of a tile: 16 or 128
+template <int R>  // rows of a tile
 __device__ __forceinline__ SeqWork seq_work(const PagedSdpaArgs& a, int b) {
   SeqWork w{0, 0, 0, 0, 0};
   if (b < a.p.B) {

@@ -628,3 +628,63 @@ def test_evict_in_chunks(gpu, hkv, d):
     table = ref.tables(rng, lengths, page, pages, width)
     mass = torch.rand((2, len(lengths), hkv, width * page), generator=gen)
     run_evict(gpu, pool, _keeps(rng, lengths, 2, hkv, count), table, lengths, mass)
+
+
+def test_evict_in_a_strided_pool(gpu):
+    """Every second page of a larger pool with the layers inside, mass of a wider tensor:
+    what lies between stays as it was."""
+    import sparkq
+
+    rng, gen = random.Random(5), torch.Generator().manual_seed(5)
+    page, lengths, count = 16, [300, 90, 200], 77
+    pool = ref.pool(gen, 40, 2, page, 128, layers=3)
+    table = ref.tables(rng, lengths, page, 40, 20)
+    mass, keep = torch.rand((3, 3, 2, 20 * page), generator=gen), _keeps(rng, lengths, 3, 2, count)
+    wide = [torch.full((40, 2, 3, *t.shape[2:]), 5, dtype=t.dtype, device=gpu) for t in pool]
+    dev = [t[:, 1].transpose(0, 1) for t in wide]
+    for a, b in zip(dev, pool):
+        a.copy_(b)
+    m = torch.full((3, 3, 3, 20 * page + 1), 7.0, device=gpu)
+    m[:, :, 1:, 1:] = mass.to(gpu)
+    got = sparkq.kv_pages_evict(dev, keep.to(gpu), _ints(table, gpu), _ints(lengths, gpu),
+                                mass=m[:, :, 1:, 1:])
+    want = long.evict(table, lengths, count, 40, page)
+    assert got[0].tolist() == want[0] and got[1].tolist() == want[1]
+    cache, after = long.moved(pool, mass, keep, table, lengths, want[0], want[1])
+    for a, b, t in zip(dev, cache, wide):
+        assert torch.equal(a.cpu(), b) and (t[:, 0] == 5).all()
+    assert torch.equal(m[:, :, 1:, 1:].cpu(), after)
+    assert (m[:, :, 0] == 7.0).all() and (m[..., 0] == 7.0).all()
+
+
+# --- gathered weight at every count of rows ----------------------------------------
+
+@pytest.mark.parametrize("new", [5, 10, 40])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [128, 256])
+def test_mass_of_all_kinds_of_batches_by_rows(gpu, new, causal, d):
+    """15, 30 and 120 rows a KV head, where the ones above have 3, 9 and 60."""
+    test_mass_of_all_kinds_of_batches(gpu, new, causal, d)
+
+
+@pytest.mark.parametrize("new", [1, 4, 8, 16, 17])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 64), (8, 2, 128), (4, 1, 256)])
+def test_mass_of_many_sequences(gpu, new, hq, hkv, d):
+    """More sequences than a wave has lanes, among them long ones that are split and idle
+    ones: 4 to 68 rows a KV head."""
+    import sparkq
+
+    rng = random.Random(new)
+    lengths = [rng.choice([new, new + 1, 40, 333]) for _ in range(70)]
+    lengths[3], lengths[66] = 4100, 1999
+    lengths = [max(n, new) for n in lengths]
+    news = [0 if i % 9 == 7 else new - (i % 2) * (new > 1) for i in range(70)]
+    q, _, _, cache, table, starts = ref.batch(new, lengths, news, hq, hkv, d, 32)
+    q = q.to(BF)
+    dev, at = tuple(t.to(gpu) for t in cache), _gpu(gpu, table, starts, lengths)
+    kw = {"scale": d ** -0.5, "max_new": new}
+    _, lse = sparkq.paged_quantized_sdpa(q.to(gpu), dev, *at, return_lse=True, **kw)
+    before = torch.rand((70, hkv, len(table[0]) * 32))
+    got = before.to(gpu)
+    sparkq.paged_kv_mass(q.to(gpu), lse, dev, got, *at, **kw)
+    check_mass(got, q, lse.cpu(), cache, before, table, starts, lengths, d ** -0.5)

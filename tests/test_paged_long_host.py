@@ -192,7 +192,7 @@ def test_abi_eviction():
         (15, 0, -1, "shape"), (21, 8, -1, "page_size"), (21, 48, -1, "page_size"), (8, 1, -1, "overlap"),
         (22, None, -4, "workspace"), (23, 8, -4, "workspace"), (13, i64(192, 64, 31), -1, "overlap"),
         (13, i64(192, 31, 32), -1, "overlap"), (12, i64(8192, 2040, 8192, 2048, 512, 64, 512, 64), -1, "apart"),
-        (14, 2 ** 30, -1, "large"), (12, i64(0, 2048, 8192, 2048, 512, 64, 512, 64), -1, "layers overlap"),
+        (14, 2 ** 30, -1, "large"), (20, 2 ** 20, -1, "large"), (12, i64(0, 2048, 8192, 2048, 512, 64, 512, 64), -1, "layers overlap"),
         (12, i64(8192, 2048, 8192, 2048, 512, 64, 48, 64), -1, "layers overlap")])
 
 
