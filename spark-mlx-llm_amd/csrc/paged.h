@@ -65,15 +65,29 @@ __device__ __forceinline__ int seq_of_row(const PagedBatch& p, int t) {
   return lo < p.B ? lo : -1;
 }
 
-// the same in one round trip for every 64 sequences: all lanes of a wave ask for the
-// same row
-__device__ __forceinline__ int wave_seq_of_row(const PagedBatch& p, int t) {
+// The sequence whose rows hold packed row t, or b = -1, in one round trip for every 64
+// sequences: all lanes of a wave ask for the same row.
+struct RowOf {
+  int b;
+  SeqRows s;
+};
+__device__ __forceinline__ RowOf wave_row(const PagedBatch& p, int t) {
   const int lane = threadIdx.x & 63;
+  RowOf r{-1, {0, 0, 0}};
   for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const unsigned long long past = __ballot(b0 + lane < p.B && p.starts[min(b0 + lane, p.B - 1) + 1] > t);
-    if (past) return b0 + __builtin_ctzll(past);
+    const int b = min(b0 + lane, p.B - 1);
+    const SeqRows s = seq_rows(p, b);
+    const unsigned long long past = __ballot(b0 + lane < p.B && p.starts[b + 1] > t);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      r = RowOf{b0 + l, {__builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.count, l),
+                         __builtin_amdgcn_readlane(s.length, l)}};
+      break;
+    }
   }
-  return -1;
+  // (the compiler does not see that a loop left on a ballot leaves scalars)
+  for (int* f : {&r.b, &r.s.first, &r.s.count, &r.s.length}) *f = __builtin_amdgcn_readfirstlane(*f);
+  return r;
 }
 
 // last token that row i of a sequence's new tokens sees (-1: none)

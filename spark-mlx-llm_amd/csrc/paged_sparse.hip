@@ -35,22 +35,24 @@ struct Listed {
   int n;
 };
 
-// Entries [e0, e1) of a list, no more than kListed, looked up by the first wave.
+// Entries [e0, e1) of a list, no more than kListed, looked up by the first wave; j are
+// its first 64.
 __device__ __forceinline__ void look_up(const SparseArgs& s, Listed& l, const int32_t* list, int b, int lim, int e0,
-                                        int e1) {
+                                        int e1, int j) {
   const PagedBatch& p = s.a.p;
   const int lane = threadIdx.x & 63;
   int n = 0;
   for (int e = e0; e < e1; e += 64) {
-    const int j = e + lane < e1 ? list[e + lane] : -1;
-    bool in = (unsigned)j < (unsigned)p.width && ((int64_t)j << p.page_log2) <= lim;
+    bool in = e + lane < e1 && (unsigned)j < (unsigned)p.width && ((int64_t)j << p.page_log2) <= lim;
     const int id = p.table[b * p.table_stride + (in ? j : 0)];
     in = in && (unsigned)id < (unsigned)p.pages;
+    const int at_j = j;
+    j = list[min(e + 64 + lane, e1 - 1)];
     const unsigned long long m = __ballot(in);
     if (in) {
       const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
       l.id[at] = id;
-      l.pos[at] = j << p.page_log2;
+      l.pos[at] = at_j << p.page_log2;
     }
     n += __builtin_popcountll(m);
   }
@@ -100,9 +102,14 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_sparse_kernel(Spa
   const int part = x % s.parts;
   x /= s.parts;
   const int tile = x % s.tiles, t = x / s.tiles;
-  const int b = wave_seq_of_row(a.p, t);
+  const int32_t* list = s.list + t * s.l_tok + kh * s.l_head;
+  const int e_first = (int)((int64_t)part * s.count / s.parts), e_end = (int)((int64_t)(part + 1) * s.count / s.parts);
+  // (asked for before it is known whose row this is)
+  const int j_first = list[min(e_first + lane, s.count - 1)];
+  const RowOf ro = wave_row(a.p, t);
+  const int b = ro.b;
   if (b < 0) return;
-  const SeqRows sq = seq_rows(a.p, b);
+  const SeqRows sq = ro.s;
   const int i_row = t - sq.first;
   if (i_row < 0 || i_row >= min(sq.count, a.max_new)) return;
   const int lim = last_seen_by(sq, i_row, a.causal);
@@ -239,11 +246,9 @@ __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_sparse_kernel(Spa
     }
   };
 
-  const int32_t* list = s.list + t * s.l_tok + kh * s.l_head;
-  const int e_end = (int)((int64_t)(part + 1) * s.count / s.parts);
-  for (int e = (int)((int64_t)part * s.count / s.parts); e < e_end; e += kListed) {
-    __syncthreads();  // the pages looked up before are done with
-    if (wave == 0) look_up(s, lst, list, b, lim, e, min(e + kListed, e_end));
+  for (int e = e_first; e < e_end; e += kListed) {
+    if (e != e_first) __syncthreads();  // the pages looked up before are done with
+    if (wave == 0) look_up(s, lst, list, b, lim, e, min(e + kListed, e_end), e == e_first ? j_first : list[min(e + lane, e_end - 1)]);
     __syncthreads();
     listed = __builtin_amdgcn_readfirstlane(lst.n);
     const int blocks = ((listed << a.p.page_log2) + kFewBlock - 1) / kFewBlock;
@@ -307,9 +312,9 @@ __global__ __launch_bounds__(256) void paged_sparse_merge_kernel(SparseArgs s) {
   const PagedSdpaArgs& a = s.a;
   const int kh = blockIdx.x % a.Hkv, gqa = a.Hq / a.Hkv, x = blockIdx.x / a.Hkv;
   const int tile = x % s.tiles, t = x / s.tiles;
-  const int b = wave_seq_of_row(a.p, t);
-  if (b < 0) return;
-  const SeqRows sq = seq_rows(a.p, b);
+  const RowOf ro = wave_row(a.p, t);
+  const SeqRows sq = ro.s;
+  if (ro.b < 0) return;
   if (t < sq.first || t - sq.first >= min(sq.count, a.max_new)) return;
   const int rows = min(gqa - 16 * tile, 16);
   const int64_t base = ((((int64_t)t * a.Hkv + kh) * s.tiles + tile) * s.parts) * s.rows_held;
