@@ -68,12 +68,12 @@ __global__ __launch_bounds__(256) void paged_mass_few_kernel(MassArgs s) {
     const int r = 16 * i + n16, rr = min(r, rows - 1), rt = rr / gqa;
     const int64_t t = it.first + rt;
     const int head = kh * gqa + rr - rt * gqa;
-    mul[i] = load_query<NK, 4>(a, a.q + t * a.q_tok + head * a.q_head, true,
-                               [&](int c) { return 16 * (grp + 4 * (c >> 1)) + 8 * (c & 1); }, qb[i]);
-    base[i] = row_base(s.lse[t * a.Hq + head]);
+    mul[i] = a.sign * load_query<NK, 4>(a, a.q + t * a.q_tok + head * a.q_head, true,
+                                        [&](int c) { return 16 * (grp + 4 * (c >> 1)) + 8 * (c & 1); }, qb[i]);
+    // (a row that is none has the last one's scores, and no weight)
+    base[i] = r < rows ? row_base(s.lse[t * a.Hq + head]) : __builtin_huge_valf();
     lim[i] = r < rows ? last_seen(a, it, rr, gqa) : -1;
   }
-  const bool full = rows == 16 * TILES;
 
   u32x4_t kr[2][PL], skr;
   float2 old;
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256) void paged_mass_few_kernel(MassArgs s) {
     };
     float ksc[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ksc[i] = ((i & 1) ? hi16<F16>(skr[i >> 1]) : lo16<F16>(skr[i >> 1])) * a.sign;
+    for (int i = 0; i < 8; ++i) ksc[i] = (i & 1) ? hi16<F16>(skr[i >> 1]) : lo16<F16>(skr[i >> 1]);
     const uint32_t ok = pages_ok;
     const float2 was = old;
     auto ahead = [&]() {
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(256) void paged_mass_few_kernel(MassArgs s) {
         for (int c = 0; c < NK; ++c) kf[h][c] = key(h, c);
       ahead();
     }
-    const bool hidden = t0 + kBlock > all || ok != 3 || !full;
+    const bool hidden = t0 + kBlock > all || ok != 3;
     float p[8];
 #pragma unroll
     for (int r = 0; r < TILES; ++r) {
