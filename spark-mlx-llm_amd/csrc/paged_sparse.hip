@@ -361,7 +361,7 @@ struct SparsePlan {
   int64_t tiles, parts, rows_held;
 };
 
-SparsePlan sparse_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t count, int64_t page) {
+SparsePlan sparse_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t count, int64_t page) {
   SparsePlan p;
   const int64_t gqa = Hq / Hkv;
   p.tiles = cdiv(gqa, 16);
@@ -370,9 +370,10 @@ SparsePlan sparse_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t count, int64_
   // 128 tokens (a block for each wave). More parts fill the chip better, but joining
   // them costs 4 us: 224 lists of 77 pages of 32 tokens at D = 256 take 51 us whole, 53
   // + 5 in two parts; 56 lists of 32 pages of 64 at D = 128 15 + 4 in four, 17 + 4 in ten.
-  // Lists of up to 512 tokens stay whole: 8 of them take 10.6 us, in four parts 10.0 in a
-  // graph and a launch more without one.
-  const int64_t most = count * page <= 512 ? 1 : std::min(cdiv(count * page, 128), count);
+  // Lists that four waves take about as long for as a join stay whole, one launch less: 8
+  // lists of 512 tokens at D = 128 10.6 us (split 9.7), of 256 at D = 256 10.9 (11.7).
+  const int64_t most =
+      count * page <= (D <= 128 ? 512 : 256) ? 1 : std::min(cdiv(count * page, 128), count);
   p.parts = std::max<int64_t>(std::min(device_cus() / std::max<int64_t>(T * Hkv * p.tiles, 1), most), 1);
   return p;
 }
@@ -387,7 +388,7 @@ void launch_sparse(const SparseArgs& s, hipStream_t st) {
 }  // namespace
 
 size_t paged_sparse_workspace(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t count, int64_t page) {
-  const SparsePlan p = sparse_plan(T, Hq, Hkv, count, page);
+  const SparsePlan p = sparse_plan(T, Hq, Hkv, D, count, page);
   return p.parts == 1 ? 0 : (size_t)(T * Hkv * p.tiles * p.parts * p.rows_held * (D + 2)) * sizeof(float);
 }
 
@@ -397,7 +398,7 @@ int paged_sparse_sdpa(const PagedBatch& p, const void* q, const int64_t* qst, co
                       hipStream_t st) {
   if (p.T == 0 || p.B == 0) return SPARKQ_OK;
   const int64_t page = 1LL << p.page_log2;
-  const SparsePlan plan = sparse_plan(p.T, Hq, Hkv, count, page);
+  const SparsePlan plan = sparse_plan(p.T, Hq, Hkv, D, count, page);
   const size_t need = paged_sparse_workspace(p.T, Hq, Hkv, D, count, page);
   if (need > 0 && (!ws || wsb < need))
     return set_error(SPARKQ_ERR_WORKSPACE, "paged_sparse_sdpa needs a workspace of %zu bytes (got %zu)", need,
