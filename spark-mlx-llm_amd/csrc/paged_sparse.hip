@@ -84,8 +84,8 @@ struct Runs {
 // Bytes bound it, 2 (D + 2) a listed token and KV head: 56 decoded tokens with lists of
 // 77 pages of 32, 4 KV heads of 256 (196 MB), take 51 us, 3.85 TB/s of the 5.1 that a
 // copy reaches: 224 workgroups of four waves are what keeps loads in flight (eight waves:
-// 54 us). One sequence of 32 pages of 64, 8 KV heads of 128 (4.3 MB), is latency: 7.5 us,
-// and 3.9 for the parts' join; unsplit lists, which need no join, take 24 there with four
+// 54 us). One sequence of 32 pages of 64, 8 KV heads of 128 (4.3 MB), is latency: 7.3 us,
+// and 3.8 for the parts' join; unsplit lists, which need no join, take 24 there with four
 // waves, 21 with eight, as a block's 380 vector instructions then follow each other.
 template <int D>
 __global__ __launch_bounds__(256, D <= 128 ? 3 : 2) void paged_sparse_kernel(SparseArgs s) {
