@@ -688,3 +688,42 @@ def test_mass_of_many_sequences(gpu, new, hq, hkv, d):
     got = before.to(gpu)
     sparkq.paged_kv_mass(q.to(gpu), lse, dev, got, *at, **kw)
     check_mass(got, q, lse.cpu(), cache, before, table, starts, lengths, d ** -0.5)
+
+
+# --- a pool whose offsets need more than 32 bits -----------------------------------
+
+def test_a_pool_past_4_gib(gpu):
+    """The same sequences in a small pool and behind 4 GiB of a large one: every result is
+    the same, bit for bit."""
+    import sparkq
+
+    hkv, d, page, lengths, news = 2, 256, 64, [700, 64, 333], [20, 0, 1]
+    q, _, _, cache, table, starts = ref.batch(21, lengths, news, 8, hkv, d, page, spare=4)
+    n = cache[0].shape[0]
+    small = [t.to(gpu) for t in cache]
+    base = 2 ** 32 // (hkv * page * d) + 3
+    large = [torch.zeros((base + n, *t.shape[1:]), dtype=t.dtype, device=gpu) for t in cache]
+    for a, b in zip(large, small):
+        a[base:] = b
+    assert large[0].numel() > 2 ** 32
+    tables = [table, [[base + p if p >= 0 else p for p in row] for row in table]]
+    mass = torch.rand((1, 3, hkv, len(table[0]) * page)).to(gpu)
+    q, keep = q.to(F16).to(gpu), _keeps(random.Random(21), lengths, 1, hkv, 250)[0].to(gpu)
+    results = []
+    for c, tab in zip((small, large), tables):
+        at, m = _gpu(gpu, tab, starts, lengths), mass[0].clone()
+        bnd = torch.zeros((c[0].shape[0], hkv, 2, d), dtype=BF, device=gpu)
+        sparkq.paged_key_bounds(c, bnd, at[0], _ints([0, 700, 764, 1097], gpu), at[2], max_new=700)
+        scores, seen = sparkq.paged_page_scores(q, bnd, *at, page_size=page, scale=0.1, max_new=20)
+        pages = sparkq.select_top(scores, 3, lengths=seen, first=1, last=1)
+        out = sparkq.paged_sparse_sdpa(q, c, pages, *at, scale=0.1, max_new=20)
+        full, lse = sparkq.paged_quantized_sdpa(q, c, *at, scale=0.1, max_new=20, return_lse=True)
+        for new in (20, 1):  # (of a sequence's first row alone, then)
+            sparkq.paged_kv_mass(q, lse, c, m, *at, scale=0.1, max_new=new)
+        evicted = sparkq.kv_pages_evict(c, keep, at[0], at[2], mass=m)
+        shift = c[0].shape[0] - n
+        new_table = torch.where(evicted[0] >= 0, evicted[0] - shift, evicted[0])
+        results.append([bnd[shift:], scores, seen, pages, out, full, lse, m, new_table, *evicted[1:],
+                        *(t[shift:] for t in c)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
