@@ -115,21 +115,20 @@ __global__ __launch_bounds__(256) void select_wave_kernel(SelectArgs a) {
 // a workgroup a row
 // ---------------------------------------------------------------------------
 // Wave w of W has the places [w per, (w + 1) per), 64 KPT of them at a time: the keys
-// of rows of up to 64 W KPT values stay in registers (HELD), those of longer ones are
-// made again from the values in every pass. (In LDS they let three workgroups on a CU
-// where four fit.)
+// of rows of up to 64 W KPT values stay in registers (HELD), those of others are made
+// again from the values in every pass. (In LDS they let three workgroups on a CU where
+// four fit.)
 //
 // The k-th largest key is found by digits of 11, 11 and 10 bits: how many of the keys
 // with the digits found so far have each next one, and down from the largest which
 // digit the k-th has. Where few enough keys share its first digit they are listed, and
 // one wave finds it among them.
-// 1024 rows of up to 8192 values (30 MB) take 20.5 us, where a copy of them takes 6: four
-// workgroups a CU go through one chain of barriers each, the counting in LDS first among
-// what they wait for.
-constexpr int kBins = 2048, kListed = 512, kPerThread = 16;
+// 1024 rows of up to 8192 values (30 MB) take 19.8 us, where a copy of them takes 6: four
+// workgroups a CU go through one chain of barriers each and fill the vector units to 62%.
+constexpr int kBins = 2048, kListed = 512;
 
-template <int W, bool HELD>
-__global__ __launch_bounds__(64 * W, 8) void select_group_kernel(SelectArgs a) {
+template <int W, int KPT, bool HELD>
+__global__ __launch_bounds__(64 * W, KPT > 16 ? 4 : 8) void select_group_kernel(SelectArgs a) {
   __shared__ int s_bins[kBins], s_pick[3], s_count[2][W], s_listed;
   __shared__ uint32_t s_list[kListed], s_theta;
   __shared__ uint8_t s_owner[kListed];
@@ -141,7 +140,6 @@ __global__ __launch_bounds__(64 * W, 8) void select_group_kernel(SelectArgs a) {
     return;
   }
   const int per = (s.n + 64 * W - 1) / (64 * W) * 64, w0 = wave * per, w1 = min(w0 + per, s.n);
-  constexpr int KPT = kPerThread;
   uint32_t key[KPT];
   // (offsets in 32 bits beside scalar addresses: n and count are below 2^30)
   auto value = [&](int i) __attribute__((always_inline)) {
@@ -230,22 +228,28 @@ __global__ __launch_bounds__(64 * W, 8) void select_group_kernel(SelectArgs a) {
       break;
     }
     if (pass == 0 && alike <= kListed) {
-      int more = 0;
+      int more = 0, own = 0;  // of the wave, of the lane
       const uint32_t next = theta + (1u << 21) - 1;  // the last key with this digit
       each([&](int, uint32_t key) __attribute__((always_inline)) {
         more += __builtin_popcountll(__ballot(key > next));
-        const unsigned long long m = __ballot(key - theta < 1u << 21);
-        if (m) {
-          int at = 0;
-          if (lane == 0) at = atomicAdd(&s_listed, __builtin_popcountll(m));
-          at = __builtin_amdgcn_readfirstlane(at) + lanes_below(m);
-          if (key - theta < 1u << 21) {
-            s_list[at] = key;
-            s_owner[at] = (uint8_t)wave;
-          }
+        own += key - theta < 1u << 21;
+      });
+      int at = own;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(at, o);
+        if (lane >= o) at += y;
+      }
+      int base = 0;
+      if (lane == 63) base = atomicAdd(&s_listed, at);
+      at += __shfl(base, 63) - own;
+      each([&](int, uint32_t key) __attribute__((always_inline)) {
+        if (key - theta < 1u << 21) {
+          s_list[at] = key;
+          s_owner[at++] = (uint8_t)wave;
         }
       });
-      if (lane == 0) atomicAdd(&s_count[0][wave], more);
+      if (lane == 0) s_count[0][wave] = more;
       __syncthreads();
       if (wave == 0) {
         uint32_t key[kListed / 64];
@@ -307,9 +311,9 @@ template <int KPT>
 void launch_wave(const SelectArgs& a, hipStream_t st) {
   hipLaunchKernelGGL(select_wave_kernel<KPT>, dim3((unsigned)cdiv(a.total, 4)), dim3(256), 0, st, a);
 }
-template <int W, bool HELD>
+template <int W, int KPT, bool HELD>
 void launch_group(const SelectArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((select_group_kernel<W, HELD>), dim3((unsigned)a.total), dim3(64 * W), 0, st, a);
+  hipLaunchKernelGGL((select_group_kernel<W, KPT, HELD>), dim3((unsigned)a.total), dim3(64 * W), 0, st, a);
 }
 
 }  // namespace
@@ -323,7 +327,8 @@ int select_top(const float* x, const int32_t* lengths, int32_t* out, int64_t lay
   // Up to 1024 values a wave a row: 2048 rows of 1000 take 10.7 us, with a workgroup each
   // 12.6 or more; rows of 2000 13.4 with a workgroup, 17.4 with a wave. The smallest
   // workgroup that holds the keys of longer ones; without (rows of 16000) 2048 rows take
-  // 83 us, with them 64.
+  // 83 us, with them 62. 32 keys a thread let one workgroup on a CU: 256 rows of 20000 take
+  // 20 us, 512 35, where keys that are made again take 32 and 45; 2048 rows 131 and 117.
   if (n <= 256)
     launch_wave<4>(a, stream);
   else if (n <= 512)
@@ -331,13 +336,15 @@ int select_top(const float* x, const int32_t* lengths, int32_t* out, int64_t lay
   else if (n <= 1024)
     launch_wave<16>(a, stream);
   else if (n <= 4096)
-    launch_group<4, true>(a, stream);
+    launch_group<4, 16, true>(a, stream);
   else if (n <= 8192)
-    launch_group<8, true>(a, stream);
+    launch_group<8, 16, true>(a, stream);
   else if (n <= 16384)
-    launch_group<16, true>(a, stream);
+    launch_group<16, 16, true>(a, stream);
+  else if (n <= 32768 && total <= 2 * device_cus())
+    launch_group<16, 32, true>(a, stream);
   else
-    launch_group<16, false>(a, stream);
+    launch_group<16, 16, false>(a, stream);
   return check_launch("select_top");
 }
 

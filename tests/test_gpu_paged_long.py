@@ -727,3 +727,22 @@ def test_a_pool_past_4_gib(gpu):
                         *(t[shift:] for t in c)])
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+# --- selection at the borders of its kernels ----------------------------------------
+
+@pytest.mark.parametrize("n", [1023, 4095, 8192, 8193, 16384, 16385, 32768, 32769])
+@pytest.mark.parametrize("kind", ["normal", "ties"])
+def test_select_at_borders(gpu, n, kind):
+    test_select(gpu, n, kind)
+
+
+def test_select_of_many_long_rows(gpu):
+    import sparkq
+
+    n = 17001
+    x = torch.randn((1, 65, 16, n), generator=torch.Generator().manual_seed(n))
+    x[:, ::2] = torch.round(x[:, ::2] * 8)
+    lengths = [n - 13 * (i % 5) for i in range(65)]
+    got = sparkq.select_top(x.to(gpu), 700, lengths=_ints(lengths, gpu), first=3, last=40)
+    assert torch.equal(got.cpu(), long.select(x, 700, lengths, 3, 40))
