@@ -682,7 +682,8 @@ int sparkq_kv_pages_compact(void* k_codes, void* v_codes, void* k_scales, void* 
 
 /* sparkq_paged_sdpa that also returns lse [T,Hq] float32: the natural logarithm of
  * the sum of each row's exp(scale * q . k) over the tokens that it sees, -inf where
- * that is none. Rows of lse are written where rows of out are. */
+ * that is none. The values have no part in it, nor have their scales, not even where
+ * these are not finite. Rows of lse are written where rows of out are. */
 int sparkq_paged_sdpa_lse(const void* q, const void* k_codes, const void* k_scales,
                           const void* v_codes, const void* v_scales,
                           const int32_t* page_table, const int32_t* starts,

@@ -251,13 +251,17 @@ template <int TOP>
 __device__ __forceinline__ float unit(const RowState& st) { return st.t - (float)TOP; }
 
 // The exponent of a value scale's size; no less than -60 (fp16 ends at -24: 0 is
-// meant), so that a row whose best token has no value keeps a finite normalizer.
+// meant), so that a row whose best token has no value keeps a finite normalizer, and no
+// more than 16 (fp16 ends at 15: what is not finite is meant), so that the scores of
+// the other tokens still count in it.
 __device__ __forceinline__ float scale_exp(float v) {
-  return (float)max((int)(__float_as_uint(v) >> 23 & 255u), 127 - 60) - 127.0f;
+  return (float)min(max((int)(__float_as_uint(v) >> 23 & 255u), 127 - 60), 127 + 16) - 127.0f;
 }
 
 // What a part of a row's context hands on: its unit, or -inf where it saw nothing
-// (scores that are all NaN leave no maximum, but a sum that is not 0).
+// (scores that are all NaN leave no maximum, but a sum that is not 0). Its sums are NaN
+// where it saw a value that is not finite, and count whatever their weight: 0 times NaN
+// is NaN.
 template <int TOP>
 __device__ __forceinline__ float part_max(const RowState& st, float z) {
   return st.t != kNegInf ? unit<TOP>(st) : (z != 0.0f ? 0.0f : kNegInf);
@@ -310,17 +314,21 @@ __device__ __forceinline__ float most_of(float v) {
 __device__ __forceinline__ float least_of(float v) { return -max_row16(-fabsf(kept_scale(v))); }
 constexpr float kSpread = 16.0f;  // of the largest to the least that one exponent stands for
 
-// Hides the scores that are not in `ok` and turns those of values that are not
-// finite to NaN; returns the largest score plus scale exponent of the others.
+// Hides the scores that are not in `ok`; returns the largest score plus scale exponent
+// of those that are visible. `odd` is NaN where the row sees a value that is not finite,
+// and takes its sums with it, but not its normalizer.
 template <int N, int G>
-__device__ __forceinline__ float hide(uint32_t ok, float s[N], float mul, const float vsc[N]) {
+__device__ __forceinline__ float hide(uint32_t ok, float s[N], float mul, const float vsc[N], float& odd) {
   float t = kNegInf;
+  uint32_t bad = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const bool live = (ok >> i) & 1u;
-    s[i] = live ? (__float_as_uint(vsc[i]) == 0x80000000u ? __builtin_nanf("") : s[i]) : kNegInf;
+    s[i] = live ? s[i] : kNegInf;
     t = fmaxf(t, fmaf(s[i], mul, scale_exp(vsc[i])));
+    bad |= live ? (uint32_t)(__float_as_uint(vsc[i]) == 0x80000000u) : 0u;
   }
+  odd = sum_groups<G>(bad ? __builtin_nanf("") : 0.0f);
   return max_groups<G>(t);
 }
 

@@ -488,7 +488,13 @@ __global__ __launch_bounds__(256, 2) void paged_tile_kernel(PagedSdpaArgs a) {
         const int j = 4 * G * (i >> 2) + 4 * grp + (i & 3);
         ok |= (uint32_t)(t0 + j <= lim && ((pages_ok >> (j / 16)) & 1u)) << i;
       }
-      t = hide<N, G>(__float_as_uint(pinned(__uint_as_float(ok))), s, mul, vsc);
+      float odd;
+      t = hide<N, G>(__float_as_uint(pinned(__uint_as_float(ok))), s, mul, vsc, odd);
+      if (__ballot(odd != odd)) {
+        const float f = pinned(odd != odd ? odd : 1.0f);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[j] *= f;
+      }
     } else {
       t = s[0];
 #pragma unroll
@@ -725,7 +731,13 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
         const int j = 32 * half + 4 * G * (i >> 2) + 4 * grp + (i & 3);
         ok |= (uint32_t)(t0 + j <= lim && ((pages_ok >> (j / 16)) & 1u)) << i;
       }
-      t = hide<N, G>(__float_as_uint(pinned(__uint_as_float(ok))), s, mul, vsc);
+      float odd;
+      t = hide<N, G>(__float_as_uint(pinned(__uint_as_float(ok))), s, mul, vsc, odd);
+      if (__ballot(odd != odd)) {
+        const float f = pinned(odd != odd ? odd : 1.0f);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[j] *= f;
+      }
     } else {
       t = s[0];
 #pragma unroll
@@ -845,11 +857,20 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
     }
   }
 
-  // the halves' sums (every wave is past its last read of the states)
+  // the halves' sums (every wave is past its last read of the states and the weights); a
+  // wave that weighed a value that is not finite has NaN in its dims, and here the other
+  // learns of it
   float z = sum_groups<G>(st.z);
+  float* const some = reinterpret_cast<float*>(smem + S::P);
   state[32 * wave + row] = z;
+  if (grp == 0) some[32 * wave + row] = acc[0][0];
   __syncthreads();
   z += state[32 * (wave ^ 1) + row];
+  const float odd = some[32 * (wave ^ 1) + row];
+  if (__builtin_expect(odd != odd, 0)) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[j] *= odd;
+  }
   const int r = 32 * (wave >> 1) + row;
   if (r >= rows) return;
   if (it.parts == 1) {
@@ -938,7 +959,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PagedSdpaArgs a) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const float f = wts[r][min(k0 + u * ways, parts - 1)];
-        if (k0 + u * ways < parts && f != 0.0f) o += v[u] * f;
+        o += v[u] * (k0 + u * ways < parts ? f : 0.0f);
       }
     }
     if (ways > 1) {

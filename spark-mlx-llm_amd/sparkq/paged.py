@@ -189,7 +189,8 @@ def paged_quantized_sdpa(queries, cache, page_table, starts, lengths, *, scale, 
     quarter more time there). Scores, normalizer and sums are fp32.
 
     With return_lse the result is (out, lse [T,Hq] float32): the natural logarithm of
-    the sum of each row's exponentiated scores, -inf where it sees nothing."""
+    the sum of each row's exponentiated scores, -inf where it sees nothing. Values and
+    their scales have no part in it, finite or not."""
     op = "paged_quantized_sdpa"
     kc, ks, vc, vs, index, (pages, hkv, page, d) = _check_cache(op, cache, 4)
     _check_attention(op, queries, hkv, d, index, mask, scale, max_new)
