@@ -755,13 +755,18 @@ class PagedKVCache:
     def evict(self, count: int, *, first: int = 0, last: int = 0):
         """Rows of more than `count` tokens keep `count` of them, in each layer and KV head
         its own: the first `first`, the last `last`, and those of the rest that gathered
-        the most attention weight. To be called between steps: the tokens of the last one
-        are then old ones. Returns `missing` (on the device, like step's): pages that the
-        pool was short of, as what is written must not be shared; when it is not 0 all is
-        as it was."""
+        the most attention weight. To be called between steps, when every layer has appended
+        and attended the last one's tokens, which are then old ones: refused before the
+        first append of a step with new tokens. Returns `missing` (on the device, like
+        step's): pages that the pool was short of, as what is written must not be shared;
+        when it is not 0 all is as it was."""
         self._ready()
         if self.mass is None:
             raise ValueError("evict needs a cache with mass=True")
+        if self._last is not None and self.max_new:
+            raise ValueError("evict comes between steps, and the last one's tokens are not in the "
+                             "cache: append and attend them, or take a step that was short of "
+                             "pages back with undo()")
         keep = select_top(self.mass, count, lengths=self._lengths, first=first, last=last)
         before = self._lengths
         self.page_table, self._lengths, self.missing = kv_pages_evict(
