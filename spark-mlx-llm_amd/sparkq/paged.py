@@ -680,10 +680,11 @@ class PagedKVCache:
             self._lengths = ints.new_tensor([min(n, room) for n in after])
             self.missing, self._full = self.missing.new_full((1,), short), True
         else:
+            # (first what may fail for want of memory: the fork cannot be taken back)
+            mass = self.mass if self.mass is None or parents is None else self._mass_of(parents)
             self.page_table, self._lengths, self.missing = kv_pages_fork(
                 self.cache, self.page_table, self._lengths, parents, ints[:rows])
-            if self.mass is not None and parents is not None:
-                self.mass = self._mass_of(parents)
+            self.mass = mass
         self._last, self._counts = last, after
         self.starts, self.max_new = ints[rows:2 * rows + 1], max(new_tokens, default=0)
         return self.starts

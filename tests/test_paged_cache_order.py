@@ -62,3 +62,20 @@ def test_eviction_after_what_has_no_new_tokens(cache):
     cache.step([0, 0], [0, 0])
     cache.evict(6)
     assert cache.calls == ["fork", "append", "evict", "fork", "evict", "fork", "evict"]
+
+
+def test_a_step_that_fails_leaves_the_cache_as_it_was(cache, monkeypatch):
+    """Weights of rows that continue others are a tensor of their own, which there may be
+    no memory for."""
+    def full(self, parents):
+        raise torch.OutOfMemoryError("no memory")
+
+    names = ("page_table", "lengths", "missing", "mass", "starts", "max_new", "_last", "_counts")
+    before = [getattr(cache, n) for n in names]
+    with monkeypatch.context() as m:
+        m.setattr(sparkq.PagedKVCache, "_mass_of", full)
+        with pytest.raises(torch.OutOfMemoryError):
+            cache.step([3, 4, 5], [0, 0, 1])
+    assert all(getattr(cache, n) is b for n, b in zip(names, before)) and not cache.calls
+    cache.step([3, 4, 5], [0, 0, 1])
+    assert cache.lengths.tolist() == [23, 24, 14] and cache.mass.shape[1] == 3
