@@ -257,6 +257,8 @@ struct MassShape {
   static constexpr int BUF = ROWS * 2 * D;
   static constexpr int JOIN = 8 * 32 * 33 * 4;
   static constexpr int BYTES = 2 * BUF > JOIN ? 2 * BUF : JOIN;
+  static constexpr int ALIGN = 2 * D;  // of the buffers: a row's pieces are addressed by xor
+  static_assert(BUF % ALIGN == 0 && ROWS * ALIGN == BUF, "rows lie at multiples of their size");
   // 16-byte piece p of row r lies at place p ^ turn(r) of its row: any 16 rows' pieces p
   // hit different banks
   static __device__ __forceinline__ int turn(int r) { return D == 64 ? (r >> 1) & 7 : r & 15; }
@@ -275,7 +277,7 @@ __global__ __launch_bounds__(512, D <= 128 ? 4 : 2) void paged_mass_many_kernel(
   constexpr int NK = D / 16, N = mass_tokens(WAYS), kRows = S::ROWS;
   constexpr int PPR = D / 8, PPT = kRows * PPR / 512;  // 16-byte pieces of a row, of a thread
   const PagedSdpaArgs& a = s.a;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[S::BYTES];
+  __shared__ __attribute__((aligned(S::ALIGN))) unsigned char smem[S::BYTES];
   __shared__ float s_base[2][kRows];
   __shared__ int s_lim[2][kRows];
   __shared__ __attribute__((aligned(16))) float s_scale[N];
@@ -344,8 +346,8 @@ __global__ __launch_bounds__(512, D <= 128 ? 4 : 2) void paged_mass_many_kernel(
 #pragma unroll
     for (int v = 0; v < 16; ++v) sum[v] = 0.0f;
     auto tile = [&](int buf, int r, bool whole) {  // rows r .. r + 31 of a buffer
-      // (16 ((2 k + grp) ^ turn) is 32 k ^ 16 (grp ^ turn): one address, where the compiler
-      // would keep one for each k)
+      // (16 ((2 k + grp) ^ turn) is 32 k ^ 16 (grp ^ turn), and below the 2 D that rows are
+      // aligned to: one address, where the compiler would keep one for each k)
       uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem + buf * S::BUF +
                     (r + col) * 2 * D + 16 * (grp ^ S::turn(r + col));
       asm volatile("" : "+v"(at));
