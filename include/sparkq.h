@@ -703,7 +703,8 @@ int sparkq_paged_sdpa_lse(const void* q, const void* k_codes, const void* k_scal
 
 /* Bounds of each page's keys: bounds bf16 [pages,Hkv,2,D], the least key of a
  * channel rounded down, then the largest rounded up, with bounds_strides[0..1] =
- * page, head in elements (multiples of 8, 16-byte aligned, [2][D] contiguous).
+ * page, head in elements (multiples of 8, 16-byte aligned, [2][D] contiguous, both
+ * no less than 2 D).
  * Written for the pages that hold the batch's new tokens (the last starts[b+1] -
  * starts[b] of sequence b, of at most max_new), from all tokens of the page that
  * the sequence has. A page with a key scale that is not finite is bounded by

@@ -1095,6 +1095,7 @@ int sparkq_paged_key_bounds(const void* k_codes, const void* k_scales, void* bou
                                 k_scales, strides))
     return rc;
   if (int rc = bounds_check("paged_key_bounds", bounds, bounds_strides, D, Hkv)) return rc;
+  REQUIRE(bounds_strides[0] >= 2 * D || pages == 1, "paged_key_bounds: bounds overlap");
   REQUIRE(starts && (B == 0 || (page_table && lengths)), "paged_key_bounds: null tensor pointer");
   REQUIRE(max_new > 0 && max_new <= kI32Max, "paged_key_bounds: max_new must be positive");
   DEVICE_OK();
