@@ -719,12 +719,14 @@ int sparkq_paged_key_bounds(const void* k_codes, const void* k_scales, void* bou
 
 /* Scores of a row's pages: scores[t,h,j] = max over the query heads g of KV head h
  * of scale * sum_d max(q[t,g,d] lo[d], q[t,g,d] hi[d]) (min where scale < 0), no less
- * than any of their logits with a key of page j of t's sequence; -inf where t sees
- * nothing of the page (causal as in sparkq_paged_sdpa) or there is none. A head
- * whose sum is NaN does not count. scores float32 [T,Hkv,max_pages] contiguous and
+ * than any of their logits with a key of page j of t's sequence, but for rounding;
+ * -inf where t sees nothing of the page (causal as in sparkq_paged_sdpa) or there is
+ * none. A head whose sum is NaN does not count. scores float32 [T,Hkv,max_pages] contiguous and
  * 16-byte aligned, seen int32 [T]: how many of its pages t sees. Rows that fall to
  * no sequence, or past max_new of one, are left as they were. Products of 16-bit
- * values are exact, sums fp32. */
+ * values are exact, sums fp32: off by (2 D + 2) 2^-24 of |scale| sum_d |q| max(|lo|,
+ * |hi|) at most, and with float16 queries, for which a page's bounds are turned to
+ * fp16, by 2^-39 of its largest bound times |scale| sum_d |q| more. */
 int sparkq_paged_page_scores(const void* q, const void* bounds, const int32_t* page_table,
                              const int32_t* starts, const int32_t* lengths, float* scores,
                              int32_t* seen, int64_t T, int64_t B, int64_t Hq, int64_t Hkv,

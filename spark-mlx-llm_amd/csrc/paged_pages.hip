@@ -8,7 +8,8 @@
 //   scale * sum_d max(q[d] lo[d], q[d] hi[d])  =  scale * (q+ . hi + q- . lo)
 //
 // with q+ and q- the positive and negative values of q (scale >= 0; q takes its
-// sign): a product of depth 2 D.
+// sign): a product of depth 2 D, in fp32 sums (so but for (2 D + 2) 2^-24 of its terms'
+// sizes).
 #include <algorithm>
 
 #include "paged.h"
@@ -149,7 +150,8 @@ __device__ __forceinline__ f32x4_t mfma16(u32x4_t x, u32x4_t y, f32x4_t c) {
 // A lane's share of the bounds of a page: dims 32 c + 8 grp .. + 8, and what the
 // scores have to be multiplied by. For fp16 queries the bounds are turned to fp16,
 // shifted by a power of two for that: exact but for what bf16 holds below 2^-28 of
-// the page's largest, which is rounded.
+// the page's largest, which is rounded, by 2^-39 of the largest at most (to nearest: a
+// bound may come out that much too narrow).
 template <typename T, int D>
 struct PageOperand {
   u32x4_t lo[D / 32], hi[D / 32];

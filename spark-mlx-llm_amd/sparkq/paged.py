@@ -267,8 +267,10 @@ def paged_page_scores(queries, bounds, page_table, starts, lengths, *, page_size
         max over the head's query heads g of  scale * sum_d max(q[t,g,d] lo, q[t,g,d] hi)
 
     with the bounds of that page [pages,Hkv,2,D]: no logit of the row with a key of
-    the page is larger. (scale < 0: with min for max.) -inf where the row sees
-    nothing of the page, or there is none; a head whose sum is NaN does not count.
+    the page is larger, but for the rounding of an fp32 sum ((2 D + 2) 2^-24 of its
+    terms' sizes; with float16 queries also 2^-39 of the page's largest bound times
+    scale * sum |q|). (scale < 0: with min for max.) -inf where the row sees nothing of
+    the page, or there is none; a head whose sum is NaN does not count.
     seen counts the pages that each row sees, for select_top:
 
         scores, seen = paged_page_scores(...)
