@@ -587,7 +587,11 @@ class PagedKVCache:
         cache.evict(count)                           # between steps
 
     leaves each row the `count` tokens that gathered most. (After it lengths are no
-    longer positions: count these apart.)"""
+    longer positions: count these apart.) What a token added to the others' weight stays
+    there when it is taken back by lowering `lengths`. A step of drafted tokens is
+    therefore attended by paged_quantized_sdpa(..., return_lse=True), and paged_kv_mass
+    adds the weights of the accepted rows to mass[l] (with starts of their own and the
+    lowered lengths) once it is known which these are."""
 
     def __init__(self, layers: int, pages: int, kv_heads: int, head_dim: int, *,
                  page_size: int = 64, max_pages: int = 128, batch: int = 0, device="cuda",
