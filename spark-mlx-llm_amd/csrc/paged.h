@@ -65,8 +65,9 @@ __device__ __forceinline__ int seq_of_row(const PagedBatch& p, int t) {
   return lo < p.B ? lo : -1;
 }
 
-// The sequence whose rows hold packed row t, or b = -1, in one round trip for every 64
-// sequences: all lanes of a wave ask for the same row.
+// The sequence whose rows hold packed row t, or b = -1: a round trip for the ends of every
+// 64 sequences' rows, and one for what is there of the one that has it (the compiler puts
+// those loads behind the ballot). All lanes of a wave ask for the same row.
 struct RowOf {
   int b;
   SeqRows s;

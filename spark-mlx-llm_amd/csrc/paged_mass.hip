@@ -192,18 +192,22 @@ __global__ __launch_bounds__(256) void paged_mass_few_kernel(MassArgs s) {
 // ---------------------------------------------------------------------------
 // A wave has 32 tokens of one KV head, their codes in registers as the first operand
 // of the 32 x 32 products. The workgroup goes over the rows that see its tokens, kRows
-// at a time: it brings their queries into LDS, the next ones' loads in flight, and a
-// wave takes tiles of 32 of them as second operands. A lane then has one row's scores of 16
+// at a time: it brings their queries into LDS, in one of two buffers, and a wave takes
+// tiles of 32 of them as second operands. A lane then has one row's scores of 16
 // tokens, and sums its rows' weights in registers; lanes (and waves) are joined at the
 // end through LDS. Codes are exact in either 16-bit type, so queries stay as they are.
 // WAYS waves share 32 tokens and take turns at the tiles: two, or four where that gives
 // less than two workgroups a CU (500 new tokens of 1000, 8 KV heads: four 22 us, two 28;
-// 3 sequences of 300 and 6000, 4 KV heads of 256: two 33, four 49).
+// 3 sequences of 300 and 6000, 4 KV heads of 256: two 33, four 49). What counts is what the
+// tables have room for, as lengths are on the device: those 500 take 28 in a table of 128
+// pages of 64.
 // What it has to do is the product and an exponential a score: 2048 new tokens of 8192, 32
-// heads of 128 on 8, take 155 us, 780 TFLOP/s. The vector units bound it (66 % busy, the
-// matrix units 42 %): a multiply-add, an exponential and an addition a score, and what
-// hides the loads. Queries go straight into LDS: through registers the same tiles take
-// 164 us, as 11 of them spill.
+// heads of 128 on 8, take 150 to 155 us, 780 to 800 TFLOP/s. Nothing is full (vector units
+// 65 %, matrix units 42 %, waves wait in 39 % of their time). The next rows' loads are issued
+// before this round's tiles, but do not run beside them: the compiler cannot tell the
+// buffer that they fill from the one that is read, and waits for them before a tile's first
+// read, so each round of two tiles a wave has a round trip to memory in it. Queries go
+// straight into LDS: through registers the same tiles take 164 us, as 11 of them spill.
 template <typename T>
 __device__ __forceinline__ u32x4_t codes_as(uint32_t lo, uint32_t hi);
 template <>

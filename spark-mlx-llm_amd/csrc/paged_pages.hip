@@ -219,8 +219,10 @@ __device__ __forceinline__ f32x4_t page_scores(const PageOperand<T, D>& b, const
 
 // One new token a sequence: a group's query heads are the product's 16 columns, and
 // the largest of their scores is taken over a row of 16 lanes. A wave has 16 pages of
-// one KV head, a workgroup 64. A chain of three round trips: one sequence of 512 pages
-// takes 4.2 us, 64 of up to 512 (39 MB) 14.5 (with 32 pages a wave 5.3 and 15.9).
+// one KV head, a workgroup 64. A chain of three round trips, starts, then length and table,
+// then bounds and queries: one sequence of 512 pages takes 4.2 us, 64 of up to 512 (39 MB)
+// 14.0 to 15.1 (with 32 pages a wave 5.3 and 15.9), where the grid, which the table's width
+// makes, is twice what the chip holds and mostly idle.
 constexpr int kOnePages = 64;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_scores_one_kernel(ScoreArgs a) {
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(256) void paged_scores_one_kernel(ScoreArgs a) {
   const int kh = blockIdx.x % a.Hkv, x = blockIdx.x / a.Hkv, b = x / a.chunks, chunk = x - b * a.chunks;
   const int gqa = a.Hq / a.Hkv;
   const int j0 = chunk * kOnePages + 16 * wave, j = j0 + n16;
-  // (asked for before the lengths are known, which say whether it is a page)
+  // (asked for beside the length, which says whether it is a page)
   const int id = a.p.table[b * a.p.table_stride + min(j, a.p.width - 1)];
   const SeqRows s = seq_rows(a.p, b);
   if (s.count == 0) return;
@@ -309,8 +311,10 @@ __device__ __forceinline__ TokenTile find_tokens(const PagedBatch& p, int max_ne
 // head at a time, and the largest over the group's heads stays in the lane. A wave
 // holds the bounds of 32 pages in registers, a workgroup takes 128. 512 new tokens of
 // 16384 (512 pages of 32, 20 heads on 4, fp16) take 13.4 us, 200 TFLOP/s: 512 workgroups,
-// each a wait for lengths, table and bounds before five heads' products; bounds turned to
-// fp16 (once a wave) and queries parted by sign are most of its instructions.
+// each a chain of lengths, the first tile's page, its bounds beside the second's page, that
+// one's bounds, and then a round trip a head: the compiler loads a head's queries right
+// before its products, not beside the ones before. Bounds turned to fp16 (once a wave) and
+// queries parted by sign are most of its instructions.
 constexpr int kManyPages = 128;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_scores_many_kernel(ScoreArgs a) {

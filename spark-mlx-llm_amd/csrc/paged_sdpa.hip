@@ -902,8 +902,10 @@ __global__ __launch_bounds__(512, 2) void paged_pair_kernel(PagedSdpaArgs a) {
 // tile. A wave per row finds the parts' weights (a lane each, one round trip);
 // then a thread sums four dims of a row over every `ways`-th part, eight loads
 // in flight, and the ways are summed through LDS. A chain of round trips: 4.2 us
-// where nothing was split, 4.4 us for 32 parts of one sequence's 32 heads. (A join
-// by the last part to end would need counters that are zero before every call.)
+// where nothing was split, 4.6 us for 32 parts of one sequence's 32 heads. What weighs
+// nothing is added all the same, which NaN needs and which lets the eight loads go out
+// together (where each was behind a test of its weight 5.5). A join by the last part to
+// end would need counters, in memory of their own that threads and captured graphs share.
 constexpr int kMaxParts = 512;
 template <int D, int R>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PagedSdpaArgs a) {

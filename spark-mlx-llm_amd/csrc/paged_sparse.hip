@@ -366,8 +366,8 @@ SparsePlan sparse_plan(int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t co
   const int64_t gqa = Hq / Hkv;
   p.tiles = cdiv(gqa, 16);
   p.rows_held = std::min<int64_t>(gqa, 16);
-  // Lists are split where there are fewer of them than CUs, into parts of no less than
-  // 128 tokens (a block for each wave). More parts fill the chip better, but joining
+  // Lists are split where there are no more of them than half the CUs, into parts of no
+  // less than 128 tokens (a block for each wave). More parts fill the chip better, but joining
   // them costs 4 us: 224 lists of 77 pages of 32 tokens at D = 256 take 51 us whole, 53
   // + 5 in two parts; 56 lists of 32 pages of 64 at D = 128 15 + 4 in four, 17 + 4 in ten.
   // Lists that four waves take about as long for as a join stay whole, one launch less: 8

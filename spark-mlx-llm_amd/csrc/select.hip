@@ -329,6 +329,8 @@ int select_top(const float* x, const int32_t* lengths, int32_t* out, int64_t lay
   // workgroup that holds the keys of longer ones; without (rows of 16000) 2048 rows take
   // 83 us, with them 62. 32 keys a thread let one workgroup on a CU: 256 rows of 20000 take
   // 20 us, 512 35, where keys that are made again take 32 and 45; 2048 rows 131 and 117.
+  // It goes by what a row has room for, as lengths are on the device: 1024 rows of 2000 take
+  // 12 us in 2000 places, 14 in 8192, 27 in 16384 and 40 in 40000.
   if (n <= 256)
     launch_wave<4>(a, stream);
   else if (n <= 512)
